@@ -327,6 +327,143 @@ int pplx_a2a_graph_end_capture(void *stream, pplx_a2a_graph_t **out);
 int pplx_a2a_graph_launch(pplx_a2a_graph_t *graph, void *stream);
 int pplx_a2a_graph_destroy(pplx_a2a_graph_t *graph);
 
+/* ---- between dispatch and combine ------------------------------------------ */
+
+/* Operators on plain device buffers: no world, no handle, nothing kept between calls.  They only
+ * enqueue kernels on `stream` of `device` (a HIP device ordinal), so they may be captured; every
+ * buffer, the workspace among them, is the caller's and stays valid until the kernels are done.
+ * Two calls that may overlap in time need workspaces of their own.  They have no counterpart in the
+ * reference, which leaves the experts to its caller. */
+
+/* Tokens sorted by expert.  Pick (t, k) is live when t < min(m, *bound_m) and indices[t, k] <
+ * num_experts; its row is slots[t, k], its rank among the live picks ordered by (expert, t, k), and
+ * -1 when it is not live.  Rows offsets[e] .. offsets[e + 1] - 1 are expert e's; out_rows[slot] is a copy of
+ * x[t], or its quantised form, and the rows of out_rows[0 .. m * experts_per_token) behind the last
+ * live one are zeros (their scales too).  Unlike dispatch every pick has a row, one that repeats an expert of
+ * its token too.  Quantised rows (out_scale not NULL): a = max(max |x[t, :]|, 2^-100),
+ * out_rows = rint(x * (127 / a)) as int8 and out_scale = a / 127; a row that holds an infinity or a NaN
+ * becomes zeros with a scale of NaN. */
+typedef struct pplx_a2a_sort_args {
+  const void *x;               /* [m, hidden_dim] of dtype, 16-byte aligned */
+  int64_t x_stride_row;        /* bytes, a multiple of 16 */
+  int32_t dtype;               /* pplx_a2a_dtype */
+  uint32_t m;
+  uint32_t experts_per_token;  /* 1..64; m * experts_per_token < 2^31 */
+  uint32_t num_experts;        /* 1..5461 */
+  uint64_t hidden_dim;         /* rows, and quantised rows, are multiples of 16 bytes */
+  const uint32_t *indices;     /* [m, K] contiguous */
+  const uint32_t *bound_m;     /* device scalar or NULL (= m) */
+  void *out_rows;              /* [m * K, hidden_dim] of dtype, or int8 */
+  int64_t out_stride_row;      /* bytes, a multiple of 16 */
+  float *out_scale;            /* [m * K] or NULL */
+  int32_t *slots;              /* [m, K] contiguous */
+  int32_t *offsets;            /* [num_experts + 1] */
+  void *workspace;             /* pplx_a2a_sort_workspace bytes, 4-byte aligned; may be NULL when that is 0 */
+} pplx_a2a_sort_args_t;
+int pplx_a2a_sort_workspace(uint32_t m, uint32_t experts_per_token, uint32_t num_experts, uint64_t *bytes);
+int pplx_a2a_sort_tokens(int device, const pplx_a2a_sort_args_t *args, void *stream);
+
+/* Sorted rows back to tokens: out[t] = sum over k of weights[t, k] * y[slots[t, k]], accumulated in
+ * fp32 in the order of k and rounded once; picks with a slot outside [0, y_rows) add nothing, whatever their
+ * weight, and a token without others becomes zeros.  Without weights the sum of the rows, which is the gradient of
+ * sort_tokens. */
+typedef struct pplx_a2a_unsort_args {
+  void *out;                 /* [m, hidden_dim] of out_dtype, 16-byte aligned */
+  int64_t out_stride_row;    /* bytes, a multiple of 16 */
+  int32_t out_dtype;         /* pplx_a2a_dtype */
+  int32_t y_dtype;           /* pplx_a2a_dtype */
+  const void *y;             /* [y_rows, hidden_dim] of y_dtype, 16-byte aligned */
+  int64_t y_stride_row;      /* bytes, a multiple of 16 */
+  int64_t y_rows;
+  const int32_t *slots;      /* [m, K] contiguous */
+  const float *weights;      /* [m, K] contiguous or NULL */
+  uint32_t m;
+  uint32_t experts_per_token; /* 1..64 */
+  uint64_t hidden_dim;       /* a multiple of 8 */
+} pplx_a2a_unsort_args_t;
+int pplx_a2a_unsort_tokens(int device, const pplx_a2a_unsort_args_t *args, void *stream);
+
+/* Gradients of unsort_tokens: grad_y[slots[t, k]] = weights[t, k] * grad_out[t] and grad_weights[t, k] =
+ * <grad_out[t], y[slots[t, k]]>, summed in fp32; rows of grad_y from offsets[num_experts] on, which no slot names,
+ * and weights of picks without a row get zeros.  Either gradient may be left out (NULL). */
+typedef struct pplx_a2a_unsort_backward_args {
+  void *grad_y;               /* [y_rows, hidden_dim] of dtype, 16-byte aligned, or NULL */
+  int64_t grad_y_stride_row;  /* bytes, a multiple of 16 */
+  float *grad_weights;        /* [m, K] contiguous or NULL */
+  const void *grad_out;       /* [m, hidden_dim] of grad_dtype, 16-byte aligned */
+  int64_t grad_out_stride_row; /* bytes, a multiple of 16 */
+  int32_t grad_dtype;         /* pplx_a2a_dtype of grad_out */
+  int32_t dtype;              /* pplx_a2a_dtype of y and grad_y */
+  const void *y;              /* read for grad_weights only */
+  int64_t y_stride_row;       /* bytes, a multiple of 16 */
+  int64_t y_rows;             /* of y and grad_y */
+  const int32_t *slots;       /* [m, K] contiguous */
+  const int32_t *num_rows;    /* device scalar: live rows, which is offsets + num_experts */
+  const float *weights;       /* [m, K] contiguous or NULL (ones) */
+  uint32_t m;
+  uint32_t experts_per_token; /* 1..64 */
+  uint64_t hidden_dim;        /* a multiple of 8 */
+} pplx_a2a_unsort_backward_args_t;
+int pplx_a2a_unsort_tokens_backward(int device, const pplx_a2a_unsort_backward_args_t *args, void *stream);
+
+/* Where the rows of the experts lie.  PADDED: [num_experts, rows], of which expert e's first starts_or_counts[e] (clamped
+ * to 0 .. rows) are there, as dispatch leaves them; SORTED: [rows], of which starts_or_counts[e] ..
+ * starts_or_counts[e + 1] - 1 are expert e's (num_experts + 1 entries that do not descend from 0 on, clamped to rows);
+ * DENSE: [rows], all of them there (one expert, starts_or_counts NULL). */
+typedef enum pplx_a2a_row_layout {
+  PPLX_A2A_ROWS_DENSE = 0,
+  PPLX_A2A_ROWS_SORTED = 1,
+  PPLX_A2A_ROWS_PADDED = 2
+} pplx_a2a_row_layout;
+typedef struct pplx_a2a_rows {
+  int32_t layout;                   /* pplx_a2a_row_layout */
+  uint32_t num_experts;             /* 1..5461 */
+  uint64_t rows;                    /* of the buffer, PADDED: of each expert's; all of them < 2^31 */
+  const int32_t *starts_or_counts;
+} pplx_a2a_rows_t;
+
+/* Rows to 8 bits with one scale each, as sort_tokens does it: of x [.., width], or with swiglu of
+ * silu(x[.., :width]) * x[.., width:2 * width] in fp32, silu(g) = g / (1 + exp(-g)).  Rows that are not there
+ * are neither read nor written. */
+typedef struct pplx_a2a_quantize_args {
+  pplx_a2a_rows_t rows;
+  void *out;                       /* int8 [.., width], 16-byte aligned */
+  int64_t out_stride_row;          /* bytes, a multiple of 16, as is the next */
+  int64_t out_stride_expert;       /* (PADDED) */
+  float *out_scale;
+  int64_t out_scale_stride_row;    /* floats */
+  int64_t out_scale_stride_expert;
+  const void *x;                   /* of dtype, 16-byte aligned */
+  int64_t x_stride_row;            /* bytes, a multiple of 16, as is the next */
+  int64_t x_stride_expert;
+  int32_t dtype;                   /* pplx_a2a_dtype */
+  int32_t swiglu;
+  uint64_t width;                  /* a multiple of 16 */
+} pplx_a2a_quantize_args_t;
+int pplx_a2a_quantize_rows(int device, const pplx_a2a_quantize_args_t *args, void *stream);
+
+/* Rows times their experts' weights in 8-bit integers: out[r, n] = x_scale[r] * weight_scale[e, n] *
+ * sum over k of x[r, k] * weight[e, n, k].  The sums are exact (int32), the scaling is fp32, rounded once to out_dtype.
+ * Rows that are not there are neither read nor written. */
+typedef struct pplx_a2a_int8_matmul_args {
+  pplx_a2a_rows_t rows;
+  void *out;                     /* [.., n] of out_dtype, aligned to its elements */
+  int64_t out_stride_row;        /* elements */
+  int64_t out_stride_expert;
+  int32_t out_dtype;             /* pplx_a2a_dtype */
+  const int8_t *x;               /* [.., k], 16-byte aligned */
+  int64_t x_stride_row;          /* bytes, a multiple of 16, as is the next */
+  int64_t x_stride_expert;
+  const float *x_scale;
+  int64_t x_scale_stride_row;    /* floats */
+  int64_t x_scale_stride_expert;
+  const int8_t *weight;          /* [num_experts, n, k] contiguous, 16-byte aligned */
+  const float *weight_scale;     /* [num_experts, n] contiguous */
+  uint64_t n;                    /* < 2^31 */
+  uint64_t k;                    /* a multiple of 16, at most 131056: 128 * 128 * k < 2^31 */
+} pplx_a2a_int8_matmul_args_t;
+int pplx_a2a_int8_matmul(int device, const pplx_a2a_int8_matmul_args_t *args, void *stream);
+
 /* ---- misc -------------------------------------------------------------- */
 
 const char *pplx_a2a_last_error(void);

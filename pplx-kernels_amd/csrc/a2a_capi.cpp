@@ -19,6 +19,7 @@
 
 #include "a2a_device.h"
 #include "a2a_device_scope.h"
+#include "a2a_host.h"
 #include "pplx_a2a.h"
 
 // Profiler ranges around the launch sequences, like the reference's nvtxRangePush("dispatch") /
@@ -43,6 +44,12 @@ int fail(int status, const char *fmt, ...) {
   g_last_error = buf;
   return status;
 }
+
+}  // namespace
+
+int pplx_amd::report_failure(int status, const char *message) { return fail(status, "%s", message); }
+
+namespace {
 
 // (hipGetLastError: an error that is returned here is not reported once more by whoever asks for the last one)
 #define HIP_TRY(expr)                                                                        \

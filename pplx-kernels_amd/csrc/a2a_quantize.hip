@@ -1,0 +1,173 @@
+// Rows to 8 bits with one scale each, with the gated activation in front: the input of the experts' products.
+#include "a2a_experts.h"
+
+namespace pplx_amd {
+namespace {
+
+struct QuantizeDev {
+  RowsDev rows;
+  uint8_t *out;
+  int64_t out_stride_row, out_stride_expert;
+  float *scale;
+  int64_t scale_stride_row, scale_stride_expert;
+  const uint8_t *x;
+  int64_t x_stride_row, x_stride_expert;
+  uint32_t width;
+};
+
+// Sixteen values of the row from element 16 * j on.
+template <class T, bool SWIGLU>
+__device__ __forceinline__ void load_values(const PPLX_GLOBAL T *row, uint32_t width, uint32_t j, f32x8 *v) {
+  typename Eight<T>::raw a = load_eight<T>(row + 16ull * j), b = load_eight<T>(row + 16ull * j + 8);
+  v[0] = Eight<T>::wide(a);
+  v[1] = Eight<T>::wide(b);
+  if constexpr (SWIGLU) {
+    const PPLX_GLOBAL T *up = row + width;
+    a = load_eight<T>(up + 16ull * j);
+    b = load_eight<T>(up + 16ull * j + 8);
+    const f32x8 u[2] = {Eight<T>::wide(a), Eight<T>::wide(b)};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[i][k] = v[i][k] / (1.f + __expf(-v[i][k])) * u[i][k];
+    }
+  }
+}
+
+// LANES threads to a row; up to 32 * LANES elements stay in registers between the search for the largest value and the
+// conversion, longer rows are read twice.
+template <class T, bool SWIGLU, int LANES>
+__device__ __forceinline__ void quantize_one(const QuantizeDev &a, uint32_t e, uint32_t r, uint32_t g) {
+  constexpr int NS = 2;
+  const PPLX_GLOBAL T *row =
+      as_global(reinterpret_cast<const T *>(a.x + (int64_t)e * a.x_stride_expert + (int64_t)r * a.x_stride_row));
+  const uint32_t groups = a.width / 16;
+  const bool held = groups <= LANES * NS;
+  f32x8 v[2 * NS];
+  uint32_t bits = 0;
+  for (uint32_t base = 0; base < groups; base += LANES * NS) {
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      uint32_t j = base + i * LANES + g;
+      j = j < groups ? j : groups - 1;
+      load_values<T, SWIGLU>(row, a.width, j, v + 2 * i);
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * NS; ++i) {
+      const uint32_t b = magnitude_bits(v[i]);
+      bits = bits > b ? bits : b;
+    }
+  }
+  const RowScale s = row_scale(row_max<LANES>(bits));
+  if (g == 0) as_global(a.scale)[(int64_t)e * a.scale_stride_expert + (int64_t)r * a.scale_stride_row] = s.scale;
+  PPLX_GLOBAL u32x4 *out =
+      as_global(reinterpret_cast<u32x4 *>(a.out + (int64_t)e * a.out_stride_expert + (int64_t)r * a.out_stride_row));
+  for (uint32_t base = 0; base < groups; base += LANES * NS) {
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      const uint32_t j = base + i * LANES + g;
+      if (!held) load_values<T, SWIGLU>(row, a.width, j < groups ? j : groups - 1, v + 2 * i);
+      if (j < groups) out[j] = quantize_sixteen(v[2 * i], v[2 * i + 1], s.inverse);
+    }
+  }
+}
+
+// Rows of one buffer: as many as are there, 256 / LANES to a workgroup.
+template <class T, bool SWIGLU, int LANES>
+__global__ __launch_bounds__(256) void quantize_flat(QuantizeDev a) {
+  uint32_t there = a.rows.rows;
+  if (a.rows.layout == PPLX_A2A_ROWS_SORTED) {
+    const int32_t last = as_global(a.rows.starts_or_counts)[a.rows.experts];
+    there = last < 0 ? 0 : (uint32_t)last < there ? (uint32_t)last : there;
+  }
+  const uint32_t r = LANES == 64 ? blockIdx.x * 4 + wave_id() : blockIdx.x;
+  if (r < there) quantize_one<T, SWIGLU, LANES>(a, 0, r, threadIdx.x % LANES);
+}
+
+// Rows of the experts' buffers: workgroups share out the rows that are there, whose experts they find in the sums of the
+// counts.
+template <class T, bool SWIGLU, int LANES>
+__global__ __launch_bounds__(256) void quantize_padded(QuantizeDev a) {
+  extern __shared__ uint32_t upto[];  // rows of the experts up to and with each
+  __shared__ uint32_t of_wave[4];
+  const uint32_t E = a.rows.experts;
+  const uint32_t per = (E + 255) / 256, first = threadIdx.x * per;
+  uint32_t own = 0;
+  for (uint32_t i = 0; i < per; ++i) own += first + i < E ? span_of(a.rows, first + i).count : 0u;
+  uint32_t sum = wave_scan(own, lane_id());
+  if (lane_id() == 63) of_wave[wave_id()] = sum;
+  __syncthreads();
+  sum -= own;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) sum += (uint32_t)w < wave_id() ? of_wave[w] : 0u;
+  for (uint32_t i = 0; i < per; ++i) {
+    if (first + i < E) upto[first + i] = sum += span_of(a.rows, first + i).count;
+  }
+  __syncthreads();
+  const uint32_t there = upto[E - 1];
+  constexpr uint32_t kAtOnce = 256 / LANES;
+  for (uint32_t i = blockIdx.x * kAtOnce; i < there; i += gridDim.x * kAtOnce) {
+    const uint32_t r = i + (LANES == 64 ? wave_id() : 0);
+    if (r >= there) break;  // (with 256 lanes to a row r is i)
+    uint32_t lo = 0, hi = E - 1;
+    while (lo < hi) {
+      const uint32_t mid = (lo + hi) / 2;
+      if (upto[mid] > r) hi = mid;
+      else lo = mid + 1;
+    }
+    const uint32_t e = __builtin_amdgcn_readfirstlane(lo);
+    quantize_one<T, SWIGLU, LANES>(a, e, r - (e ? upto[e - 1] : 0u), threadIdx.x % LANES);
+  }
+}
+
+template <class T, bool SWIGLU, int LANES> int launch_quantize(const QuantizeDev &a, hipStream_t s) {
+  constexpr uint32_t kAtOnce = 256 / LANES;
+  if (a.rows.layout == PPLX_A2A_ROWS_PADDED) {
+    const uint64_t groups = ((uint64_t)a.rows.rows * a.rows.experts + kAtOnce - 1) / kAtOnce;
+    const uint32_t grid = groups < 2048 ? (uint32_t)groups : 2048;  // eight workgroups to a compute unit
+    PPLX_LAUNCH(launch_kernel(quantize_padded<T, SWIGLU, LANES>, dim3(grid), dim3(256), 4 * a.rows.experts, s, a));
+  } else {
+    PPLX_LAUNCH(launch_kernel(quantize_flat<T, SWIGLU, LANES>, dim3((a.rows.rows + kAtOnce - 1) / kAtOnce), dim3(256), 0, s, a));
+  }
+  return PPLX_A2A_OK;
+}
+
+}  // namespace
+}  // namespace pplx_amd
+
+using namespace pplx_amd;
+
+extern "C" int pplx_a2a_quantize_rows(int device, const pplx_a2a_quantize_args_t *args, void *stream) {
+  PPLX_REQUIRE(args, "args is NULL");
+  const pplx_a2a_quantize_args_t &p = *args;
+  QuantizeDev a{};
+  const int st = check_rows(p.rows, &a.rows);
+  if (st) return st;
+  PPLX_REQUIRE(is_dtype(p.dtype), "unsupported dtype of x");
+  PPLX_REQUIRE(p.width > 0 && p.width < (1ull << 27) && p.width % 16 == 0, "width must be a multiple of 16 below 2^27");
+  if (p.rows.rows == 0) return PPLX_A2A_OK;
+  PPLX_REQUIRE(p.out && p.out_scale && p.x, "out / out_scale / x is NULL");
+  PPLX_REQUIRE(is_aligned(p.out, 16) && p.out_stride_row % 16 == 0 && p.out_stride_expert % 16 == 0,
+               "out must be 16-byte aligned with 16-byte strides");
+  PPLX_REQUIRE(is_aligned(p.x, 16) && p.x_stride_row % 16 == 0 && p.x_stride_expert % 16 == 0,
+               "x must be 16-byte aligned with 16-byte strides");
+  PPLX_REQUIRE(is_aligned(p.out_scale, 4), "out_scale must be aligned to its elements");
+  a.out = static_cast<uint8_t *>(p.out);
+  a.out_stride_row = p.out_stride_row;
+  a.out_stride_expert = p.out_stride_expert;
+  a.scale = p.out_scale;
+  a.scale_stride_row = p.out_scale_stride_row;
+  a.scale_stride_expert = p.out_scale_stride_expert;
+  a.x = static_cast<const uint8_t *>(p.x);
+  a.x_stride_row = p.x_stride_row;
+  a.x_stride_expert = p.x_stride_expert;
+  a.width = (uint32_t)p.width;
+  return guarded(device, [&] {
+    return with_type(p.dtype, [&](auto tag) {
+      typedef typename decltype(tag)::type T;
+      hipStream_t s = (hipStream_t)stream;
+      if (a.width <= 1024) return p.swiglu ? launch_quantize<T, true, 64>(a, s) : launch_quantize<T, false, 64>(a, s);
+      return p.swiglu ? launch_quantize<T, true, 256>(a, s) : launch_quantize<T, false, 256>(a, s);
+    });
+  });
+}

@@ -1,0 +1,271 @@
+// Sorted rows back to tokens, weighted, and the gradients of that.  The gradient of the sort itself is the gather without
+// weights.  Both go by token: a token's picks are gathered (or written) by the lanes that hold its row, so nothing is
+// added by atomics and every sum has one order.
+#include "a2a_experts.h"
+
+namespace pplx_amd {
+namespace {
+
+struct UnsortDev {
+  void *out;
+  int64_t out_stride;  // bytes
+  const uint8_t *y;
+  int64_t y_stride;    // bytes
+  uint32_t y_rows;
+  const int32_t *slots;
+  const float *weights;
+  uint32_t m, K, width;
+};
+
+// Adds N rows of the token to acc, in the order of `left`'s bits, which it takes away.
+template <class Y, int N>
+__device__ __forceinline__ void gather_some(const UnsortDev &a, int32_t slot, float w, uint64_t &left, uint32_t col, f32x8 &acc) {
+  typename Eight<Y>::raw raw[N];
+  float weight[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int k = __builtin_ctzll(left);
+    left &= left - 1;
+    const uint32_t s = (uint32_t)__builtin_amdgcn_readlane(slot, k);
+    weight[i] = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(w), k));
+    raw[i] = load_eight<Y>(as_global(reinterpret_cast<const Y *>(a.y + (int64_t)s * a.y_stride)) + col);
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const f32x8 v = Eight<Y>::wide(raw[i]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] = __builtin_fmaf(weight[i], v[j], acc[j]);
+  }
+}
+
+// One wave to 512 elements of a token's row, eight to a lane, and up to eight rows in flight.
+template <class Y, class O>
+__global__ __launch_bounds__(256) void unsort_gather(UnsortDev a, uint32_t pieces, FastDiv by_pieces) {
+  const uint32_t lane = lane_id();
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + threadIdx.x / kWave);
+  const uint32_t t = fast_div(wave, by_pieces);
+  if (t >= a.m) return;
+  const uint32_t col = (wave - t * pieces) * 512 + lane * 8;
+  const uint32_t from = col < a.width ? col : a.width - 8;  // (loads stay unconditional)
+  int32_t slot = -1;
+  float w = 1.f;
+  if (lane < a.K) {
+    slot = as_global(a.slots)[(size_t)t * a.K + lane];
+    if (a.weights) w = as_global(a.weights)[(size_t)t * a.K + lane];
+  }
+  uint64_t left = __ballot((uint32_t)slot < a.y_rows);
+  f32x8 acc = {0, 0, 0, 0, 0, 0, 0, 0};
+  uint32_t n = __builtin_popcountll(left);
+  for (; n >= 8; n -= 8) gather_some<Y, 8>(a, slot, w, left, from, acc);
+  if (n & 4) gather_some<Y, 4>(a, slot, w, left, from, acc);
+  if (n & 2) gather_some<Y, 2>(a, slot, w, left, from, acc);
+  if (n & 1) gather_some<Y, 1>(a, slot, w, left, from, acc);
+  if (col < a.width) {
+    store_eight<O>(as_global(reinterpret_cast<O *>(static_cast<uint8_t *>(a.out) + (int64_t)t * a.out_stride)) + col, acc);
+  }
+}
+
+struct UnsortBackwardDev {
+  uint8_t *grad_y;
+  int64_t grad_y_stride;
+  float *grad_weights;
+  const uint8_t *grad_out;
+  int64_t grad_out_stride;
+  const uint8_t *y;
+  int64_t y_stride;
+  uint32_t y_rows;
+  const int32_t *slots;
+  const int32_t *num_rows;
+  const float *weights;
+  uint32_t m, K, width;
+};
+
+// LANES threads to a token (a wave, or the workgroup).  Eight picks at a time: their rows of y are read, their rows of
+// grad_y written, and the eight products summed over the row at the end.
+template <class T, class G, int LANES>
+__global__ __launch_bounds__(256) void unsort_backward(UnsortBackwardDev a) {
+  constexpr int kPicks = 8;
+  const uint32_t lane = lane_id(), wave = wave_id(), g = threadIdx.x % LANES;
+  const uint32_t t = LANES == 64 ? blockIdx.x * 4 + wave : blockIdx.x;
+  if (t >= a.m) return;  // (with 256 lanes to a token the grid has one workgroup a token)
+  int32_t slot = -1;
+  float w = 1.f;
+  if (lane < a.K) {
+    slot = as_global(a.slots)[(size_t)t * a.K + lane];
+    if (a.weights) w = as_global(a.weights)[(size_t)t * a.K + lane];
+  }
+  const uint64_t live = __ballot((uint32_t)slot < a.y_rows);
+  const PPLX_GLOBAL G *go_row = as_global(reinterpret_cast<const G *>(a.grad_out + (int64_t)t * a.grad_out_stride));
+  const bool want_y = a.grad_y != nullptr, want_w = a.grad_weights != nullptr;
+  __shared__ float partial[LANES / 64][kPicks];
+  for (uint32_t first = 0; first < a.K; first += kPicks) {
+    float acc[kPicks] = {};
+    for (uint32_t col = g * 8; col < a.width; col += LANES * 8) {
+      typename Eight<T>::raw raw[kPicks];
+      if (want_w) {
+#pragma unroll
+        for (int i = 0; i < kPicks; ++i) {
+          const uint32_t k = first + i;
+          if (k < a.K && (live >> k) & 1) {
+            const uint32_t s = (uint32_t)__builtin_amdgcn_readlane(slot, k);
+            raw[i] = load_eight<T>(as_global(reinterpret_cast<const T *>(a.y + (int64_t)s * a.y_stride)) + col);
+          }
+        }
+      }
+      const f32x8 go = Eight<G>::wide(load_eight<G>(go_row + col));
+#pragma unroll
+      for (int i = 0; i < kPicks; ++i) {
+        const uint32_t k = first + i;
+        if (!(k < a.K && (live >> k) & 1)) continue;
+        if (want_w) {
+          const f32x8 v = Eight<T>::wide(raw[i]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) acc[i] = __builtin_fmaf(go[j], v[j], acc[i]);
+        }
+        if (want_y) {
+          const float weight = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(w), k));
+          const uint32_t s = (uint32_t)__builtin_amdgcn_readlane(slot, k);
+          store_eight<T>(as_global(reinterpret_cast<T *>(a.grad_y + (int64_t)s * a.grad_y_stride)) + col, go * weight);
+        }
+      }
+    }
+    if (want_w) {
+#pragma unroll
+      for (int i = 0; i < kPicks; ++i) acc[i] = wave_sum(acc[i]);
+      if constexpr (LANES > 64) {
+        __syncthreads();  // (the picks before have been read)
+#pragma unroll
+        for (int i = 0; i < kPicks; ++i) {
+          if (lane == 0) partial[wave][i] = acc[i];
+        }
+        __syncthreads();
+        if (threadIdx.x < kPicks && first + threadIdx.x < a.K) {
+          float sum = 0.f;
+#pragma unroll
+          for (int v = 0; v < LANES / 64; ++v) sum += partial[v][threadIdx.x];
+          const uint32_t k = first + threadIdx.x;
+          as_global(a.grad_weights)[(size_t)t * a.K + k] = (live >> k) & 1 ? sum : 0.f;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPicks; ++i) {
+          if (lane == (uint32_t)i && first + i < a.K) {
+            as_global(a.grad_weights)[(size_t)t * a.K + first + i] = (live >> (first + i)) & 1 ? acc[i] : 0.f;
+          }
+        }
+      }
+    }
+  }
+  if (!want_y) return;
+  // The rows that no slot names lie behind the others; they are shared out over the tokens.
+  const int32_t there = *as_global(a.num_rows);
+  const uint32_t total = there > 0 ? (uint32_t)there : 0u;
+  const uint64_t stride = (uint64_t)a.m * a.K;
+  for (uint32_t k = 0; k < a.K; ++k) {
+    for (uint64_t r = (uint64_t)t * a.K + k; r < a.y_rows; r += stride) {
+      if (r < total) continue;
+      PPLX_GLOBAL T *row = as_global(reinterpret_cast<T *>(a.grad_y + (int64_t)r * a.grad_y_stride));
+      for (uint32_t col = g * 8; col < a.width; col += LANES * 8) store_eight<T>(row + col, f32x8{0, 0, 0, 0, 0, 0, 0, 0});
+    }
+  }
+}
+
+}  // namespace
+}  // namespace pplx_amd
+
+using namespace pplx_amd;
+
+namespace {
+int check_unsort_size(uint64_t m, uint64_t K, uint64_t hidden_dim, int64_t y_rows) {
+  PPLX_REQUIRE(K >= 1 && K <= 64, "experts_per_token must be in [1, 64]");
+  PPLX_REQUIRE(hidden_dim > 0 && hidden_dim < (1ull << 28) && hidden_dim % 8 == 0,
+               "hidden_dim must be a multiple of 8 below 2^28");
+  PPLX_REQUIRE(y_rows >= 0 && y_rows < (1ll << 31), "y must have fewer than 2^31 rows");
+  if (m * K >= (1ull << 31) || m * ((hidden_dim + 511) / 512) >= (1ull << 32))
+    return refuse(PPLX_A2A_UNSUPPORTED, "too many picks or elements");
+  return PPLX_A2A_OK;
+}
+}  // namespace
+
+extern "C" int pplx_a2a_unsort_tokens(int device, const pplx_a2a_unsort_args_t *args, void *stream) {
+  PPLX_REQUIRE(args, "args is NULL");
+  const pplx_a2a_unsort_args_t &p = *args;
+  const int st = check_unsort_size(p.m, p.experts_per_token, p.hidden_dim, p.y_rows);
+  if (st) return st;
+  PPLX_REQUIRE(is_dtype(p.y_dtype) && is_dtype(p.out_dtype), "unsupported dtype of y or out");
+  if (p.m == 0) return PPLX_A2A_OK;
+  PPLX_REQUIRE(p.out && p.slots && (p.y || p.y_rows == 0), "out / slots / y is NULL");
+  PPLX_REQUIRE(is_aligned(p.out, 16) && p.out_stride_row % 16 == 0, "out must be 16-byte aligned with a 16-byte row stride");
+  PPLX_REQUIRE(is_aligned(p.y, 16) && p.y_stride_row % 16 == 0, "y must be 16-byte aligned with a 16-byte row stride");
+  PPLX_REQUIRE(is_aligned(p.slots, 4) && is_aligned(p.weights, 4), "slots and weights must be aligned to their elements");
+  UnsortDev a{};
+  a.out = p.out;
+  a.out_stride = p.out_stride_row;
+  a.y = static_cast<const uint8_t *>(p.y);
+  a.y_stride = p.y_stride_row;
+  a.y_rows = (uint32_t)p.y_rows;
+  a.slots = p.slots;
+  a.weights = p.weights;
+  a.m = p.m;
+  a.K = p.experts_per_token;
+  a.width = (uint32_t)p.hidden_dim;
+  const uint32_t pieces = (a.width + 511) / 512;
+  const dim3 grid((uint32_t)(((uint64_t)a.m * pieces + 3) / 4));
+  return guarded(device, [&] {
+    return with_type(p.y_dtype, [&](auto y) {
+      return with_type(p.out_dtype, [&](auto out) {
+        PPLX_LAUNCH(launch_kernel(unsort_gather<typename decltype(y)::type, typename decltype(out)::type>, grid, dim3(256), 0,
+                                  (hipStream_t)stream, a, pieces, make_fast_div(pieces)));
+        return (int)PPLX_A2A_OK;
+      });
+    });
+  });
+}
+
+extern "C" int pplx_a2a_unsort_tokens_backward(int device, const pplx_a2a_unsort_backward_args_t *args, void *stream) {
+  PPLX_REQUIRE(args, "args is NULL");
+  const pplx_a2a_unsort_backward_args_t &p = *args;
+  const int st = check_unsort_size(p.m, p.experts_per_token, p.hidden_dim, p.y_rows);
+  if (st) return st;
+  PPLX_REQUIRE(is_dtype(p.dtype) && is_dtype(p.grad_dtype), "unsupported dtype of y or grad_out");
+  if (!p.grad_y && !p.grad_weights) return PPLX_A2A_OK;
+  PPLX_REQUIRE(p.m > 0 || !p.grad_y || p.y_rows == 0, "without tokens there is no gradient of rows");
+  if (p.m == 0) return PPLX_A2A_OK;
+  PPLX_REQUIRE(p.grad_out && p.slots, "grad_out / slots is NULL");
+  PPLX_REQUIRE(!p.grad_y || (p.num_rows && is_aligned(p.num_rows, 4)), "num_rows is NULL or not aligned");
+  PPLX_REQUIRE(!p.grad_weights || p.y || p.y_rows == 0, "y is NULL, which grad_weights needs");
+  PPLX_REQUIRE(is_aligned(p.grad_out, 16) && p.grad_out_stride_row % 16 == 0 && is_aligned(p.grad_y, 16) &&
+                   p.grad_y_stride_row % 16 == 0 && is_aligned(p.y, 16) && p.y_stride_row % 16 == 0,
+               "grad_out, grad_y and y must be 16-byte aligned with 16-byte row strides");
+  PPLX_REQUIRE(is_aligned(p.slots, 4) && is_aligned(p.weights, 4) && is_aligned(p.grad_weights, 4),
+               "slots, weights and grad_weights must be aligned to their elements");
+  UnsortBackwardDev a{};
+  a.grad_y = static_cast<uint8_t *>(p.grad_y);
+  a.grad_y_stride = p.grad_y_stride_row;
+  a.grad_weights = p.grad_weights;
+  a.grad_out = static_cast<const uint8_t *>(p.grad_out);
+  a.grad_out_stride = p.grad_out_stride_row;
+  a.y = static_cast<const uint8_t *>(p.y);
+  a.y_stride = p.y_stride_row;
+  a.y_rows = (uint32_t)p.y_rows;
+  a.slots = p.slots;
+  a.num_rows = p.num_rows;
+  a.weights = p.weights;
+  a.m = p.m;
+  a.K = p.experts_per_token;
+  a.width = (uint32_t)p.hidden_dim;
+  return guarded(device, [&] {
+    return with_type(p.dtype, [&](auto y) {
+      return with_type(p.grad_dtype, [&](auto grad) {
+        typedef typename decltype(y)::type Y;
+        typedef typename decltype(grad)::type G;
+        if (a.width <= 1024) {
+          PPLX_LAUNCH(launch_kernel(unsort_backward<Y, G, 64>, dim3((a.m + 3) / 4), dim3(256), 0, (hipStream_t)stream, a));
+        } else {
+          PPLX_LAUNCH(launch_kernel(unsort_backward<Y, G, 256>, dim3(a.m), dim3(256), 0, (hipStream_t)stream, a));
+        }
+        return (int)PPLX_A2A_OK;
+      });
+    });
+  });
+}

@@ -35,26 +35,13 @@
 #include <vector>
 
 #include "pplx_a2a.h"
+#include "torch_common.h"
+
+PyMethodDef *experts_methods();  // the functions of torch_experts.cpp
 
 namespace {
 
 using fptr_t = int64_t;
-
-const char *status_name(int status) {
-  switch (status) {
-    case PPLX_A2A_INVALID_ARGUMENT: return "invalid argument";
-    case PPLX_A2A_INVALID_STATE: return "invalid state";
-    case PPLX_A2A_HIP_ERROR: return "HIP error";
-    case PPLX_A2A_UNSUPPORTED: return "unsupported";
-    default: return "error";
-  }
-}
-
-#define A2A_CHECK(status)                                                                     \
-  do {                                                                                        \
-    const int st_ = (status);                                                                 \
-    TORCH_CHECK(st_ == PPLX_A2A_OK, "pplx_kernels: ", status_name(st_), ": ", pplx_a2a_last_error()); \
-  } while (0)
 
 // ---------------------------------------------------------------------------
 // Worlds and rank handles
@@ -348,33 +335,11 @@ fptr_t create_internode(int64_t maxNumTokens, int64_t numExperts, int64_t expert
 // ---------------------------------------------------------------------------
 // Tensor checks (csrc/bindings/all_to_all_ops.cpp:19-24,135-161,249-259)
 // ---------------------------------------------------------------------------
-void check_tensor(const at::Tensor &x, int64_t ndim, const char *name) {
-  TORCH_CHECK(x.is_cuda(), "Tensor ", name, " must be on GPU");
-  TORCH_CHECK(x.is_contiguous(), "Tensor ", name, " must be contiguous");
-  TORCH_CHECK(x.dim() == ndim, "Tensor ", name, " must be ", ndim, " dimensional");
-}
-
-void check_bound_m(const at::Tensor *bound_m) {
-  if (!bound_m) return;
-  check_tensor(*bound_m, 1, "boundM.value()");
-  TORCH_CHECK(bound_m->scalar_type() == at::kUInt32, "boundM must be of type UInt32");
-  TORCH_CHECK(bound_m->numel() == 1, "boundM must be a scalar tensor");
-}
-
 // getSplitMode, csrc/bindings/all_to_all_ops.cpp:110-120
 int split_mode_of(bool do_send, bool do_recv) {
   TORCH_CHECK(do_send || do_recv, "Invalid split mode");
   if (do_send && do_recv) return PPLX_A2A_SPLIT_NONE;
   return do_send ? PPLX_A2A_SPLIT_SEND : PPLX_A2A_SPLIT_RECV;
-}
-
-int dtype_code(at::ScalarType t) {
-  switch (t) {
-    case at::kFloat: return PPLX_A2A_F32;
-    case at::kBFloat16: return PPLX_A2A_BF16;
-    case at::kHalf: return PPLX_A2A_F16;
-    default: return -1;
-  }
 }
 
 void check_dispatch(const at::Tensor &outExpertNumTokens, const at::Tensor &outExpertX,
@@ -537,10 +502,6 @@ uint32_t abandon_assembly(World *world, int op, Released &released) {
               " step that was being assembled has been abandoned: ", (dropped),                   \
               " recorded call(s) dropped, every rank calls again)")
 
-void *current_stream_of(const at::Tensor &t) {
-  return (void *)c10::hip::getCurrentHIPStream(t.device().index()).stream();
-}
-
 // csrc/bindings/all_to_all_ops.cpp:122-196.  Optional tensors arrive as pointers (NULL = None).
 void dispatch_core(fptr_t ptr, const at::Tensor &outExpertNumTokens, const at::Tensor &outExpertX,
                    const at::Tensor *outExpertXScale, const at::Tensor &dpX, const at::Tensor *dpXScale,
@@ -615,8 +576,6 @@ void combine_core(fptr_t ptr, const at::Tensor &outTokens, const at::Tensor &ind
   }
 }
 
-const at::Tensor *opt(const std::optional<at::Tensor> &t) { return t.has_value() ? &*t : nullptr; }
-
 // The registered ops (the reference's signatures).
 void dispatch_op(fptr_t ptr, at::Tensor &outExpertNumTokens, at::Tensor &outExpertX,
                  const std::optional<at::Tensor> &outExpertXScale, const at::Tensor &dpX,
@@ -670,28 +629,6 @@ TORCH_LIBRARY(pplx_kernels, m) {
 // ---------------------------------------------------------------------------
 namespace {
 
-const at::Tensor &tensor_arg(PyObject *obj, const char *name) {
-  TORCH_CHECK_TYPE(THPVariable_Check(obj), name, " must be a Tensor, not ", Py_TYPE(obj)->tp_name);
-  return THPVariable_Unpack(obj);
-}
-
-const at::Tensor *optional_tensor_arg(PyObject *obj, const char *name) {
-  return obj == Py_None ? nullptr : &tensor_arg(obj, name);
-}
-
-int64_t int_arg(PyObject *obj, const char *name) {
-  const long long v = PyLong_AsLongLong(obj);
-  if (v == -1 && PyErr_Occurred()) {
-    PyErr_Clear();
-    TORCH_CHECK_TYPE(false, name, " must be an int, not ", Py_TYPE(obj)->tp_name);
-  }
-  return v;
-}
-
-void arity(const char *fn, Py_ssize_t got, Py_ssize_t want) {
-  TORCH_CHECK_TYPE(got == want, fn, "() takes ", want, " positional arguments but ", got, " were given");
-}
-
 // dispatch(fptr, out_expert_num_tokens, out_expert_x, out_expert_x_scale, dp_x, dp_x_scale, indices,
 //          bound_m, do_send, do_recv)
 PyObject *py_dispatch(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
@@ -742,18 +679,6 @@ PyObject *entry(PyObject *seq, Py_ssize_t r, Owned &keep) {
   if (!item) throw python_error();  // (the pending exception: an IndexError where a sequence is too short)
   keep.refs.push_back(item);
   return item;
-}
-
-// The library call itself runs without the interpreter lock.
-struct WithoutGil {
-  PyThreadState *state = PyEval_SaveThread();
-  ~WithoutGil() { PyEval_RestoreThread(state); }
-};
-
-template <class Fn>
-int without_gil(Fn &&fn) {
-  WithoutGil released;
-  return fn();
 }
 
 std::shared_ptr<World> world_arg(PyObject *obj) { return live_world((uint64_t)int_arg(obj, "world")); }
@@ -1050,4 +975,8 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_C", "torch operator layer of ppl
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__C(void) { return PyModule_Create(&kModule); }
+PyMODINIT_FUNC PyInit__C(void) {
+  PyObject *module = PyModule_Create(&kModule);
+  if (module && PyModule_AddFunctions(module, experts_methods()) != 0) Py_CLEAR(module);
+  return module;
+}

@@ -70,6 +70,12 @@ EXPORTED_SYMBOLS = (
     "pplx_a2a_graph_end_capture",
     "pplx_a2a_graph_launch",
     "pplx_a2a_graph_destroy",
+    "pplx_a2a_sort_workspace",
+    "pplx_a2a_sort_tokens",
+    "pplx_a2a_unsort_tokens",
+    "pplx_a2a_unsort_tokens_backward",
+    "pplx_a2a_quantize_rows",
+    "pplx_a2a_int8_matmul",
     "pplx_a2a_last_error",
     "pplx_a2a_version",
     "pplx_a2a_build_id",
