@@ -5,9 +5,9 @@
 // on the matrix cores (v_mfma_i32_*_i8), whose int32 sums are exact for every k that the entry point admits.  The weights
 // are the first operand, so that the accumulators of a lane are consecutive columns of one row of the result.
 //
-// Tiles of BM rows by BN columns go through LDS, 128 bytes of k at a time, which loads write there directly.  A row of a
-// tile is a line of eight 16-byte chunks; chunk c of row r lies at place c ^ (r & 7) of its line, so that the lanes of a
-// fragment, which read one chunk each of consecutive rows, read all banks.  How many rows each expert has is known on the
+// Tiles of BM rows by BN columns go through LDS, BK bytes of k at a time, which loads write there directly.  A row of a
+// tile is a line of 16-byte chunks, whose places are exchanged from row to row so that the lanes of a fragment, which read one
+// chunk each of consecutive rows, read all banks.  How many rows each expert has is known on the
 // device only: every workgroup sums the experts' blocks of rows and takes tiles from the list that follows from them.
 #include "a2a_experts.h"
 
@@ -29,38 +29,32 @@ struct MatmulDev {
   const float *weight_scale;
   uint32_t n, k;
   uint32_t n_blocks;
-  uint32_t vector_stores;  // out rows are aligned to four elements
+  uint32_t vector_stores;  // the rows of out are 16-byte aligned
 };
 
-constexpr uint32_t kStepBytes = 128;
-
-// Waits until at most `left` of the wave's loads and stores are under way.
-template <int LEFT> __device__ __forceinline__ void wait_loads() {
-  __builtin_amdgcn_s_waitcnt((LEFT & 15) | ((LEFT >> 4) << 14) | (7 << 4) | (15 << 8));
+// Waits until at most LEFT of the wave's loads are under way, and for its LDS reads where asked to.
+template <int LEFT, bool LDS = false> __device__ __forceinline__ void wait_loads() {
+  __builtin_amdgcn_s_waitcnt((LEFT & 15) | ((LEFT >> 4) << 14) | (7 << 4) | ((LDS ? 0 : 15) << 8));
   asm volatile("" ::: "memory");
 }
 
-// Sixteen bytes a lane from global memory to LDS, lane i's at `lds` + 16 i.
-__device__ __forceinline__ void load_to_lds(const PPLX_GLOBAL int8_t *p, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory", "m0");
+// Sixteen bytes a lane from `base` + `offset` to LDS, lane i's at `lds` + 16 i; `lanes` is ~0, or 0 for a load that only
+// counts.  (asm: behind the builtin the compiler waits for the loads of the steps to come before it reads the step at
+// hand out of LDS.  Nothing is returned to registers, and the kernel waits by itself.  All lanes are active where it
+// stands.  m0 wants one wait state before the load, which the writes of exec are.)
+__device__ __forceinline__ void load_to_lds(const int8_t *base, uint32_t offset, uint32_t lds, uint32_t lanes) {
+  asm volatile(
+      "s_mov_b32 m0, %2\n\t"
+      "s_mov_b32 exec_lo, %3\n\t"
+      "s_mov_b32 exec_hi, %3\n\t"
+      "global_load_lds_dwordx4 %0, %1\n\t"
+      "s_mov_b64 exec, -1"
+      ::"v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds)), "s"(__builtin_amdgcn_readfirstlane(lanes))
+      : "memory");
 }
 
 __device__ __forceinline__ uint32_t lds_address(const void *p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p;
-}
-
-// Four consecutive columns of a row of the result, of which `n` exist.
-template <class O>
-__device__ __forceinline__ void store_four(PPLX_GLOBAL O *p, f32x4 v, uint32_t n, bool whole) {
-  if (whole && n >= 4) {
-    typedef O four __attribute__((ext_vector_type(4)));
-    *reinterpret_cast<PPLX_GLOBAL four *>(p) = __builtin_convertvector(v, four);
-  } else {
-#pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-      if (i < n) p[i] = (O)v[i];
-    }
-  }
 }
 
 // Inclusive sums of the experts' blocks of BM rows in `upto`, by all THREADS threads of the workgroup.
@@ -110,32 +104,25 @@ template <int BM, int BN> __device__ __forceinline__ Tile tile_of(const MatmulDe
   return t;
 }
 
-// The fragments of one matrix instruction: 32 rows and 32 bytes of k, or 16 rows and 64 bytes of k, 16 bytes to a lane.
-template <int F> struct Mfma;
-template <> struct Mfma<32> {
-  typedef i32x16 acc;
-  static constexpr int kChunks = 2;
-  static __device__ __forceinline__ acc run(i32x4 a, i32x4 b, acc c) {
-    return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);
-  }
-};
-template <> struct Mfma<16> {
-  typedef i32x4 acc;
-  static constexpr int kChunks = 4;
-  static __device__ __forceinline__ acc run(i32x4 a, i32x4 b, acc c) {
-    return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
-  }
-};
-
-// WM by WN waves, each BM / WM rows by BN / WN columns in fragments of F; STAGES steps of k in LDS.
-template <int BM, int BN, int WM, int WN, int F, int STAGES, class O>
+// WM by WN waves, each BM / WM rows by BN / WN columns in fragments of 32 by 32; STAGES steps of BK bytes of k in LDS.  A wave
+// reads the fragments of the next 32 bytes of k before it multiplies those at hand, over the border between two steps too:
+// there it waits for the next step's loads, and behind the barrier this step's place takes those of a step to come.
+// TAIL: k is no multiple of BK.
+template <int BM, int BN, int WM, int WN, int BK, int STAGES, bool TAIL, class O>
 __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev a) {
   constexpr int kWaves = WM * WN, kThreads = kWaves * 64;
-  constexpr int MF = BM / WM / F, NF = BN / WN / F;  // fragments of a wave
-  constexpr int kLoads = (BM + BN) / 8 / kWaves;     // of a wave in a step, eight rows each
-  static_assert((BM + BN) % (8 * kWaves) == 0 && BM % (WM * F) == 0 && BN % (WN * F) == 0, "tile");
-  constexpr int kStage = (BM + BN) * (int)kStepBytes;
-  extern __shared__ __align__(128) uint8_t lds[];  // [STAGES][BM rows of x, BN of the weight][128], then the sums
+  constexpr int kRows = BM / WM, kColumns = BN / WN, MF = kRows / 32, NF = kColumns / 32;
+  constexpr int kChunks = BK / 16, kRowsPerLoad = 64 / kChunks;
+  constexpr int kLoads = (BM + BN) / kRowsPerLoad / kWaves;  // of a wave in a step
+  constexpr int kSteps = BK / 32;                            // matrix instructions along k in a step
+  static_assert(BK == 64 || BK == 128, "a line is four or eight chunks");
+  static_assert((BM + BN) % (kRowsPerLoad * kWaves) == 0 && BM % kRowsPerLoad == 0, "whole loads");
+  static_assert(kRows % 32 == 0 && kColumns % 32 == 0, "whole fragments");
+  static_assert((STAGES - 1) * kLoads < 63, "loads that can be counted");
+  constexpr int kStage = (BM + BN) * BK;
+  constexpr int kOutStride = kColumns * 4 + 16;  // bytes of a row of sums in LDS, one chunk apart in banks
+  static_assert(kWaves * 32 * kOutStride <= STAGES * kStage, "32 rows of each wave's sums fit the stages");
+  extern __shared__ __align__(128) uint8_t lds[];  // [STAGES][BM rows of x, BN of the weight][BK], then the sums
   uint32_t *upto = reinterpret_cast<uint32_t *>(lds + STAGES * kStage);
   __shared__ uint32_t of_wave[kWaves];
   sum_blocks<kThreads, BM>(a.rows, upto, of_wave);
@@ -143,116 +130,168 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev a) {
   const uint32_t lane = lane_id(), wave = wave_id();
   const uint32_t wm = wave % WM, wn = wave / WM;
   const uint32_t lds0 = lds_address(lds);
-  const uint32_t steps = (a.k + kStepBytes - 1) / kStepBytes;
-  const uint32_t chunk = ((lane & 7) ^ (lane >> 3)) * 16;  // of its line that this lane fetches
-  // Places of the fragments' chunks in their lines (rows of a fragment differ by 8 or more in what the lanes share).
-  const uint32_t frag_row = (lane % F) * kStepBytes, frag_chunk = lane / F;
+  const uint32_t steps = (a.k + BK - 1) / BK;
+  // Chunk c of row r lies at c ^ swizzle(r): sixteen consecutive rows hold a chunk at sixteen places of 256 bytes, which is
+  // what LDS reads at a time.  (With exchanges for 128 bytes reads took 8.8 cycles instead of 4.9.)
+  auto swizzle = [](uint32_t row) { return kChunks == 8 ? (row >> 1) & 7 : (row >> 2) & 3; };
+  static_assert(kWaves * kRowsPerLoad % 16 == 0 && BM % 16 == 0, "a lane's rows have one exchange");
+  const uint32_t load_row = lane / kChunks;
+  const uint32_t load_chunk = (lane % kChunks) ^ swizzle(wave * kRowsPerLoad + load_row);
+  const uint32_t frag_base = (lane % 32) * BK;
+  uint32_t frag_place[kSteps];
+#pragma unroll
+  for (int kk = 0; kk < kSteps; ++kk) frag_place[kk] = ((2 * kk + lane / 32) ^ swizzle(lane % 32)) * 16;
 
   // (blockIdx goes round the eight XCDs)
   const uint32_t block = (blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;
   for (uint32_t id = block; id < tiles; id += gridDim.x) {
     const Tile t = tile_of<BM, BN>(a, upto, id);
     if (t.m0 >= t.count) continue;  // (offsets that descend make a list that is too long)
-    const int8_t *x = a.x + (int64_t)t.e * a.x_stride_expert + (int64_t)t.begin * a.x_stride_row;
-    const int8_t *weight = a.weight + (uint64_t)t.e * a.n * a.k;
-    const PPLX_GLOBAL int8_t *from[kLoads];
+    const int8_t *x = a.x + (int64_t)t.e * a.x_stride_expert + (int64_t)(t.begin + t.m0) * a.x_stride_row;
+    const int8_t *weight = a.weight + ((uint64_t)t.e * a.n + t.n0) * a.k;
+    const uint32_t rows_left = t.count - t.m0, columns_left = a.n - t.n0;
+    uint32_t offset[kLoads];
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const uint32_t row = (i * kWaves + wave) * 8 + (lane >> 3);  // of the stage
-      if ((i * kWaves + wave) * 8 < BM) {
-        const uint32_t r = t.m0 + row;
-        from[i] = as_global(x + (int64_t)(r < t.count ? r : t.count - 1) * a.x_stride_row);
+      const uint32_t first = (i * kWaves + wave) * kRowsPerLoad;  // row of the stage
+      if (first < BM) {
+        const uint32_t r = first + load_row;
+        offset[i] = (r < rows_left ? r : rows_left - 1) * (uint32_t)a.x_stride_row + load_chunk * 16;
       } else {
-        const uint32_t r = t.n0 + row - BM;
-        from[i] = as_global(weight + (uint64_t)(r < a.n ? r : a.n - 1) * a.k);
+        const uint32_t r = first - BM + load_row;
+        offset[i] = (r < columns_left ? r : columns_left - 1) * a.k + load_chunk * 16;
       }
     }
-    auto fetch = [&](uint32_t step, uint32_t stage) __attribute__((always_inline)) {
-      const uint32_t k = step * kStepBytes + chunk;
-      const uint32_t at = k < a.k ? k : 0;  // (bytes behind k are taken for zeros when they are used)
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        load_to_lds(from[i] + at, __builtin_amdgcn_readfirstlane(lds0 + stage * kStage + (i * kWaves + wave) * 1024));
+    // Load number i of a step.  Behind k a lane fetches the first chunk of its line; what it brings is taken for zeros.  Loads of
+    // steps that do not exist bring nothing, and count: the loop has one path.
+    auto fetch = [&](int i, uint32_t step, uint32_t stage) __attribute__((always_inline)) {
+      const uint32_t first = (i * kWaves + wave) * kRowsPerLoad;
+      const int8_t *base = (first < BM ? x : weight) + step * BK;
+      const bool behind = TAIL && step * BK + load_chunk * 16 >= a.k;
+      load_to_lds(base, behind ? offset[i] - load_chunk * 16 : offset[i], lds0 + stage * kStage + first * BK,
+                  step < steps ? ~0u : 0u);
+    };
+    i32x4 fx[2][MF], fw[2][NF];
+    // Fragment number i (of the rows, then of the columns) for matrix instructions kk of a step.
+    auto read = [&](int i, int to, int kk, uint32_t step, uint32_t stage) __attribute__((always_inline)) {
+      const uint8_t *lines = lds + stage * kStage + frag_base + frag_place[kk];
+      if (i < MF) {
+        fx[to][i] = *reinterpret_cast<const i32x4 *>(lines + (wm * kRows + i * 32) * BK);
+        if constexpr (TAIL) fx[to][i] &= step * BK + kk * 32 + (lane / 32) * 16 < a.k ? -1 : 0;
+      } else {
+        fw[to][i - MF] = *reinterpret_cast<const i32x4 *>(lines + (BM + wn * kColumns + (i - MF) * 32) * BK);
       }
     };
 
-    typename Mfma<F>::acc acc[NF][MF] = {};
+    i32x16 acc[NF][MF] = {};
     // The tile before has been read; its stores are done, so that what is counted below are loads.
     wait_loads<0>();
     __syncthreads();
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) {
-      if ((uint32_t)s < steps) fetch(s, s);
+    for (int s = 0; s < STAGES; ++s) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) fetch(i, s, s);
     }
+    wait_loads<(STAGES - 1) * kLoads>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < MF + NF; ++i) read(i, 0, 0, 0, 0);
+    // The matrix instructions of 32 bytes of k, between which the reads of the next 32 and the loads of a step go out: a wave issues in order, and one that hands over all its reads or loads at once waits for them to be taken.
+    constexpr int kProducts = MF * NF;
+    auto multiply = [&](int from, auto read_next, auto fetch_next) __attribute__((always_inline)) {
+#pragma unroll
+      for (int q = 0; q < kProducts; ++q) {
+        const int j = q / MF, i = q % MF;
+        acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[from][j], fx[from][i], acc[j][i], 0, 0, 0);
+#pragma unroll
+        for (int r = q * (MF + NF) / kProducts; r < (q + 1) * (MF + NF) / kProducts; ++r) read_next(r);
+#pragma unroll
+        for (int l = q * kLoads / kProducts; l < (q + 1) * kLoads / kProducts; ++l) fetch_next(l);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    auto nothing = [](int) {};
     uint32_t stage = 0;
     for (uint32_t step = 0; step < steps; ++step) {
-      if (step + STAGES - 1 <= steps) wait_loads<(STAGES - 2) * kLoads>();
-      else wait_loads<0>();
+      const uint32_t next = stage + 1 == STAGES ? 0 : stage + 1;
+#pragma unroll
+      for (int kk = 0; kk + 1 < kSteps; ++kk) {
+        multiply(kk % 2, [&](int r) { read(r, (kk + 1) % 2, kk + 1, step, stage); }, nothing);
+      }
+      // Loads under way are those of steps step + 1 .. step + STAGES - 1; this step's place is free behind the barrier.
+      wait_loads<(STAGES - 2) * kLoads, true>();
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      if (step + STAGES - 1 < steps) fetch(step + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
-      const uint8_t *rows_x = lds + stage * kStage + wm * (BM / WM) * kStepBytes + frag_row;
-      const uint8_t *rows_w = lds + stage * kStage + (BM + wn * (BN / WN)) * kStepBytes + frag_row;
-      const uint32_t left = a.k - step * kStepBytes;
-      constexpr int kChunks = Mfma<F>::kChunks;
-#pragma unroll
-      for (int kk = 0; kk < 8 / kChunks; ++kk) {
-        const uint32_t c = kk * kChunks + frag_chunk;
-        const uint32_t place = (c ^ (lane & 7)) * 16;
-        i32x4 fx[MF], fw[NF];
-#pragma unroll
-        for (int i = 0; i < MF; ++i) fx[i] = *reinterpret_cast<const i32x4 *>(rows_x + i * F * kStepBytes + place);
-#pragma unroll
-        for (int i = 0; i < NF; ++i) fw[i] = *reinterpret_cast<const i32x4 *>(rows_w + i * F * kStepBytes + place);
-        if (left < kStepBytes) {
-          const bool there = c * 16 < left;
-#pragma unroll
-          for (int i = 0; i < MF; ++i) fx[i] = there ? fx[i] : i32x4{0, 0, 0, 0};
-        }
-#pragma unroll
-        for (int j = 0; j < NF; ++j) {
-#pragma unroll
-          for (int i = 0; i < MF; ++i) acc[j][i] = Mfma<F>::run(fw[j], fx[i], acc[j][i]);
-        }
-      }
-      stage = stage + 1 == STAGES ? 0 : stage + 1;
+      multiply((kSteps - 1) % 2, [&](int r) { read(r, kSteps % 2, 0, step + 1, next); },
+               [&](int l) { fetch(l, step + STAGES, stage); });
+      stage = next;
     }
 
-    // Lane l holds row l % F of each fragment and, in its accumulators, columns 4 (l / F) .. + 3 of every 256 / F.
-    constexpr uint32_t kSpan = 256 / F;
-    const float *ws = a.weight_scale + (uint64_t)t.e * a.n;
+    static_assert(kSteps % 2 == 0, "a step begins with the first fragments");
+    // Lane l holds row l % 32 of each fragment and, in its accumulators, columns 4 (l / 32) .. + 3 of every eight.  The sums of 32
+    // rows of the wave at a time go through its part of LDS, so that they are scaled where a lane has the same
+    // columns of every row, and leave as whole lines.
+    wait_loads<0, true>();
+    __syncthreads();
+    uint8_t *own = lds + wave * 32 * kOutStride;
+    constexpr uint32_t kVec = 16 / sizeof(O), kVecs = kColumns / kVec, kRowsAtOnce = 64 / kVecs;
+    const uint32_t column = (lane % kVecs) * kVec, n = t.n0 + wn * kColumns + column;
+    float ws[kVec];
+#pragma unroll
+    for (uint32_t u = 0; u < kVec; ++u) {
+      ws[u] = as_global(a.weight_scale)[(uint64_t)t.e * a.n + (n + u < a.n ? n + u : a.n - 1)];
+    }
 #pragma unroll
     for (int i = 0; i < MF; ++i) {
-      const uint32_t r = t.m0 + wm * (BM / WM) + i * F + lane % F;
-      if (r >= t.count) continue;
-      const float xs = as_global(a.x_scale)[(int64_t)t.e * a.x_scale_stride_expert + (int64_t)(t.begin + r) * a.x_scale_stride_row];
-      PPLX_GLOBAL O *out = as_global(reinterpret_cast<O *>(a.out)) + (int64_t)t.e * a.out_stride_expert +
-                           (int64_t)(t.begin + r) * a.out_stride_row;
+      const uint32_t r0 = t.m0 + wm * kRows + i * 32;
+      if (r0 >= t.count) break;  // (waves are on their own here)
+      const uint32_t r = r0 + lane % 32;
+      const float xs = as_global(a.x_scale)[(int64_t)t.e * a.x_scale_stride_expert +
+                                            (int64_t)(t.begin + (r < t.count ? r : t.count - 1)) * a.x_scale_stride_row];
 #pragma unroll
       for (int j = 0; j < NF; ++j) {
 #pragma unroll
-        for (int q = 0; q < F * F / 256; ++q) {
-          const uint32_t n = t.n0 + wn * (BN / WN) + j * F + q * kSpan + 4 * (lane / F);
-          if (n >= a.n) continue;
-          const uint32_t exist = a.n - n;
-          f32x4 v;
-#pragma unroll
-          for (uint32_t u = 0; u < 4; ++u) {
-            v[u] = (float)acc[j][i][4 * q + u] * (xs * as_global(ws)[n + (u < exist ? u : 0)]);
-          }
-          store_four<O>(out + n, v, exist, a.vector_stores);
+        for (int q = 0; q < 4; ++q) {
+          *reinterpret_cast<i32x4 *>(own + (lane % 32) * kOutStride + (j * 32 + q * 8 + 4 * (lane / 32)) * 4) =
+              i32x4{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
         }
       }
+      wait_loads<63, true>();
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (uint32_t first = 0; first < 32; first += kRowsAtOnce) {
+        const uint32_t row = first + lane / kVecs;
+        const float row_scale = __shfl(xs, (int)row);
+        const i32x4 *from = reinterpret_cast<const i32x4 *>(own + row * kOutStride + column * 4);
+        typedef O vec __attribute__((ext_vector_type(kVec)));
+        vec v;
+#pragma unroll
+        for (uint32_t u = 0; u < kVec; ++u) v[u] = (O)((float)from[u / 4][u % 4] * (row_scale * ws[u]));
+        if (r0 + row >= t.count || n >= a.n) continue;
+        PPLX_GLOBAL O *out = as_global(reinterpret_cast<O *>(a.out)) + (int64_t)t.e * a.out_stride_expert +
+                             (int64_t)(t.begin + r0 + row) * a.out_stride_row + n;
+        if (a.vector_stores && a.n - n >= kVec) {
+          *reinterpret_cast<PPLX_GLOBAL vec *>(out) = v;
+        } else {
+#pragma unroll
+          for (uint32_t u = 0; u < kVec; ++u) {
+            if (u < a.n - n) out[u] = v[u];
+          }
+        }
+      }
+      wait_loads<63, true>();
+      __builtin_amdgcn_wave_barrier();
     }
   }
 }
 
 constexpr uint32_t kComputeUnits = 256;
 
-template <int BM, int BN, int WM, int WN, int F, int STAGES, class O>
+template <int BM, int BN, int WM, int WN, int BK, int STAGES, class O>
 int launch_tiles(const MatmulDev &from, uint64_t most_blocks, hipStream_t s) {
   MatmulDev a = from;
-  constexpr uint32_t kTileLds = STAGES * (BM + BN) * kStepBytes;
+  constexpr uint32_t kTileLds = STAGES * (BM + BN) * BK;
   const uint32_t lds = kTileLds + 4 * a.rows.experts;
   constexpr uint32_t kPerUnit = kTileLds <= 64 * 1024 ? 2 : 1;
   a.n_blocks = (a.n + BN - 1) / BN;
@@ -260,7 +299,7 @@ int launch_tiles(const MatmulDev &from, uint64_t most_blocks, hipStream_t s) {
   if (tiles >= (1ull << 31)) return refuse(PPLX_A2A_UNSUPPORTED, "too many tiles");
   uint64_t grid = kPerUnit * kComputeUnits;
   grid = tiles < grid ? (tiles + 7) / 8 * 8 : grid;  // (whole rounds of the XCDs)
-  auto kernel = matmul_tiles<BM, BN, WM, WN, F, STAGES, O>;
+  auto kernel = a.k % BK ? matmul_tiles<BM, BN, WM, WN, BK, STAGES, true, O> : matmul_tiles<BM, BN, WM, WN, BK, STAGES, false, O>;
   if (lds > 64 * 1024) {
     const hipError_t err =
         hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
@@ -278,9 +317,9 @@ template <class O> int launch_matmul(const MatmulDev &a, hipStream_t s) {
     return (all + bm - 1) / bm + (E < all ? E : all) - 1;
   };
   const uint64_t even = all / E;
-  if (even <= 24) return launch_tiles<32, 128, 1, 4, 32, 3, O>(a, most_blocks(32), s);
-  if (even <= 128) return launch_tiles<64, 128, 1, 4, 32, 3, O>(a, most_blocks(64), s);
-  return launch_tiles<256, 256, 2, 4, 32, 2, O>(a, most_blocks(256), s);
+  if (even <= 24) return launch_tiles<32, 128, 1, 4, 128, 3, O>(a, most_blocks(32), s);
+  if (even <= 128) return launch_tiles<64, 128, 1, 4, 128, 3, O>(a, most_blocks(64), s);
+  return launch_tiles<256, 256, 2, 2, 64, 4, O>(a, most_blocks(256), s);
 }
 
 }  // namespace
@@ -301,6 +340,8 @@ extern "C" int pplx_a2a_int8_matmul(int device, const pplx_a2a_int8_matmul_args_
   PPLX_REQUIRE(p.out && p.x && p.x_scale && p.weight && p.weight_scale, "out / x / x_scale / weight / weight_scale is NULL");
   PPLX_REQUIRE(is_aligned(p.x, 16) && p.x_stride_row % 16 == 0 && p.x_stride_expert % 16 == 0,
                "x must be 16-byte aligned with 16-byte strides");
+  if (p.x_stride_row < 0 || p.x_stride_row >= (1 << 23))  // (a tile's rows are reached by 32-bit offsets)
+    return refuse(PPLX_A2A_UNSUPPORTED, "rows of x must be less than 8 MiB apart");
   PPLX_REQUIRE(is_aligned(p.weight, 16), "weight must be 16-byte aligned");
   PPLX_REQUIRE(is_aligned(p.out, dtype_bytes(p.out_dtype)) && is_aligned(p.x_scale, 4) && is_aligned(p.weight_scale, 4),
                "out, x_scale and weight_scale must be aligned to their elements");
@@ -317,7 +358,8 @@ extern "C" int pplx_a2a_int8_matmul(int device, const pplx_a2a_int8_matmul_args_
   a.weight_scale = p.weight_scale;
   a.n = (uint32_t)p.n;
   a.k = (uint32_t)p.k;
-  a.vector_stores = is_aligned(p.out, 4 * dtype_bytes(p.out_dtype)) && p.out_stride_row % 4 == 0 && p.out_stride_expert % 4 == 0;
+  const int64_t vec = 16 / dtype_bytes(p.out_dtype);
+  a.vector_stores = is_aligned(p.out, 16) && p.out_stride_row % vec == 0 && p.out_stride_expert % vec == 0;
   return guarded(device, [&] {
     return with_type(p.out_dtype, [&](auto tag) { return launch_matmul<typename decltype(tag)::type>(a, (hipStream_t)stream); });
   });
