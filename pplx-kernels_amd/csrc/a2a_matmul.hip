@@ -29,7 +29,7 @@ struct MatmulDev {
   const float *weight_scale;
   uint32_t n, k;
   uint32_t n_blocks;
-  uint32_t vector_stores;  // the rows of out are 16-byte aligned
+  uint32_t vector_stores;  // the rows of out are 16-byte aligned, and multiples of that
 };
 
 // Waits until at most LEFT of the wave's loads are under way, and for its LDS reads where asked to.
@@ -50,6 +50,18 @@ __device__ __forceinline__ void load_to_lds(const int8_t *base, uint32_t offset,
       "global_load_lds_dwordx4 %0, %1\n\t"
       "s_mov_b64 exec, -1"
       ::"v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds)), "s"(__builtin_amdgcn_readfirstlane(lanes))
+      : "memory");
+}
+
+// A store of the lanes in `lanes` that counts whether there are any or not.  (All lanes are active where it stands.  Its data
+// registers may be written again two wait states later.)
+__device__ __forceinline__ void store_counted(PPLX_GLOBAL void *p, u32x4 v, uint64_t lanes) {
+  asm volatile(
+      "s_mov_b64 exec, %2\n\t"
+      "global_store_dwordx4 %0, %1, off\n\t"
+      "s_mov_b64 exec, -1\n\t"
+      "s_nop 1"
+      ::"v"(p), "v"(v), "s"(lanes)
       : "memory");
 }
 
@@ -104,9 +116,24 @@ template <int BM, int BN> __device__ __forceinline__ Tile tile_of(const MatmulDe
   return t;
 }
 
+// Four columns of a row, 4 bytes or 2 each, as words.
+template <class O> __device__ __forceinline__ void pack_four(f32x4 v, uint32_t *words) {
+  if constexpr (sizeof(O) == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) words[i] = __float_as_uint(v[i]);
+  } else {
+    typedef O four __attribute__((ext_vector_type(4)));
+    typedef uint32_t two __attribute__((ext_vector_type(2)));
+    const two w = __builtin_bit_cast(two, __builtin_convertvector(v, four));
+    words[0] = w[0];
+    words[1] = w[1];
+  }
+}
+
 // WM by WN waves, each BM / WM rows by BN / WN columns in fragments of 32 by 32; STAGES steps of BK bytes of k in LDS.  A wave
 // reads the fragments of the next 32 bytes of k before it multiplies those at hand, over the border between two steps too:
-// there it waits for the next step's loads, and behind the barrier this step's place takes those of a step to come.
+// there it waits for the next step's loads, and behind the barrier this step's place takes those of a step to come.  The
+// loads of the next tile's first steps go out before this tile's results are stored.
 // TAIL: k is no multiple of BK.
 template <int BM, int BN, int WM, int WN, int BK, int STAGES, bool TAIL, class O>
 __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev a) {
@@ -119,11 +146,12 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev a) {
   static_assert((BM + BN) % (kRowsPerLoad * kWaves) == 0 && BM % kRowsPerLoad == 0, "whole loads");
   static_assert(kRows % 32 == 0 && kColumns % 32 == 0, "whole fragments");
   static_assert((STAGES - 1) * kLoads < 63, "loads that can be counted");
+  static_assert(BM + BN <= kThreads, "a scale to a thread");
+  static_assert(kSteps % 2 == 0, "a step begins with the first fragments");
   constexpr int kStage = (BM + BN) * BK;
-  constexpr int kOutStride = kColumns * 4 + 16;  // bytes of a row of sums in LDS, one chunk apart in banks
-  static_assert(kWaves * 32 * kOutStride <= STAGES * kStage, "32 rows of each wave's sums fit the stages");
-  extern __shared__ __align__(128) uint8_t lds[];  // [STAGES][BM rows of x, BN of the weight][BK], then the sums
-  uint32_t *upto = reinterpret_cast<uint32_t *>(lds + STAGES * kStage);
+  extern __shared__ __align__(128) uint8_t lds[];  // [STAGES][BM rows of x, BN of the weight][BK], scales, sums of blocks
+  float *scales = reinterpret_cast<float *>(lds + STAGES * kStage);  // of BM rows and BN columns
+  uint32_t *upto = reinterpret_cast<uint32_t *>(scales + BM + BN);
   __shared__ uint32_t of_wave[kWaves];
   sum_blocks<kThreads, BM>(a.rows, upto, of_wave);
   const uint32_t tiles = __builtin_amdgcn_readfirstlane(upto[a.rows.experts - 1] * a.n_blocks);
@@ -142,62 +170,83 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev a) {
 #pragma unroll
   for (int kk = 0; kk < kSteps; ++kk) frag_place[kk] = ((2 * kk + lane / 32) ^ swizzle(lane % 32)) * 16;
 
-  // (blockIdx goes round the eight XCDs)
-  const uint32_t block = (blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;
-  for (uint32_t id = block; id < tiles; id += gridDim.x) {
-    const Tile t = tile_of<BM, BN>(a, upto, id);
-    if (t.m0 >= t.count) continue;  // (offsets that descend make a list that is too long)
-    const int8_t *x = a.x + (int64_t)t.e * a.x_stride_expert + (int64_t)(t.begin + t.m0) * a.x_stride_row;
-    const int8_t *weight = a.weight + ((uint64_t)t.e * a.n + t.n0) * a.k;
+  // The tile whose steps are loaded: where its operands begin, and what the lane's loads add to that.
+  const int8_t *x = nullptr, *weight = nullptr;
+  uint32_t offset[kLoads];
+  float scale = 0.f;  // of row threadIdx.x of the tile, or of its column threadIdx.x - BM
+  // Load number i of a step.  Behind k a lane fetches the first chunk of its line; what it brings is taken for zeros.  Loads of
+  // steps that do not exist bring nothing, and count: the loop has one path.
+  auto fetch = [&](int i, uint32_t step, uint32_t stage) __attribute__((always_inline)) {
+    const uint32_t first = (i * kWaves + wave) * kRowsPerLoad;
+    const int8_t *base = (first < BM ? x : weight) + step * BK;
+    const bool behind = TAIL && step * BK + load_chunk * 16 >= a.k;
+    load_to_lds(base, behind ? offset[i] - load_chunk * 16 : offset[i], lds0 + stage * kStage + first * BK,
+                step < steps ? ~0u : 0u);
+  };
+  auto begin = [&](const Tile &t) __attribute__((always_inline)) {
+    x = a.x + (int64_t)t.e * a.x_stride_expert + (int64_t)(t.begin + t.m0) * a.x_stride_row;
+    weight = a.weight + ((uint64_t)t.e * a.n + t.n0) * a.k;
     const uint32_t rows_left = t.count - t.m0, columns_left = a.n - t.n0;
-    uint32_t offset[kLoads];
+    if (threadIdx.x < BM) {
+      const uint32_t r = threadIdx.x < rows_left ? threadIdx.x : rows_left - 1;
+      scale = as_global(a.x_scale)[(int64_t)t.e * a.x_scale_stride_expert + (int64_t)(t.begin + t.m0 + r) * a.x_scale_stride_row];
+    } else if (threadIdx.x < BM + BN) {
+      const uint32_t c = threadIdx.x - BM < columns_left ? threadIdx.x - BM : columns_left - 1;
+      scale = as_global(a.weight_scale)[(uint64_t)t.e * a.n + t.n0 + c];
+    }
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const uint32_t first = (i * kWaves + wave) * kRowsPerLoad;  // row of the stage
-      if (first < BM) {
-        const uint32_t r = first + load_row;
-        offset[i] = (r < rows_left ? r : rows_left - 1) * (uint32_t)a.x_stride_row + load_chunk * 16;
-      } else {
-        const uint32_t r = first - BM + load_row;
-        offset[i] = (r < columns_left ? r : columns_left - 1) * a.k + load_chunk * 16;
-      }
+      const uint32_t r = first + load_row - (first < BM ? 0 : BM);
+      offset[i] = load_chunk * 16 + (first < BM ? (r < rows_left ? r : rows_left - 1) * (uint32_t)a.x_stride_row
+                                                : (r < columns_left ? r : columns_left - 1) * a.k);
     }
-    // Load number i of a step.  Behind k a lane fetches the first chunk of its line; what it brings is taken for zeros.  Loads of
-    // steps that do not exist bring nothing, and count: the loop has one path.
-    auto fetch = [&](int i, uint32_t step, uint32_t stage) __attribute__((always_inline)) {
-      const uint32_t first = (i * kWaves + wave) * kRowsPerLoad;
-      const int8_t *base = (first < BM ? x : weight) + step * BK;
-      const bool behind = TAIL && step * BK + load_chunk * 16 >= a.k;
-      load_to_lds(base, behind ? offset[i] - load_chunk * 16 : offset[i], lds0 + stage * kStage + first * BK,
-                  step < steps ? ~0u : 0u);
-    };
-    i32x4 fx[2][MF], fw[2][NF];
-    // Fragment number i (of the rows, then of the columns) for matrix instructions kk of a step.
-    auto read = [&](int i, int to, int kk, uint32_t step, uint32_t stage) __attribute__((always_inline)) {
-      const uint8_t *lines = lds + stage * kStage + frag_base + frag_place[kk];
-      if (i < MF) {
-        fx[to][i] = *reinterpret_cast<const i32x4 *>(lines + (wm * kRows + i * 32) * BK);
-        if constexpr (TAIL) fx[to][i] &= step * BK + kk * 32 + (lane / 32) * 16 < a.k ? -1 : 0;
-      } else {
-        fw[to][i - MF] = *reinterpret_cast<const i32x4 *>(lines + (BM + wn * kColumns + (i - MF) * 32) * BK);
-      }
-    };
-
-    i32x16 acc[NF][MF] = {};
-    // The tile before has been read; its stores are done, so that what is counted below are loads.
-    wait_loads<0>();
-    __syncthreads();
 #pragma unroll
     for (int s = 0; s < STAGES; ++s) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) fetch(i, s, s);
     }
-    wait_loads<(STAGES - 1) * kLoads>();
+  };
+  i32x4 fx[2][MF], fw[2][NF];
+  // Fragment number i (of the rows, then of the columns) for matrix instructions kk of a step.
+  auto read = [&](int i, int to, int kk, uint32_t step, uint32_t stage) __attribute__((always_inline)) {
+    const uint8_t *lines = lds + stage * kStage + frag_base + frag_place[kk];
+    if (i < MF) {
+      fx[to][i] = *reinterpret_cast<const i32x4 *>(lines + (wm * kRows + i * 32) * BK);
+      if constexpr (TAIL) fx[to][i] &= step * BK + kk * 32 + (lane / 32) * 16 < a.k ? -1 : 0;
+    } else {
+      fw[to][i - MF] = *reinterpret_cast<const i32x4 *>(lines + (BM + wn * kColumns + (i - MF) * 32) * BK);
+    }
+  };
+
+  // (blockIdx goes round the eight XCDs)
+  uint32_t id = (blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;
+  Tile t{};
+  auto find = [&]() __attribute__((always_inline)) {
+    for (; id < tiles; id += gridDim.x) {
+      t = tile_of<BM, BN>(a, upto, id);
+      if (t.m0 < t.count) break;  // (offsets that descend make a list that is too long)
+    }
+    return id < tiles;
+  };
+  // Stores of a tile's results by a wave, where they are counted: columns are whole stores.
+  constexpr int kStores = MF * NF * (sizeof(O) == 4 ? 4 : 2);
+  static_assert((STAGES - 1) * kLoads + kStores < 63, "loads and stores that can be counted");
+  const bool counted = a.vector_stores;
+  bool stored = false;  // the stores of the tile before stand behind the loads of the first steps
+  bool more = find();
+  if (more) begin(t);
+  while (more) {
+    const Tile at = t;
+    i32x16 acc[NF][MF] = {};
+    if (stored) wait_loads<(STAGES - 1) * kLoads + kStores>();
+    else wait_loads<(STAGES - 1) * kLoads>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 #pragma unroll
     for (int i = 0; i < MF + NF; ++i) read(i, 0, 0, 0, 0);
-    // The matrix instructions of 32 bytes of k, between which the reads of the next 32 and the loads of a step go out: a wave issues in order, and one that hands over all its reads or loads at once waits for them to be taken.
+    // The matrix instructions of 32 bytes of k, between which the reads of the next 32 and the loads of a step go out: a wave
+    // issues in order, and one that hands over all its reads or loads at once waits for them to be taken.
     constexpr int kProducts = MF * NF;
     auto multiply = [&](int from, auto read_next, auto fetch_next) __attribute__((always_inline)) {
 #pragma unroll
@@ -211,16 +260,16 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev a) {
         __builtin_amdgcn_sched_barrier(0);
       }
     };
-    auto nothing = [](int) {};
     uint32_t stage = 0;
     for (uint32_t step = 0; step < steps; ++step) {
       const uint32_t next = stage + 1 == STAGES ? 0 : stage + 1;
 #pragma unroll
       for (int kk = 0; kk + 1 < kSteps; ++kk) {
-        multiply(kk % 2, [&](int r) { read(r, (kk + 1) % 2, kk + 1, step, stage); }, nothing);
+        multiply(kk % 2, [&](int r) { read(r, (kk + 1) % 2, kk + 1, step, stage); }, [](int) {});
       }
       // Loads under way are those of steps step + 1 .. step + STAGES - 1; this step's place is free behind the barrier.
-      wait_loads<(STAGES - 2) * kLoads, true>();
+      if (stored && step < STAGES - 1) wait_loads<(STAGES - 2) * kLoads + kStores, true>();
+      else wait_loads<(STAGES - 2) * kLoads, true>();
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       multiply((kSteps - 1) % 2, [&](int r) { read(r, kSteps % 2, 0, step + 1, next); },
@@ -228,60 +277,65 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev a) {
       stage = next;
     }
 
-    static_assert(kSteps % 2 == 0, "a step begins with the first fragments");
-    // Lane l holds row l % 32 of each fragment and, in its accumulators, columns 4 (l / 32) .. + 3 of every eight.  The sums of 32
-    // rows of the wave at a time go through its part of LDS, so that they are scaled where a lane has the same
-    // columns of every row, and leave as whole lines.
     wait_loads<0, true>();
-    __syncthreads();
-    uint8_t *own = lds + wave * 32 * kOutStride;
-    constexpr uint32_t kVec = 16 / sizeof(O), kVecs = kColumns / kVec, kRowsAtOnce = 64 / kVecs;
-    const uint32_t column = (lane % kVecs) * kVec, n = t.n0 + wn * kColumns + column;
-    float ws[kVec];
-#pragma unroll
-    for (uint32_t u = 0; u < kVec; ++u) {
-      ws[u] = as_global(a.weight_scale)[(uint64_t)t.e * a.n + (n + u < a.n ? n + u : a.n - 1)];
-    }
+    if (threadIdx.x < BM + BN) scales[threadIdx.x] = scale;
+    __syncthreads();  // (the stages have been read, the scales are there)
+    id += gridDim.x;
+    more = find();
+    if (more) begin(t);
+    stored = counted;
+
+    // Lane l holds row l % 32 of each fragment and, in its accumulators, columns 4 (l / 32) .. + 3 of every eight.  Of 2-byte
+    // results two such groups change places between the halves of the wave, so that every lane has 16 bytes of its row.
+    const uint32_t half = lane / 32;
 #pragma unroll
     for (int i = 0; i < MF; ++i) {
-      const uint32_t r0 = t.m0 + wm * kRows + i * 32;
-      if (r0 >= t.count) break;  // (waves are on their own here)
-      const uint32_t r = r0 + lane % 32;
-      const float xs = as_global(a.x_scale)[(int64_t)t.e * a.x_scale_stride_expert +
-                                            (int64_t)(t.begin + (r < t.count ? r : t.count - 1)) * a.x_scale_stride_row];
+      const uint32_t row = wm * kRows + i * 32 + lane % 32;
+      const float xs = scales[row];
+      const bool there = at.m0 + row < at.count;
+      PPLX_GLOBAL O *out = as_global(reinterpret_cast<O *>(a.out)) + (int64_t)at.e * a.out_stride_expert +
+                           (int64_t)(at.begin + at.m0 + row) * a.out_stride_row;
 #pragma unroll
       for (int j = 0; j < NF; ++j) {
+        constexpr int kGroups = sizeof(O) == 4 ? 1 : 2;  // of eight columns in a store
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          *reinterpret_cast<i32x4 *>(own + (lane % 32) * kOutStride + (j * 32 + q * 8 + 4 * (lane / 32)) * 4) =
-              i32x4{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
-        }
-      }
-      wait_loads<63, true>();
-      __builtin_amdgcn_wave_barrier();
+        for (int q = 0; q < 4; q += kGroups) {
+          uint32_t words[4];
 #pragma unroll
-      for (uint32_t first = 0; first < 32; first += kRowsAtOnce) {
-        const uint32_t row = first + lane / kVecs;
-        const float row_scale = __shfl(xs, (int)row);
-        const i32x4 *from = reinterpret_cast<const i32x4 *>(own + row * kOutStride + column * 4);
-        typedef O vec __attribute__((ext_vector_type(kVec)));
-        vec v;
+          for (int g = 0; g < kGroups; ++g) {
+            const uint32_t column = wn * kColumns + j * 32 + (q + g) * 8 + 4 * half;
+            const f32x4 ws = *reinterpret_cast<const f32x4 *>(scales + BM + column);
+            f32x4 v;
 #pragma unroll
-        for (uint32_t u = 0; u < kVec; ++u) v[u] = (O)((float)from[u / 4][u % 4] * (row_scale * ws[u]));
-        if (r0 + row >= t.count || n >= a.n) continue;
-        PPLX_GLOBAL O *out = as_global(reinterpret_cast<O *>(a.out)) + (int64_t)t.e * a.out_stride_expert +
-                             (int64_t)(t.begin + r0 + row) * a.out_stride_row + n;
-        if (a.vector_stores && a.n - n >= kVec) {
-          *reinterpret_cast<PPLX_GLOBAL vec *>(out) = v;
-        } else {
+            for (int u = 0; u < 4; ++u) v[u] = (float)acc[j][i][4 * (q + g) + u] * (xs * ws[u]);
+            pack_four<O>(v, words + 2 * g);
+          }
+          uint32_t n = at.n0 + wn * kColumns + j * 32 + q * 8;
+          if constexpr (kGroups == 2) {
+            const auto first = __builtin_amdgcn_permlane32_swap(words[0], words[2], false, false);
+            const auto second = __builtin_amdgcn_permlane32_swap(words[1], words[3], false, false);
+            words[0] = first[0];
+            words[1] = second[0];
+            words[2] = first[1];
+            words[3] = second[1];
+            n += 8 * half;
+          } else {
+            n += 4 * half;
+          }
+          constexpr uint32_t kVec = 16 / sizeof(O);
+          if (counted) {
+            const uint64_t lanes = __ballot(there && n < a.n);
+            store_counted(out + n, u32x4{words[0], words[1], words[2], words[3]}, lanes);
+          } else if (there && n < a.n) {
+            typedef O vec __attribute__((ext_vector_type(kVec)));
+            const vec v = __builtin_bit_cast(vec, u32x4{words[0], words[1], words[2], words[3]});
 #pragma unroll
-          for (uint32_t u = 0; u < kVec; ++u) {
-            if (u < a.n - n) out[u] = v[u];
+            for (uint32_t u = 0; u < kVec; ++u) {
+              if (u < a.n - n) out[n + u] = v[u];
+            }
           }
         }
       }
-      wait_loads<63, true>();
-      __builtin_amdgcn_wave_barrier();
     }
   }
 }
@@ -292,7 +346,7 @@ template <int BM, int BN, int WM, int WN, int BK, int STAGES, class O>
 int launch_tiles(const MatmulDev &from, uint64_t most_blocks, hipStream_t s) {
   MatmulDev a = from;
   constexpr uint32_t kTileLds = STAGES * (BM + BN) * BK;
-  const uint32_t lds = kTileLds + 4 * a.rows.experts;
+  const uint32_t lds = kTileLds + 4 * (BM + BN) + 4 * a.rows.experts;
   constexpr uint32_t kPerUnit = kTileLds <= 64 * 1024 ? 2 : 1;
   a.n_blocks = (a.n + BN - 1) / BN;
   const uint64_t tiles = most_blocks * a.n_blocks;
@@ -319,7 +373,7 @@ template <class O> int launch_matmul(const MatmulDev &a, hipStream_t s) {
   const uint64_t even = all / E;
   if (even <= 24) return launch_tiles<32, 128, 1, 4, 128, 3, O>(a, most_blocks(32), s);
   if (even <= 128) return launch_tiles<64, 128, 1, 4, 128, 3, O>(a, most_blocks(64), s);
-  return launch_tiles<256, 256, 2, 2, 64, 4, O>(a, most_blocks(256), s);
+  return launch_tiles<256, 256, 2, 4, 64, 4, O>(a, most_blocks(256), s);
 }
 
 }  // namespace
@@ -359,7 +413,7 @@ extern "C" int pplx_a2a_int8_matmul(int device, const pplx_a2a_int8_matmul_args_
   a.n = (uint32_t)p.n;
   a.k = (uint32_t)p.k;
   const int64_t vec = 16 / dtype_bytes(p.out_dtype);
-  a.vector_stores = is_aligned(p.out, 16) && p.out_stride_row % vec == 0 && p.out_stride_expert % vec == 0;
+  a.vector_stores = is_aligned(p.out, 16) && p.n % vec == 0 && p.out_stride_row % vec == 0 && p.out_stride_expert % vec == 0;
   return guarded(device, [&] {
     return with_type(p.out_dtype, [&](auto tag) { return launch_matmul<typename decltype(tag)::type>(a, (hipStream_t)stream); });
   });
