@@ -41,12 +41,14 @@ template <int LEFT, bool LDS = false> __device__ __forceinline__ void wait_loads
 // Sixteen bytes a lane from `base` + `offset` to LDS, lane i's at `lds` + 16 i; `lanes` is ~0, or 0 for a load that only
 // counts.  (asm: behind the builtin the compiler waits for the loads of the steps to come before it reads the step at
 // hand out of LDS.  Nothing is returned to registers, and the kernel waits by itself.  All lanes are active where it
-// stands.  m0 wants one wait state before the load, which the writes of exec are.)
+// stands.  The load wants one wait state behind the write of m0, and five behind a vector instruction that wrote the
+// registers of `base`, of which the compiler keeps count for its own loads only.)
 __device__ __forceinline__ void load_to_lds(const int8_t *base, uint32_t offset, uint32_t lds, uint32_t lanes) {
   asm volatile(
       "s_mov_b32 m0, %2\n\t"
       "s_mov_b32 exec_lo, %3\n\t"
       "s_mov_b32 exec_hi, %3\n\t"
+      "s_nop 1\n\t"
       "global_load_lds_dwordx4 %0, %1\n\t"
       "s_mov_b64 exec, -1"
       ::"v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds)), "s"(__builtin_amdgcn_readfirstlane(lanes))
@@ -146,7 +148,7 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev a) {
   static_assert((BM + BN) % (kRowsPerLoad * kWaves) == 0 && BM % kRowsPerLoad == 0, "whole loads");
   static_assert(kRows % 32 == 0 && kColumns % 32 == 0, "whole fragments");
   static_assert((STAGES - 1) * kLoads < 63, "loads that can be counted");
-  static_assert(BM + BN <= kThreads, "a scale to a thread");
+  constexpr int kScales = (BM + BN + kThreads - 1) / kThreads;  // of a thread
   static_assert(kSteps % 2 == 0, "a step begins with the first fragments");
   constexpr int kStage = (BM + BN) * BK;
   extern __shared__ __align__(128) uint8_t lds[];  // [STAGES][BM rows of x, BN of the weight][BK], scales, sums of blocks
@@ -173,7 +175,7 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev a) {
   // The tile whose steps are loaded: where its operands begin, and what the lane's loads add to that.
   const int8_t *x = nullptr, *weight = nullptr;
   uint32_t offset[kLoads];
-  float scale = 0.f;  // of row threadIdx.x of the tile, or of its column threadIdx.x - BM
+  float scale[kScales];  // of row threadIdx.x, threadIdx.x + kThreads .. of the tile, its columns behind its rows
   // Load number i of a step.  Behind k a lane fetches the first chunk of its line; what it brings is taken for zeros.  Loads of
   // steps that do not exist bring nothing, and count: the loop has one path.
   auto fetch = [&](int i, uint32_t step, uint32_t stage) __attribute__((always_inline)) {
@@ -187,12 +189,16 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev a) {
     x = a.x + (int64_t)t.e * a.x_stride_expert + (int64_t)(t.begin + t.m0) * a.x_stride_row;
     weight = a.weight + ((uint64_t)t.e * a.n + t.n0) * a.k;
     const uint32_t rows_left = t.count - t.m0, columns_left = a.n - t.n0;
-    if (threadIdx.x < BM) {
-      const uint32_t r = threadIdx.x < rows_left ? threadIdx.x : rows_left - 1;
-      scale = as_global(a.x_scale)[(int64_t)t.e * a.x_scale_stride_expert + (int64_t)(t.begin + t.m0 + r) * a.x_scale_stride_row];
-    } else if (threadIdx.x < BM + BN) {
-      const uint32_t c = threadIdx.x - BM < columns_left ? threadIdx.x - BM : columns_left - 1;
-      scale = as_global(a.weight_scale)[(uint64_t)t.e * a.n + t.n0 + c];
+#pragma unroll
+    for (int i = 0; i < kScales; ++i) {
+      const uint32_t p = threadIdx.x + i * kThreads;
+      if (p < BM) {
+        const uint32_t r = p < rows_left ? p : rows_left - 1;
+        scale[i] = as_global(a.x_scale)[(int64_t)t.e * a.x_scale_stride_expert + (int64_t)(t.begin + t.m0 + r) * a.x_scale_stride_row];
+      } else if (p < BM + BN) {
+        const uint32_t c = p - BM < columns_left ? p - BM : columns_left - 1;
+        scale[i] = as_global(a.weight_scale)[(uint64_t)t.e * a.n + t.n0 + c];
+      }
     }
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
@@ -231,7 +237,7 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev a) {
   };
   // Stores of a tile's results by a wave, where they are counted: columns are whole stores.
   constexpr int kStores = MF * NF * (sizeof(O) == 4 ? 4 : 2);
-  static_assert((STAGES - 1) * kLoads + kStores < 63, "loads and stores that can be counted");
+  constexpr int kBehind = (STAGES - 1) * kLoads + kStores <= 63 ? kStores : 0;  // as far as the counter goes
   const bool counted = a.vector_stores;
   bool stored = false;  // the stores of the tile before stand behind the loads of the first steps
   bool more = find();
@@ -239,7 +245,7 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev a) {
   while (more) {
     const Tile at = t;
     i32x16 acc[NF][MF] = {};
-    if (stored) wait_loads<(STAGES - 1) * kLoads + kStores>();
+    if (stored) wait_loads<(STAGES - 1) * kLoads + kBehind>();
     else wait_loads<(STAGES - 1) * kLoads>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -268,7 +274,7 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev a) {
         multiply(kk % 2, [&](int r) { read(r, (kk + 1) % 2, kk + 1, step, stage); }, [](int) {});
       }
       // Loads under way are those of steps step + 1 .. step + STAGES - 1; this step's place is free behind the barrier.
-      if (stored && step < STAGES - 1) wait_loads<(STAGES - 2) * kLoads + kStores, true>();
+      if (stored && step < STAGES - 1) wait_loads<(STAGES - 2) * kLoads + kBehind, true>();
       else wait_loads<(STAGES - 2) * kLoads, true>();
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
@@ -278,7 +284,10 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev a) {
     }
 
     wait_loads<0, true>();
-    if (threadIdx.x < BM + BN) scales[threadIdx.x] = scale;
+#pragma unroll
+    for (int i = 0; i < kScales; ++i) {
+      if (threadIdx.x + i * kThreads < BM + BN) scales[threadIdx.x + i * kThreads] = scale[i];
+    }
     __syncthreads();  // (the stages have been read, the scales are there)
     id += gridDim.x;
     more = find();
@@ -340,18 +349,20 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev a) {
   }
 }
 
-constexpr uint32_t kComputeUnits = 256;
+// Of a compute unit's LDS the tiles use the first 128 KiB: what lies behind has not been loaded to without registers.
+constexpr uint32_t kComputeUnits = 256, kLdsBytes = 128 * 1024;
 
 template <int BM, int BN, int WM, int WN, int BK, int STAGES, class O>
 int launch_tiles(const MatmulDev &from, uint64_t most_blocks, hipStream_t s) {
   MatmulDev a = from;
   constexpr uint32_t kTileLds = STAGES * (BM + BN) * BK;
   const uint32_t lds = kTileLds + 4 * (BM + BN) + 4 * a.rows.experts;
-  constexpr uint32_t kPerUnit = kTileLds <= 64 * 1024 ? 2 : 1;
+  constexpr uint32_t per_unit = kLdsBytes / kTileLds;
+  static_assert(per_unit >= 1, "a tile's steps fit");
   a.n_blocks = (a.n + BN - 1) / BN;
   const uint64_t tiles = most_blocks * a.n_blocks;
   if (tiles >= (1ull << 31)) return refuse(PPLX_A2A_UNSUPPORTED, "too many tiles");
-  uint64_t grid = kPerUnit * kComputeUnits;
+  uint64_t grid = per_unit * kComputeUnits;
   grid = tiles < grid ? (tiles + 7) / 8 * 8 : grid;  // (whole rounds of the XCDs)
   auto kernel = a.k % BK ? matmul_tiles<BM, BN, WM, WN, BK, STAGES, true, O> : matmul_tiles<BM, BN, WM, WN, BK, STAGES, false, O>;
   if (lds > 64 * 1024) {
@@ -371,7 +382,7 @@ template <class O> int launch_matmul(const MatmulDev &a, hipStream_t s) {
     return (all + bm - 1) / bm + (E < all ? E : all) - 1;
   };
   const uint64_t even = all / E;
-  if (even <= 24) return launch_tiles<32, 128, 1, 4, 128, 3, O>(a, most_blocks(32), s);
+  if (even <= 64) return launch_tiles<32, 128, 1, 4, 128, 3, O>(a, most_blocks(32), s);
   if (even <= 128) return launch_tiles<64, 128, 1, 4, 128, 3, O>(a, most_blocks(64), s);
   return launch_tiles<256, 256, 2, 4, 64, 4, O>(a, most_blocks(256), s);
 }
