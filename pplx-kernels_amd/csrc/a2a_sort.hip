@@ -283,7 +283,7 @@ __global__ __launch_bounds__(1024) void sort_count(SortDev a) {
 // consecutive, counts them first, and then goes through them 64 at a time.
 template <int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void sort_slots(SortDev a, uint32_t id_bits) {
-  extern __shared__ uint32_t tables[];  // [E] first rows, then [WAVES][E] the next row of an expert for each wave
+  extern __shared__ uint32_t tables[];  // [E] first rows of the experts, then for each wave [E] its next rows behind those
   __shared__ uint32_t of_wave[WAVES];
   uint32_t *start = tables, *next = tables + a.E;
   const uint32_t lane = lane_id(), wave = wave_id();
@@ -292,17 +292,7 @@ __global__ __launch_bounds__(WAVES * 64) void sort_slots(SortDev a, uint32_t id_
   const uint32_t first = blockIdx.x * a.tile + wave * part;
   const PPLX_GLOBAL uint32_t *idx = as_global(a.indices);
   for (uint32_t e = threadIdx.x; e < WAVES * a.E; e += WAVES * 64) next[e] = 0;
-  for (uint32_t e = threadIdx.x; e < a.E; e += WAVES * 64) {
-    uint32_t all = 0;
-    for (uint32_t i = 0; i < a.tiles; ++i) all += as_global(a.tile_counts)[(size_t)i * a.E + e];
-    start[e] = all;
-  }
   __syncthreads();
-  const uint32_t total = scan_experts<WAVES * 64>(start, start, a.E, of_wave);
-  if (blockIdx.x == 0) {
-    for (uint32_t e = threadIdx.x; e < a.E; e += WAVES * 64) as_global(a.offsets)[e] = (int32_t)start[e];
-    if (threadIdx.x == 0) as_global(a.offsets)[a.E] = (int32_t)total;
-  }
   uint32_t *own = next + (size_t)wave * a.E;
   for (uint32_t i = lane; i < part; i += 64) {
     const uint32_t p = first + i;
@@ -311,8 +301,22 @@ __global__ __launch_bounds__(WAVES * 64) void sort_slots(SortDev a, uint32_t id_
   }
   __syncthreads();
   for (uint32_t e = threadIdx.x; e < a.E; e += WAVES * 64) {
-    uint32_t row = start[e];
-    for (uint32_t i = 0; i < blockIdx.x; ++i) row += as_global(a.tile_counts)[(size_t)i * a.E + e];
+    // (sixteen tiles' counts in flight: one behind the other they are 64 trips to the L2)
+    uint32_t all = 0, row = 0;
+    constexpr uint32_t kAtOnce = 16;
+    for (uint32_t i = 0; i < a.tiles; i += kAtOnce) {
+      uint32_t n[kAtOnce];
+#pragma unroll
+      for (uint32_t u = 0; u < kAtOnce; ++u) {
+        n[u] = as_global(a.tile_counts)[(size_t)(i + u < a.tiles ? i + u : 0) * a.E + e];
+      }
+#pragma unroll
+      for (uint32_t u = 0; u < kAtOnce; ++u) {
+        all += i + u < a.tiles ? n[u] : 0;
+        row += i + u < blockIdx.x ? n[u] : 0;
+      }
+    }
+    start[e] = all;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
       const uint32_t n = next[(size_t)w * a.E + e];
@@ -321,6 +325,11 @@ __global__ __launch_bounds__(WAVES * 64) void sort_slots(SortDev a, uint32_t id_
     }
   }
   __syncthreads();
+  const uint32_t total = scan_experts<WAVES * 64>(start, start, a.E, of_wave);
+  if (blockIdx.x == 0) {
+    for (uint32_t e = threadIdx.x; e < a.E; e += WAVES * 64) as_global(a.offsets)[e] = (int32_t)start[e];
+    if (threadIdx.x == 0) as_global(a.offsets)[a.E] = (int32_t)total;
+  }
   for (uint32_t i = lane; i < part; i += 64) {
     const uint32_t p = first + i;
     if (p - lane >= all_picks) break;
@@ -330,7 +339,7 @@ __global__ __launch_bounds__(WAVES * 64) void sort_slots(SortDev a, uint32_t id_
     int32_t slot = -1;
     if (live) {
       const uint32_t leader = (uint32_t)__builtin_ctzll(same);
-      slot = (int32_t)(own[e] + lanes_below(same));
+      slot = (int32_t)(start[e] + own[e] + lanes_below(same));
       __builtin_amdgcn_wave_barrier();
       if (lane == leader) atomicAdd(&own[e], (uint32_t)__builtin_popcountll(same));
       __builtin_amdgcn_wave_barrier();
