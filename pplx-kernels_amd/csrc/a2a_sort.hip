@@ -26,9 +26,6 @@ struct SortDev {
   uint32_t tile, tiles;     // picks of a tile, tiles
 };
 
-// Rows that more than the last-level cache's share takes stream past it, the others stay there for the experts.
-constexpr uint64_t kKeepMaxBytes = 128ull << 20;
-
 __device__ __forceinline__ uint32_t tokens_there(const SortDev &a) {
   if (!a.bound_m) return a.m;
   const uint32_t n = *as_global(a.bound_m);
@@ -78,9 +75,14 @@ __device__ __forceinline__ uint32_t scan_experts(const uint32_t *counts, uint32_
   return total;
 }
 
+// Rows are stored through to memory at agent scope and stay in the last-level cache as far as it goes.  8192 tokens x 8
+// rows of 14 KiB, us: so 214, non-temporal 225, non-temporal through 220, plain 218; whole rows in a wave's registers
+// 220-227, four to sixteen waves to a compute unit 213-227.  5.2 TB/s, of which eight parts in nine are writes to rows
+// all over the buffer, is what the memory takes of these.
+//
 // The copies of one token's row, by LANES threads of which `g` is this one's number.  Lane k of every wave holds the
 // slot of pick k; rows t * K + k from `total` on are the ones that nobody else fills.
-template <int LANES, RowStore POLICY>
+template <int LANES>
 __device__ __forceinline__ void copy_row(const SortDev &a, uint32_t t, int32_t slot, uint32_t total, uint32_t g) {
   const uint32_t lane = lane_id();
   const uint32_t spare = t * a.K + lane;
@@ -103,7 +105,7 @@ __device__ __forceinline__ void copy_row(const SortDev &a, uint32_t t, int32_t s
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           const uint32_t j = base + i * LANES + g;
-          if (j < a.row_vecs) row_store<POLICY>(v[i], out + j);
+          if (j < a.row_vecs) row_store<RowStore::kKeep>(v[i], out + j);
         }
       }
     }
@@ -113,7 +115,7 @@ __device__ __forceinline__ void copy_row(const SortDev &a, uint32_t t, int32_t s
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const uint32_t j = base + i * LANES + g;
-        if (j < a.row_vecs) row_store<POLICY>(u32x4{0, 0, 0, 0}, out + j);
+        if (j < a.row_vecs) row_store<RowStore::kKeep>(u32x4{0, 0, 0, 0}, out + j);
       }
     }
   }
@@ -121,7 +123,7 @@ __device__ __forceinline__ void copy_row(const SortDev &a, uint32_t t, int32_t s
 
 // The same with quantised copies.  Up to 32 * LANES elements of the row stay in registers between the search for its
 // largest value and its conversion, longer rows are read twice.
-template <int LANES, RowStore POLICY, class T>
+template <int LANES, class T>
 __device__ __forceinline__ void quantize_row(const SortDev &a, uint32_t t, int32_t slot, uint32_t total, uint32_t g) {
   const uint32_t lane = lane_id();
   const uint32_t spare = t * a.K + lane;
@@ -177,7 +179,7 @@ __device__ __forceinline__ void quantize_row(const SortDev &a, uint32_t t, int32
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
           const uint32_t j = base + i * LANES + g;
-          if (j < groups) row_store<POLICY>(q[i], out + j);
+          if (j < groups) row_store<RowStore::kKeep>(q[i], out + j);
         }
       }
     }
@@ -187,24 +189,24 @@ __device__ __forceinline__ void quantize_row(const SortDev &a, uint32_t t, int32
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         const uint32_t j = base + i * LANES + g;
-        if (j < groups) row_store<POLICY>(u32x4{0, 0, 0, 0}, out + j);
+        if (j < groups) row_store<RowStore::kKeep>(u32x4{0, 0, 0, 0}, out + j);
       }
     }
   }
 }
 
 // T: the element type of quantised rows, void for copies.
-template <int LANES, RowStore POLICY, class T>
+template <int LANES, class T>
 __device__ __forceinline__ void place_row(const SortDev &a, uint32_t t, int32_t slot, uint32_t total, uint32_t g) {
-  if constexpr (std::is_void_v<T>) copy_row<LANES, POLICY>(a, t, slot, total, g);
-  else quantize_row<LANES, POLICY, T>(a, t, slot, total, g);
+  if constexpr (std::is_void_v<T>) copy_row<LANES>(a, t, slot, total, g);
+  else quantize_row<LANES, T>(a, t, slot, total, g);
 }
 
 // One launch: `per` tokens to a workgroup of 256 threads, 256 / LANES of them at a time.
 constexpr uint32_t kMaxPer = 16;
-template <int LANES, RowStore POLICY, class T>
+template <int LANES, class T>
 __global__ __launch_bounds__(256) void sort_one_launch(SortDev a, uint32_t per, uint32_t id_bits) {
-  extern __shared__ uint32_t tables[];  // [E] counts, then first rows; [E] picks in front of this workgroup's
+  extern __shared__ uint32_t tables[];  // [E] picks from this workgroup's on, then first rows; [E] picks in front of them
   __shared__ uint32_t of_wave[4];
   __shared__ int32_t own_slots[kMaxPer * 64];
   uint32_t *all = tables, *before = tables + a.E;
@@ -215,13 +217,21 @@ __global__ __launch_bounds__(256) void sort_one_launch(SortDev a, uint32_t per, 
   for (uint32_t e = threadIdx.x; e < 2 * a.E; e += 256) tables[e] = 0;
   __syncthreads();
   const PPLX_GLOBAL uint32_t *idx = as_global(a.indices);
-  for (uint32_t p = threadIdx.x; p < picks; p += 256) {
-    const uint32_t e = idx[p];
-    if (e < a.E) {
-      atomicAdd(&all[e], 1u);
-      if (p < first) atomicAdd(&before[e], 1u);
+  constexpr uint32_t kAtOnce = 8;  // loads in flight
+  for (uint32_t base = 0; base < picks; base += 256 * kAtOnce) {
+    uint32_t e[kAtOnce];
+#pragma unroll
+    for (uint32_t u = 0; u < kAtOnce; ++u) {
+      const uint32_t p = base + u * 256 + threadIdx.x;
+      e[u] = p < picks ? idx[p] : a.E;
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < kAtOnce; ++u) {
+      if (e[u] < a.E) atomicAdd(base + u * 256 + threadIdx.x < first ? &before[e[u]] : &all[e[u]], 1u);
     }
   }
+  __syncthreads();
+  for (uint32_t e = threadIdx.x; e < a.E; e += 256) all[e] += before[e];
   __syncthreads();
   const uint32_t total = scan_experts<256>(all, all, a.E, of_wave);
   if (blockIdx.x == 0) {
@@ -252,13 +262,13 @@ __global__ __launch_bounds__(256) void sort_one_launch(SortDev a, uint32_t per, 
     }
   }
   __syncthreads();
-  constexpr uint32_t kAtOnce = 256 / LANES;
+  constexpr uint32_t kRowsAtOnce = 256 / LANES;
   const uint32_t g = threadIdx.x % LANES;
-  for (uint32_t i = 0; i < per; i += kAtOnce) {
+  for (uint32_t i = 0; i < per; i += kRowsAtOnce) {
     const uint32_t mine = i + (LANES == 64 ? wave : 0);
     if (mine >= tokens) break;  // (with 256 lanes to a row the whole workgroup leaves)
     const int32_t slot = lane < a.K ? own_slots[mine * a.K + lane] : -1;
-    place_row<LANES, POLICY, T>(a, t0 + mine, slot, total, g);
+    place_row<LANES, T>(a, t0 + mine, slot, total, g);
   }
 }
 
@@ -349,17 +359,19 @@ __global__ __launch_bounds__(WAVES * 64) void sort_slots(SortDev a, uint32_t id_
 }
 
 // Third launch: the rows.
-template <int LANES, RowStore POLICY, class T>
+template <int LANES, class T>
 __global__ __launch_bounds__(256) void sort_rows(SortDev a) {
   const uint32_t lane = lane_id();
   const uint32_t t = LANES == 64 ? blockIdx.x * 4 + wave_id() : blockIdx.x;
   if (t >= a.m) return;  // (with 256 lanes to a row the grid has one workgroup a token)
   const uint32_t total = (uint32_t)as_global(a.offsets)[a.E];
   const int32_t slot = lane < a.K ? as_global(a.slots)[(size_t)t * a.K + lane] : -1;
-  place_row<LANES, POLICY, T>(a, t, slot, total, threadIdx.x % LANES);
+  place_row<LANES, T>(a, t, slot, total, threadIdx.x % LANES);
 }
 
-constexpr uint32_t kOneLaunchPicks = 4096;
+// us a call, one launch / three: 1024 x 8 picks of rows of 4 KiB 10.2 / 14.9, 2048 x 4 of 8 KiB 17.8 / 19.7; beyond, 2048 x 6 of
+// quantised 8 KiB 20.3 / 19.1, 8192 x 2 of 8 KiB (with the gradients) 185.6 / 181.3.
+constexpr uint32_t kOneLaunchPicks = 8192;
 constexpr uint32_t kMaxTiles = 64;
 
 uint32_t sort_waves(uint32_t E) {
@@ -375,7 +387,7 @@ void sort_tiling(uint32_t picks, uint32_t E, uint32_t *tile, uint32_t *tiles) {
   *tiles = (picks + per - 1) / per;
 }
 
-template <int LANES, RowStore POLICY, class T> int launch_sort(const SortDev &a, hipStream_t s) {
+template <int LANES, class T> int launch_sort(const SortDev &a, hipStream_t s) {
   uint32_t bits = 0;
   while ((1u << bits) < a.E) ++bits;
   if (a.tiles == 0) {
@@ -384,7 +396,7 @@ template <int LANES, RowStore POLICY, class T> int launch_sort(const SortDev &a,
     const uint32_t at_once = 256 / LANES;
     per = per < at_once ? at_once : per > kMaxPer ? kMaxPer : per;
     const uint32_t groups = a.m ? (a.m + per - 1) / per : 1;  // (without tokens the offsets are still written)
-    PPLX_LAUNCH(launch_kernel(sort_one_launch<LANES, POLICY, T>, dim3(groups), dim3(256), 8 * a.E, s, a, per, bits));
+    PPLX_LAUNCH(launch_kernel(sort_one_launch<LANES, T>, dim3(groups), dim3(256), 8 * a.E, s, a, per, bits));
     return PPLX_A2A_OK;
   }
   PPLX_LAUNCH(launch_kernel(sort_count, dim3(a.tiles), dim3(1024), 4 * a.E, s, a));
@@ -393,17 +405,13 @@ template <int LANES, RowStore POLICY, class T> int launch_sort(const SortDev &a,
   if (waves == 16) PPLX_LAUNCH(launch_kernel(sort_slots<16>, grid, block, lds, s, a, bits));
   else if (waves == 8) PPLX_LAUNCH(launch_kernel(sort_slots<8>, grid, block, lds, s, a, bits));
   else PPLX_LAUNCH(launch_kernel(sort_slots<2>, grid, block, lds, s, a, bits));
-  PPLX_LAUNCH(launch_kernel(sort_rows<LANES, POLICY, T>, dim3(LANES == 64 ? (a.m + 3) / 4 : a.m), dim3(256), 0, s, a));
+  PPLX_LAUNCH(launch_kernel(sort_rows<LANES, T>, dim3(LANES == 64 ? (a.m + 3) / 4 : a.m), dim3(256), 0, s, a));
   return PPLX_A2A_OK;
 }
 
-template <class T> int launch_sort_form(const SortDev &a, uint64_t row_bytes, hipStream_t s) {
-  const bool keep = (uint64_t)a.m * a.K * row_bytes <= kKeepMaxBytes;
-  const bool wave_rows = std::is_void_v<T> ? a.row_vecs <= 256 : a.width <= 2048;
-  if (wave_rows) {
-    return keep ? launch_sort<64, RowStore::kKeep, T>(a, s) : launch_sort<64, RowStore::kStream, T>(a, s);
-  }
-  return keep ? launch_sort<256, RowStore::kKeep, T>(a, s) : launch_sort<256, RowStore::kStream, T>(a, s);
+template <class T> int launch_sort_form(const SortDev &a, hipStream_t s) {
+  const bool wave_rows = std::is_void_v<T> ? a.row_vecs <= 256 : a.width <= 2048;  // what its registers hold
+  return wave_rows ? launch_sort<64, T>(a, s) : launch_sort<256, T>(a, s);
 }
 
 }  // namespace
@@ -469,7 +477,7 @@ extern "C" int pplx_a2a_sort_tokens(int device, const pplx_a2a_sort_args_t *args
   a.tile_counts = static_cast<uint32_t *>(p.workspace);
   return guarded(device, [&] {
     hipStream_t s = (hipStream_t)stream;
-    if (!p.out_scale || a.m == 0) return launch_sort_form<void>(a, out_bytes, s);
-    return with_type(p.dtype, [&](auto tag) { return launch_sort_form<typename decltype(tag)::type>(a, out_bytes, s); });
+    if (!p.out_scale || a.m == 0) return launch_sort_form<void>(a, s);
+    return with_type(p.dtype, [&](auto tag) { return launch_sort_form<typename decltype(tag)::type>(a, s); });
   });
 }

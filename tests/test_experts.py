@@ -89,8 +89,11 @@ SORTS = [
     (33, 3, 7, 520, BF16, 0, "any"),
     (100, 10, 128, 4328, BF16, 77, "mixed"),
     (127, 8, 5461, 24, BF16, None, "any"),
-    (512, 8, 256, 264, F32, None, "mixed"),  # the most picks that take one launch
-    (513, 8, 256, 264, F32, 500, "mixed"),  # the fewest that take three
+    (512, 8, 256, 264, F32, None, "mixed"),
+    (513, 8, 256, 264, F32, 500, "mixed"),
+    (1024, 8, 256, 264, F16, None, "mixed"),  # the most picks that take one launch
+    (8192, 1, 5461, 16, BF16, 8191, "any"),
+    (1025, 8, 256, 264, F16, 1000, "mixed"),  # few more: three
     (1500, 7, 5461, 40, BF16, 1499, "any"),
     (1500, 7, 1700, 40, BF16, None, "mixed"),
     (9001, 9, 33, 136, F16, 8000, "mixed"),
