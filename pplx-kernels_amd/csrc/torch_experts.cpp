@@ -4,10 +4,14 @@
 
 #include <ATen/MemoryOverlap.h>
 #include <ATen/ops/empty.h>
-#include <torch/csrc/utils/disable_torch_function.h>
+#include <ATen/ops/empty_like.h>
+#include <torch/csrc/Dtype.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
 #include <string>
+#include <tuple>
 
 #include "pplx_a2a.h"
 #include "torch_common.h"
@@ -374,6 +378,165 @@ int64_t sort_workspace_op(int64_t m, int64_t k, int64_t experts) {
   return (int64_t)((sort_workspace(m, k, experts) + 3) / 4);
 }
 
+// ---------------------------------------------------------------------------
+// The differentiable ones, which make their results
+// ---------------------------------------------------------------------------
+at::Tensor fresh(at::IntArrayRef sizes, const at::Tensor &with, at::ScalarType type) {
+  return at::empty(sizes, at::TensorOptions(with.device()).dtype(type));
+}
+
+struct Sorted {
+  at::Tensor rows, scale, slots, offsets, workspace;
+};
+
+Sorted new_sorted(const at::Tensor &x, const at::Tensor &indices, int64_t experts, bool int8) {
+  TORCH_CHECK(x.dim() == 2, "Tensor x must be 2 dimensional");
+  TORCH_CHECK(indices.dim() == 2, "Tensor indices must be 2 dimensional");
+  TORCH_CHECK(experts >= 1, "pplx_kernels: invalid argument: num_experts must be positive");
+  const int64_t m = indices.sizes()[0], k = indices.sizes()[1], words = (int64_t)(sort_workspace(m, k, experts) / 4);
+  Sorted s;
+  s.rows = fresh({m * k, x.sizes()[1]}, x, int8 ? at::kChar : x.scalar_type());
+  if (int8) s.scale = fresh({m * k}, x, at::kFloat);
+  s.slots = fresh({m, k}, x, at::kInt);
+  s.offsets = fresh({experts + 1}, x, at::kInt);
+  if (words) s.workspace = fresh({words}, x, at::kInt);
+  return s;
+}
+
+const at::Tensor *defined(const at::Tensor &t) { return t.defined() ? &t : nullptr; }
+
+Sorted sort_new(const at::Tensor &x, const at::Tensor &indices, int64_t experts, const at::Tensor *bound_m, bool int8) {
+  TORCH_CHECK(x.is_cuda(), "Tensor x must be on GPU");
+  Sorted s = new_sorted(x, indices, experts, int8);
+  sort_tokens(s.rows, defined(s.scale), s.slots, s.offsets, defined(s.workspace), x, indices, bound_m);
+  return s;
+}
+
+using SortedTuple = std::tuple<at::Tensor, at::Tensor, at::Tensor>;
+SortedTuple sorted_tokens_op(const at::Tensor &x, const at::Tensor &indices, int64_t experts, opt_tensor bound_m) {
+  Sorted s = sort_new(x, indices, experts, opt(bound_m), false);
+  return {s.rows, s.slots, s.offsets};
+}
+SortedTuple sorted_tokens_meta(const at::Tensor &x, const at::Tensor &indices, int64_t experts, opt_tensor) {
+  Sorted s = new_sorted(x, indices, experts, false);
+  return {s.rows, s.slots, s.offsets};
+}
+
+at::Tensor unsorted_tokens_meta(const at::Tensor &y, const at::Tensor &slots, const at::Tensor &, opt_tensor,
+                                std::optional<at::ScalarType> out_dtype) {
+  TORCH_CHECK(y.dim() == 2, "Tensor y must be 2 dimensional");
+  TORCH_CHECK(slots.dim() == 2, "Tensor slots must be 2 dimensional");
+  return fresh({slots.sizes()[0], y.sizes()[1]}, y, out_dtype.value_or(y.scalar_type()));
+}
+at::Tensor unsorted_tokens_op(const at::Tensor &y, const at::Tensor &slots, const at::Tensor &offsets, opt_tensor weights,
+                              std::optional<at::ScalarType> out_dtype) {
+  TORCH_CHECK(y.is_cuda(), "Tensor y must be on GPU");
+  at::Tensor out = unsorted_tokens_meta(y, slots, offsets, weights, out_dtype);
+  unsort_tokens(out, y, slots, opt(weights));
+  return out;
+}
+
+// The ops above and those on tensors of the caller, through the dispatcher, so that a step can be traced.
+template <class Fn> auto op_handle(const char *name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Fn>();
+}
+
+// Gradients come in any layout (that of a sum is one element, expanded).
+at::Tensor as_rows(const at::Tensor &g) {
+  const int64_t bytes = (int64_t)g.element_size();
+  const bool fits = g.strides()[1] == 1 && g.strides()[0] * bytes % 16 == 0 &&
+                    (g.is_meta() || reinterpret_cast<uintptr_t>(g.data_ptr()) % 16 == 0);
+  return fits ? g : g.clone(at::MemoryFormat::Contiguous);
+}
+
+// Gradients that are asked for their own (create_graph) say that they have none when they are.
+torch::autograd::variable_list differentiable_once(torch::autograd::variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  torch::autograd::variable_list made;
+  for (const at::Tensor &g : grads) {
+    if (g.defined()) made.push_back(g);
+  }
+  auto error = std::make_shared<torch::autograd::DelayedError>(
+      "pplx_kernels: the gradients of sort_tokens and unsort_tokens are differentiable once", (int64_t)made.size());
+  for (at::Tensor &g : made) {
+    g = g.detach();
+    g.requires_grad_(true);
+  }
+  made = (*error)(std::move(made));
+  size_t next = 0;
+  for (at::Tensor &g : grads) {
+    if (g.defined()) g = made[next++];
+  }
+  return grads;
+}
+
+struct SortFunction : torch::autograd::Function<SortFunction> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x,
+                                                const at::Tensor &indices, int64_t experts,
+                                                const std::optional<at::Tensor> &bound_m) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static auto op = op_handle<SortedTuple(const at::Tensor &, const at::Tensor &, int64_t, opt_tensor)>(
+        "pplx_kernels::sorted_tokens");
+    auto [rows, slots, offsets] = op.call(x, indices, experts, bound_m);
+    ctx->save_for_backward({slots});
+    ctx->mark_non_differentiable({slots, offsets});
+    ctx->set_materialize_grads(false);
+    return {rows, slots, offsets};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
+                                                 torch::autograd::variable_list grads) {
+    at::Tensor grad_x;
+    if (grads[0].defined()) {
+      const at::Tensor slots = ctx->get_saved_variables()[0];
+      at::NoGradGuard plain;
+      static auto op = op_handle<void(at::Tensor &, const at::Tensor &, const at::Tensor &, opt_tensor)>(
+          "pplx_kernels::unsort_tokens");
+      const at::Tensor g = as_rows(grads[0]);
+      grad_x = fresh({slots.sizes()[0], g.sizes()[1]}, g, g.scalar_type());
+      op.call(grad_x, g, slots, std::nullopt);
+    }
+    return differentiable_once({grad_x, at::Tensor(), at::Tensor(), at::Tensor()});
+  }
+};
+
+struct UnsortFunction : torch::autograd::Function<UnsortFunction> {
+  static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &y, const at::Tensor &slots,
+                            const at::Tensor &offsets, const std::optional<at::Tensor> &weights,
+                            std::optional<at::ScalarType> out_dtype) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static auto op = op_handle<at::Tensor(const at::Tensor &, const at::Tensor &, const at::Tensor &, opt_tensor,
+                                          std::optional<at::ScalarType>)>("pplx_kernels::unsorted_tokens");
+    at::Tensor out = op.call(y, slots, offsets, weights, out_dtype);
+    ctx->save_for_backward({y, slots, offsets, weights.value_or(at::Tensor())});
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &y = saved[0], &weights = saved[3];
+    at::Tensor grad_y, grad_weights;
+    {
+      at::NoGradGuard plain;
+      static auto op = op_handle<void(opt_tensor, opt_tensor, const at::Tensor &, const at::Tensor &, const at::Tensor &,
+                                      const at::Tensor &, opt_tensor)>("pplx_kernels::unsort_tokens_backward");
+      if (ctx->needs_input_grad(0)) grad_y = fresh(y.sizes(), y, y.scalar_type());
+      if (weights.defined() && ctx->needs_input_grad(3)) grad_weights = fresh(weights.sizes(), weights, at::kFloat);
+      auto maybe = [](const at::Tensor &t) { return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt; };
+      op.call(maybe(grad_y), maybe(grad_weights), as_rows(grads[0]), y, saved[1], saved[2], maybe(weights));
+    }
+    return differentiable_once({grad_y, at::Tensor(), at::Tensor(), grad_weights, at::Tensor()});
+  }
+};
+
+SortedTuple sorted_tokens_autograd(const at::Tensor &x, const at::Tensor &indices, int64_t experts, opt_tensor bound_m) {
+  auto made = SortFunction::apply(x, indices, experts, bound_m);
+  return {made[0], made[1], made[2]};
+}
+at::Tensor unsorted_tokens_autograd(const at::Tensor &y, const at::Tensor &slots, const at::Tensor &offsets,
+                                    opt_tensor weights, std::optional<at::ScalarType> out_dtype) {
+  return UnsortFunction::apply(y, slots, offsets, weights, out_dtype);
+}
+
 // Meta kernels: a traced call does nothing.
 template <class Fn> struct Nothing;
 template <class... A> struct Nothing<void (*)(A...)> {
@@ -404,6 +567,14 @@ TORCH_LIBRARY_FRAGMENT(pplx_kernels, m) {
          "(Tensor! out, Tensor x, Tensor x_scale, Tensor weight, Tensor weight_scale, Tensor? num_tokens, Tensor? offsets) "
          "-> ()",
          &int8_matmul_op);
+  m.def("sorted_tokens(Tensor x, Tensor indices, int num_experts, Tensor? bound_m) -> (Tensor, Tensor, Tensor)");
+  m.impl("sorted_tokens", c10::kCUDA, &sorted_tokens_op);
+  m.impl("sorted_tokens", c10::kMeta, &sorted_tokens_meta);
+  m.impl("sorted_tokens", c10::DispatchKey::Autograd, &sorted_tokens_autograd);
+  m.def("unsorted_tokens(Tensor y, Tensor slots, Tensor offsets, Tensor? weights, ScalarType? out_dtype) -> Tensor");
+  m.impl("unsorted_tokens", c10::kCUDA, &unsorted_tokens_op);
+  m.impl("unsorted_tokens", c10::kMeta, &unsorted_tokens_meta);
+  m.impl("unsorted_tokens", c10::DispatchKey::Autograd, &unsorted_tokens_autograd);
   m.def("sort_workspace", &sort_workspace_op);
 }
 
@@ -411,10 +582,6 @@ TORCH_LIBRARY_FRAGMENT(pplx_kernels, m) {
 // Functions of pplx_kernels._C
 // ---------------------------------------------------------------------------
 namespace {
-
-at::Tensor fresh(at::IntArrayRef sizes, const at::Tensor &with, at::ScalarType type) {
-  return at::empty(sizes, at::TensorOptions(with.device()).dtype(type));
-}
 
 PyObject *wrap_or_none(const at::Tensor &t) {
   if (!t.defined()) Py_RETURN_NONE;
@@ -425,23 +592,11 @@ PyObject *wrap_or_none(const at::Tensor &t) {
 PyObject *py_sort_tokens(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   arity("sort_tokens", nargs, 5);
-  const at::Tensor &x = tensor_arg(args[0], "x"), &indices = tensor_arg(args[1], "indices");
-  const int64_t experts = int_arg(args[2], "num_experts");
-  const at::Tensor *bound_m = optional_tensor_arg(args[3], "bound_m");
-  const bool int8 = PyObject_IsTrue(args[4]) == 1;
-  TORCH_CHECK(x.is_cuda(), "Tensor x must be on GPU");
-  TORCH_CHECK(x.dim() == 2, "Tensor x must be 2 dimensional");
-  TORCH_CHECK(indices.dim() == 2, "Tensor indices must be 2 dimensional");
-  TORCH_CHECK(experts >= 1, "pplx_kernels: invalid argument: num_experts must be positive");
-  const int64_t m = indices.sizes()[0], k = indices.sizes()[1], words = (int64_t)(sort_workspace(m, k, experts) / 4);
-  at::Tensor rows = fresh({m * k, x.sizes()[1]}, x, int8 ? at::kChar : x.scalar_type()), scale, workspace;
-  if (int8) scale = fresh({m * k}, x, at::kFloat);
-  at::Tensor slots = fresh({m, k}, x, at::kInt), offsets = fresh({experts + 1}, x, at::kInt);
-  if (words) workspace = fresh({words}, x, at::kInt);
-  sort_tokens(rows, int8 ? &scale : nullptr, slots, offsets, words ? &workspace : nullptr, x, indices, bound_m);
+  const Sorted s = sort_new(tensor_arg(args[0], "x"), tensor_arg(args[1], "indices"), int_arg(args[2], "num_experts"),
+                            optional_tensor_arg(args[3], "bound_m"), PyObject_IsTrue(args[4]) == 1);
   PyObject *out = PyTuple_New(5);
   if (!out) throw python_error();
-  const at::Tensor *made[] = {&rows, &scale, &slots, &offsets, &workspace};
+  const at::Tensor *made[] = {&s.rows, &s.scale, &s.slots, &s.offsets, &s.workspace};
   for (int i = 0; i < 5; ++i) PyTuple_SET_ITEM(out, i, wrap_or_none(*made[i]));
   return out;
   END_HANDLE_TH_ERRORS
@@ -455,6 +610,39 @@ PyObject *py_sort_tokens_out(PyObject *, PyObject *const *args, Py_ssize_t nargs
               tensor_arg(args[3], "offsets"), optional_tensor_arg(args[4], "workspace"), tensor_arg(args[5], "x"),
               tensor_arg(args[6], "indices"), optional_tensor_arg(args[7], "bound_m"));
   Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+// differentiable: sorted_tokens(x, indices, num_experts, bound_m) -> (rows, slots, offsets)
+PyObject *py_sorted_tokens(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  arity("sorted_tokens", nargs, 4);
+  const at::Tensor *bound_m = optional_tensor_arg(args[3], "bound_m");
+  auto [rows, slots, offsets] =
+      sorted_tokens_autograd(tensor_arg(args[0], "x"), tensor_arg(args[1], "indices"), int_arg(args[2], "num_experts"),
+                             bound_m ? std::optional<at::Tensor>(*bound_m) : std::nullopt);
+  PyObject *out = PyTuple_New(3);
+  if (!out) throw python_error();
+  PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(rows));
+  PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(slots));
+  PyTuple_SET_ITEM(out, 2, THPVariable_Wrap(offsets));
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
+// differentiable: unsorted_tokens(y, slots, offsets, weights, out_dtype) -> out
+PyObject *py_unsorted_tokens(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  arity("unsorted_tokens", nargs, 5);
+  const at::Tensor *weights = optional_tensor_arg(args[3], "weights");
+  std::optional<at::ScalarType> dtype;
+  if (args[4] != Py_None) {
+    TORCH_CHECK_TYPE(THPDtype_Check(args[4]), "out_dtype must be a torch.dtype");
+    dtype = reinterpret_cast<THPDtype *>(args[4])->scalar_type;
+  }
+  return THPVariable_Wrap(unsorted_tokens_autograd(tensor_arg(args[0], "y"), tensor_arg(args[1], "slots"),
+                                                   tensor_arg(args[2], "offsets"),
+                                                   weights ? std::optional<at::Tensor>(*weights) : std::nullopt, dtype));
   END_HANDLE_TH_ERRORS
 }
 
@@ -512,6 +700,10 @@ PyMethodDef kExpertsMethods[] = {
      "sort_tokens(x, indices, num_experts, bound_m, int8) -> (rows, scale, slots, offsets, workspace)"},
     {"sort_tokens_out", PPLX_FASTCALL(py_sort_tokens_out),
      "sort_tokens_out(rows, scale, slots, offsets, workspace, x, indices, bound_m)"},
+    {"sorted_tokens", PPLX_FASTCALL(py_sorted_tokens),
+     "sorted_tokens(x, indices, num_experts, bound_m) -> (rows, slots, offsets), differentiable"},
+    {"unsorted_tokens", PPLX_FASTCALL(py_unsorted_tokens),
+     "unsorted_tokens(y, slots, offsets, weights, out_dtype) -> out, differentiable"},
     {"unsort_tokens", PPLX_FASTCALL(py_unsort_tokens), "unsort_tokens(out, y, slots, weights)"},
     {"unsort_tokens_backward", PPLX_FASTCALL(py_unsort_tokens_backward),
      "unsort_tokens_backward(grad_y, grad_weights, grad_out, y, slots, offsets, weights)"},

@@ -97,12 +97,9 @@ def sort_tokens(
         return out
     if not int8 and _wants_grad(x):
         _check_recording()
-        rows, slots, offsets = _Sort.apply(x, indices, num_experts, bound_m)
+        fn = _ops.sorted_tokens if _is_compiling() else _C.sorted_tokens
+        rows, slots, offsets = fn(x, indices, num_experts, bound_m)
         return SortedTokens(rows, None, slots, offsets, None)
-    return _sort_new(x, indices, num_experts, bound_m, int8)
-
-
-def _sort_new(x, indices, num_experts, bound_m, int8) -> SortedTokens:
     if not _is_compiling():
         return SortedTokens._make(_C.sort_tokens(x, indices, num_experts, bound_m, int8))
     m, k = indices.shape
@@ -132,7 +129,8 @@ def unsort_tokens(
     float16, ``H`` a multiple of 8.  Differentiable in ``y`` and ``weights`` unless ``out`` is given."""
     if out is None and _wants_grad(y, weights):
         _check_recording()
-        return _Unsort.apply(y, slots, offsets, weights, out_dtype)
+        fn = _ops.unsorted_tokens if _is_compiling() else _C.unsorted_tokens
+        return fn(y, slots, offsets, weights, out_dtype)
     return _unsort(y, slots, weights, out_dtype, out)
 
 
@@ -163,49 +161,6 @@ def unsort_tokens_backward(
     fn = _ops.unsort_tokens_backward if _is_compiling() else _C.unsort_tokens_backward
     fn(out[0], out[1], grad_out, y, slots, offsets, weights)
     return out
-
-
-def _as_rows(grad: torch.Tensor) -> torch.Tensor:
-    """Gradients come in any layout (that of a sum is one element, expanded)."""
-    bytes_ = grad.element_size()
-    fits = grad.stride(-1) == 1 and grad.stride(0) * bytes_ % 16 == 0 and grad.data_ptr() % 16 == 0
-    return grad if fits else grad.clone(memory_format=torch.contiguous_format)
-
-
-class _Sort(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, indices, num_experts, bound_m):
-        made = _sort_new(x, indices, num_experts, bound_m, False)
-        ctx.save_for_backward(made.slots)
-        ctx.mark_non_differentiable(made.slots, made.offsets)
-        ctx.set_materialize_grads(False)
-        return made.rows, made.slots, made.offsets
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_rows, _slots, _offsets):
-        if grad_rows is None:
-            return None, None, None, None
-        (slots,) = ctx.saved_tensors
-        return sort_tokens_backward(_as_rows(grad_rows), slots), None, None, None
-
-
-class _Unsort(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, y, slots, offsets, weights, out_dtype):
-        ctx.save_for_backward(y, slots, offsets, weights)
-        return _unsort(y, slots, weights, out_dtype, None)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_out):
-        y, slots, offsets, weights = ctx.saved_tensors
-        grads = (
-            torch.empty_like(y, memory_format=torch.contiguous_format) if ctx.needs_input_grad[0] else None,
-            torch.empty_like(weights) if ctx.needs_input_grad[3] else None,
-        )
-        unsort_tokens_backward(_as_rows(grad_out), y, slots, offsets, weights, out=grads)
-        return grads[0], None, None, grads[1], None
 
 
 def quantize_rows(

@@ -316,6 +316,20 @@ def test_autograd_layouts_of_gradients(device):
 
 
 @gpu
+def test_gradients_are_differentiable_once(device):
+    m, k, experts, hidden = 8, 2, 4, 32
+    indices = to_u32(make_indices(m, k, experts, torch.Generator().manual_seed(1), "any"), device)
+    x = torch.randn(m, hidden, device=device, requires_grad=True)
+    weights = torch.rand(m, k, device=device, requires_grad=True)
+    s = sort_tokens(x, indices, experts)
+    out = unsort_tokens(s.rows, s.slots, s.offsets, weights)
+    gx, gw = torch.autograd.grad(out.sum(), [x, weights], create_graph=True)
+    assert torch.isfinite(gx).all() and torch.isfinite(gw).all()
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        (gx.sum() + gw.sum()).backward()
+
+
+@gpu
 def test_a_saved_tensor_that_is_written_over_is_noticed(device):
     m, k, experts, hidden = 8, 2, 4, 32
     gen = torch.Generator().manual_seed(1)
