@@ -32,6 +32,8 @@ struct MatmulDev {
   uint32_t vector_stores;  // the rows of out are 16-byte aligned, and multiples of that
 };
 
+#define PPLX_CONSTANT __attribute__((address_space(4)))
+
 // Waits until at most LEFT of the wave's loads are under way, and for its LDS reads where asked to.
 template <int LEFT, bool LDS = false> __device__ __forceinline__ void wait_loads() {
   __builtin_amdgcn_s_waitcnt((LEFT & 15) | ((LEFT >> 4) << 14) | (7 << 4) | ((LDS ? 0 : 15) << 8));
@@ -94,23 +96,24 @@ struct Tile {
 // Tile number `id` of the list: by expert, then by groups of kGroup blocks of rows, in a group by columns.  Workgroups
 // that run at the same time on one XCD take consecutive ones, about kGroup by eight of them, whose operands its L2 serves.
 constexpr uint32_t kGroup = 4;
-template <int BM, int BN> __device__ __forceinline__ Tile tile_of(const MatmulDev &a, const uint32_t *upto, uint32_t id) {
-  uint32_t lo = 0, hi = a.rows.experts - 1;
+template <int BM, int BN>
+__device__ __forceinline__ Tile tile_of(const RowsDev &rows, uint32_t n_blocks, const uint32_t *upto, uint32_t id) {
+  uint32_t lo = 0, hi = rows.experts - 1;
   while (lo < hi) {
     const uint32_t mid = (lo + hi) / 2;
-    if (upto[mid] * a.n_blocks > id) hi = mid;
+    if (upto[mid] * n_blocks > id) hi = mid;
     else lo = mid + 1;
   }
   Tile t;
   t.e = __builtin_amdgcn_readfirstlane(lo);
   const uint32_t before = t.e ? upto[t.e - 1] : 0u;
   const uint32_t blocks = upto[t.e] - before;
-  const uint32_t local = id - before * a.n_blocks;
-  const uint32_t group = local / (kGroup * a.n_blocks);
-  const uint32_t in_group = local - group * kGroup * a.n_blocks;
+  const uint32_t local = id - before * n_blocks;
+  const uint32_t group = local / (kGroup * n_blocks);
+  const uint32_t in_group = local - group * kGroup * n_blocks;
   const uint32_t size = blocks - group * kGroup < kGroup ? blocks - group * kGroup : kGroup;
   const uint32_t nb = in_group / size;
-  const Span s = span_of(a.rows, t.e);
+  const Span s = span_of(rows, t.e);
   t.m0 = __builtin_amdgcn_readfirstlane((group * kGroup + in_group - nb * size) * BM);
   t.n0 = __builtin_amdgcn_readfirstlane(nb * BN);
   t.begin = __builtin_amdgcn_readfirstlane(s.begin);
@@ -138,7 +141,7 @@ template <class O> __device__ __forceinline__ void pack_four(f32x4 v, uint32_t *
 // loads of the next tile's first steps go out before this tile's results are stored.
 // TAIL: k is no multiple of BK.
 template <int BM, int BN, int WM, int WN, int BK, int STAGES, bool TAIL, class O>
-__global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev a) {
+__global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev) {
   constexpr int kWaves = WM * WN, kThreads = kWaves * 64;
   constexpr int kRows = BM / WM, kColumns = BN / WN, MF = kRows / 32, NF = kColumns / 32;
   constexpr int kChunks = BK / 16, kRowsPerLoad = 64 / kChunks;
@@ -155,12 +158,24 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev a) {
   float *scales = reinterpret_cast<float *>(lds + STAGES * kStage);  // of BM rows and BN columns
   uint32_t *upto = reinterpret_cast<uint32_t *>(scales + BM + BN);
   __shared__ uint32_t of_wave[kWaves];
-  sum_blocks<kThreads, BM>(a.rows, upto, of_wave);
-  const uint32_t tiles = __builtin_amdgcn_readfirstlane(upto[a.rows.experts - 1] * a.n_blocks);
+  // The arguments are read where they are used, once a tile: kept in scalar registers they are more than there are.
+  auto arguments = []() __attribute__((always_inline)) {
+    auto *p = (const PPLX_CONSTANT MatmulDev *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return p;
+  };
+  uint32_t tiles;
+  {
+    const auto *a = arguments();
+    const RowsDev rows{a->rows.starts_or_counts, a->rows.rows, a->rows.experts, a->rows.layout};
+    sum_blocks<kThreads, BM>(rows, upto, of_wave);
+    tiles = __builtin_amdgcn_readfirstlane(upto[rows.experts - 1] * a->n_blocks);
+  }
   const uint32_t lane = lane_id(), wave = wave_id();
   const uint32_t wm = wave % WM, wn = wave / WM;
   const uint32_t lds0 = lds_address(lds);
-  const uint32_t steps = (a.k + BK - 1) / BK;
+  const uint32_t depth = arguments()->k;
+  const uint32_t steps = (depth + BK - 1) / BK;
   // Chunk c of row r lies at c ^ swizzle(r): sixteen consecutive rows hold a chunk at sixteen places of 256 bytes, which is
   // what LDS reads at a time.  (With exchanges for 128 bytes reads took 8.8 cycles instead of 4.9.)
   auto swizzle = [](uint32_t row) { return kChunks == 8 ? (row >> 1) & 7 : (row >> 2) & 3; };
@@ -181,31 +196,32 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev a) {
   auto fetch = [&](int i, uint32_t step, uint32_t stage) __attribute__((always_inline)) {
     const uint32_t first = (i * kWaves + wave) * kRowsPerLoad;
     const int8_t *base = (first < BM ? x : weight) + step * BK;
-    const bool behind = TAIL && step * BK + load_chunk * 16 >= a.k;
+    const bool behind = TAIL && step * BK + load_chunk * 16 >= depth;
     load_to_lds(base, behind ? offset[i] - load_chunk * 16 : offset[i], lds0 + stage * kStage + first * BK,
                 step < steps ? ~0u : 0u);
   };
   auto begin = [&](const Tile &t) __attribute__((always_inline)) {
-    x = a.x + (int64_t)t.e * a.x_stride_expert + (int64_t)(t.begin + t.m0) * a.x_stride_row;
-    weight = a.weight + ((uint64_t)t.e * a.n + t.n0) * a.k;
-    const uint32_t rows_left = t.count - t.m0, columns_left = a.n - t.n0;
+    const auto *a = arguments();
+    x = a->x + (int64_t)t.e * a->x_stride_expert + (int64_t)(t.begin + t.m0) * a->x_stride_row;
+    weight = a->weight + ((uint64_t)t.e * a->n + t.n0) * depth;
+    const uint32_t rows_left = t.count - t.m0, columns_left = a->n - t.n0;
 #pragma unroll
     for (int i = 0; i < kScales; ++i) {
       const uint32_t p = threadIdx.x + i * kThreads;
       if (p < BM) {
         const uint32_t r = p < rows_left ? p : rows_left - 1;
-        scale[i] = as_global(a.x_scale)[(int64_t)t.e * a.x_scale_stride_expert + (int64_t)(t.begin + t.m0 + r) * a.x_scale_stride_row];
+        scale[i] = as_global(a->x_scale)[(int64_t)t.e * a->x_scale_stride_expert + (int64_t)(t.begin + t.m0 + r) * a->x_scale_stride_row];
       } else if (p < BM + BN) {
         const uint32_t c = p - BM < columns_left ? p - BM : columns_left - 1;
-        scale[i] = as_global(a.weight_scale)[(uint64_t)t.e * a.n + t.n0 + c];
+        scale[i] = as_global(a->weight_scale)[(uint64_t)t.e * a->n + t.n0 + c];
       }
     }
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const uint32_t first = (i * kWaves + wave) * kRowsPerLoad;  // row of the stage
       const uint32_t r = first + load_row - (first < BM ? 0 : BM);
-      offset[i] = load_chunk * 16 + (first < BM ? (r < rows_left ? r : rows_left - 1) * (uint32_t)a.x_stride_row
-                                                : (r < columns_left ? r : columns_left - 1) * a.k);
+      offset[i] = load_chunk * 16 + (first < BM ? (r < rows_left ? r : rows_left - 1) * (uint32_t)a->x_stride_row
+                                                : (r < columns_left ? r : columns_left - 1) * depth);
     }
 #pragma unroll
     for (int s = 0; s < STAGES; ++s) {
@@ -219,7 +235,7 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev a) {
     const uint8_t *lines = lds + stage * kStage + frag_base + frag_place[kk];
     if (i < MF) {
       fx[to][i] = *reinterpret_cast<const i32x4 *>(lines + (wm * kRows + i * 32) * BK);
-      if constexpr (TAIL) fx[to][i] &= step * BK + kk * 32 + (lane / 32) * 16 < a.k ? -1 : 0;
+      if constexpr (TAIL) fx[to][i] &= step * BK + kk * 32 + (lane / 32) * 16 < depth ? -1 : 0;
     } else {
       fw[to][i - MF] = *reinterpret_cast<const i32x4 *>(lines + (BM + wn * kColumns + (i - MF) * 32) * BK);
     }
@@ -229,8 +245,11 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev a) {
   uint32_t id = (blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;
   Tile t{};
   auto find = [&]() __attribute__((always_inline)) {
+    const auto *a = arguments();
+    const RowsDev rows{a->rows.starts_or_counts, a->rows.rows, a->rows.experts, a->rows.layout};
+    const uint32_t n_blocks = a->n_blocks;
     for (; id < tiles; id += gridDim.x) {
-      t = tile_of<BM, BN>(a, upto, id);
+      t = tile_of<BM, BN>(rows, n_blocks, upto, id);
       if (t.m0 < t.count) break;  // (offsets that descend make a list that is too long)
     }
     return id < tiles;
@@ -238,7 +257,7 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev a) {
   // Stores of a tile's results by a wave, where they are counted: columns are whole stores.
   constexpr int kStores = MF * NF * (sizeof(O) == 4 ? 4 : 2);
   constexpr int kBehind = (STAGES - 1) * kLoads + kStores <= 63 ? kStores : 0;  // as far as the counter goes
-  const bool counted = a.vector_stores;
+  const bool counted = arguments()->vector_stores;
   bool stored = false;  // the stores of the tile before stand behind the loads of the first steps
   bool more = find();
   if (more) begin(t);
@@ -296,14 +315,18 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev a) {
 
     // Lane l holds row l % 32 of each fragment and, in its accumulators, columns 4 (l / 32) .. + 3 of every eight.  Of 2-byte
     // results two such groups change places between the halves of the wave, so that every lane has 16 bytes of its row.
+    const auto *a = arguments();
+    const uint32_t columns = a->n;
+    const int64_t out_stride = a->out_stride_row;
+    PPLX_GLOBAL O *out_first = as_global(reinterpret_cast<O *>(a->out)) + (int64_t)at.e * a->out_stride_expert +
+                               (int64_t)(at.begin + at.m0) * out_stride;
     const uint32_t half = lane / 32;
 #pragma unroll
     for (int i = 0; i < MF; ++i) {
       const uint32_t row = wm * kRows + i * 32 + lane % 32;
       const float xs = scales[row];
       const bool there = at.m0 + row < at.count;
-      PPLX_GLOBAL O *out = as_global(reinterpret_cast<O *>(a.out)) + (int64_t)at.e * a.out_stride_expert +
-                           (int64_t)(at.begin + at.m0 + row) * a.out_stride_row;
+      PPLX_GLOBAL O *out = out_first + (int64_t)row * out_stride;
 #pragma unroll
       for (int j = 0; j < NF; ++j) {
         constexpr int kGroups = sizeof(O) == 4 ? 1 : 2;  // of eight columns in a store
@@ -333,14 +356,14 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev a) {
           }
           constexpr uint32_t kVec = 16 / sizeof(O);
           if (counted) {
-            const uint64_t lanes = __ballot(there && n < a.n);
+            const uint64_t lanes = __ballot(there && n < columns);
             store_counted(out + n, u32x4{words[0], words[1], words[2], words[3]}, lanes);
-          } else if (there && n < a.n) {
+          } else if (there && n < columns) {
             typedef O vec __attribute__((ext_vector_type(kVec)));
             const vec v = __builtin_bit_cast(vec, u32x4{words[0], words[1], words[2], words[3]});
 #pragma unroll
             for (uint32_t u = 0; u < kVec; ++u) {
-              if (u < a.n - n) out[n + u] = v[u];
+              if (u < columns - n) out[n + u] = v[u];
             }
           }
         }
