@@ -153,6 +153,10 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev) {
   static_assert((STAGES - 1) * kLoads < 63, "loads that can be counted");
   constexpr int kScales = (BM + BN + kThreads - 1) / kThreads;  // of a thread
   static_assert(kSteps % 2 == 0, "a step begins with the first fragments");
+  // A wave of few products reads a step's fragments all at once: read for the next product only, each waits for LDS.
+  constexpr bool kWhole = MF * NF <= 2;
+  constexpr int kSets = kWhole ? kSteps : 2;            // of fragments in registers
+  constexpr int kAhead = kWhole ? STAGES - 1 : STAGES;  // steps loaded in front of a tile's first
   constexpr int kStage = (BM + BN) * BK;
   extern __shared__ __align__(128) uint8_t lds[];  // [STAGES][BM rows of x, BN of the weight][BK], scales, sums of blocks
   float *scales = reinterpret_cast<float *>(lds + STAGES * kStage);  // of BM rows and BN columns
@@ -224,12 +228,12 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev) {
                                                 : (r < columns_left ? r : columns_left - 1) * depth);
     }
 #pragma unroll
-    for (int s = 0; s < STAGES; ++s) {
+    for (int s = 0; s < kAhead; ++s) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) fetch(i, s, s);
     }
   };
-  i32x4 fx[2][MF], fw[2][NF];
+  i32x4 fx[kSets][MF], fw[kSets][NF];
   // Fragment number i (of the rows, then of the columns) for matrix instructions kk of a step.
   auto read = [&](int i, int to, int kk, uint32_t step, uint32_t stage) __attribute__((always_inline)) {
     const uint8_t *lines = lds + stage * kStage + frag_base + frag_place[kk];
@@ -264,42 +268,72 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev) {
   while (more) {
     const Tile at = t;
     i32x16 acc[NF][MF] = {};
-    if (stored) wait_loads<(STAGES - 1) * kLoads + kBehind>();
-    else wait_loads<(STAGES - 1) * kLoads>();
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
+    if constexpr (kWhole) {
+      uint32_t stage = 0;
+      for (uint32_t step = 0; step < steps; ++step) {
+        const uint32_t before = stage == 0 ? STAGES - 1 : stage - 1;
+        // Loads under way are those of steps step .. step + STAGES - 2; the place of the step before is free behind the barrier.
+        if (stored && step < STAGES - 1) wait_loads<(STAGES - 2) * kLoads + kBehind>();
+        else wait_loads<(STAGES - 2) * kLoads>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < MF + NF; ++i) read(i, 0, 0, 0, 0);
-    // The matrix instructions of 32 bytes of k, between which the reads of the next 32 and the loads of a step go out: a wave
-    // issues in order, and one that hands over all its reads or loads at once waits for them to be taken.
-    constexpr int kProducts = MF * NF;
-    auto multiply = [&](int from, auto read_next, auto fetch_next) __attribute__((always_inline)) {
+        for (int kk = 0; kk < kSteps; ++kk) {
 #pragma unroll
-      for (int q = 0; q < kProducts; ++q) {
-        const int j = q / MF, i = q % MF;
-        acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[from][j], fx[from][i], acc[j][i], 0, 0, 0);
+          for (int i = 0; i < MF + NF; ++i) read(i, kk, kk, step, stage);
+        }
 #pragma unroll
-        for (int r = q * (MF + NF) / kProducts; r < (q + 1) * (MF + NF) / kProducts; ++r) read_next(r);
+        for (int i = 0; i < kLoads; ++i) fetch(i, step + STAGES - 1, before);
 #pragma unroll
-        for (int l = q * kLoads / kProducts; l < (q + 1) * kLoads / kProducts; ++l) fetch_next(l);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int kk = 0; kk < kSteps; ++kk) {
+#pragma unroll
+          for (int j = 0; j < NF; ++j) {
+#pragma unroll
+            for (int i = 0; i < MF; ++i) {
+              acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[kk][j], fx[kk][i], acc[j][i], 0, 0, 0);
+            }
+          }
+        }
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
       }
-    };
-    uint32_t stage = 0;
-    for (uint32_t step = 0; step < steps; ++step) {
-      const uint32_t next = stage + 1 == STAGES ? 0 : stage + 1;
-#pragma unroll
-      for (int kk = 0; kk + 1 < kSteps; ++kk) {
-        multiply(kk % 2, [&](int r) { read(r, (kk + 1) % 2, kk + 1, step, stage); }, [](int) {});
-      }
-      // Loads under way are those of steps step + 1 .. step + STAGES - 1; this step's place is free behind the barrier.
-      if (stored && step < STAGES - 1) wait_loads<(STAGES - 2) * kLoads + kBehind, true>();
-      else wait_loads<(STAGES - 2) * kLoads, true>();
+    } else {
+      if (stored) wait_loads<(STAGES - 1) * kLoads + kBehind>();
+      else wait_loads<(STAGES - 1) * kLoads>();
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      multiply((kSteps - 1) % 2, [&](int r) { read(r, kSteps % 2, 0, step + 1, next); },
-               [&](int l) { fetch(l, step + STAGES, stage); });
-      stage = next;
+#pragma unroll
+      for (int i = 0; i < MF + NF; ++i) read(i, 0, 0, 0, 0);
+      // The matrix instructions of 32 bytes of k, between which the reads of the next 32 and the loads of a step go out: a wave
+      // issues in order, and one that hands over all its reads or loads at once waits for them to be taken.
+      constexpr int kProducts = MF * NF;
+      auto multiply = [&](int from, auto read_next, auto fetch_next) __attribute__((always_inline)) {
+#pragma unroll
+        for (int q = 0; q < kProducts; ++q) {
+          const int j = q / MF, i = q % MF;
+          acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[from][j], fx[from][i], acc[j][i], 0, 0, 0);
+#pragma unroll
+          for (int r = q * (MF + NF) / kProducts; r < (q + 1) * (MF + NF) / kProducts; ++r) read_next(r);
+#pragma unroll
+          for (int l = q * kLoads / kProducts; l < (q + 1) * kLoads / kProducts; ++l) fetch_next(l);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      };
+      uint32_t stage = 0;
+      for (uint32_t step = 0; step < steps; ++step) {
+        const uint32_t next = stage + 1 == STAGES ? 0 : stage + 1;
+#pragma unroll
+        for (int kk = 0; kk + 1 < kSteps; ++kk) {
+          multiply(kk % 2, [&](int r) { read(r, (kk + 1) % 2, kk + 1, step, stage); }, [](int) {});
+        }
+        // Loads under way are those of steps step + 1 .. step + STAGES - 1; this step's place is free behind the barrier.
+        if (stored && step < STAGES - 1) wait_loads<(STAGES - 2) * kLoads + kBehind, true>();
+        else wait_loads<(STAGES - 2) * kLoads, true>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        multiply((kSteps - 1) % 2, [&](int r) { read(r, kSteps % 2, 0, step + 1, next); },
+                 [&](int l) { fetch(l, step + STAGES, stage); });
+        stage = next;
+      }
     }
 
     wait_loads<0, true>();
@@ -397,17 +431,184 @@ int launch_tiles(const MatmulDev &from, uint64_t most_blocks, hipStream_t s) {
   return PPLX_A2A_OK;
 }
 
+// Products of few tiles: one workgroup to 16 RF rows by 32 columns, whose eight waves share out k, 128 bytes at a time, and
+// add their sums in LDS (whole numbers: in any order the same).  Operands go straight to registers, in fragments of 16 rows by
+// 64 bytes: the lanes of an instruction take 64 bytes in one piece of each row (32 by 32 bytes, which takes 16, was 1.2
+// to 1.6 times as long).  AHEAD units of a wave are in flight.
+constexpr int kSplitWaves = 8;
+template <int RF, int CF, int AHEAD, class O> __global__ __launch_bounds__(kSplitWaves * 64) void matmul_split(MatmulDev a) {
+  constexpr int kRows = 16 * RF, kColumns = 16 * CF;
+  extern __shared__ uint32_t upto[];
+  __shared__ uint32_t of_wave[kSplitWaves];
+  __shared__ int32_t sums[kSplitWaves][RF * CF * 4 * 64];
+  const uint32_t lane = lane_id(), wave = wave_id();
+  Tile t;
+  if (a.rows.layout == PPLX_A2A_ROWS_DENSE) {
+    t.e = t.begin = 0;
+    t.count = a.rows.rows;
+    const uint32_t block = blockIdx.x / a.n_blocks;
+    t.m0 = block * kRows;
+    t.n0 = (blockIdx.x - block * a.n_blocks) * kColumns;
+  } else {
+    sum_blocks<kSplitWaves * 64, kRows>(a.rows, upto, of_wave);
+    if (blockIdx.x >= upto[a.rows.experts - 1] * a.n_blocks) return;
+    t = tile_of<kRows, kColumns>(a.rows, a.n_blocks, upto, blockIdx.x);
+    if (t.m0 >= t.count) return;  // (offsets that descend make a list that is too long)
+  }
+  const int8_t *x_first = a.x + (int64_t)t.e * a.x_stride_expert + (int64_t)(t.begin + t.m0) * a.x_stride_row;
+  const int8_t *w_first = a.weight + ((uint64_t)t.e * a.n + t.n0) * a.k;
+  const uint32_t rows_left = t.count - t.m0, columns_left = a.n - t.n0;
+  const PPLX_GLOBAL int8_t *x[RF], *weight[CF];
+#pragma unroll
+  for (int i = 0; i < RF; ++i) {
+    const uint32_t r = i * 16 + lane % 16;
+    x[i] = as_global(x_first + (int64_t)(r < rows_left ? r : rows_left - 1) * a.x_stride_row);
+  }
+#pragma unroll
+  for (int i = 0; i < CF; ++i) {
+    const uint32_t c = i * 16 + lane % 16;
+    weight[i] = as_global(w_first + (uint64_t)(c < columns_left ? c : columns_left - 1) * a.k);
+  }
+  const uint32_t units = (a.k + 127) / 128, own = lane / 16 * 16;
+  struct Unit {
+    i32x4 x[2][RF], w[2][CF];
+  };
+  Unit u[AHEAD];
+  auto load = [&](Unit &to, uint32_t unit) __attribute__((always_inline)) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t k = unit * 128 + h * 64 + own;
+      const uint32_t at = k < a.k ? k : 0;
+#pragma unroll
+      for (int i = 0; i < CF; ++i) to.w[h][i] = *reinterpret_cast<const PPLX_GLOBAL i32x4 *>(weight[i] + at);
+#pragma unroll
+      for (int i = 0; i < RF; ++i) to.x[h][i] = *reinterpret_cast<const PPLX_GLOBAL i32x4 *>(x[i] + at);
+    }
+  };
+  i32x4 acc[CF][RF] = {};
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) {
+    if (wave + i * kSplitWaves < units) load(u[i], wave + i * kSplitWaves);
+  }
+  for (uint32_t first = wave; first < units; first += AHEAD * kSplitWaves) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const uint32_t unit = first + i * kSplitWaves;
+      if (unit >= units) break;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int there = unit * 128 + h * 64 + own < a.k ? -1 : 0;  // (bytes behind k are taken for zeros)
+#pragma unroll
+        for (int r = 0; r < RF; ++r) {
+          const i32x4 fx = u[i].x[h][r] & there;
+#pragma unroll
+          for (int c = 0; c < CF; ++c) acc[c][r] = __builtin_amdgcn_mfma_i32_16x16x64_i8(u[i].w[h][c], fx, acc[c][r], 0, 0, 0);
+        }
+      }
+      if (unit + AHEAD * kSplitWaves < units) load(u[i], unit + AHEAD * kSplitWaves);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < CF; ++c) {
+#pragma unroll
+    for (int r = 0; r < RF; ++r) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sums[wave][((c * RF + r) * 4 + i) * 64 + lane] = acc[c][r][i];
+    }
+  }
+  __syncthreads();
+  // Lane l of fragment (c, r) has columns 16 c + 4 (l / 16) .. + 3 of row 16 r + l % 16.
+  if (threadIdx.x >= RF * CF * 64) return;
+  const uint32_t fragment = threadIdx.x / 64, c = fragment / RF, r = fragment % RF;
+  const uint32_t row = t.m0 + r * 16 + lane % 16, n = t.n0 + c * 16 + 4 * (lane / 16);
+  if (row >= t.count || n >= a.n) return;
+  const float xs = as_global(a.x_scale)[(int64_t)t.e * a.x_scale_stride_expert + (int64_t)(t.begin + row) * a.x_scale_stride_row];
+  const PPLX_GLOBAL float *ws = as_global(a.weight_scale) + (uint64_t)t.e * a.n;
+  PPLX_GLOBAL O *out = as_global(reinterpret_cast<O *>(a.out)) + (int64_t)t.e * a.out_stride_expert +
+                       (int64_t)(t.begin + row) * a.out_stride_row;
+#pragma unroll
+  for (uint32_t i = 0; i < 4; ++i) {
+    if (n + i >= a.n) break;
+    int32_t sum = 0;
+#pragma unroll
+    for (int w = 0; w < kSplitWaves; ++w) sum += sums[w][(fragment * 4 + i) * 64 + lane];
+    out[n + i] = (O)((float)sum * (xs * ws[n + i]));
+  }
+}
+
+template <int RF, int CF, int AHEAD, class O> int launch_split(const MatmulDev &from, uint64_t most_blocks, hipStream_t s) {
+  MatmulDev a = from;
+  a.n_blocks = (a.n + 16 * CF - 1) / (16 * CF);
+  const uint64_t tiles = most_blocks * a.n_blocks;
+  if (tiles >= (1ull << 31)) return refuse(PPLX_A2A_UNSUPPORTED, "too many tiles");
+  PPLX_LAUNCH(launch_kernel(matmul_split<RF, CF, AHEAD, O>, dim3((uint32_t)tiles), dim3(kSplitWaves * 64), 4 * a.rows.experts, s, a));
+  return PPLX_A2A_OK;
+}
+
+// What a form costs, in microseconds, from the number of workgroups that its blocks make: `start` once, and for every round
+// of the compute units `per_line` for each 128 bytes of k and `per_tile`.  (The loads of a workgroup's steps go to LDS
+// at some 32 bytes a cycle, which is what the lines of the tiles cost.)  Fitted to products of 1 to 49152 rows with 1 to 64
+// experts, k of 496 to 8192 and n of 300 to 16384, for which the form with the least estimate is within
+// 10 % of the fastest (in buffers of the experts, of whose rows the device knows, within a third).
+// Measured, us, with the tiles of 32 x 128 / 64 x 128 / 128 x 128 / 128 x 256 / 256 x 256:
+//   4096 x 4096, one weight   128 rows 13.4 / 14.5 / 19.8 / 28.5 / 40.6    512  21.7 / 16.8 / 20.8 / 28.8 / 43.1
+//                             1024  39.6 / 29.9 / 25.2 / 30.8 / 43.6       2048 74 / 56 / 47.7 / 43.0 / 48.7     4096 142 / 111 / 91 / 83 / 69
+//   2816 x 2048, 64 experts   4096 rows 108 / 103 / 96 / 92 / 111          16384 286 / 248 / 193 / 178 / 184     49152 775 / 650 / 473 / 445 / 378
+// and, for few rows, split 16 x 16 / split 16 x 32 / split 32 x 32 / tiles of 32 x 128:
+//   4096 x 4096   1 row 5.6 / 7.0 / 7.5 / 13.0     16 rows 7.0 / 8.5 / 9.1 / 13.2     64 rows 18.3 / 13.8 / 10.6 / 13.0
+//   16384 x 4096  8 rows 16.6 / 14.4 / 15.9 / 13.5     2048 x 7168  8 rows 8.2 / 11.1 / 11.7 / 20.0
+struct MatmulForm {
+  uint32_t bm, bn;
+  double start, per_line, per_tile;
+};
+constexpr MatmulForm kForms[] = {
+    {16, 16, 3.0, 0.105, 0.0}, {16, 32, 3.0, 0.17, 0.0},  {32, 32, 3.0, 0.26, 0.0},  // split
+    {32, 128, 1.5, 0.29, 2.2}, {64, 128, 1.5, 0.42, 3.0}, {128, 128, 1.5, 0.69, 3.5}, {128, 256, 1.5, 1.25, 5.0},
+    {256, 256, 1.5, 2.05, 7.0},
+};
+
+int matmul_form(const MatmulDev &a) {
+  const double E = a.rows.experts;
+  // Of an expert's buffer an eighth is taken to be there: how much it is only the device knows.
+  const double rows = a.rows.layout == PPLX_A2A_ROWS_PADDED ? E * ((a.rows.rows + 7) / 8) : a.rows.rows;
+  const double with_rows = rows < E ? rows : E, lines = (a.k + 127) / 128;
+  int best = 0;
+  double least = 0;
+  for (int f = 0; f < (int)(sizeof(kForms) / sizeof(kForms[0])); ++f) {
+    const MatmulForm &form = kForms[f];
+    // (the last block of an expert is half full, and each that has rows has one)
+    double blocks = E == 1 ? (double)((a.rows.rows + form.bm - 1) / form.bm) : rows / form.bm + 0.5 * with_rows;
+    if (blocks < with_rows) blocks = with_rows;
+    const double tiles = blocks * ((a.n + form.bn - 1) / form.bn);
+    double rounds = tiles / kComputeUnits;
+    if (form.per_tile != 0.0) rounds = (double)(uint64_t)(rounds + 0.999);  // (small workgroups share the units)
+    else if (rounds < 1) rounds = 1;
+    const double cost = form.start + rounds * (lines * form.per_line + form.per_tile);
+    if (f == 0 || cost < least) {
+      best = f;
+      least = cost;
+    }
+  }
+  return best;
+}
+
 template <class O> int launch_matmul(const MatmulDev &a, hipStream_t s) {
   const uint64_t E = a.rows.experts;
-  const uint64_t all = a.rows.layout == PPLX_A2A_ROWS_PADDED ? E * a.rows.rows : a.rows.rows;
-  auto most_blocks = [&](uint64_t bm) {  // that the rows of all experts can make
-    if (a.rows.layout == PPLX_A2A_ROWS_PADDED) return E * ((a.rows.rows + bm - 1) / bm);
-    return (all + bm - 1) / bm + (E < all ? E : all) - 1;
+  auto most_blocks = [&](uint64_t bm) -> uint64_t {  // that the rows of all experts can make
+    const uint64_t rows = a.rows.rows;
+    if (a.rows.layout == PPLX_A2A_ROWS_PADDED) return E * ((rows + bm - 1) / bm);
+    return (rows + bm - 1) / bm + (E < rows ? E : rows) - 1;
   };
-  const uint64_t even = all / E;
-  if (even <= 64) return launch_tiles<32, 128, 1, 4, 128, 3, O>(a, most_blocks(32), s);
-  if (even <= 128) return launch_tiles<64, 128, 1, 4, 128, 3, O>(a, most_blocks(64), s);
-  return launch_tiles<256, 256, 2, 4, 64, 4, O>(a, most_blocks(256), s);
+  switch (matmul_form(a)) {
+    case 0: return launch_split<1, 1, 4, O>(a, most_blocks(16), s);
+    case 1: return launch_split<1, 2, 4, O>(a, most_blocks(16), s);
+    case 2: return launch_split<2, 2, 2, O>(a, most_blocks(32), s);
+    case 3: return launch_tiles<32, 128, 1, 4, 128, 3, O>(a, most_blocks(32), s);
+    case 4: return launch_tiles<64, 128, 1, 4, 128, 3, O>(a, most_blocks(64), s);
+    case 5: return launch_tiles<128, 128, 2, 2, 64, 4, O>(a, most_blocks(128), s);
+    case 6: return launch_tiles<128, 256, 2, 4, 64, 4, O>(a, most_blocks(128), s);
+    default: return launch_tiles<256, 256, 2, 4, 64, 4, O>(a, most_blocks(256), s);
+  }
 }
 
 }  // namespace

@@ -577,8 +577,8 @@ def test_refused_tensors(device):
         (lambda: sort_tokens(x, idx, 3, out=s, int8=True), "int8"),
         (lambda: sort_tokens(x[:2], idx[:2], 3, out=s), "slots"),
         (lambda: sort_tokens(y[:4], idx, 3, out=s), "overlaps"),
-        (lambda: sort_tokens(t(3000, 8), t(3000, 2, dtype=u32), 3, out=SortedTokens.empty(
-            3000, 8, 3, 2, BF16, device)._replace(workspace=None)), "workspace"),
+        (lambda: sort_tokens(t(9000, 8), t(9000, 2, dtype=u32), 3, out=SortedTokens.empty(
+            9000, 8, 3, 2, BF16, device)._replace(workspace=None)), "workspace"),
         (lambda: unsort_tokens(y, s.slots, s.offsets, w.to(BF16)), "weights must be of type"),
         (lambda: unsort_tokens(y, s.slots, s.offsets, w[:, :1]), "weights"),
         (lambda: unsort_tokens(y, s.slots.long(), s.offsets), "slots must be of type"),
