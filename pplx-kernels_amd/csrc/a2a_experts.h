@@ -69,14 +69,19 @@ template <> struct Eight<float> {
   static __device__ __forceinline__ f32x8 wide(raw v) { return v; }
   static __device__ __forceinline__ raw narrow(f32x8 v) { return v; }
 };
-template <class T> __device__ __forceinline__ typename Eight<T>::raw load_eight(const PPLX_GLOBAL T *p) {
+// NT: past the caches.
+template <bool NT, class V> __device__ __forceinline__ V load_vector(const PPLX_GLOBAL V *p) {
+  if constexpr (NT) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+template <class T, bool NT = false> __device__ __forceinline__ typename Eight<T>::raw load_eight(const PPLX_GLOBAL T *p) {
   if constexpr (sizeof(T) == 4) {
     // (two 16-byte loads: rows are 16-byte aligned, not 32)
     const PPLX_GLOBAL f32x4 *q = reinterpret_cast<const PPLX_GLOBAL f32x4 *>(p);
-    const f32x4 a = q[0], b = q[1];
+    const f32x4 a = load_vector<NT>(q), b = load_vector<NT>(q + 1);
     return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
   } else {
-    return *reinterpret_cast<const PPLX_GLOBAL typename Eight<T>::raw *>(p);
+    return load_vector<NT>(reinterpret_cast<const PPLX_GLOBAL typename Eight<T>::raw *>(p));
   }
 }
 template <class T> __device__ __forceinline__ void store_eight(PPLX_GLOBAL T *p, f32x8 v) {
@@ -86,6 +91,17 @@ template <class T> __device__ __forceinline__ void store_eight(PPLX_GLOBAL T *p,
     q[1] = f32x4{v[4], v[5], v[6], v[7]};
   } else {
     *reinterpret_cast<PPLX_GLOBAL typename Eight<T>::raw *>(p) = Eight<T>::narrow(v);
+  }
+}
+
+// The same past the caches.
+template <class T> __device__ __forceinline__ void stream_eight(PPLX_GLOBAL T *p, f32x8 v) {
+  if constexpr (sizeof(T) == 4) {
+    PPLX_GLOBAL f32x4 *q = reinterpret_cast<PPLX_GLOBAL f32x4 *>(p);
+    __builtin_nontemporal_store(f32x4{v[0], v[1], v[2], v[3]}, q);
+    __builtin_nontemporal_store(f32x4{v[4], v[5], v[6], v[7]}, q + 1);
+  } else {
+    __builtin_nontemporal_store(Eight<T>::narrow(v), reinterpret_cast<PPLX_GLOBAL typename Eight<T>::raw *>(p));
   }
 }
 

@@ -4,6 +4,8 @@
 namespace pplx_amd {
 namespace {
 
+constexpr uint64_t kStreamBytes = 64ull << 20;
+
 struct QuantizeDev {
   RowsDev rows;
   uint8_t *out;
@@ -39,7 +41,7 @@ __device__ __forceinline__ void load_values(const PPLX_GLOBAL T *row, uint32_t w
 
 // LANES threads to a row; up to 32 * LANES elements stay in registers between the search for the largest value and the
 // conversion, longer rows are read twice.
-template <class T, bool SWIGLU, int LANES>
+template <class T, bool SWIGLU, int LANES, bool STREAM>
 __device__ __forceinline__ void quantize_one(const QuantizeDev &a, uint32_t e, uint32_t r, uint32_t g) {
   constexpr int NS = 2;
   const PPLX_GLOBAL T *row =
@@ -70,13 +72,17 @@ __device__ __forceinline__ void quantize_one(const QuantizeDev &a, uint32_t e, u
     for (int i = 0; i < NS; ++i) {
       const uint32_t j = base + i * LANES + g;
       if (!held) load_values<T, SWIGLU>(row, a.width, j < groups ? j : groups - 1, v + 2 * i);
-      if (j < groups) out[j] = quantize_sixteen(v[2 * i], v[2 * i + 1], s.inverse);
+      if (j < groups) {
+        const u32x4 q = quantize_sixteen(v[2 * i], v[2 * i + 1], s.inverse);
+        if constexpr (STREAM) __builtin_nontemporal_store(q, out + j);
+        else out[j] = q;
+      }
     }
   }
 }
 
 // Rows of one buffer: as many as are there, 256 / LANES to a workgroup.
-template <class T, bool SWIGLU, int LANES>
+template <class T, bool SWIGLU, int LANES, bool STREAM>
 __global__ __launch_bounds__(256) void quantize_flat(QuantizeDev a) {
   uint32_t there = a.rows.rows;
   if (a.rows.layout == PPLX_A2A_ROWS_SORTED) {
@@ -84,7 +90,7 @@ __global__ __launch_bounds__(256) void quantize_flat(QuantizeDev a) {
     there = last < 0 ? 0 : (uint32_t)last < there ? (uint32_t)last : there;
   }
   const uint32_t r = LANES == 64 ? blockIdx.x * 4 + wave_id() : blockIdx.x;
-  if (r < there) quantize_one<T, SWIGLU, LANES>(a, 0, r, threadIdx.x % LANES);
+  if (r < there) quantize_one<T, SWIGLU, LANES, STREAM>(a, 0, r, threadIdx.x % LANES);
 }
 
 // Rows of the experts' buffers: workgroups share out the rows that are there, whose experts they find in the sums of the
@@ -119,7 +125,7 @@ __global__ __launch_bounds__(256) void quantize_padded(QuantizeDev a) {
       else lo = mid + 1;
     }
     const uint32_t e = __builtin_amdgcn_readfirstlane(lo);
-    quantize_one<T, SWIGLU, LANES>(a, e, r - (e ? upto[e - 1] : 0u), threadIdx.x % LANES);
+    quantize_one<T, SWIGLU, LANES, false>(a, e, r - (e ? upto[e - 1] : 0u), threadIdx.x % LANES);
   }
 }
 
@@ -130,7 +136,12 @@ template <class T, bool SWIGLU, int LANES> int launch_quantize(const QuantizeDev
     const uint32_t grid = groups < 2048 ? (uint32_t)groups : 2048;  // eight workgroups to a compute unit
     PPLX_LAUNCH(launch_kernel(quantize_padded<T, SWIGLU, LANES>, dim3(grid), dim3(256), 4 * a.rows.experts, s, a));
   } else {
-    PPLX_LAUNCH(launch_kernel(quantize_flat<T, SWIGLU, LANES>, dim3((a.rows.rows + kAtOnce - 1) / kAtOnce), dim3(256), 0, s, a));
+    // Rows that are more than a share of the last-level cache are stored past it.  us, plain / so: 49152 activated rows of 1408
+    // (277 MB read) 71.6 / 61.8, 16384 of 2048 34.9 / 31.8, 32768 plain ones of 7168 126.3 / 121.9; 2000 of 1408 5.2 / 5.1: there
+    // they stay for the product.  Large ones run at 5.3-5.8 TB/s.
+    const bool stream = (uint64_t)a.rows.rows * a.width * sizeof(T) * (SWIGLU ? 2 : 1) > kStreamBytes;
+    auto kernel = stream ? quantize_flat<T, SWIGLU, LANES, true> : quantize_flat<T, SWIGLU, LANES, false>;
+    PPLX_LAUNCH(launch_kernel(kernel, dim3((a.rows.rows + kAtOnce - 1) / kAtOnce), dim3(256), 0, s, a));
   }
   return PPLX_A2A_OK;
 }

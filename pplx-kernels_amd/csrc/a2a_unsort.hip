@@ -6,6 +6,8 @@
 namespace pplx_amd {
 namespace {
 
+constexpr uint64_t kStreamRowsBytes = 96ull << 20, kStreamGradientBytes = 56ull << 20;
+
 struct UnsortDev {
   void *out;
   int64_t out_stride;  // bytes
@@ -17,9 +19,27 @@ struct UnsortDev {
   uint32_t m, K, width;
 };
 
+// Where the eight elements of a lane lie in a piece of 512: together where they are 16 bytes, in two halves of the piece where
+// they are 32, so that each load of the wave takes whole lines.
+template <class Y> __device__ __forceinline__ void lane_columns(uint32_t lane, uint32_t *at) {
+  at[0] = sizeof(Y) == 4 ? lane * 4 : lane * 8;
+  at[1] = sizeof(Y) == 4 ? 256 + lane * 4 : lane * 8 + 4;
+}
+template <class Y, bool NT>
+__device__ __forceinline__ typename Eight<Y>::raw load_columns(const PPLX_GLOBAL Y *row, const uint32_t *at) {
+  if constexpr (sizeof(Y) == 4) {
+    const f32x4 a = load_vector<NT>(reinterpret_cast<const PPLX_GLOBAL f32x4 *>(row + at[0]));
+    const f32x4 b = load_vector<NT>(reinterpret_cast<const PPLX_GLOBAL f32x4 *>(row + at[1]));
+    return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  } else {
+    return load_vector<NT>(reinterpret_cast<const PPLX_GLOBAL typename Eight<Y>::raw *>(row + at[0]));
+  }
+}
+
 // Adds N rows of the token to acc, in the order of `left`'s bits, which it takes away.
-template <class Y, int N>
-__device__ __forceinline__ void gather_some(const UnsortDev &a, int32_t slot, float w, uint64_t &left, uint32_t col, f32x8 &acc) {
+template <class Y, int N, bool NT>
+__device__ __forceinline__ void gather_some(const UnsortDev &a, int32_t slot, float w, uint64_t &left, const uint32_t *from,
+                                            f32x8 &acc) {
   typename Eight<Y>::raw raw[N];
   float weight[N];
 #pragma unroll
@@ -28,7 +48,7 @@ __device__ __forceinline__ void gather_some(const UnsortDev &a, int32_t slot, fl
     left &= left - 1;
     const uint32_t s = (uint32_t)__builtin_amdgcn_readlane(slot, k);
     weight[i] = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(w), k));
-    raw[i] = load_eight<Y>(as_global(reinterpret_cast<const Y *>(a.y + (int64_t)s * a.y_stride)) + col);
+    raw[i] = load_columns<Y, NT>(as_global(reinterpret_cast<const Y *>(a.y + (int64_t)s * a.y_stride)), from);
   }
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -39,14 +59,20 @@ __device__ __forceinline__ void gather_some(const UnsortDev &a, int32_t slot, fl
 }
 
 // One wave to 512 elements of a token's row, eight to a lane, and up to eight rows in flight.
-template <class Y, class O>
+template <class Y, class O, bool NT>
 __global__ __launch_bounds__(256) void unsort_gather(UnsortDev a, uint32_t pieces, FastDiv by_pieces) {
   const uint32_t lane = lane_id();
   const uint32_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + threadIdx.x / kWave);
   const uint32_t t = fast_div(wave, by_pieces);
   if (t >= a.m) return;
-  const uint32_t col = (wave - t * pieces) * 512 + lane * 8;
-  const uint32_t from = col < a.width ? col : a.width - 8;  // (loads stay unconditional)
+  const uint32_t piece = (wave - t * pieces) * 512;
+  uint32_t at[2], from[2];
+  lane_columns<Y>(lane, at);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    at[h] += piece;
+    from[h] = at[h] < a.width ? at[h] : a.width - 8 + 4 * h;  // (loads stay unconditional)
+  }
   int32_t slot = -1;
   float w = 1.f;
   if (lane < a.K) {
@@ -56,12 +82,23 @@ __global__ __launch_bounds__(256) void unsort_gather(UnsortDev a, uint32_t piece
   uint64_t left = __ballot((uint32_t)slot < a.y_rows);
   f32x8 acc = {0, 0, 0, 0, 0, 0, 0, 0};
   uint32_t n = __builtin_popcountll(left);
-  for (; n >= 8; n -= 8) gather_some<Y, 8>(a, slot, w, left, from, acc);
-  if (n & 4) gather_some<Y, 4>(a, slot, w, left, from, acc);
-  if (n & 2) gather_some<Y, 2>(a, slot, w, left, from, acc);
-  if (n & 1) gather_some<Y, 1>(a, slot, w, left, from, acc);
-  if (col < a.width) {
-    store_eight<O>(as_global(reinterpret_cast<O *>(static_cast<uint8_t *>(a.out) + (int64_t)t * a.out_stride)) + col, acc);
+  for (; n >= 8; n -= 8) gather_some<Y, 8, NT>(a, slot, w, left, from, acc);
+  if (n & 4) gather_some<Y, 4, NT>(a, slot, w, left, from, acc);
+  if (n & 2) gather_some<Y, 2, NT>(a, slot, w, left, from, acc);
+  if (n & 1) gather_some<Y, 1, NT>(a, slot, w, left, from, acc);
+  PPLX_GLOBAL O *out = as_global(reinterpret_cast<O *>(static_cast<uint8_t *>(a.out) + (int64_t)t * a.out_stride));
+  if constexpr (sizeof(Y) == 4) {
+    typedef O four __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const f32x4 v = {acc[4 * h], acc[4 * h + 1], acc[4 * h + 2], acc[4 * h + 3]};
+      if (at[h] < a.width) {
+        PPLX_GLOBAL four *p = reinterpret_cast<PPLX_GLOBAL four *>(out + at[h]);
+        __builtin_nontemporal_store(__builtin_convertvector(v, four), p);
+      }
+    }
+  } else if (at[0] < a.width) {
+    stream_eight<O>(out + at[0], acc);
   }
 }
 
@@ -82,7 +119,7 @@ struct UnsortBackwardDev {
 
 // LANES threads to a token (a wave, or the workgroup).  Eight picks at a time: their rows of y are read, their rows of
 // grad_y written, and the eight products summed over the row at the end.
-template <class T, class G, int LANES>
+template <class T, class G, int LANES, bool NT>
 __global__ __launch_bounds__(256) void unsort_backward(UnsortBackwardDev a) {
   constexpr int kPicks = 8;
   const uint32_t lane = lane_id(), wave = wave_id(), g = threadIdx.x % LANES;
@@ -108,7 +145,7 @@ __global__ __launch_bounds__(256) void unsort_backward(UnsortBackwardDev a) {
           const uint32_t k = first + i;
           if (k < a.K && (live >> k) & 1) {
             const uint32_t s = (uint32_t)__builtin_amdgcn_readlane(slot, k);
-            raw[i] = load_eight<T>(as_global(reinterpret_cast<const T *>(a.y + (int64_t)s * a.y_stride)) + col);
+            raw[i] = load_eight<T, NT>(as_global(reinterpret_cast<const T *>(a.y + (int64_t)s * a.y_stride)) + col);
           }
         }
       }
@@ -125,7 +162,7 @@ __global__ __launch_bounds__(256) void unsort_backward(UnsortBackwardDev a) {
         if (want_y) {
           const float weight = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(w), k));
           const uint32_t s = (uint32_t)__builtin_amdgcn_readlane(slot, k);
-          store_eight<T>(as_global(reinterpret_cast<T *>(a.grad_y + (int64_t)s * a.grad_y_stride)) + col, go * weight);
+          stream_eight<T>(as_global(reinterpret_cast<T *>(a.grad_y + (int64_t)s * a.grad_y_stride)) + col, go * weight);
         }
       }
     }
@@ -214,8 +251,15 @@ extern "C" int pplx_a2a_unsort_tokens(int device, const pplx_a2a_unsort_args_t *
   return guarded(device, [&] {
     return with_type(p.y_dtype, [&](auto y) {
       return with_type(p.out_dtype, [&](auto out) {
-        PPLX_LAUNCH(launch_kernel(unsort_gather<typename decltype(y)::type, typename decltype(out)::type>, grid, dim3(256), 0,
-                                  (hipStream_t)stream, a, pieces, make_fast_div(pieces)));
+        typedef typename decltype(y)::type Y;
+        typedef typename decltype(out)::type O;
+        // Results go past the caches, and rows that are more than the last-level cache's share come past them.  us, plain /
+        // stores / loads and stores non-temporal: 8192 x 2 rows of 4096 bf16 (134 MB) 39.4 / 36.6 / 33.0, 8192 x 8 of 7168
+        // 204 / 189 / 176, 3001 x 5 of 2880 fp32 (173 MB) 38.9 / 35.4 / 31.5; 4096 x 3 of 2880 (71 MB) 17.9 / 15.4 / 16.6,
+        // 8192 of 4096 (67 MB) 26.7 / 20.6 / 23.0, 1024 x 2 of 7168 8.6 / 8.2 / 8.9.  Large ones run at 6.0 TB/s.
+        const uint64_t bytes = (uint64_t)a.m * a.K * a.width * sizeof(Y);
+        auto kernel = bytes > kStreamRowsBytes ? unsort_gather<Y, O, true> : unsort_gather<Y, O, false>;
+        PPLX_LAUNCH(launch_kernel(kernel, grid, dim3(256), 0, (hipStream_t)stream, a, pieces, make_fast_div(pieces)));
         return (int)PPLX_A2A_OK;
       });
     });
@@ -259,12 +303,17 @@ extern "C" int pplx_a2a_unsort_tokens_backward(int device, const pplx_a2a_unsort
       return with_type(p.grad_dtype, [&](auto grad) {
         typedef typename decltype(y)::type Y;
         typedef typename decltype(grad)::type G;
-        if (a.width <= 1024) {
-          PPLX_LAUNCH(launch_kernel(unsort_backward<Y, G, 64>, dim3((a.m + 3) / 4), dim3(256), 0, (hipStream_t)stream, a));
-        } else {
-          PPLX_LAUNCH(launch_kernel(unsort_backward<Y, G, 256>, dim3(a.m), dim3(256), 0, (hipStream_t)stream, a));
-        }
-        return (int)PPLX_A2A_OK;
+        // us, plain / stores / loads and stores non-temporal: 8192 x 2 rows of 4096 bf16 (134 MB) 71.7 / 68.3 / 56.5, 8192 x 8 of
+        // 2048 (268 MB) 112 / 109 / 100, 16384 x 2 of 1024 (67 MB) 36.3 / 31.4 / 30.2; 2048 x 6 of 2048 (50 MB) 24.6 / 19.6 /
+        // 23.0, 1024 x 2 of 7168 (29 MB) 13.8 / 13.9 / 15.1.
+        const bool stream = (uint64_t)a.m * a.K * a.width * sizeof(Y) > kStreamGradientBytes;
+        auto launch = [&](auto lanes) {
+          constexpr int L = decltype(lanes)::value;
+          auto kernel = stream ? unsort_backward<Y, G, L, true> : unsort_backward<Y, G, L, false>;
+          PPLX_LAUNCH(launch_kernel(kernel, dim3(L == 64 ? (a.m + 3) / 4 : a.m), dim3(256), 0, (hipStream_t)stream, a));
+          return (int)PPLX_A2A_OK;
+        };
+        return a.width <= 1024 ? launch(std::integral_constant<int, 64>{}) : launch(std::integral_constant<int, 256>{});
       });
     });
   });
