@@ -139,8 +139,8 @@ template <class T, bool SWIGLU, int LANES> int launch_quantize(const QuantizeDev
     // Rows that are more than a share of the last-level cache are stored past it.  us, plain / so: 49152 activated rows of 1408
     // (277 MB read) 71.6 / 61.8, 16384 of 2048 34.9 / 31.8, 32768 plain ones of 7168 126.3 / 121.9; 2000 of 1408 5.2 / 5.1: there
     // they stay for the product.  Large ones run at 5.3-5.8 TB/s.
-    const bool stream = (uint64_t)a.rows.rows * a.width * sizeof(T) * (SWIGLU ? 2 : 1) > kStreamBytes;
-    auto kernel = stream ? quantize_flat<T, SWIGLU, LANES, true> : quantize_flat<T, SWIGLU, LANES, false>;
+    const bool large = (uint64_t)a.rows.rows * a.width * sizeof(T) * (SWIGLU ? 2 : 1) > kStreamBytes;
+    auto kernel = large ? quantize_flat<T, SWIGLU, LANES, true> : quantize_flat<T, SWIGLU, LANES, false>;
     PPLX_LAUNCH(launch_kernel(kernel, dim3((a.rows.rows + kAtOnce - 1) / kAtOnce), dim3(256), 0, s, a));
   }
   return PPLX_A2A_OK;

@@ -306,10 +306,10 @@ extern "C" int pplx_a2a_unsort_tokens_backward(int device, const pplx_a2a_unsort
         // us, plain / stores / loads and stores non-temporal: 8192 x 2 rows of 4096 bf16 (134 MB) 71.7 / 68.3 / 56.5, 8192 x 8 of
         // 2048 (268 MB) 112 / 109 / 100, 16384 x 2 of 1024 (67 MB) 36.3 / 31.4 / 30.2; 2048 x 6 of 2048 (50 MB) 24.6 / 19.6 /
         // 23.0, 1024 x 2 of 7168 (29 MB) 13.8 / 13.9 / 15.1.
-        const bool stream = (uint64_t)a.m * a.K * a.width * sizeof(Y) > kStreamGradientBytes;
+        const bool large = (uint64_t)a.m * a.K * a.width * sizeof(Y) > kStreamGradientBytes;
         auto launch = [&](auto lanes) {
           constexpr int L = decltype(lanes)::value;
-          auto kernel = stream ? unsort_backward<Y, G, L, true> : unsort_backward<Y, G, L, false>;
+          auto kernel = large ? unsort_backward<Y, G, L, true> : unsort_backward<Y, G, L, false>;
           PPLX_LAUNCH(launch_kernel(kernel, dim3(L == 64 ? (a.m + 3) / 4 : a.m), dim3(256), 0, (hipStream_t)stream, a));
           return (int)PPLX_A2A_OK;
         };
