@@ -5,7 +5,8 @@ token counts); ``baseline_configs()`` returns the five benchmark workloads C1..C
 draws one DP group's inputs on the CPU from a seeded generator (fp8 block quantisation with an
 fp32 absmax scale per 128 columns, uniform or Zipf-skewed routing without replacement, softmax
 weights); ``DeviceStep`` holds all ranks' device tensors of one step and runs it through a
-``LoopbackWorld`` or through per-rank ``AllToAll`` objects.  Used by ``bench.py`` and by the tests.
+``LoopbackWorld`` or through per-rank ``AllToAll`` objects; ``Int8Experts`` is what stands between the two halves of a
+step of int8 rows.  Used by ``bench.py`` and by the tests.
 """
 
 from __future__ import annotations
@@ -52,6 +53,8 @@ class WorkloadSpec:
     def scale_dim(self) -> int:
         if self.in_dtype.itemsize != 1:
             return 0
+        if self.in_dtype == torch.int8:
+            return 4  # one scale a row; rows of scales are multiples of 16 bytes
         return (self.hidden_dim + self.block_size - 1) // self.block_size
 
     @property
@@ -100,6 +103,16 @@ def quantize_fp8_blockwise(x: torch.Tensor, block: int = 128) -> tuple[torch.Ten
     return q.contiguous(), scale.contiguous()
 
 
+def quantize_int8_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """bf16/f32 [n, H] -> (int8 [n, H], f32 scales [n, 4], of which the first is the row's), as ``quantize_rows`` does it."""
+    xf = x.float()
+    most = torch.full((x.shape[0],), 127.0)
+    a = xf.abs().amax(dim=1).clamp_min(2.0**-100)
+    scale = torch.zeros(x.shape[0], 4)
+    scale[:, 0] = torch.div(a, most)
+    return torch.round(xf * torch.div(most, a)[:, None]).to(torch.int8), scale
+
+
 def sample_routing(n: int, E: int, K: int, routing: str, rng: torch.Generator) -> torch.Tensor:
     """[n, K] int32 expert ids, distinct per row."""
     if n == 0:
@@ -134,6 +147,8 @@ def generate_group(spec: WorkloadSpec, group: int, seed: int | None = None, n: i
     x_scale = None
     if spec.in_dtype == FP8:
         x, x_scale = quantize_fp8_blockwise(x, spec.block_size)
+    elif spec.in_dtype == torch.int8:
+        x, x_scale = quantize_int8_rows(x)
     else:
         x = x.to(spec.in_dtype)
     return GroupInputs(x, x_scale, indices, weights.contiguous(), n)
@@ -257,6 +272,43 @@ class DeviceStep:
             + T * s.dp_size * s.hidden_dim * s.out_dtype.itemsize
         )
         return dispatch, combine
+
+
+class Int8Experts:
+    """Experts of 8-bit weights between the dispatch and the combine of a :class:`DeviceStep` whose rows are int8: the product
+    with the gate and up weights, the gated activation, quantised again, and the product with the down weights, for the
+    experts of all ranks at once.  Random weights with one scale a row."""
+
+    def __init__(self, step: DeviceStep, intermediate: int, seed: int = 0) -> None:
+        spec, dev = step.spec, step.expert_x_all.device
+        assert spec.in_dtype == torch.int8
+        gen = torch.Generator(device=dev).manual_seed(seed)
+        experts, hidden = spec.num_experts, spec.hidden_dim
+
+        def weights(rows: int, columns: int) -> tuple[torch.Tensor, torch.Tensor]:
+            w = torch.randint(-127, 128, (experts, rows, columns), generator=gen, dtype=torch.int8, device=dev)
+            scale = (0.5 + torch.rand(experts, rows, generator=gen, device=dev)) / (73.0 * columns**0.5)  # (outputs of size 1)
+            return w, scale
+
+        self.gate_up, self.gate_up_scale = weights(2 * intermediate, hidden)
+        self.down, self.down_scale = weights(hidden, intermediate)
+        shape = (experts, step.cap)
+        self.num_tokens = step.expert_num_tokens_all.view(experts)
+        self.x = step.expert_x_all.view(*shape, hidden)
+        self.x_scale = step.expert_x_scale_all.view(*shape, spec.scale_dim)[..., 0]
+        self.h = torch.empty((*shape, 2 * intermediate), dtype=torch.bfloat16, device=dev)
+        self.q = torch.empty((*shape, intermediate), dtype=torch.int8, device=dev)
+        self.q_scale = torch.empty(shape, dtype=torch.float32, device=dev)
+        self.y = step.expert_y_all.view(*shape, hidden)
+
+    def run(self) -> None:
+        """From what dispatch left to what combine takes; allocates nothing."""
+        from .experts import int8_matmul, quantize_rows
+
+        n = self.num_tokens
+        int8_matmul(self.x, self.x_scale, self.gate_up, self.gate_up_scale, num_tokens=n, out=self.h)
+        quantize_rows(self.h, num_tokens=n, swiglu=True, out=(self.q, self.q_scale))
+        int8_matmul(self.q, self.q_scale, self.down, self.down_scale, num_tokens=n, out=self.y)
 
 
 def make_world(spec: WorkloadSpec, group_name: str = "loopback"):
