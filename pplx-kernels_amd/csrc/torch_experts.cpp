@@ -412,14 +412,16 @@ Sorted sort_new(const at::Tensor &x, const at::Tensor &indices, int64_t experts,
   return s;
 }
 
-using SortedTuple = std::tuple<at::Tensor, at::Tensor, at::Tensor>;
-SortedTuple sorted_tokens_op(const at::Tensor &x, const at::Tensor &indices, int64_t experts, opt_tensor bound_m) {
-  Sorted s = sort_new(x, indices, experts, opt(bound_m), false);
-  return {s.rows, s.slots, s.offsets};
+// (rows, scale, slots, offsets); without int8 the scale is empty
+using SortedTuple = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
+SortedTuple as_tuple(const Sorted &s) {
+  return {s.rows, s.scale.defined() ? s.scale : fresh({0}, s.rows, at::kFloat), s.slots, s.offsets};
 }
-SortedTuple sorted_tokens_meta(const at::Tensor &x, const at::Tensor &indices, int64_t experts, opt_tensor) {
-  Sorted s = new_sorted(x, indices, experts, false);
-  return {s.rows, s.slots, s.offsets};
+SortedTuple sorted_tokens_op(const at::Tensor &x, const at::Tensor &indices, int64_t experts, opt_tensor bound_m, bool int8) {
+  return as_tuple(sort_new(x, indices, experts, opt(bound_m), int8));
+}
+SortedTuple sorted_tokens_meta(const at::Tensor &x, const at::Tensor &indices, int64_t experts, opt_tensor, bool int8) {
+  return as_tuple(new_sorted(x, indices, experts, int8));
 }
 
 at::Tensor unsorted_tokens_meta(const at::Tensor &y, const at::Tensor &slots, const at::Tensor &, opt_tensor,
@@ -441,11 +443,12 @@ template <class Fn> auto op_handle(const char *name) {
   return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Fn>();
 }
 
-// Gradients come in any layout (that of a sum is one element, expanded).
+// Gradients come in any layout (that of a sum is one element, expanded).  Those of a traced step have no address yet.
 at::Tensor as_rows(const at::Tensor &g) {
   const int64_t bytes = (int64_t)g.element_size();
-  const bool fits = g.strides()[1] == 1 && g.strides()[0] * bytes % 16 == 0 &&
-                    (g.is_meta() || reinterpret_cast<uintptr_t>(g.data_ptr()) % 16 == 0);
+  const bool traced = g.is_meta() || g.key_set().has(c10::DispatchKey::Python) || g.key_set().has(c10::DispatchKey::Functionalize);
+  const bool aligned = traced ? g.storage_offset() * bytes % 16 == 0 : reinterpret_cast<uintptr_t>(g.data_ptr()) % 16 == 0;
+  const bool fits = g.strides()[1] == 1 && g.strides()[0] * bytes % 16 == 0 && aligned;
   return fits ? g : g.clone(at::MemoryFormat::Contiguous);
 }
 
@@ -470,18 +473,22 @@ torch::autograd::variable_list differentiable_once(torch::autograd::variable_lis
   return grads;
 }
 
+SortedTuple call_sorted_tokens(const at::Tensor &x, const at::Tensor &indices, int64_t experts, opt_tensor bound_m, bool int8) {
+  at::AutoDispatchBelowADInplaceOrView below;
+  static auto op = op_handle<SortedTuple(const at::Tensor &, const at::Tensor &, int64_t, opt_tensor, bool)>(
+      "pplx_kernels::sorted_tokens");
+  return op.call(x, indices, experts, bound_m, int8);
+}
+
 struct SortFunction : torch::autograd::Function<SortFunction> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x,
                                                 const at::Tensor &indices, int64_t experts,
                                                 const std::optional<at::Tensor> &bound_m) {
-    at::AutoDispatchBelowADInplaceOrView below;
-    static auto op = op_handle<SortedTuple(const at::Tensor &, const at::Tensor &, int64_t, opt_tensor)>(
-        "pplx_kernels::sorted_tokens");
-    auto [rows, slots, offsets] = op.call(x, indices, experts, bound_m);
+    auto [rows, scale, slots, offsets] = call_sorted_tokens(x, indices, experts, bound_m, false);
     ctx->save_for_backward({slots});
-    ctx->mark_non_differentiable({slots, offsets});
+    ctx->mark_non_differentiable({scale, slots, offsets});
     ctx->set_materialize_grads(false);
-    return {rows, slots, offsets};
+    return {rows, scale, slots, offsets};
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
                                                  torch::autograd::variable_list grads) {
@@ -528,9 +535,11 @@ struct UnsortFunction : torch::autograd::Function<UnsortFunction> {
   }
 };
 
-SortedTuple sorted_tokens_autograd(const at::Tensor &x, const at::Tensor &indices, int64_t experts, opt_tensor bound_m) {
+SortedTuple sorted_tokens_autograd(const at::Tensor &x, const at::Tensor &indices, int64_t experts, opt_tensor bound_m,
+                                   bool int8) {
+  if (int8) return call_sorted_tokens(x, indices, experts, bound_m, true);
   auto made = SortFunction::apply(x, indices, experts, bound_m);
-  return {made[0], made[1], made[2]};
+  return {made[0], made[1], made[2], made[3]};
 }
 at::Tensor unsorted_tokens_autograd(const at::Tensor &y, const at::Tensor &slots, const at::Tensor &offsets,
                                     opt_tensor weights, std::optional<at::ScalarType> out_dtype) {
@@ -567,7 +576,7 @@ TORCH_LIBRARY_FRAGMENT(pplx_kernels, m) {
          "(Tensor! out, Tensor x, Tensor x_scale, Tensor weight, Tensor weight_scale, Tensor? num_tokens, Tensor? offsets) "
          "-> ()",
          &int8_matmul_op);
-  m.def("sorted_tokens(Tensor x, Tensor indices, int num_experts, Tensor? bound_m) -> (Tensor, Tensor, Tensor)");
+  m.def("sorted_tokens(Tensor x, Tensor indices, int num_experts, Tensor? bound_m, bool int8) -> (Tensor, Tensor, Tensor, Tensor)");
   m.impl("sorted_tokens", c10::kCUDA, &sorted_tokens_op);
   m.impl("sorted_tokens", c10::kMeta, &sorted_tokens_meta);
   m.impl("sorted_tokens", c10::DispatchKey::Autograd, &sorted_tokens_autograd);
@@ -618,9 +627,9 @@ PyObject *py_sorted_tokens(PyObject *, PyObject *const *args, Py_ssize_t nargs) 
   HANDLE_TH_ERRORS
   arity("sorted_tokens", nargs, 4);
   const at::Tensor *bound_m = optional_tensor_arg(args[3], "bound_m");
-  auto [rows, slots, offsets] =
+  auto [rows, scale, slots, offsets] =
       sorted_tokens_autograd(tensor_arg(args[0], "x"), tensor_arg(args[1], "indices"), int_arg(args[2], "num_experts"),
-                             bound_m ? std::optional<at::Tensor>(*bound_m) : std::nullopt);
+                             bound_m ? std::optional<at::Tensor>(*bound_m) : std::nullopt, false);
   PyObject *out = PyTuple_New(3);
   if (!out) throw python_error();
   PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(rows));

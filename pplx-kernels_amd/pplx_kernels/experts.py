@@ -65,7 +65,7 @@ def _wants_grad(*tensors: torch.Tensor | None) -> bool:
 
 
 def _check_recording() -> None:
-    if not _is_compiling() and torch.cuda.is_current_stream_capturing():
+    if torch.cuda.is_current_stream_capturing():
         raise RuntimeError(
             "pplx_kernels: gradients are not recorded under stream capture: capture sort_tokens_backward and "
             "unsort_tokens_backward, under torch.no_grad()"
@@ -95,17 +95,14 @@ def sort_tokens(
         fn = _ops.sort_tokens if _is_compiling() else _C.sort_tokens_out
         fn(out.rows, out.scale, out.slots, out.offsets, out.workspace, x, indices, bound_m)
         return out
+    if _is_compiling():
+        rows, scale, slots, offsets = _ops.sorted_tokens(x, indices, num_experts, bound_m, int8)
+        return SortedTokens(rows, scale if int8 else None, slots, offsets, None)
     if not int8 and _wants_grad(x):
         _check_recording()
-        fn = _ops.sorted_tokens if _is_compiling() else _C.sorted_tokens
-        rows, slots, offsets = fn(x, indices, num_experts, bound_m)
+        rows, slots, offsets = _C.sorted_tokens(x, indices, num_experts, bound_m)
         return SortedTokens(rows, None, slots, offsets, None)
-    if not _is_compiling():
-        return SortedTokens._make(_C.sort_tokens(x, indices, num_experts, bound_m, int8))
-    m, k = indices.shape
-    made = SortedTokens.empty(m, x.size(1), num_experts, k, x.dtype, x.device, int8)
-    _ops.sort_tokens(*made, x, indices, bound_m)
-    return made
+    return SortedTokens._make(_C.sort_tokens(x, indices, num_experts, bound_m, int8))
 
 
 def sort_tokens_backward(
@@ -127,10 +124,11 @@ def unsort_tokens(
     """``out[t] = sum_k weights[t, k] * y[slots[t, k]]`` over the picks that have a row, fp32 accumulation in pick order;
     a token without one becomes zeros.  ``weights`` are float32 (None: ones).  ``y`` is ``[rows, H]`` of float32, bfloat16 or
     float16, ``H`` a multiple of 8.  Differentiable in ``y`` and ``weights`` unless ``out`` is given."""
+    if out is None and _is_compiling():
+        return _ops.unsorted_tokens(y, slots, offsets, weights, out_dtype)
     if out is None and _wants_grad(y, weights):
         _check_recording()
-        fn = _ops.unsorted_tokens if _is_compiling() else _C.unsorted_tokens
-        return fn(y, slots, offsets, weights, out_dtype)
+        return _C.unsorted_tokens(y, slots, offsets, weights, out_dtype)
     return _unsort(y, slots, weights, out_dtype, out)
 
 
