@@ -164,22 +164,32 @@ __device__ __forceinline__ uint32_t magnitude_bits(f32x8 v) {
   }
   return m;
 }
-// Sixteen values as bytes.  (A row with an infinity or a NaN has inverse 0 and becomes zeros: its products, which may be
-// NaN, are not converted.)
-__device__ __forceinline__ u32x4 quantize_sixteen(f32x8 a, f32x8 b, float inverse) {
-  uint32_t q[4];
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// Eight values as bytes.  1.5 * 2^23 + p is p rounded to an integer, ties to even, whose low byte is the low byte of the sum's
+// bits: |p| <= 127.  (A row with an infinity or a NaN has inverse 0 and becomes zeros, whatever its products are.)
+__device__ __forceinline__ u32x2 quantize_eight(f32x8 v, float inverse) {
+#pragma clang fp contract(off)
+  uint32_t bits[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t word = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float v = i < 2 ? a[4 * i + j] : b[4 * (i - 2) + j];
-      const int r = inverse != 0.f ? (int)__builtin_rintf(v * inverse) : 0;
-      word |= ((uint32_t)r & 0xffu) << (8 * j);
-    }
-    q[i] = word;
+  for (int i = 0; i < 8; ++i) {
+    const float p = v[i] * inverse;  // (rounded, as the oracle's product is)
+    bits[i] = __float_as_uint(p + 12582912.f);
   }
-  return u32x4{q[0], q[1], q[2], q[3]};
+  const uint32_t keep = inverse != 0.f ? 0xffffffffu : 0u;
+  uint32_t q[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t *b = bits + 4 * i;
+    // (a selector's bytes 0-3 are of the second operand, 4-7 of the first)
+    const uint32_t low = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400), high = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0c);
+    q[i] = (low | high) & keep;
+  }
+  return u32x2{q[0], q[1]};
+}
+__device__ __forceinline__ u32x4 quantize_sixteen(f32x8 a, f32x8 b, float inverse) {
+  const u32x2 lo = quantize_eight(a, inverse), hi = quantize_eight(b, inverse);
+  return u32x4{lo[0], lo[1], hi[0], hi[1]};
 }
 
 // The largest of the magnitudes that the LANES threads of a row found (64, or the 256 of a workgroup, which all call).

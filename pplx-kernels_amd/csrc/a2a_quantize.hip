@@ -4,7 +4,7 @@
 namespace pplx_amd {
 namespace {
 
-constexpr uint64_t kStreamBytes = 64ull << 20;
+constexpr uint64_t kStreamBytes = 192ull << 20;
 
 struct QuantizeDev {
   RowsDev rows;
@@ -17,72 +17,79 @@ struct QuantizeDev {
   uint32_t width;
 };
 
-// Sixteen values of the row from element 16 * j on.
-template <class T, bool SWIGLU>
-__device__ __forceinline__ void load_values(const PPLX_GLOBAL T *row, uint32_t width, uint32_t j, f32x8 *v) {
-  typename Eight<T>::raw a = load_eight<T>(row + 16ull * j), b = load_eight<T>(row + 16ull * j + 8);
-  v[0] = Eight<T>::wide(a);
-  v[1] = Eight<T>::wide(b);
-  if constexpr (SWIGLU) {
-    const PPLX_GLOBAL T *up = row + width;
-    a = load_eight<T>(up + 16ull * j);
-    b = load_eight<T>(up + 16ull * j + 8);
-    const f32x8 u[2] = {Eight<T>::wide(a), Eight<T>::wide(b)};
+// What one thread holds of a row: PIECES times eight elements, eight elements apart from the next thread's.
+template <class T, bool SWIGLU, int LANES, int PIECES, bool NT> struct Piece {
+  const PPLX_GLOBAL T *row;
+  uint32_t width, groups, g, first_of_wave;
+  f32x8 v[PIECES];
+
+  // (the same for all lanes of a wave: pieces that no lane has cost nothing)
+  __device__ __forceinline__ bool any(uint32_t base, int i) const { return base + i * LANES + first_of_wave < groups; }
+
+  __device__ __forceinline__ void load(uint32_t base) {
+    typename Eight<T>::raw gate[PIECES], up[SWIGLU ? PIECES : 1];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < PIECES; ++i) {
+      if (!any(base, i)) continue;
+      uint32_t j = base + i * LANES + g;
+      j = j < groups ? j : groups - 1;
+      gate[i] = load_eight<T, NT>(row + 8ull * j);
+      if constexpr (SWIGLU) up[i] = load_eight<T, NT>(row + width + 8ull * j);
+    }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        // (a reciprocal of one ulp: a quotient to the last bit is ten instructions more, which the rows' bytes do not hide)
-        v[i][k] = v[i][k] * __builtin_amdgcn_rcpf(1.f + __expf(-v[i][k])) * u[i][k];
+    for (int i = 0; i < PIECES; ++i) {
+      if (!any(base, i)) continue;
+      v[i] = Eight<T>::wide(gate[i]);
+      if constexpr (SWIGLU) {
+        const f32x8 u = Eight<T>::wide(up[i]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          // (a reciprocal of one ulp: a quotient to the last bit is ten instructions more, which the rows' bytes do not hide)
+          v[i][k] = v[i][k] * __builtin_amdgcn_rcpf(1.f + __expf(-v[i][k])) * u[k];
+        }
       }
     }
   }
-}
+};
 
-// LANES threads to a row; up to 32 * LANES elements stay in registers between the search for the largest value and the
+// LANES threads to a row; up to 8 * PIECES * LANES elements stay in registers between the search for the largest value and the
 // conversion, longer rows are read twice.
-template <class T, bool SWIGLU, int LANES, bool STREAM>
+template <class T, bool SWIGLU, int LANES, int PIECES, bool NT>
 __device__ __forceinline__ void quantize_one(const QuantizeDev &a, uint32_t e, uint32_t r, uint32_t g) {
-  constexpr int NS = 2;
-  const PPLX_GLOBAL T *row =
-      as_global(reinterpret_cast<const T *>(a.x + (int64_t)e * a.x_stride_expert + (int64_t)r * a.x_stride_row));
-  const uint32_t groups = a.width / 16;
-  const bool held = groups <= LANES * NS;
-  f32x8 v[2 * NS];
+  constexpr uint32_t kStep = LANES * PIECES;
+  Piece<T, SWIGLU, LANES, PIECES, NT> p;
+  p.row = as_global(reinterpret_cast<const T *>(a.x + (int64_t)e * a.x_stride_expert + (int64_t)r * a.x_stride_row));
+  p.width = a.width;
+  p.groups = a.width / 8;
+  p.g = g;
+  p.first_of_wave = LANES == 64 ? 0 : wave_id() * 64;
   uint32_t bits = 0;
-  for (uint32_t base = 0; base < groups; base += LANES * NS) {
+  for (uint32_t base = 0; base < p.groups; base += kStep) {
+    p.load(base);
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
-      uint32_t j = base + i * LANES + g;
-      j = j < groups ? j : groups - 1;
-      load_values<T, SWIGLU>(row, a.width, j, v + 2 * i);
-    }
-#pragma unroll
-    for (int i = 0; i < 2 * NS; ++i) {
-      const uint32_t b = magnitude_bits(v[i]);
+    for (int i = 0; i < PIECES; ++i) {
+      if (!p.any(base, i)) continue;
+      const uint32_t b = magnitude_bits(p.v[i]);
       bits = bits > b ? bits : b;
     }
   }
   const RowScale s = row_scale(row_max<LANES>(bits));
   if (g == 0) as_global(a.scale)[(int64_t)e * a.scale_stride_expert + (int64_t)r * a.scale_stride_row] = s.scale;
-  PPLX_GLOBAL u32x4 *out =
-      as_global(reinterpret_cast<u32x4 *>(a.out + (int64_t)e * a.out_stride_expert + (int64_t)r * a.out_stride_row));
-  for (uint32_t base = 0; base < groups; base += LANES * NS) {
+  PPLX_GLOBAL u32x2 *out =
+      as_global(reinterpret_cast<u32x2 *>(a.out + (int64_t)e * a.out_stride_expert + (int64_t)r * a.out_stride_row));
+  for (uint32_t base = 0; base < p.groups; base += kStep) {
+    if (p.groups > kStep) p.load(base);
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
+    for (int i = 0; i < PIECES; ++i) {
+      if (!p.any(base, i)) continue;
       const uint32_t j = base + i * LANES + g;
-      if (!held) load_values<T, SWIGLU>(row, a.width, j < groups ? j : groups - 1, v + 2 * i);
-      if (j < groups) {
-        const u32x4 q = quantize_sixteen(v[2 * i], v[2 * i + 1], s.inverse);
-        if constexpr (STREAM) __builtin_nontemporal_store(q, out + j);
-        else out[j] = q;
-      }
+      if (j < p.groups) out[j] = quantize_eight(p.v[i], s.inverse);
     }
   }
 }
 
 // Rows of one buffer: as many as are there, 256 / LANES to a workgroup.
-template <class T, bool SWIGLU, int LANES, bool STREAM>
+template <class T, bool SWIGLU, int LANES, int PIECES, bool NT>
 __global__ __launch_bounds__(256) void quantize_flat(QuantizeDev a) {
   uint32_t there = a.rows.rows;
   if (a.rows.layout == PPLX_A2A_ROWS_SORTED) {
@@ -90,12 +97,12 @@ __global__ __launch_bounds__(256) void quantize_flat(QuantizeDev a) {
     there = last < 0 ? 0 : (uint32_t)last < there ? (uint32_t)last : there;
   }
   const uint32_t r = LANES == 64 ? blockIdx.x * 4 + wave_id() : blockIdx.x;
-  if (r < there) quantize_one<T, SWIGLU, LANES, STREAM>(a, 0, r, threadIdx.x % LANES);
+  if (r < there) quantize_one<T, SWIGLU, LANES, PIECES, NT>(a, 0, r, threadIdx.x % LANES);
 }
 
 // Rows of the experts' buffers: workgroups share out the rows that are there, whose experts they find in the sums of the
 // counts.
-template <class T, bool SWIGLU, int LANES>
+template <class T, bool SWIGLU, int LANES, int PIECES>
 __global__ __launch_bounds__(256) void quantize_padded(QuantizeDev a) {
   extern __shared__ uint32_t upto[];  // rows of the experts up to and with each
   __shared__ uint32_t of_wave[4];
@@ -125,22 +132,26 @@ __global__ __launch_bounds__(256) void quantize_padded(QuantizeDev a) {
       else lo = mid + 1;
     }
     const uint32_t e = __builtin_amdgcn_readfirstlane(lo);
-    quantize_one<T, SWIGLU, LANES, false>(a, e, r - (e ? upto[e - 1] : 0u), threadIdx.x % LANES);
+    quantize_one<T, SWIGLU, LANES, PIECES, false>(a, e, r - (e ? upto[e - 1] : 0u), threadIdx.x % LANES);
   }
 }
 
-template <class T, bool SWIGLU, int LANES> int launch_quantize(const QuantizeDev &a, hipStream_t s) {
+template <class T, bool SWIGLU, int LANES, int PIECES> int launch_quantize(const QuantizeDev &a, hipStream_t s) {
   constexpr uint32_t kAtOnce = 256 / LANES;
   if (a.rows.layout == PPLX_A2A_ROWS_PADDED) {
     const uint64_t groups = ((uint64_t)a.rows.rows * a.rows.experts + kAtOnce - 1) / kAtOnce;
     const uint32_t grid = groups < 2048 ? (uint32_t)groups : 2048;  // eight workgroups to a compute unit
-    PPLX_LAUNCH(launch_kernel(quantize_padded<T, SWIGLU, LANES>, dim3(grid), dim3(256), 4 * a.rows.experts, s, a));
+    PPLX_LAUNCH(launch_kernel(quantize_padded<T, SWIGLU, LANES, PIECES>, dim3(grid), dim3(256), 4 * a.rows.experts, s, a));
   } else {
-    // Rows that are more than a share of the last-level cache are stored past it.  us, plain / so: 49152 activated rows of 1408
-    // (277 MB read) 71.6 / 61.8, 16384 of 2048 34.9 / 31.8, 32768 plain ones of 7168 126.3 / 121.9; 2000 of 1408 5.2 / 5.1: there
-    // they stay for the product.  Large ones run at 5.3-5.8 TB/s.
-    const bool large = (uint64_t)a.rows.rows * a.width * sizeof(T) * (SWIGLU ? 2 : 1) > kStreamBytes;
-    auto kernel = large ? quantize_flat<T, SWIGLU, LANES, true> : quantize_flat<T, SWIGLU, LANES, false>;
+    // Bound by its bytes: 49152 activated rows of 1408 (277 MB read, 69 MB written) take 62.6 us, 5.5 TB/s, 8192 of 14336 102.6, 5.7
+    // TB/s, and 32768 plain ones of 7168 120, 5.9 TB/s.  (Pieces of sixteen elements instead of eight leave lanes idle, and
+    // arithmetic then binds the activated ones: 74.7 us, 4.6 TB/s.)
+    // Rows that would fill the last-level cache are read past it, unless they are read twice, so that the result is in it for
+    // whoever reads it next.  us with a read of the result behind it, plain / so: 49152 rows of 1408 231.9 / 226.2; 16384 of 2048
+    // (134 MB) with their product 95.4 / 97.7.  Storing the result past the cache is faster alone and slower with its reader
+    // (253.5).
+    const bool large = (uint64_t)a.rows.rows * a.width * sizeof(T) * (SWIGLU ? 2 : 1) > kStreamBytes && a.width <= 8 * PIECES * LANES;
+    auto kernel = large ? quantize_flat<T, SWIGLU, LANES, PIECES, true> : quantize_flat<T, SWIGLU, LANES, PIECES, false>;
     PPLX_LAUNCH(launch_kernel(kernel, dim3((a.rows.rows + kAtOnce - 1) / kAtOnce), dim3(256), 0, s, a));
   }
   return PPLX_A2A_OK;
@@ -180,8 +191,12 @@ extern "C" int pplx_a2a_quantize_rows(int device, const pplx_a2a_quantize_args_t
     return with_type(p.dtype, [&](auto tag) {
       typedef typename decltype(tag)::type T;
       hipStream_t s = (hipStream_t)stream;
-      if (a.width <= 2048) return p.swiglu ? launch_quantize<T, true, 64>(a, s) : launch_quantize<T, false, 64>(a, s);
-      return p.swiglu ? launch_quantize<T, true, 256>(a, s) : launch_quantize<T, false, 256>(a, s);
+      // A wave to a row, whose largest value needs no barrier, where four pieces a thread hold the row; us, 64 threads / 256:
+      // 32768 plain rows of 512 11.2 / 29.3, of 2048 37.2 / 44.0, activated 54.4 / 63.1; with eight pieces in one wave rows of 4096
+      // 115 / 111, 2000 of them 11.7 / 9.2.  Eight pieces a thread hold rows of up to 16384.
+      if (a.width <= 2048) return p.swiglu ? launch_quantize<T, true, 64, 4>(a, s) : launch_quantize<T, false, 64, 4>(a, s);
+      if (a.width <= 8192) return p.swiglu ? launch_quantize<T, true, 256, 4>(a, s) : launch_quantize<T, false, 256, 4>(a, s);
+      return p.swiglu ? launch_quantize<T, true, 256, 8>(a, s) : launch_quantize<T, false, 256, 8>(a, s);
     });
   });
 }

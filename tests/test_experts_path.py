@@ -271,6 +271,18 @@ def test_the_same_inputs_give_the_same_bits(device):
 
 
 @gpu
+@pytest.mark.parametrize("rows,width", [(12800, 2032), (3500, 14352), (3000, 17008)])
+def test_large_rows_are_quantised_as_small_ones(device, rows, width):
+    """More than the last-level cache may hold: read another way, with the same results."""
+    x = torch.empty(rows, 2 * width, dtype=torch.float32, device=device).normal_(generator=torch.Generator(device).manual_seed(9))
+    q, scale = quantize_rows(x, swiglu=True)
+    for r in range(0, rows, 1000):
+        part, part_scale = quantize_rows(x[r : r + 1000], swiglu=True)
+        assert torch.equal(q[r : r + 1000], part) and torch.equal(scale[r : r + 1000], part_scale)
+    check_quantized(q[:20], scale[:20], *swiglu64(x[:20].cpu()))
+
+
+@gpu
 def test_traced_calls(device):
     """Under torch.compile the calls are the registered ops; gradients flow through them."""
     gen = torch.Generator().manual_seed(9)
