@@ -9,6 +9,8 @@
 // tile is a line of 16-byte chunks, whose places are exchanged from row to row so that the lanes of a fragment, which read one
 // chunk each of consecutive rows, read all banks.  How many rows each expert has is known on the
 // device only: every workgroup sums the experts' blocks of rows and takes tiles from the list that follows from them.
+#include <cmath>
+
 #include "a2a_experts.h"
 
 namespace pplx_amd {
@@ -29,6 +31,7 @@ struct MatmulDev {
   const float *weight_scale;
   uint32_t n, k;
   uint32_t n_blocks;
+  uint32_t large_weights;  // more than the last-level cache is likely to hold until they are read again
   uint32_t vector_stores;  // the rows of out are 16-byte aligned, and multiples of that
 };
 
@@ -55,6 +58,28 @@ __device__ __forceinline__ void load_to_lds(const int8_t *base, uint32_t offset,
       "s_mov_b64 exec, -1"
       ::"v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds)), "s"(__builtin_amdgcn_readfirstlane(lanes))
       : "memory");
+}
+
+// The same, past the caches if `past`.  (The branch stands in the asm: one of the compiler's, between the matrix instructions,
+// costs registers.)
+__device__ __forceinline__ void load_past_to_lds(const int8_t *base, uint32_t offset, uint32_t lds, uint32_t lanes, uint32_t past) {
+  asm volatile(
+      "s_mov_b32 m0, %2\n\t"
+      "s_cmp_eq_u32 %4, 0\n\t"
+      "s_mov_b32 exec_lo, %3\n\t"
+      "s_mov_b32 exec_hi, %3\n\t"
+      "s_cbranch_scc1 .Lkept%=\n\t"
+      "s_nop 1\n\t"
+      "global_load_lds_dwordx4 %0, %1 nt\n\t"
+      "s_branch .Lloaded%=\n"
+      ".Lkept%=:\n\t"
+      "s_nop 1\n\t"
+      "global_load_lds_dwordx4 %0, %1\n"
+      ".Lloaded%=:\n\t"
+      "s_mov_b64 exec, -1"
+      ::"v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds)), "s"(__builtin_amdgcn_readfirstlane(lanes)),
+        "s"(__builtin_amdgcn_readfirstlane(past))
+      : "memory", "scc");
 }
 
 // A store of the lanes in `lanes` that counts whether there are any or not.  (All lanes are active where it stands.  Its data
@@ -156,6 +181,11 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev) {
   // A wave of few products reads a step's fragments all at once: read for the next product only, each waits for LDS.
   constexpr bool kWhole = MF * NF <= 2;
   constexpr int kSets = kWhole ? kSteps : 2;            // of fragments in registers
+  // Weights that one tile reads, and no other, go past the caches: 32 rows or fewer of each of 32 experts, 4096 x 7168, take
+  // 138 us instead of 159 (6.8 TB/s).  Not in pieces of 64 bytes, half of what a read brings: the other half, read a step later,
+  // is gone by then (64 rows each 254 us instead of 193), and not weights that the last-level cache may hold from one call to
+  // the next (32 rows of 16384 x 4096 20.8 instead of 15.2).
+  constexpr bool kLines = BK == 128;
   constexpr int kAhead = kWhole ? STAGES - 1 : STAGES;  // steps loaded in front of a tile's first
   constexpr int kStage = (BM + BN) * BK;
   extern __shared__ __align__(128) uint8_t lds[];  // [STAGES][BM rows of x, BN of the weight][BK], scales, sums of blocks
@@ -173,7 +203,9 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev) {
     const auto *a = arguments();
     const RowsDev rows{a->rows.starts_or_counts, a->rows.rows, a->rows.experts, a->rows.layout};
     sum_blocks<kThreads, BM>(rows, upto, of_wave);
-    tiles = __builtin_amdgcn_readfirstlane(upto[rows.experts - 1] * a->n_blocks);
+    // (offsets that do not ascend give a list of any length, of which only tiles that exist are taken)
+    const uint32_t listed = upto[rows.experts - 1] * a->n_blocks;
+    tiles = __builtin_amdgcn_readfirstlane(listed < 1u << 31 ? listed : 1u << 31);
   }
   const uint32_t lane = lane_id(), wave = wave_id();
   const uint32_t wm = wave % WM, wn = wave / WM;
@@ -193,6 +225,7 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev) {
 
   // The tile whose steps are loaded: where its operands begin, and what the lane's loads add to that.
   const int8_t *x = nullptr, *weight = nullptr;
+  uint32_t once = 0;  // no other tile reads this one's part of the weight
   uint32_t offset[kLoads];
   float scale[kScales];  // of row threadIdx.x, threadIdx.x + kThreads .. of the tile, its columns behind its rows
   // Load number i of a step.  Behind k a lane fetches the first chunk of its line; what it brings is taken for zeros.  Loads of
@@ -201,14 +234,17 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev) {
     const uint32_t first = (i * kWaves + wave) * kRowsPerLoad;
     const int8_t *base = (first < BM ? x : weight) + step * BK;
     const bool behind = TAIL && step * BK + load_chunk * 16 >= depth;
-    load_to_lds(base, behind ? offset[i] - load_chunk * 16 : offset[i], lds0 + stage * kStage + first * BK,
-                step < steps ? ~0u : 0u);
+    const uint32_t at = behind ? offset[i] - load_chunk * 16 : offset[i], place = lds0 + stage * kStage + first * BK;
+    const uint32_t lanes = step < steps ? ~0u : 0u;
+    if (kLines && i * kWaves * kRowsPerLoad >= BM) load_past_to_lds(base, at, place, lanes, once);
+    else load_to_lds(base, at, place, lanes);
   };
   auto begin = [&](const Tile &t) __attribute__((always_inline)) {
     const auto *a = arguments();
     x = a->x + (int64_t)t.e * a->x_stride_expert + (int64_t)(t.begin + t.m0) * a->x_stride_row;
     weight = a->weight + ((uint64_t)t.e * a->n + t.n0) * depth;
     const uint32_t rows_left = t.count - t.m0, columns_left = a->n - t.n0;
+    once = a->large_weights && t.count <= BM;
 #pragma unroll
     for (int i = 0; i < kScales; ++i) {
       const uint32_t p = threadIdx.x + i * kThreads;
@@ -254,7 +290,7 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev) {
     const uint32_t n_blocks = a->n_blocks;
     for (; id < tiles; id += gridDim.x) {
       t = tile_of<BM, BN>(rows, n_blocks, upto, id);
-      if (t.m0 < t.count) break;  // (offsets that descend make a list that is too long)
+      if (t.m0 < t.count && t.n0 < a->n) break;
     }
     return id < tiles;
   };
@@ -406,7 +442,7 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev) {
   }
 }
 
-// Of a compute unit's LDS the tiles use the first 128 KiB: what lies behind has not been loaded to without registers.
+// The steps in flight take 128 KiB of a compute unit's LDS, the tables of the experts lie behind them.
 constexpr uint32_t kComputeUnits = 256, kLdsBytes = 128 * 1024;
 
 template <int BM, int BN, int WM, int WN, int BK, int STAGES, class O>
@@ -453,7 +489,7 @@ template <int RF, int CF, int AHEAD, class O> __global__ __launch_bounds__(kSpli
     sum_blocks<kSplitWaves * 64, kRows>(a.rows, upto, of_wave);
     if (blockIdx.x >= upto[a.rows.experts - 1] * a.n_blocks) return;
     t = tile_of<kRows, kColumns>(a.rows, a.n_blocks, upto, blockIdx.x);
-    if (t.m0 >= t.count) return;  // (offsets that descend make a list that is too long)
+    if (t.m0 >= t.count || t.n0 >= a.n) return;  // (offsets that do not ascend)
   }
   const int8_t *x_first = a.x + (int64_t)t.e * a.x_stride_expert + (int64_t)(t.begin + t.m0) * a.x_stride_row;
   const int8_t *w_first = a.weight + ((uint64_t)t.e * a.n + t.n0) * a.k;
@@ -546,44 +582,51 @@ template <int RF, int CF, int AHEAD, class O> int launch_split(const MatmulDev &
 }
 
 // What a form costs, in microseconds, from the number of workgroups that its blocks make: `start` once, and for every round
-// of the compute units `per_line` for each 128 bytes of k and `per_tile`.  (The loads of a workgroup's steps go to LDS
-// at some 32 bytes a cycle, which is what the lines of the tiles cost.)  Fitted to products of 1 to 49152 rows with 1 to 64
-// experts, k of 496 to 8192 and n of 300 to 16384, for which the form with the least estimate is within
-// 10 % of the fastest (in buffers of the experts, of whose rows the device knows, within a third).
-// Measured, us, with the tiles of 32 x 128 / 64 x 128 / 128 x 128 / 128 x 256 / 256 x 256:
-//   4096 x 4096, one weight   128 rows 13.4 / 14.5 / 19.8 / 28.5 / 40.6    512  21.7 / 16.8 / 20.8 / 28.8 / 43.1
-//                             1024  39.6 / 29.9 / 25.2 / 30.8 / 43.6       2048 74 / 56 / 47.7 / 43.0 / 48.7     4096 142 / 111 / 91 / 83 / 69
-//   2816 x 2048, 64 experts   4096 rows 108 / 103 / 96 / 92 / 111          16384 286 / 248 / 193 / 178 / 184     49152 775 / 650 / 473 / 445 / 378
+// of the compute units `per_line` for each 128 bytes of k and `per_tile`, or what the weights take at `rate` megabytes a
+// microsecond.  (The loads of a workgroup's steps go to LDS at some 32 bytes a cycle, which is what the lines of the tiles
+// cost.)  Fitted to 3670 products of 1 to 32768 rows with 1 to 64
+// experts, even and skewed, k of 256 to 16384 and n of 100 to 16384, each run in every form.  The form with the least estimate is
+// on average 2 % slower than the fastest with one weight, 4 % with sorted rows, and 11 % in buffers of the experts: how their
+// rows spread is known on the device only.  Without any one of the forms the fastest is 1 to 4 % slower, at worst 1.3 to 1.6 times.
+// Measured, us, with the tiles of 32 x 128 / 64 x 128 / 64 x 256 / 128 x 128 / 128 x 256 / 256 x 256:
+//   2816 x 2048, 64 experts   2048 rows 84 / 76 / 72 / 86 / 84 / 107      16384 278 / 250 / 204 / 184 / 175 / 170
+//   4096 x 7168, 32 experts   512 rows 142 / 148 / 144 / 185 / 176 / 205  1500  214 / 165 / 153 / 199 / 187 / 211
+//                             3000 309 / 262 / 218 / 215 / 200 / 227      6000  510 / 409 / 331 / 342 / 318 / 252
+//   131072 x 4096, one weight 32 rows 112 / 116 / 122 / 120 / 132 / 139   128   209 / 164 / 151 / 139 / 141 / 149
 // and, for few rows, split 16 x 16 / split 16 x 32 / split 32 x 32 / tiles of 32 x 128:
 //   4096 x 4096   1 row 5.6 / 7.0 / 7.5 / 13.0     16 rows 7.0 / 8.5 / 9.1 / 13.2     64 rows 18.3 / 13.8 / 10.6 / 13.0
 //   16384 x 4096  8 rows 16.6 / 14.4 / 15.9 / 13.5     2048 x 7168  8 rows 8.2 / 11.1 / 11.7 / 20.0
 struct MatmulForm {
   uint32_t bm, bn;
-  double start, per_line, per_tile;
+  double start, per_line, per_tile, rate;
 };
+constexpr int kSplitForms = 3;
 constexpr MatmulForm kForms[] = {
-    {16, 16, 3.0, 0.105, 0.0}, {16, 32, 3.0, 0.17, 0.0},  {32, 32, 3.0, 0.26, 0.0},  // split
-    {32, 128, 1.5, 0.29, 2.2}, {64, 128, 1.5, 0.42, 3.0}, {128, 128, 1.5, 0.69, 3.5}, {128, 256, 1.5, 1.25, 5.0},
-    {256, 256, 1.5, 2.05, 7.0},
+    {16, 16, 1.3, 0.10, 1.25, 5.0},  {16, 32, 1.1, 0.14, 1.77, 6.2},  {32, 32, 0.9, 0.16, 2.30, 4.5},  // split
+    {32, 128, 4.4, 0.29, 0.78, 6.5}, {64, 128, 1.5, 0.34, 4.16, 6.0}, {128, 128, 5.2, 0.70, 1.07, 4.2},
+    {128, 256, 0.1, 0.95, 7.01, 3.0}, {256, 256, 0.7, 1.38, 9.15, 2.8}, {64, 256, 5.7, 0.56, 3.35, 5.3},
 };
 
 int matmul_form(const MatmulDev &a) {
   const double E = a.rows.experts;
-  // Of an expert's buffer an eighth is taken to be there: how much it is only the device knows.
-  const double rows = a.rows.layout == PPLX_A2A_ROWS_PADDED ? E * ((a.rows.rows + 7) / 8) : a.rows.rows;
+  // Of the experts' buffers an eighth is taken to be there.
+  double rows = a.rows.rows;
+  if (a.rows.layout == PPLX_A2A_ROWS_PADDED) rows = rows * E < 8 ? 1 : rows * E / 8;
   const double with_rows = rows < E ? rows : E, lines = (a.k + 127) / 128;
   int best = 0;
   double least = 0;
   for (int f = 0; f < (int)(sizeof(kForms) / sizeof(kForms[0])); ++f) {
     const MatmulForm &form = kForms[f];
-    // (the last block of an expert is half full, and each that has rows has one)
-    double blocks = E == 1 ? (double)((a.rows.rows + form.bm - 1) / form.bm) : rows / form.bm + 0.5 * with_rows;
-    if (blocks < with_rows) blocks = with_rows;
-    const double tiles = blocks * ((a.n + form.bn - 1) / form.bn);
-    double rounds = tiles / kComputeUnits;
-    if (form.per_tile != 0.0) rounds = (double)(uint64_t)(rounds + 0.999);  // (small workgroups share the units)
-    else if (rounds < 1) rounds = 1;
-    const double cost = form.start + rounds * (lines * form.per_line + form.per_tile);
+    // (between experts of even sizes, and sizes that spread as an exponential does)
+    const double blocks = a.rows.layout == PPLX_A2A_ROWS_DENSE ? (double)((a.rows.rows + form.bm - 1) / form.bm)
+                                                               : with_rows / -std::expm1(-0.75 * form.bm * with_rows / rows);
+    double rounds = blocks * ((a.n + form.bn - 1) / form.bn) / kComputeUnits;
+    if (rounds < 1) rounds = 1;
+    // (small workgroups share the units; the last round of tiles is a whole one, of which a guess at their number makes a quarter)
+    if (f >= kSplitForms) rounds += (std::ceil(rounds) - rounds) * (a.rows.layout == PPLX_A2A_ROWS_DENSE ? 1.0 : 0.25);
+    const double work = rounds * (lines * form.per_line + form.per_tile);
+    const double weights = with_rows * a.n * a.k / (1e6 * form.rate);
+    const double cost = form.start + (work < weights ? weights : work);
     if (f == 0 || cost < least) {
       best = f;
       least = cost;
@@ -607,7 +650,8 @@ template <class O> int launch_matmul(const MatmulDev &a, hipStream_t s) {
     case 4: return launch_tiles<64, 128, 1, 4, 128, 3, O>(a, most_blocks(64), s);
     case 5: return launch_tiles<128, 128, 2, 2, 64, 4, O>(a, most_blocks(128), s);
     case 6: return launch_tiles<128, 256, 2, 4, 64, 4, O>(a, most_blocks(128), s);
-    default: return launch_tiles<256, 256, 2, 4, 64, 4, O>(a, most_blocks(256), s);
+    case 7: return launch_tiles<256, 256, 2, 4, 64, 4, O>(a, most_blocks(256), s);
+    default: return launch_tiles<64, 256, 1, 4, 128, 3, O>(a, most_blocks(64), s);
   }
 }
 
@@ -647,6 +691,7 @@ extern "C" int pplx_a2a_int8_matmul(int device, const pplx_a2a_int8_matmul_args_
   a.weight_scale = p.weight_scale;
   a.n = (uint32_t)p.n;
   a.k = (uint32_t)p.k;
+  a.large_weights = (uint64_t)a.rows.experts * p.n * p.k > (96ull << 20);
   const int64_t vec = 16 / dtype_bytes(p.out_dtype);
   a.vector_stores = is_aligned(p.out, 16) && p.n % vec == 0 && p.out_stride_row % vec == 0 && p.out_stride_expert % vec == 0;
   return guarded(device, [&] {

@@ -282,6 +282,71 @@ def test_large_rows_are_quantised_as_small_ones(device, rows, width):
     check_quantized(q[:20], scale[:20], *swiglu64(x[:20].cpu()))
 
 
+def product64(x, xs, w, ws):
+    sums = x.double() @ w.double().t()  # (whole numbers below 2^53)
+    return sums * xs.double()[:, None] * ws.double()
+
+
+def random_int8(shape, gen, device):
+    return torch.randint(-128, 128, shape, generator=gen, dtype=torch.int8, device=device)
+
+
+def assert_product(got, ref):
+    # as in check_product, on the device
+    bound = ref.abs() * ((torch.finfo(got.dtype).eps / 2 if got.dtype != F32 else 0) * (1 + 3 * U32) + 3 * U32) + 2.0**-130
+    assert bool(((got.double() - ref).abs() <= bound).all())
+
+
+@gpu
+@pytest.mark.parametrize("out_dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,n,k", [
+    (700, 136, 272), (1025, 136, 272), (401, 1160, 256), (401, 1159, 272), (5000, 136, 256), (4999, 133, 272),
+    (2049, 1000, 128), (2049, 1000, 272), (400, 8200, 128), (397, 8193, 272), (3000, 4104, 128), (2049, 4101, 272),
+    (400, 8200, 1024), (399, 8199, 528),
+])  # fmt: skip
+def test_products_of_every_tile(device, rows, n, k, out_dtype):
+    """Sizes for which each form of the product is chosen, with k that fills its steps and k that does not."""
+    gen = torch.Generator(device).manual_seed(rows)
+    x, w = random_int8((rows, k), gen, device), random_int8((n, k), gen, device)
+    xs, ws = (torch.rand(size, generator=gen, device=device) * 1e-2 for size in (rows, n))
+    out = torch.full((rows + 3, n), 7.0, dtype=out_dtype, device=device)
+    int8_matmul(x, xs, w, ws, out=out[:rows])
+    assert_product(out[:rows], product64(x, xs, w, ws))
+    assert (out[rows:] == 7).all()
+
+
+@gpu
+@pytest.mark.parametrize("k", [2064, 2176])
+@pytest.mark.parametrize("counts", [
+    [3] * 10 + [0] * 14, [0] * 5 + [1, 400, 0, 33] + [20] * 15, [65, 64, 1, 900, 0, 0] + [30] * 18, [100] * 24,
+])  # fmt: skip
+def test_products_of_weights_beyond_the_caches(device, counts, k):
+    """Weights that some experts' rows read once, past the caches, and others' several times."""
+    experts, n, total = len(counts), 2056, sum(counts)
+    gen = torch.Generator(device).manual_seed(total)
+    w, ws = random_int8((experts, n, k), gen, device), torch.rand(experts, n, generator=gen, device=device)
+    x, xs = random_int8((total, k), gen, device), torch.rand(total, generator=gen, device=device)
+    starts = [0, *torch.tensor(counts).cumsum(0).tolist()]
+    got = int8_matmul(x, xs, w, ws, offsets=torch.tensor(starts, dtype=torch.int32, device=device), out_dtype=F32)
+    for e, c in enumerate(counts):
+        rows = slice(starts[e], starts[e] + c)
+        assert_product(got[rows], product64(x[rows], xs[rows], w[e], ws[e]))
+
+
+@gpu
+def test_offsets_that_do_not_ascend(device):
+    """What belongs to two experts is one's or the other's; everything else is as it should be."""
+    gen = torch.Generator(device).manual_seed(3)
+    for rows, n, k in ((30, 264, 512), (3000, 2056, 1024)):
+        a, b = rows // 3, 2 * rows // 3
+        starts = torch.tensor([0, b, a, rows + 5, rows, -3], dtype=torch.int32, device=device)  # [0, b), none, [a, rows), none, none
+        x, xs = random_int8((rows, k), gen, device), torch.ones(rows, device=device)
+        w, ws = random_int8((5, n, k), gen, device), torch.ones(5, n, device=device)
+        got = int8_matmul(x, xs, w, ws, offsets=starts, out_dtype=F32)
+        assert_product(got[:a], product64(x[:a], xs[:a], w[0], ws[0]))
+        assert_product(got[b:], product64(x[b:], xs[b:], w[2], ws[2]))
+
+
 @gpu
 def test_traced_calls(device):
     """Under torch.compile the calls are the registered ops; gradients flow through them."""
