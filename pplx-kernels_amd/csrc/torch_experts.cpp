@@ -148,6 +148,11 @@ void check_slots(const at::Tensor &slots, const at::Tensor *weights, const at::T
   TORCH_CHECK(weights->sizes() == slots.sizes(), "weights must have the shape of slots");
 }
 
+void check_offsets(const at::Tensor &offsets, const at::Tensor &with) {
+  check_dense(offsets, at::kInt, 1, with, "offsets");
+  TORCH_CHECK(offsets.numel() >= 1, "offsets must not be empty");
+}
+
 void unsort_tokens(const at::Tensor &out, const at::Tensor &y, const at::Tensor &slots, const at::Tensor *weights) {
   TORCH_CHECK(y.is_cuda(), "Tensor y must be on GPU");
   TORCH_CHECK(y.dim() == 2, "Tensor y must be 2 dimensional");
@@ -192,8 +197,7 @@ void unsort_tokens_backward(const at::Tensor *grad_y, const at::Tensor *grad_wei
   check_rows_of(grad_out, "grad_out");
   const int64_t m = grad_out.sizes()[0];
   check_slots(slots, weights, y, m);
-  check_dense(offsets, at::kInt, 1, y, "offsets");
-  TORCH_CHECK(offsets.numel() >= 1, "offsets must not be empty");
+  check_offsets(offsets, y);
   TORCH_CHECK(m <= UINT32_MAX, "pplx_kernels: unsupported: 2^32 tokens or more");
   if (grad_y) {
     check_on(*grad_y, y, "grad_y");
@@ -385,6 +389,11 @@ at::Tensor fresh(at::IntArrayRef sizes, const at::Tensor &with, at::ScalarType t
   return at::empty(sizes, at::TensorOptions(with.device()).dtype(type));
 }
 
+// The same of sizes that a trace may not know.
+at::Tensor fresh_traced(c10::SymIntArrayRef sizes, const at::Tensor &with, at::ScalarType type) {
+  return at::empty_symint(sizes, at::TensorOptions(with.device()).dtype(type));
+}
+
 struct Sorted {
   at::Tensor rows, scale, slots, offsets, workspace;
 };
@@ -421,19 +430,27 @@ SortedTuple sorted_tokens_op(const at::Tensor &x, const at::Tensor &indices, int
   return as_tuple(sort_new(x, indices, experts, opt(bound_m), int8));
 }
 SortedTuple sorted_tokens_meta(const at::Tensor &x, const at::Tensor &indices, int64_t experts, opt_tensor, bool int8) {
-  return as_tuple(new_sorted(x, indices, experts, int8));
+  TORCH_CHECK(x.dim() == 2, "Tensor x must be 2 dimensional");
+  TORCH_CHECK(indices.dim() == 2, "Tensor indices must be 2 dimensional");
+  const c10::SymInt m = indices.sym_size(0), k = indices.sym_size(1);
+  return {fresh_traced({m * k, x.sym_size(1)}, x, int8 ? at::kChar : x.scalar_type()),
+          fresh_traced({int8 ? m * k : c10::SymInt(0)}, x, at::kFloat), fresh_traced({m, k}, x, at::kInt),
+          fresh({experts + 1}, x, at::kInt)};
 }
 
 at::Tensor unsorted_tokens_meta(const at::Tensor &y, const at::Tensor &slots, const at::Tensor &, opt_tensor,
                                 std::optional<at::ScalarType> out_dtype) {
   TORCH_CHECK(y.dim() == 2, "Tensor y must be 2 dimensional");
   TORCH_CHECK(slots.dim() == 2, "Tensor slots must be 2 dimensional");
-  return fresh({slots.sizes()[0], y.sizes()[1]}, y, out_dtype.value_or(y.scalar_type()));
+  return fresh_traced({slots.sym_size(0), y.sym_size(1)}, y, out_dtype.value_or(y.scalar_type()));
 }
 at::Tensor unsorted_tokens_op(const at::Tensor &y, const at::Tensor &slots, const at::Tensor &offsets, opt_tensor weights,
                               std::optional<at::ScalarType> out_dtype) {
   TORCH_CHECK(y.is_cuda(), "Tensor y must be on GPU");
-  at::Tensor out = unsorted_tokens_meta(y, slots, offsets, weights, out_dtype);
+  TORCH_CHECK(y.dim() == 2, "Tensor y must be 2 dimensional");
+  TORCH_CHECK(slots.dim() == 2, "Tensor slots must be 2 dimensional");
+  check_offsets(offsets, y);  // (the gradient reads them)
+  at::Tensor out = fresh({slots.sizes()[0], y.sizes()[1]}, y, out_dtype.value_or(y.scalar_type()));
   unsort_tokens(out, y, slots, opt(weights));
   return out;
 }
@@ -443,12 +460,13 @@ template <class Fn> auto op_handle(const char *name) {
   return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Fn>();
 }
 
-// Gradients come in any layout (that of a sum is one element, expanded).  Those of a traced step have no address yet.
+// Gradients come in any layout (that of a sum is one element, expanded).  Those of a traced step have no address, and sizes
+// that may not be known.
 at::Tensor as_rows(const at::Tensor &g) {
+  if (g.is_meta() || g.key_set().has(c10::DispatchKey::Python) || g.key_set().has(c10::DispatchKey::Functionalize)) return g.contiguous();
   const int64_t bytes = (int64_t)g.element_size();
-  const bool traced = g.is_meta() || g.key_set().has(c10::DispatchKey::Python) || g.key_set().has(c10::DispatchKey::Functionalize);
-  const bool aligned = traced ? g.storage_offset() * bytes % 16 == 0 : reinterpret_cast<uintptr_t>(g.data_ptr()) % 16 == 0;
-  const bool fits = g.strides()[1] == 1 && g.strides()[0] * bytes % 16 == 0 && aligned;
+  const bool fits =
+      g.strides()[1] == 1 && g.strides()[0] * bytes % 16 == 0 && reinterpret_cast<uintptr_t>(g.data_ptr()) % 16 == 0;
   return fits ? g : g.clone(at::MemoryFormat::Contiguous);
 }
 
@@ -484,6 +502,7 @@ struct SortFunction : torch::autograd::Function<SortFunction> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x,
                                                 const at::Tensor &indices, int64_t experts,
                                                 const std::optional<at::Tensor> &bound_m) {
+    TORCH_CHECK(x.dim() == 2 && x.sym_size(1) % 8 == 0, "x must have rows of a multiple of 8 elements for its gradient");
     auto [rows, scale, slots, offsets] = call_sorted_tokens(x, indices, experts, bound_m, false);
     ctx->save_for_backward({slots});
     ctx->mark_non_differentiable({scale, slots, offsets});
@@ -499,7 +518,7 @@ struct SortFunction : torch::autograd::Function<SortFunction> {
       static auto op = op_handle<void(at::Tensor &, const at::Tensor &, const at::Tensor &, opt_tensor)>(
           "pplx_kernels::unsort_tokens");
       const at::Tensor g = as_rows(grads[0]);
-      grad_x = fresh({slots.sizes()[0], g.sizes()[1]}, g, g.scalar_type());
+      grad_x = fresh_traced({slots.sym_size(0), g.sym_size(1)}, g, g.scalar_type());
       op.call(grad_x, g, slots, std::nullopt);
     }
     return differentiable_once({grad_x, at::Tensor(), at::Tensor(), at::Tensor()});
@@ -526,10 +545,14 @@ struct UnsortFunction : torch::autograd::Function<UnsortFunction> {
       at::NoGradGuard plain;
       static auto op = op_handle<void(opt_tensor, opt_tensor, const at::Tensor &, const at::Tensor &, const at::Tensor &,
                                       const at::Tensor &, opt_tensor)>("pplx_kernels::unsort_tokens_backward");
-      if (ctx->needs_input_grad(0)) grad_y = fresh(y.sizes(), y, y.scalar_type());
-      if (weights.defined() && ctx->needs_input_grad(3)) grad_weights = fresh(weights.sizes(), weights, at::kFloat);
+      if (ctx->needs_input_grad(0)) grad_y = fresh_traced(y.sym_sizes(), y, y.scalar_type());
+      if (weights.defined() && ctx->needs_input_grad(3)) grad_weights = fresh_traced(weights.sym_sizes(), weights, at::kFloat);
       auto maybe = [](const at::Tensor &t) { return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt; };
-      op.call(maybe(grad_y), maybe(grad_weights), as_rows(grads[0]), y, saved[1], saved[2], maybe(weights));
+      if (saved[1].sym_size(0) == 0) {  // (without tokens)
+        if (grad_y.defined()) grad_y.zero_();
+      } else {
+        op.call(maybe(grad_y), maybe(grad_weights), as_rows(grads[0]), y, saved[1], saved[2], maybe(weights));
+      }
     }
     return differentiable_once({grad_y, at::Tensor(), at::Tensor(), grad_weights, at::Tensor()});
   }

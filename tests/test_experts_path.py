@@ -372,6 +372,69 @@ def test_traced_calls(device):
     assert torch.equal(got, want)
 
 
+@gpu
+def test_traced_calls_of_unknown_sizes(device):
+    """Traced once for any number of tokens."""
+    gen = torch.Generator().manual_seed(10)
+    k, experts, hidden, traces = 2, 4, 64, []
+
+    def backend(graph, inputs):
+        traces.append(len(inputs))
+        return torch._dynamo.lookup_backend("aot_eager")(graph, inputs)
+
+    def layer(x, weights, indices):
+        s = sort_tokens(x, indices, experts)
+        q = sort_tokens(x.detach(), indices, experts, int8=True)
+        return unsort_tokens(s.rows * 2.0, s.slots, s.offsets, weights), q.rows, q.scale
+
+    compiled = torch.compile(layer, backend=backend, fullgraph=True, dynamic=True)
+    for m in (30, 41, 7):
+        x = torch.randn(m, hidden, generator=gen).to(device).requires_grad_(True)
+        weights = torch.rand(m, k, generator=gen).to(device).requires_grad_(True)
+        indices = to_u32(make_indices(m, k, experts, gen, "mixed"), device)
+        want = layer(x, weights, indices)
+        want_grads = torch.autograd.grad(want[0].sum(), [x, weights])
+        got = compiled(x, weights, indices)
+        assert len(traces) == 1
+        got_grads = torch.autograd.grad(got[0].sum(), [x, weights])
+        assert all(torch.equal(a, b) for a, b in zip(got, want)) and all(torch.equal(a, b) for a, b in zip(got_grads, want_grads))
+
+
+@gpu
+def test_gradients_at_the_edges(device):
+    """What the gradient could not do is refused when it is recorded; without tokens it is zeros."""
+    x = torch.randn(4, 12, device=device, requires_grad=True)
+    indices = torch.zeros(4, 2, dtype=torch.int32, device=device).view(torch.uint32)
+    with pytest.raises(RuntimeError, match="multiple of 8"):
+        sort_tokens(x, indices, 3)
+    s = sort_tokens(x.detach(), indices, 3)
+    assert torch.equal(s.rows[s.slots.long()], x.detach()[:, None].expand(-1, 2, -1))
+    y = torch.randn(8, 16, device=device, requires_grad=True)
+    for offsets in (s.offsets.float(), s.offsets[None], s.offsets[:0], s.offsets.cpu()):
+        with pytest.raises(RuntimeError, match="offsets"):
+            unsort_tokens(y, s.slots, offsets)
+    none = torch.empty(0, 2, dtype=torch.int32, device=device)
+    weights = torch.empty(0, 2, device=device, requires_grad=True)
+    out = unsort_tokens(y, none, torch.zeros(4, dtype=torch.int32, device=device), weights)
+    grad_y, grad_w = torch.autograd.grad(out.sum(), [y, weights])
+    assert out.shape == (0, 16) and (grad_y == 0).all() and grad_w.shape == (0, 2)
+
+
+@gpu
+@pytest.mark.parametrize("experts", [963, 964, 1820, 1821, 5461])
+def test_sort_of_many_picks_and_experts(device, experts):
+    """The tables of the experts at the sizes where they fill a workgroup's share of the memory that it counts in."""
+    m, k = 1100, 8
+    gen = torch.Generator().manual_seed(experts)
+    x = torch.randn(m, 8, generator=gen)
+    indices = make_indices(m, k, experts, gen, "mixed")
+    s = sort_tokens(x.to(device), to_u32(indices, device), experts)
+    slots, offsets, order = ref_sort(indices, experts, m)
+    rows = torch.zeros(m * k, 8)
+    rows[: order.numel()] = x[order // k]
+    assert torch.equal(s.slots.cpu(), slots) and torch.equal(s.offsets.cpu(), offsets) and torch.equal(s.rows.cpu(), rows)
+
+
 # ---------------------------------------------------------------------------
 # The C entry points refuse before anything reaches a device
 # ---------------------------------------------------------------------------
