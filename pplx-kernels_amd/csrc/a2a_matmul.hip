@@ -32,7 +32,6 @@ struct MatmulDev {
   uint32_t n, k;
   uint32_t n_blocks;
   uint32_t large_weights;  // more than the last-level cache is likely to hold until they are read again
-  uint32_t vector_stores;  // the rows of out are 16-byte aligned, and multiples of that
 };
 
 #define PPLX_CONSTANT __attribute__((address_space(4)))
@@ -145,6 +144,18 @@ __device__ __forceinline__ Tile tile_of(const RowsDev &rows, uint32_t n_blocks, 
   t.count = __builtin_amdgcn_readfirstlane(s.count);
   return t;
 }
+
+// Four results at any address that one may have.
+template <class O> struct FourOf;
+template <> struct FourOf<float> {
+  typedef float type __attribute__((ext_vector_type(4), aligned(4)));
+};
+template <> struct FourOf<__bf16> {
+  typedef __bf16 type __attribute__((ext_vector_type(4), aligned(2)));
+};
+template <> struct FourOf<_Float16> {
+  typedef _Float16 type __attribute__((ext_vector_type(4), aligned(2)));
+};
 
 // Four columns of a row, 4 bytes or 2 each, as words.
 template <class O> __device__ __forceinline__ void pack_four(f32x4 v, uint32_t *words) {
@@ -294,10 +305,9 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev) {
     }
     return id < tiles;
   };
-  // Stores of a tile's results by a wave, where they are counted: columns are whole stores.
+  // Stores of a tile's results by a wave that are counted.
   constexpr int kStores = MF * NF * (sizeof(O) == 4 ? 4 : 2);
   constexpr int kBehind = (STAGES - 1) * kLoads + kStores <= 63 ? kStores : 0;  // as far as the counter goes
-  const bool counted = arguments()->vector_stores;
   bool stored = false;  // the stores of the tile before stand behind the loads of the first steps
   bool more = find();
   if (more) begin(t);
@@ -381,7 +391,7 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev) {
     id += gridDim.x;
     more = find();
     if (more) begin(t);
-    stored = counted;
+    stored = true;
 
     // Lane l holds row l % 32 of each fragment and, in its accumulators, columns 4 (l / 32) .. + 3 of every eight.  Of 2-byte
     // results two such groups change places between the halves of the wave, so that every lane has 16 bytes of its row.
@@ -425,15 +435,17 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev) {
             n += 4 * half;
           }
           constexpr uint32_t kVec = 16 / sizeof(O);
-          if (counted) {
-            const uint64_t lanes = __ballot(there && n < columns);
-            store_counted(out + n, u32x4{words[0], words[1], words[2], words[3]}, lanes);
-          } else if (there && n < columns) {
+          // Rows that begin anywhere take whole vectors all the same, at any address; what is left of a row goes one by one (behind
+          // stores that count, where more of them make the waits longer and not shorter).
+          const u32x4 v = {words[0], words[1], words[2], words[3]};
+          asm volatile("" : "+v"(n));  // (the masks of a column for all rows at once are more scalar registers than there are)
+          store_counted(out + n, v, __ballot(there && n + kVec <= columns));
+          if (there && n < columns && n + kVec > columns) {
             typedef O vec __attribute__((ext_vector_type(kVec)));
-            const vec v = __builtin_bit_cast(vec, u32x4{words[0], words[1], words[2], words[3]});
+            const vec one = __builtin_bit_cast(vec, v);
 #pragma unroll
-            for (uint32_t u = 0; u < kVec; ++u) {
-              if (u < columns - n) out[n + u] = v[u];
+            for (uint32_t u = 0; u + 1 < kVec; ++u) {
+              if (u < columns - n) out[n + u] = one[u];
             }
           }
         }
@@ -562,13 +574,25 @@ template <int RF, int CF, int AHEAD, class O> __global__ __launch_bounds__(kSpli
   const PPLX_GLOBAL float *ws = as_global(a.weight_scale) + (uint64_t)t.e * a.n;
   PPLX_GLOBAL O *out = as_global(reinterpret_cast<O *>(a.out)) + (int64_t)t.e * a.out_stride_expert +
                        (int64_t)(t.begin + row) * a.out_stride_row;
+  float sum[4];
 #pragma unroll
   for (uint32_t i = 0; i < 4; ++i) {
-    if (n + i >= a.n) break;
-    int32_t sum = 0;
+    int32_t whole = 0;
 #pragma unroll
-    for (int w = 0; w < kSplitWaves; ++w) sum += sums[w][(fragment * 4 + i) * 64 + lane];
-    out[n + i] = (O)((float)sum * (xs * ws[n + i]));
+    for (int w = 0; w < kSplitWaves; ++w) whole += sums[w][(fragment * 4 + i) * 64 + lane];
+    sum[i] = (float)whole * (xs * ws[n + i < a.n ? n + i : n]);
+  }
+  if (a.n - n >= 4) {
+    typedef typename FourOf<O>::type four;
+    four v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (O)sum[i];
+    *reinterpret_cast<PPLX_GLOBAL four *>(out + n) = v;
+  } else {
+#pragma unroll
+    for (uint32_t i = 0; i < 3; ++i) {
+      if (i < a.n - n) out[n + i] = (O)sum[i];
+    }
   }
 }
 
@@ -692,8 +716,6 @@ extern "C" int pplx_a2a_int8_matmul(int device, const pplx_a2a_int8_matmul_args_
   a.n = (uint32_t)p.n;
   a.k = (uint32_t)p.k;
   a.large_weights = (uint64_t)a.rows.experts * p.n * p.k > (96ull << 20);
-  const int64_t vec = 16 / dtype_bytes(p.out_dtype);
-  a.vector_stores = is_aligned(p.out, 16) && p.n % vec == 0 && p.out_stride_row % vec == 0 && p.out_stride_expert % vec == 0;
   return guarded(device, [&] {
     return with_type(p.out_dtype, [&](auto tag) { return launch_matmul<typename decltype(tag)::type>(a, (hipStream_t)stream); });
   });
