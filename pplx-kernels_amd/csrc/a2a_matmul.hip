@@ -394,58 +394,70 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev) {
     stored = true;
 
     // Lane l holds row l % 32 of each fragment and, in its accumulators, columns 4 (l / 32) .. + 3 of every eight.  Of 2-byte
-    // results two such groups change places between the halves of the wave, so that every lane has 16 bytes of its row.
+    // results two such groups change places between the halves of the wave, so that every lane has 16 bytes of its row; then two
+    // such stores change places between the quarters, so that each takes 64 bytes of sixteen rows instead of 32 of 32: 16384 x
+    // 14336 of 1024 304 to 298 us, of 14340, whose rows do not begin at lines, 344 to 323.  (Odd numbers of 2-byte results take 428.)
     const auto *a = arguments();
     const uint32_t columns = a->n;
     const int64_t out_stride = a->out_stride_row;
     PPLX_GLOBAL O *out_first = as_global(reinterpret_cast<O *>(a->out)) + (int64_t)at.e * a->out_stride_expert +
                                (int64_t)(at.begin + at.m0) * out_stride;
     const uint32_t half = lane / 32;
+    constexpr uint32_t kVec = 16 / sizeof(O);        // results of a lane in a store
+    constexpr int kGroups = sizeof(O) == 4 ? 1 : 2;  // of eight columns in a store
+    const uint32_t lane_column = kVec * (half + lane / 16 % 2 * 2);
 #pragma unroll
     for (int i = 0; i < MF; ++i) {
-      const uint32_t row = wm * kRows + i * 32 + lane % 32;
-      const float xs = scales[row];
-      const bool there = at.m0 + row < at.count;
-      PPLX_GLOBAL O *out = out_first + (int64_t)row * out_stride;
+      const float xs = scales[wm * kRows + i * 32 + lane % 32];
 #pragma unroll
       for (int j = 0; j < NF; ++j) {
-        constexpr int kGroups = sizeof(O) == 4 ? 1 : 2;  // of eight columns in a store
 #pragma unroll
-        for (int q = 0; q < 4; q += kGroups) {
-          uint32_t words[4];
+        for (int q = 0; q < 4; q += 2 * kGroups) {
+          uint32_t words[2][4];
 #pragma unroll
-          for (int g = 0; g < kGroups; ++g) {
-            const uint32_t column = wn * kColumns + j * 32 + (q + g) * 8 + 4 * half;
-            const f32x4 ws = *reinterpret_cast<const f32x4 *>(scales + BM + column);
-            f32x4 v;
+          for (int p = 0; p < 2; ++p) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) v[u] = (float)acc[j][i][4 * (q + g) + u] * (xs * ws[u]);
-            pack_four<O>(v, words + 2 * g);
+            for (int g = 0; g < kGroups; ++g) {
+              const int group = q + p * kGroups + g;
+              const f32x4 ws = *reinterpret_cast<const f32x4 *>(scales + BM + wn * kColumns + j * 32 + group * 8 + 4 * half);
+              f32x4 v;
+#pragma unroll
+              for (int u = 0; u < 4; ++u) v[u] = (float)acc[j][i][4 * group + u] * (xs * ws[u]);
+              pack_four<O>(v, words[p] + 2 * g);
+            }
+            if constexpr (kGroups == 2) {
+              const auto first = __builtin_amdgcn_permlane32_swap(words[p][0], words[p][2], false, false);
+              const auto second = __builtin_amdgcn_permlane32_swap(words[p][1], words[p][3], false, false);
+              words[p][0] = first[0];
+              words[p][1] = second[0];
+              words[p][2] = first[1];
+              words[p][3] = second[1];
+            }
           }
-          uint32_t n = at.n0 + wn * kColumns + j * 32 + q * 8;
-          if constexpr (kGroups == 2) {
-            const auto first = __builtin_amdgcn_permlane32_swap(words[0], words[2], false, false);
-            const auto second = __builtin_amdgcn_permlane32_swap(words[1], words[3], false, false);
-            words[0] = first[0];
-            words[1] = second[0];
-            words[2] = first[1];
-            words[3] = second[1];
-            n += 8 * half;
-          } else {
-            n += 4 * half;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const auto both = __builtin_amdgcn_permlane16_swap(words[0][w], words[1][w], false, false);
+            words[0][w] = both[0];
+            words[1][w] = both[1];
           }
-          constexpr uint32_t kVec = 16 / sizeof(O);
-          // Rows that begin anywhere take whole vectors all the same, at any address; what is left of a row goes one by one (behind
-          // stores that count, where more of them make the waits longer and not shorter).
-          const u32x4 v = {words[0], words[1], words[2], words[3]};
+          uint32_t n = at.n0 + wn * kColumns + j * 32 + q * 8 + lane_column;
           asm volatile("" : "+v"(n));  // (the masks of a column for all rows at once are more scalar registers than there are)
-          store_counted(out + n, v, __ballot(there && n + kVec <= columns));
-          if (there && n < columns && n + kVec > columns) {
-            typedef O vec __attribute__((ext_vector_type(kVec)));
-            const vec one = __builtin_bit_cast(vec, v);
 #pragma unroll
-            for (uint32_t u = 0; u + 1 < kVec; ++u) {
-              if (u < columns - n) out[n + u] = one[u];
+          for (int p = 0; p < 2; ++p) {
+            const uint32_t row = wm * kRows + i * 32 + p * 16 + lane % 16;
+            const bool there = at.m0 + row < at.count;
+            PPLX_GLOBAL O *out = out_first + (int64_t)row * out_stride;
+            // Rows that begin anywhere take whole vectors all the same, at any address; what is left of a row goes one by one
+            // (behind stores that count, where more of them make the waits longer and not shorter).
+            const u32x4 v = {words[p][0], words[p][1], words[p][2], words[p][3]};
+            store_counted(out + n, v, __ballot(there && n + kVec <= columns));
+            if (there && n < columns && n + kVec > columns) {
+              typedef O vec __attribute__((ext_vector_type(kVec)));
+              const vec one = __builtin_bit_cast(vec, v);
+#pragma unroll
+              for (uint32_t u = 0; u + 1 < kVec; ++u) {
+                if (u < columns - n) out[n + u] = one[u];
+              }
             }
           }
         }
