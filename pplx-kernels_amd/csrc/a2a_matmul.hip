@@ -396,7 +396,7 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev) {
     // Lane l holds row l % 32 of each fragment and, in its accumulators, columns 4 (l / 32) .. + 3 of every eight.  Of 2-byte
     // results two such groups change places between the halves of the wave, so that every lane has 16 bytes of its row; then two
     // such stores change places between the quarters, so that each takes 64 bytes of sixteen rows instead of 32 of 32: 16384 x
-    // 14336 of 1024 304 to 298 us, of 14340, whose rows do not begin at lines, 344 to 323.  (Odd numbers of 2-byte results take 428.)
+    // 14336 of 1024 304 to 298 us, of 14340, whose rows do not begin at lines, 344 to 323.
     const auto *a = arguments();
     const uint32_t columns = a->n;
     const int64_t out_stride = a->out_stride_row;
@@ -406,8 +406,14 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev) {
     constexpr uint32_t kVec = 16 / sizeof(O);        // results of a lane in a store
     constexpr int kGroups = sizeof(O) == 4 ? 1 : 2;  // of eight columns in a store
     const uint32_t lane_column = kVec * (half + lane / 16 % 2 * 2);
+    // Rows of 2-byte results that begin between two words are stored one result earlier, by words, where a lane has the result
+    // before its own from the lane that holds it; the strip's first lanes, which do not, store as they are.  (Stores that split words
+    // are slow: 14335 columns 428 us, so 339.)
+    const bool odd = sizeof(O) == 2 && (((uintptr_t)out_first | (uintptr_t)(out_stride * 2)) & 2);
+    const uint32_t before = 4 * (half ? lane - 32 : lane < 16 ? lane + 48 : lane + 16);
 #pragma unroll
     for (int i = 0; i < MF; ++i) {
+      uint32_t carry[2] = {0, 0};  // the last words of the columns before, for the first lanes
       const float xs = scales[wm * kRows + i * 32 + lane % 32];
 #pragma unroll
       for (int j = 0; j < NF; ++j) {
@@ -447,13 +453,28 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev) {
             const uint32_t row = wm * kRows + i * 32 + p * 16 + lane % 16;
             const bool there = at.m0 + row < at.count;
             PPLX_GLOBAL O *out = out_first + (int64_t)row * out_stride;
-            // Rows that begin anywhere take whole vectors all the same, at any address; what is left of a row goes one by one
-            // (behind stores that count, where more of them make the waits longer and not shorter).
-            const u32x4 v = {words[p][0], words[p][1], words[p][2], words[p][3]};
-            store_counted(out + n, v, __ballot(there && n + kVec <= columns));
+            // Rows that begin anywhere take whole vectors all the same; what is left of a row goes one by one (behind stores that
+            // count, where more of them make the waits longer and not shorter).
+            u32x4 v = {words[p][0], words[p][1], words[p][2], words[p][3]};
+            const uint64_t whole = __ballot(there && n + kVec <= columns);
+            if (odd) {
+              const uint32_t last = (uint32_t)__builtin_amdgcn_ds_bpermute((int)before, (int)v[3]);
+              const bool shift = ((uintptr_t)out & 2) && !(j == 0 && q == 0 && lane < 16);
+              const uint32_t own[5] = {lane < 16 ? carry[p] : last, v[0], v[1], v[2], v[3]};
+              carry[p] = last;
+#pragma unroll
+              for (int w = 0; w < 4; ++w) v[w] = shift ? __builtin_amdgcn_alignbit(own[w + 1], own[w], 16) : own[w + 1];
+              store_counted(out + n - (shift ? 1 : 0), v, whole);
+              // (nobody behind it stores its last result)
+              if (shift && there && n + kVec <= columns && (n + 2 * kVec > columns || (j == NF - 1 && lane >= 48))) {
+                reinterpret_cast<PPLX_GLOBAL uint16_t *>(out)[n + kVec - 1] = (uint16_t)(own[4] >> 16);
+              }
+            } else {
+              store_counted(out + n, v, whole);
+            }
             if (there && n < columns && n + kVec > columns) {
               typedef O vec __attribute__((ext_vector_type(kVec)));
-              const vec one = __builtin_bit_cast(vec, v);
+              const vec one = __builtin_bit_cast(vec, u32x4{words[p][0], words[p][1], words[p][2], words[p][3]});
 #pragma unroll
               for (uint32_t u = 0; u + 1 < kVec; ++u) {
                 if (u < columns - n) out[n + u] = one[u];

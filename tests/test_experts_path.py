@@ -316,6 +316,24 @@ def test_products_of_every_tile(device, rows, n, k, out_dtype):
 
 
 @gpu
+@pytest.mark.parametrize("rows,n,k", [
+    (9, 40, 64), (401, 1160, 256), (4999, 133, 272), (2049, 1000, 128), (397, 8193, 272), (2049, 4101, 272), (399, 8199, 528),
+])  # fmt: skip
+def test_products_into_rows_that_begin_anywhere(device, rows, n, k):
+    """Rows of out at every address that a result may have, with what lies between them left as it is."""
+    gen = torch.Generator(device).manual_seed(n)
+    x, w = random_int8((rows, k), gen, device), random_int8((n + 9, k), gen, device)
+    xs, ws = (torch.rand(size, generator=gen, device=device) * 1e-2 for size in (rows, n + 9))
+    ref = product64(x, xs, w, ws)
+    for first, pitch, less in ((0, n + 1, 0), (1, n + 8, -1), (3, n + 11, -2), (5, n + 17, -9), (2, n + 9, 1), (7, n + 16, 2), (1, n + 9, 3)):
+        columns = n + less
+        out = torch.full((rows, max(pitch, first + columns)), 7.0, dtype=BF16, device=device)
+        int8_matmul(x, xs, w[:columns], ws[:columns], out=out[:, first : first + columns])
+        assert_product(out[:, first : first + columns], ref[:, :columns])
+        assert (out[:, :first] == 7).all() and (out[:, first + columns :] == 7).all()
+
+
+@gpu
 @pytest.mark.parametrize("k", [2064, 2176])
 @pytest.mark.parametrize("counts", [
     [3] * 10 + [0] * 14, [0] * 5 + [1, 400, 0, 33] + [20] * 15, [65, 64, 1, 900, 0, 0] + [30] * 18, [100] * 24,
