@@ -384,8 +384,9 @@ typedef struct pplx_a2a_unsort_args {
 int pplx_a2a_unsort_tokens(int device, const pplx_a2a_unsort_args_t *args, void *stream);
 
 /* Gradients of unsort_tokens: grad_y[slots[t, k]] = weights[t, k] * grad_out[t] and grad_weights[t, k] =
- * <grad_out[t], y[slots[t, k]]>, summed in fp32; rows of grad_y from offsets[num_experts] on, which no slot names,
- * and weights of picks without a row get zeros.  Either gradient may be left out (NULL). */
+ * <grad_out[t], y[slots[t, k]]>, summed in fp32; rows of grad_y that no slot names and weights of picks without a
+ * row get zeros.  The slots are those of a sort, of all its tokens or of some, with any of them taken out (-1): no two
+ * name one row, and none names a row from *num_rows on.  Either gradient may be left out (NULL). */
 typedef struct pplx_a2a_unsort_backward_args {
   void *grad_y;               /* [y_rows, hidden_dim] of dtype, 16-byte aligned, or NULL */
   int64_t grad_y_stride_row;  /* bytes, a multiple of 16 */

@@ -115,7 +115,75 @@ struct UnsortBackwardDev {
   const int32_t *num_rows;
   const float *weights;
   uint32_t m, K, width;
+  uint32_t sweeps, sweep_rows;  // workgroups in front of the tokens', rows of grad_y that one looks at
 };
+
+// Rows of grad_y that no slot names are zeros.  Those from *num_rows on are shared out over the tokens.  In front of it every
+// row is named by the slots of a whole sort, but not by those of some of its tokens, or with picks taken out: workgroups in
+// front of the tokens' count the slots that name a row, and where these are fewer than the rows go through them once more, for
+// sweep_rows rows each, mark in LDS what is named and clear the rest.  They write what nobody else writes, so they run beside
+// the others.
+constexpr uint32_t kMaxSweepRows = 16384;
+template <uint32_t AT_ONCE, class Fn> __device__ __forceinline__ void for_slots(const UnsortBackwardDev &a, Fn &&fn) {
+  typedef uint32_t four __attribute__((ext_vector_type(4), aligned(4)));
+  const PPLX_GLOBAL four *slots = as_global(reinterpret_cast<const four *>(a.slots));
+  const uint32_t picks = a.m * a.K, fours = picks / 4;
+  uint32_t base = threadIdx.x;
+  for (; base + 256 * (AT_ONCE - 1) < fours; base += 256 * AT_ONCE) {
+    four s[AT_ONCE];
+#pragma unroll
+    for (uint32_t u = 0; u < AT_ONCE; ++u) s[u] = slots[base + u * 256];
+#pragma unroll
+    for (uint32_t u = 0; u < AT_ONCE; ++u) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) fn(s[u][i]);
+    }
+  }
+  for (; base < fours; base += 256) {
+    const four s = slots[base];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) fn(s[i]);
+  }
+  if (threadIdx.x < picks % 4) fn((uint32_t)as_global(a.slots)[4 * fours + threadIdx.x]);
+}
+
+template <class T> __device__ void clear_unnamed(const UnsortBackwardDev &a, uint32_t total, uint32_t *named) {
+  const uint32_t rows = total < a.y_rows ? total : a.y_rows;
+  const uint32_t first = blockIdx.x * a.sweep_rows;
+  if (first >= rows) return;
+  const uint32_t count = rows - first < a.sweep_rows ? rows - first : a.sweep_rows;
+  uint32_t own = 0;
+  for_slots<16>(a, [&](uint32_t slot) { own += slot < rows ? 1u : 0u; });
+#pragma unroll
+  for (int d = 32; d; d >>= 1) own += (uint32_t)__shfl_xor((int)own, d);
+  if (lane_id() == 0) named[wave_id()] = own;
+  __syncthreads();
+  if (named[0] + named[1] + named[2] + named[3] >= rows) return;
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < (count + 31) / 32; i += 256) named[i] = 0;
+  __syncthreads();
+  for_slots<8>(a, [&](uint32_t slot) {
+    const uint32_t r = slot - first;
+    if (r < count) atomicOr(&named[r / 32], 1u << (r % 32));
+  });
+  __syncthreads();
+  for (uint32_t r = wave_id(); r < count; r += 4) {
+    if ((named[r / 32] >> (r % 32)) & 1) continue;
+    PPLX_GLOBAL T *row = as_global(reinterpret_cast<T *>(a.grad_y + (int64_t)(first + r) * a.grad_y_stride));
+    for (uint32_t col = lane_id() * 8; col < a.width; col += 64 * 8) store_eight<T>(row + col, f32x8{0, 0, 0, 0, 0, 0, 0, 0});
+  }
+}
+
+// All rows of grad_y, in front of the gradient.
+template <class T> __global__ __launch_bounds__(256) void clear_rows(UnsortBackwardDev a) {
+  const uint32_t pieces = a.width / 8;
+  const uint64_t all = (uint64_t)a.y_rows * pieces, step = (uint64_t)gridDim.x * 256;
+  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += step) {
+    const uint64_t r = i / pieces;
+    PPLX_GLOBAL T *row = as_global(reinterpret_cast<T *>(a.grad_y + (int64_t)r * a.grad_y_stride));
+    store_eight<T>(row + (i - r * pieces) * 8, f32x8{0, 0, 0, 0, 0, 0, 0, 0});
+  }
+}
 
 // LANES threads to a token (a wave, or the workgroup).  Eight picks at a time: their rows of y are read, their rows of
 // grad_y written, and the eight products summed over the row at the end.
@@ -123,7 +191,14 @@ template <class T, class G, int LANES, bool NT>
 __global__ __launch_bounds__(256) void unsort_backward(UnsortBackwardDev a) {
   constexpr int kPicks = 8;
   const uint32_t lane = lane_id(), wave = wave_id(), g = threadIdx.x % LANES;
-  const uint32_t t = LANES == 64 ? blockIdx.x * 4 + wave : blockIdx.x;
+  __shared__ uint32_t named[kMaxSweepRows / 32];
+  if (blockIdx.x < a.sweeps) {
+    const int32_t live_rows = *as_global(a.num_rows);
+    clear_unnamed<T>(a, live_rows > 0 ? (uint32_t)live_rows : 0u, named);
+    return;
+  }
+  const uint32_t group = blockIdx.x - a.sweeps;
+  const uint32_t t = LANES == 64 ? group * 4 + wave : group;
   if (t >= a.m) return;  // (with 256 lanes to a token the grid has one workgroup a token)
   int32_t slot = -1;
   float w = 1.f;
@@ -194,7 +269,7 @@ __global__ __launch_bounds__(256) void unsort_backward(UnsortBackwardDev a) {
     }
   }
   if (!want_y) return;
-  // The rows that no slot names lie behind the others; they are shared out over the tokens.
+  // The rows behind the last live one.
   const int32_t there = *as_global(a.num_rows);
   const uint32_t total = there > 0 ? (uint32_t)there : 0u;
   const uint64_t stride = (uint64_t)a.m * a.K;
@@ -221,6 +296,17 @@ int check_unsort_size(uint64_t m, uint64_t K, uint64_t hidden_dim, int64_t y_row
   if (m * K >= (1ull << 31) || m * ((hidden_dim + 511) / 512) >= (1ull << 32))
     return refuse(PPLX_A2A_UNSUPPORTED, "too many picks or elements");
   return PPLX_A2A_OK;
+}
+
+// Rows of grad_y to each of the workgroups that look for rows without a name, 0 for all rows cleared in front.  128 of them
+// or more each go through all slots, which grows with the square of the picks.  us, as if all rows had names / so / cleared:
+// 4096 x 8 rows of 64 bytes 9.2 / 8.9 / 11.9, 8192 x 8 of 128 13.3 / 13.9 / 16.7, of 4096 101 / 102 / 141; 131072 x 8 of 128
+// 146 / 163 / 166, of 512 202 / 223 / 293, of 4096 1785 / 1755 / 2709; 1000000 x 8 of 256 1202 / 1733 / 1614.
+uint32_t rows_to_sweep(uint32_t y_rows, uint64_t picks, uint64_t row_bytes) {
+  uint32_t rows = (y_rows + 127) / 128;
+  rows = rows < 256 ? 256 : rows > kMaxSweepRows ? kMaxSweepRows : rows;
+  const uint64_t sweeps = (y_rows + rows - 1) / rows;
+  return picks <= 1 << 18 || sweeps <= 2 * row_bytes ? rows : 0;
 }
 }  // namespace
 
@@ -307,10 +393,20 @@ extern "C" int pplx_a2a_unsort_tokens_backward(int device, const pplx_a2a_unsort
         // 2048 (268 MB) 112 / 109 / 100, 16384 x 2 of 1024 (67 MB) 36.3 / 31.4 / 30.2; 2048 x 6 of 2048 (50 MB) 24.6 / 19.6 /
         // 23.0, 1024 x 2 of 7168 (29 MB) 13.8 / 13.9 / 15.1.
         const bool large = (uint64_t)a.m * a.K * a.width * sizeof(Y) > kStreamGradientBytes;
+        if (a.grad_y && a.y_rows > 0) {
+          if (const uint32_t rows = rows_to_sweep(a.y_rows, (uint64_t)a.m * a.K, a.width * sizeof(Y))) {
+            a.sweep_rows = rows;
+            a.sweeps = (a.y_rows + rows - 1) / rows;
+          } else {
+            const uint64_t groups = ((uint64_t)a.y_rows * (a.width / 8) + 255) / 256;
+            PPLX_LAUNCH(launch_kernel(clear_rows<Y>, dim3(groups < 4096 ? (uint32_t)groups : 4096), dim3(256), 0, (hipStream_t)stream, a));
+          }
+        }
         auto launch = [&](auto lanes) {
           constexpr int L = decltype(lanes)::value;
           auto kernel = large ? unsort_backward<Y, G, L, true> : unsort_backward<Y, G, L, false>;
-          PPLX_LAUNCH(launch_kernel(kernel, dim3(L == 64 ? (a.m + 3) / 4 : a.m), dim3(256), 0, (hipStream_t)stream, a));
+          const uint32_t groups = a.sweeps + (L == 64 ? (a.m + 3) / 4 : a.m);
+          PPLX_LAUNCH(launch_kernel(kernel, dim3(groups), dim3(256), 0, (hipStream_t)stream, a));
           return (int)PPLX_A2A_OK;
         };
         return a.width <= 1024 ? launch(std::integral_constant<int, 64>{}) : launch(std::integral_constant<int, 256>{});

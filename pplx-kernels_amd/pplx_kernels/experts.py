@@ -152,8 +152,9 @@ def unsort_tokens_backward(
     out: tuple[torch.Tensor | None, torch.Tensor | None] | None = None,
 ) -> tuple[torch.Tensor | None, torch.Tensor | None]:
     """The gradients of :func:`unsort_tokens`: ``grad_y[slots[t, k]] = weights[t, k] * grad_out[t]``, zeros in rows that no
-    pick has, and ``grad_weights[t, k] = <grad_out[t], y[slots[t, k]]>`` (None without weights).  In ``out`` either may be
-    None, which leaves it out."""
+    pick has, and ``grad_weights[t, k] = <grad_out[t], y[slots[t, k]]>`` (None without weights).  ``slots`` are a sort's, of
+    all its tokens or of some, with any of them taken out (-1); no two name one row.  In ``out`` either may be None, which
+    leaves it out."""
     if out is None:
         out = torch.empty_like(y, memory_format=torch.contiguous_format), None if weights is None else torch.empty_like(weights)
     fn = _ops.unsort_tokens_backward if _is_compiling() else _C.unsort_tokens_backward

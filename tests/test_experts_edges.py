@@ -1,0 +1,80 @@
+"""The operators between dispatch and combine where their callers may reach and the other tests do not: parts of a sort's slots,
+sizes beyond a form's limits, ways of calling that see through the calls.
+
+Tolerances count roundings as in test_experts.py."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from pplx_kernels import sort_tokens, unsort_tokens, unsort_tokens_backward
+from tests.test_experts import (
+    BF16,
+    F16,
+    F32,
+    U32,
+    assert_within,
+    make_indices,
+    make_sorted,
+    rounded,
+    to_u32,
+)
+
+gpu = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------
+# Rows of the gradient that no slot names
+# ---------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("m,k,more,hidden,dtype", [
+    (3, 2, 0, 8, F32), (40, 3, 5, 520, BF16), (700, 4, 0, 1032, F16), (9000, 5, 0, 64, F32), (9000, 5, 0, 16, BF16), (9000, 5, 300, 1040, BF16),
+    (60001, 5, 7, 8, F16),
+])  # fmt: skip
+@pytest.mark.parametrize("part", ["first", "middle", "none", "taken out"])
+def test_rows_of_the_gradient_without_a_name(device, m, k, more, hidden, dtype, part):
+    """Slots of some of a sort's tokens, or with picks taken out: rows in front of the last live one that nobody names."""
+    gen = torch.Generator().manual_seed(m + hidden)
+    slots, offsets = make_sorted(m, k, 13, gen, device)
+    if part == "taken out":
+        slots[torch.rand(m, k, generator=gen) < 0.3] = -1
+        tokens = slice(0, m)
+    else:
+        tokens = {"first": slice(0, m // 3 + 1), "middle": slice(m // 3, m - 1), "none": slice(0, m)}[part]
+        if part == "none":
+            slots[:] = -1
+    slots = slots[tokens].contiguous()
+    rows, n = m * k + more, slots.shape[0]
+    y = torch.randn(rows, hidden, generator=gen).to(dtype)
+    weights, grad_out = torch.rand(n, k, generator=gen), torch.randn(n, hidden, generator=gen).to(dtype)
+    grad_y = torch.full((rows, hidden), float("nan"), dtype=dtype, device=device)
+    grad_w = torch.full((n, k), float("nan"), device=device)
+    unsort_tokens_backward(*(t.to(device) for t in (grad_out, y, slots, offsets, weights)), out=(grad_y, grad_w))
+    ref_y = torch.zeros(rows, hidden, dtype=torch.float64)
+    t, p = torch.nonzero(slots >= 0, as_tuple=True)
+    ref_y[slots[t, p].long()] = grad_out.double()[t] * weights.double()[t, p][:, None]
+    assert_within(grad_y, ref_y, rounded(ref_y, dtype, U32 * ref_y.abs()))
+    named = torch.zeros(rows, dtype=torch.bool)
+    named[slots[t, p].long()] = True
+    assert (grad_y.cpu()[~named] == 0).all()
+    assert torch.isfinite(grad_w).all() and (grad_w.cpu()[slots < 0] == 0).all()
+
+
+@gpu
+def test_gradients_of_tokens_in_parts(device):
+    """A step whose tokens go back in parts, each through a call of its own, has the gradients of the whole step."""
+    m, k, experts, hidden = 300, 3, 8, 264
+    gen = torch.Generator().manual_seed(11)
+    x = torch.randn(m, hidden, generator=gen).to(device)
+    indices = to_u32(make_indices(m, k, experts, gen, "mixed"), device)
+    weights = torch.rand(m, k, generator=gen).to(device).requires_grad_(True)
+    grad = torch.randn(m, hidden, generator=gen).to(device)
+    s = sort_tokens(x, indices, experts)
+    y = s.rows.clone().requires_grad_(True)
+    whole = torch.autograd.grad(unsort_tokens(y, s.slots, s.offsets, weights), [y, weights], grad)
+    torch.full((4, *y.shape), float("nan"), device=device)  # (memory that the gradients may get holds no zeros)
+    parts = [unsort_tokens(y, s.slots[a : a + 70], s.offsets, weights[a : a + 70]) for a in range(0, m, 70)]
+    got = torch.autograd.grad(torch.cat(parts), [y, weights], grad)
+    # (a row's gradient is one part's; the others add zeros)
+    assert all(torch.equal(a, b) for a, b in zip(got, whole))
