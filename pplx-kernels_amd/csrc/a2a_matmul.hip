@@ -171,6 +171,9 @@ template <class O> __device__ __forceinline__ void pack_four(f32x4 v, uint32_t *
   }
 }
 
+// The steps in flight take 128 KiB of a compute unit's LDS, the tables of the experts lie behind them.
+constexpr uint32_t kLdsBytes = 128 * 1024;
+
 // WM by WN waves, each BM / WM rows by BN / WN columns in fragments of 32 by 32; STAGES steps of BK bytes of k in LDS.  A wave
 // reads the fragments of the next 32 bytes of k before it multiplies those at hand, over the border between two steps too:
 // there it waits for the next step's loads, and behind the barrier this step's place takes those of a step to come.  The
@@ -199,10 +202,12 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev) {
   constexpr bool kLines = BK == 128;
   constexpr int kAhead = kWhole ? STAGES - 1 : STAGES;  // steps loaded in front of a tile's first
   constexpr int kStage = (BM + BN) * BK;
-  extern __shared__ __align__(128) uint8_t lds[];  // [STAGES][BM rows of x, BN of the weight][BK], scales, sums of blocks
+  // [STAGES][BM rows of x, BN of the weight][BK], scales, sums of blocks, sums of waves.  All of a workgroup's share is in here,
+  // so that the stages, which loads write directly, begin at its first byte.
+  extern __shared__ __align__(128) uint8_t lds[];
+  static_assert(STAGES * kStage <= kLdsBytes, "loads to LDS stay in front of kLdsBytes");
   float *scales = reinterpret_cast<float *>(lds + STAGES * kStage);  // of BM rows and BN columns
   uint32_t *upto = reinterpret_cast<uint32_t *>(scales + BM + BN);
-  __shared__ uint32_t of_wave[kWaves];
   // The arguments are read where they are used, once a tile: kept in scalar registers they are more than there are.
   auto arguments = []() __attribute__((always_inline)) {
     auto *p = (const PPLX_CONSTANT MatmulDev *)__builtin_amdgcn_kernarg_segment_ptr();
@@ -213,7 +218,7 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev) {
   {
     const auto *a = arguments();
     const RowsDev rows{a->rows.starts_or_counts, a->rows.rows, a->rows.experts, a->rows.layout};
-    sum_blocks<kThreads, BM>(rows, upto, of_wave);
+    sum_blocks<kThreads, BM>(rows, upto, upto + rows.experts);
     // (offsets that do not ascend give a list of any length, of which only tiles that exist are taken)
     const uint32_t listed = upto[rows.experts - 1] * a->n_blocks;
     tiles = __builtin_amdgcn_readfirstlane(listed < 1u << 31 ? listed : 1u << 31);
@@ -487,14 +492,13 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev) {
   }
 }
 
-// The steps in flight take 128 KiB of a compute unit's LDS, the tables of the experts lie behind them.
-constexpr uint32_t kComputeUnits = 256, kLdsBytes = 128 * 1024;
+constexpr uint32_t kComputeUnits = 256;
 
 template <int BM, int BN, int WM, int WN, int BK, int STAGES, class O>
 int launch_tiles(const MatmulDev &from, uint64_t most_blocks, hipStream_t s) {
   MatmulDev a = from;
   constexpr uint32_t kTileLds = STAGES * (BM + BN) * BK;
-  const uint32_t lds = kTileLds + 4 * (BM + BN) + 4 * a.rows.experts;
+  const uint32_t lds = kTileLds + 4 * (BM + BN) + 4 * a.rows.experts + 4 * WM * WN;
   constexpr uint32_t per_unit = kLdsBytes / kTileLds;
   static_assert(per_unit >= 1, "a tile's steps fit");
   a.n_blocks = (a.n + BN - 1) / BN;

@@ -8,7 +8,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from pplx_kernels import sort_tokens, unsort_tokens, unsort_tokens_backward
+from pplx_kernels import ops, sort_tokens, unsort_tokens, unsort_tokens_backward
+from tests.test_capi_cpu import _gpu_kernels_of
 from tests.test_experts import (
     BF16,
     F16,
@@ -78,3 +79,15 @@ def test_gradients_of_tokens_in_parts(device):
     got = torch.autograd.grad(torch.cat(parts), [y, weights], grad)
     # (a row's gradient is one part's; the others add zeros)
     assert all(torch.equal(a, b) for a, b in zip(got, whole))
+
+
+# ---------------------------------------------------------------------------
+# What the kernels take of a workgroup
+# ---------------------------------------------------------------------------
+def test_product_tiles_begin_at_the_first_byte_of_lds():
+    """The steps of a tile, which loads write to LDS directly, lie in front of everything else that a workgroup has there, and
+    no kernel of the products spills."""
+    kernels = [k for k in _gpu_kernels_of(ops._LIB_PATH) if "matmul_tiles" in k[".name"]]
+    assert len(kernels) == 6 * 2 * 3  # forms, k that fills the steps or not, types
+    assert {k[".group_segment_fixed_size"] for k in kernels} == {0}
+    assert {k[".vgpr_spill_count"] for k in kernels} == {0} and {k[".sgpr_spill_count"] for k in kernels} == {0}
