@@ -5,6 +5,7 @@
 #include <ATen/MemoryOverlap.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
+#include <c10/core/AutogradState.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -491,6 +492,15 @@ torch::autograd::variable_list differentiable_once(torch::autograd::variable_lis
   return grads;
 }
 
+// Tangents of forward-mode differentiation are refused, not dropped.
+void check_no_tangent(std::initializer_list<const at::Tensor *> read) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const at::Tensor *x : read) {
+    TORCH_CHECK(!x || !x->defined() || !x->_fw_grad(0).defined(),
+                "pplx_kernels: sort_tokens, unsort_tokens and their gradients have no forward-mode derivatives");
+  }
+}
+
 SortedTuple call_sorted_tokens(const at::Tensor &x, const at::Tensor &indices, int64_t experts, opt_tensor bound_m, bool int8) {
   at::AutoDispatchBelowADInplaceOrView below;
   static auto op = op_handle<SortedTuple(const at::Tensor &, const at::Tensor &, int64_t, opt_tensor, bool)>(
@@ -512,6 +522,7 @@ struct SortFunction : torch::autograd::Function<SortFunction> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
                                                  torch::autograd::variable_list grads) {
     at::Tensor grad_x;
+    check_no_tangent({&grads[0]});
     if (grads[0].defined()) {
       const at::Tensor slots = ctx->get_saved_variables()[0];
       at::NoGradGuard plain;
@@ -541,6 +552,7 @@ struct UnsortFunction : torch::autograd::Function<UnsortFunction> {
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &y = saved[0], &weights = saved[3];
     at::Tensor grad_y, grad_weights;
+    check_no_tangent({&grads[0], &y, &weights});
     {
       at::NoGradGuard plain;
       static auto op = op_handle<void(opt_tensor, opt_tensor, const at::Tensor &, const at::Tensor &, const at::Tensor &,
@@ -561,11 +573,13 @@ struct UnsortFunction : torch::autograd::Function<UnsortFunction> {
 SortedTuple sorted_tokens_autograd(const at::Tensor &x, const at::Tensor &indices, int64_t experts, opt_tensor bound_m,
                                    bool int8) {
   if (int8) return call_sorted_tokens(x, indices, experts, bound_m, true);
+  check_no_tangent({&x});
   auto made = SortFunction::apply(x, indices, experts, bound_m);
   return {made[0], made[1], made[2], made[3]};
 }
 at::Tensor unsorted_tokens_autograd(const at::Tensor &y, const at::Tensor &slots, const at::Tensor &offsets,
                                     opt_tensor weights, std::optional<at::ScalarType> out_dtype) {
+  check_no_tangent({&y, opt(weights)});
   return UnsortFunction::apply(y, slots, offsets, weights, out_dtype);
 }
 

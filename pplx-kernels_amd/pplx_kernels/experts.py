@@ -12,7 +12,7 @@ back for a rank that holds its experts itself, with the gradients of both.
 
 ``quantize_rows`` and ``int8_matmul`` take the buffers that ``AllToAll.dispatch`` fills as well, with its
 ``out_expert_num_tokens`` as ``num_tokens``.  All of it runs on the current stream of the tensors' device and keeps
-nothing between calls.  With ``out=`` a call allocates nothing, so it can be captured as it is; without, the results are
+nothing between calls.  Gradients are those of reverse mode; forward mode is refused.  With ``out=`` a call allocates nothing, so it can be captured as it is; without, the results are
 new tensors.  Under capture gradients go through ``unsort_tokens_backward`` and ``sort_tokens_backward``: a capture that
 autograd recorded would depend on graphs of the same leaves that live outside.
 """
@@ -22,6 +22,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from .ops import _C, _ops
 
@@ -61,11 +62,16 @@ class SortedTokens(NamedTuple):
 
 
 def _wants_grad(*tensors: torch.Tensor | None) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    # (a tensor with a tangent need not require a gradient)
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors
+    )
 
 
-def _check_recording() -> None:
-    if torch.cuda.is_current_stream_capturing():
+def _check_recording(x: torch.Tensor) -> None:
+    if x.is_cuda and torch.cuda.is_current_stream_capturing():
         raise RuntimeError(
             "pplx_kernels: gradients are not recorded under stream capture: capture sort_tokens_backward and "
             "unsort_tokens_backward, under torch.no_grad()"
@@ -99,7 +105,7 @@ def sort_tokens(
         rows, scale, slots, offsets = _ops.sorted_tokens(x, indices, num_experts, bound_m, int8)
         return SortedTokens(rows, scale if int8 else None, slots, offsets, None)
     if not int8 and _wants_grad(x):
-        _check_recording()
+        _check_recording(x)
         rows, slots, offsets = _C.sorted_tokens(x, indices, num_experts, bound_m)
         return SortedTokens(rows, None, slots, offsets, None)
     return SortedTokens._make(_C.sort_tokens(x, indices, num_experts, bound_m, int8))
@@ -127,7 +133,7 @@ def unsort_tokens(
     if out is None and _is_compiling():
         return _ops.unsorted_tokens(y, slots, offsets, weights, out_dtype)
     if out is None and _wants_grad(y, weights):
-        _check_recording()
+        _check_recording(y)
         return _C.unsorted_tokens(y, slots, offsets, weights, out_dtype)
     return _unsort(y, slots, weights, out_dtype, out)
 

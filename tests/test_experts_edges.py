@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from pplx_kernels import ops, sort_tokens, unsort_tokens, unsort_tokens_backward
 from tests.test_capi_cpu import _gpu_kernels_of
@@ -79,6 +80,53 @@ def test_gradients_of_tokens_in_parts(device):
     got = torch.autograd.grad(torch.cat(parts), [y, weights], grad)
     # (a row's gradient is one part's; the others add zeros)
     assert all(torch.equal(a, b) for a, b in zip(got, whole))
+
+
+# ---------------------------------------------------------------------------
+# Forward-mode differentiation
+# ---------------------------------------------------------------------------
+def check_tangents_are_refused(device):
+    """No derivative is lost: a tensor with a tangent, which need not require a gradient, is refused wherever it comes in."""
+    idx, offsets = torch.zeros(4, 2, dtype=torch.uint32, device=device), torch.tensor([0, 8], dtype=torch.int32, device=device)
+    slots = torch.arange(8, dtype=torch.int32, device=device).view(4, 2)
+    x, y, weights = (torch.ones(*shape, device=device) for shape in ((4, 16), (8, 16), (4, 2)))
+    with forward_ad.dual_level():
+        dx, dy, dw = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, y, weights))
+        assert not dx.requires_grad
+        for call in (
+            lambda: sort_tokens(dx, idx, 1),
+            lambda: unsort_tokens(dy, slots, offsets),
+            lambda: unsort_tokens(dy, slots, offsets, weights),
+            lambda: unsort_tokens(y, slots, offsets, dw),
+            lambda: torch.ops.pplx_kernels.sorted_tokens(dx, idx, 1, None, False),
+            lambda: torch.ops.pplx_kernels.unsorted_tokens(y, slots, offsets, dw, None),
+        ):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+
+
+def test_tangents_are_refused_before_the_device_is_looked_at():
+    check_tangents_are_refused("cpu")
+
+
+@gpu
+def test_tangents_are_refused(device):
+    check_tangents_are_refused(device)
+    idx = torch.zeros(4, 2, dtype=torch.uint32, device=device)
+    x, y, weights = (torch.randn(*shape, device=device, requires_grad=True) for shape in ((4, 16), (8, 16), (4, 2)))
+    s = sort_tokens(x, idx, 1)
+    out = unsort_tokens(y, s.slots, s.offsets, weights)
+    with forward_ad.dual_level():  # (forward over reverse)
+        for made, leaf in ((s.rows, x), (out, y), (out, weights)):
+            grad = forward_ad.make_dual(torch.ones_like(made), torch.ones_like(made))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(made, leaf, grad, retain_graph=True)
+        # what is not differentiable takes the values
+        d = forward_ad.make_dual(x.detach(), torch.ones_like(x))
+        assert torch.equal(sort_tokens(d, idx, 1, int8=True).rows, sort_tokens(x.detach(), idx, 1, int8=True).rows)
+    assert torch.equal(torch.autograd.grad(s.rows.sum(), x)[0], torch.full_like(x, 2))
 
 
 # ---------------------------------------------------------------------------
