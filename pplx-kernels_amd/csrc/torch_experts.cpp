@@ -559,11 +559,11 @@ struct UnsortFunction : torch::autograd::Function<UnsortFunction> {
                                       const at::Tensor &, opt_tensor)>("pplx_kernels::unsort_tokens_backward");
       if (ctx->needs_input_grad(0)) grad_y = fresh_traced(y.sym_sizes(), y, y.scalar_type());
       if (weights.defined() && ctx->needs_input_grad(3)) grad_weights = fresh_traced(weights.sym_sizes(), weights, at::kFloat);
-      auto maybe = [](const at::Tensor &t) { return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt; };
+      auto if_defined = [](const at::Tensor &t) { return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt; };
       if (saved[1].sym_size(0) == 0) {  // (without tokens)
         if (grad_y.defined()) grad_y.zero_();
       } else {
-        op.call(maybe(grad_y), maybe(grad_weights), as_rows(grads[0]), y, saved[1], saved[2], maybe(weights));
+        op.call(if_defined(grad_y), if_defined(grad_weights), as_rows(grads[0]), y, saved[1], saved[2], if_defined(weights));
       }
     }
     return differentiable_once({grad_y, at::Tensor(), at::Tensor(), grad_weights, at::Tensor()});
@@ -629,6 +629,24 @@ TORCH_LIBRARY_FRAGMENT(pplx_kernels, m) {
 // ---------------------------------------------------------------------------
 namespace {
 
+// Whether the dispatcher would go straight to the kernel (or to autograd, which the functions see to).  A tracer, a mode, a
+// transform or a tensor that is more than its data has to see the registered op: behind its back the results would be taken for
+// what `empty` made.
+bool straight(std::initializer_list<const at::Tensor *> tensors) {
+  static const uint64_t usual =
+      c10::full_backend_mask | c10::autocast_dispatch_keyset.raw_repr() |
+      c10::DispatchKeySet({c10::DispatchKey::Dense, c10::DispatchKey::BackendSelect, c10::DispatchKey::ADInplaceOrView,
+                           c10::DispatchKey::AutogradFunctionality}).raw_repr();
+  const auto local = c10::impl::tls_local_dispatch_key_set();
+  c10::DispatchKeySet keys = local.included_;
+  for (const at::Tensor *x : tensors) {
+    if (x) keys = keys | x->key_set();
+  }
+  return ((keys - local.excluded_).raw_repr() & ~usual) == 0;
+}
+
+std::optional<at::Tensor> maybe(const at::Tensor *x) { return x ? std::optional<at::Tensor>(*x) : std::nullopt; }
+
 PyObject *wrap_or_none(const at::Tensor &t) {
   if (!t.defined()) Py_RETURN_NONE;
   return THPVariable_Wrap(t);
@@ -638,8 +656,18 @@ PyObject *wrap_or_none(const at::Tensor &t) {
 PyObject *py_sort_tokens(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   arity("sort_tokens", nargs, 5);
-  const Sorted s = sort_new(tensor_arg(args[0], "x"), tensor_arg(args[1], "indices"), int_arg(args[2], "num_experts"),
-                            optional_tensor_arg(args[3], "bound_m"), PyObject_IsTrue(args[4]) == 1);
+  const at::Tensor &x = tensor_arg(args[0], "x"), &indices = tensor_arg(args[1], "indices");
+  const int64_t experts = int_arg(args[2], "num_experts");
+  const at::Tensor *bound_m = optional_tensor_arg(args[3], "bound_m");
+  const bool int8 = PyObject_IsTrue(args[4]) == 1;
+  Sorted s;
+  if (straight({&x, &indices, bound_m})) {
+    s = sort_new(x, indices, experts, bound_m, int8);
+  } else {
+    static auto op = op_handle<decltype(sorted_tokens_op)>("pplx_kernels::sorted_tokens");
+    std::tie(s.rows, s.scale, s.slots, s.offsets) = op.call(x, indices, experts, maybe(bound_m), int8);
+    if (!int8) s.scale = at::Tensor();
+  }
   PyObject *out = PyTuple_New(5);
   if (!out) throw python_error();
   const at::Tensor *made[] = {&s.rows, &s.scale, &s.slots, &s.offsets, &s.workspace};
@@ -652,9 +680,18 @@ PyObject *py_sort_tokens(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
 PyObject *py_sort_tokens_out(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   arity("sort_tokens_out", nargs, 8);
-  sort_tokens(tensor_arg(args[0], "rows"), optional_tensor_arg(args[1], "scale"), tensor_arg(args[2], "slots"),
-              tensor_arg(args[3], "offsets"), optional_tensor_arg(args[4], "workspace"), tensor_arg(args[5], "x"),
-              tensor_arg(args[6], "indices"), optional_tensor_arg(args[7], "bound_m"));
+  const at::Tensor &rows = tensor_arg(args[0], "rows"), &slots = tensor_arg(args[2], "slots"),
+                   &offsets = tensor_arg(args[3], "offsets"), &x = tensor_arg(args[5], "x"),
+                   &indices = tensor_arg(args[6], "indices");
+  const at::Tensor *scale = optional_tensor_arg(args[1], "scale"), *workspace = optional_tensor_arg(args[4], "workspace"),
+                   *bound_m = optional_tensor_arg(args[7], "bound_m");
+  if (straight({&rows, scale, &slots, &offsets, workspace, &x, &indices, bound_m})) {
+    sort_tokens(rows, scale, slots, offsets, workspace, x, indices, bound_m);
+  } else {
+    static auto op = op_handle<decltype(sort_tokens_op)>("pplx_kernels::sort_tokens");
+    at::Tensor to_rows = rows, to_slots = slots, to_offsets = offsets;
+    op.call(to_rows, maybe(scale), to_slots, to_offsets, maybe(workspace), x, indices, maybe(bound_m));
+  }
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -696,8 +733,15 @@ PyObject *py_unsorted_tokens(PyObject *, PyObject *const *args, Py_ssize_t nargs
 PyObject *py_unsort_tokens(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   arity("unsort_tokens", nargs, 4);
-  unsort_tokens(tensor_arg(args[0], "out"), tensor_arg(args[1], "y"), tensor_arg(args[2], "slots"),
-                optional_tensor_arg(args[3], "weights"));
+  const at::Tensor &out = tensor_arg(args[0], "out"), &y = tensor_arg(args[1], "y"), &slots = tensor_arg(args[2], "slots");
+  const at::Tensor *weights = optional_tensor_arg(args[3], "weights");
+  if (straight({&out, &y, &slots, weights})) {
+    unsort_tokens(out, y, slots, weights);
+  } else {
+    static auto op = op_handle<decltype(unsort_tokens_op)>("pplx_kernels::unsort_tokens");
+    at::Tensor to = out;
+    op.call(to, y, slots, maybe(weights));
+  }
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -706,9 +750,16 @@ PyObject *py_unsort_tokens(PyObject *, PyObject *const *args, Py_ssize_t nargs) 
 PyObject *py_unsort_tokens_backward(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   arity("unsort_tokens_backward", nargs, 7);
-  unsort_tokens_backward(optional_tensor_arg(args[0], "grad_y"), optional_tensor_arg(args[1], "grad_weights"),
-                         tensor_arg(args[2], "grad_out"), tensor_arg(args[3], "y"), tensor_arg(args[4], "slots"),
-                         tensor_arg(args[5], "offsets"), optional_tensor_arg(args[6], "weights"));
+  const at::Tensor *grad_y = optional_tensor_arg(args[0], "grad_y"), *grad_weights = optional_tensor_arg(args[1], "grad_weights"),
+                   *weights = optional_tensor_arg(args[6], "weights");
+  const at::Tensor &grad_out = tensor_arg(args[2], "grad_out"), &y = tensor_arg(args[3], "y"), &slots = tensor_arg(args[4], "slots"),
+                   &offsets = tensor_arg(args[5], "offsets");
+  if (straight({grad_y, grad_weights, &grad_out, &y, &slots, &offsets, weights})) {
+    unsort_tokens_backward(grad_y, grad_weights, grad_out, y, slots, offsets, weights);
+  } else {
+    static auto op = op_handle<decltype(unsort_tokens_backward_op)>("pplx_kernels::unsort_tokens_backward");
+    op.call(maybe(grad_y), maybe(grad_weights), grad_out, y, slots, offsets, maybe(weights));
+  }
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -717,9 +768,16 @@ PyObject *py_unsort_tokens_backward(PyObject *, PyObject *const *args, Py_ssize_
 PyObject *py_quantize_rows(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   arity("quantize_rows", nargs, 6);
-  quantize_rows(tensor_arg(args[0], "out"), tensor_arg(args[1], "scale"), tensor_arg(args[2], "x"),
-                optional_tensor_arg(args[3], "num_tokens"), optional_tensor_arg(args[4], "offsets"),
-                PyObject_IsTrue(args[5]) == 1);
+  const at::Tensor &out = tensor_arg(args[0], "out"), &scale = tensor_arg(args[1], "scale"), &x = tensor_arg(args[2], "x");
+  const at::Tensor *num_tokens = optional_tensor_arg(args[3], "num_tokens"), *offsets = optional_tensor_arg(args[4], "offsets");
+  const bool swiglu = PyObject_IsTrue(args[5]) == 1;
+  if (straight({&out, &scale, &x, num_tokens, offsets})) {
+    quantize_rows(out, scale, x, num_tokens, offsets, swiglu);
+  } else {
+    static auto op = op_handle<decltype(quantize_rows_op)>("pplx_kernels::quantize_rows");
+    at::Tensor to = out, to_scale = scale;
+    op.call(to, to_scale, x, maybe(num_tokens), maybe(offsets), swiglu);
+  }
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -728,9 +786,16 @@ PyObject *py_quantize_rows(PyObject *, PyObject *const *args, Py_ssize_t nargs) 
 PyObject *py_int8_matmul(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   arity("int8_matmul", nargs, 7);
-  int8_matmul(tensor_arg(args[0], "out"), tensor_arg(args[1], "x"), tensor_arg(args[2], "x_scale"),
-              tensor_arg(args[3], "weight"), tensor_arg(args[4], "weight_scale"), optional_tensor_arg(args[5], "num_tokens"),
-              optional_tensor_arg(args[6], "offsets"));
+  const at::Tensor &out = tensor_arg(args[0], "out"), &x = tensor_arg(args[1], "x"), &x_scale = tensor_arg(args[2], "x_scale"),
+                   &weight = tensor_arg(args[3], "weight"), &weight_scale = tensor_arg(args[4], "weight_scale");
+  const at::Tensor *num_tokens = optional_tensor_arg(args[5], "num_tokens"), *offsets = optional_tensor_arg(args[6], "offsets");
+  if (straight({&out, &x, &x_scale, &weight, &weight_scale, num_tokens, offsets})) {
+    int8_matmul(out, x, x_scale, weight, weight_scale, num_tokens, offsets);
+  } else {
+    static auto op = op_handle<decltype(int8_matmul_op)>("pplx_kernels::int8_matmul");
+    at::Tensor to = out;
+    op.call(to, x, x_scale, weight, weight_scale, maybe(num_tokens), maybe(offsets));
+  }
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }

@@ -7,9 +7,21 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
+from torch.utils._python_dispatch import TorchDispatchMode
 
-from pplx_kernels import ops, sort_tokens, unsort_tokens, unsort_tokens_backward
+from pplx_kernels import (
+    SortedTokens,
+    int8_matmul,
+    ops,
+    quantize_rows,
+    sort_tokens,
+    sort_tokens_backward,
+    unsort_tokens,
+    unsort_tokens_backward,
+)
 from tests.test_capi_cpu import _gpu_kernels_of
 from tests.test_experts import (
     BF16,
@@ -127,6 +139,83 @@ def test_tangents_are_refused(device):
         d = forward_ad.make_dual(x.detach(), torch.ones_like(x))
         assert torch.equal(sort_tokens(d, idx, 1, int8=True).rows, sort_tokens(x.detach(), idx, 1, int8=True).rows)
     assert torch.equal(torch.autograd.grad(s.rows.sum(), x)[0], torch.full_like(x, 2))
+
+
+# ---------------------------------------------------------------------------
+# Modes, tracers and tensors that are more than their data
+# ---------------------------------------------------------------------------
+def every_call(x, idx, q, scale, weight, weight_scale, w):
+    """Each call of the operators, with results of its own and in the caller's."""
+    s = sort_tokens(x, idx, 3)
+    t = sort_tokens(x, idx, 3, int8=True)
+    room = SortedTokens(*(None if a is None else torch.empty_like(a) for a in (s.rows, None, s.slots, s.offsets, None)))
+    r = sort_tokens(x, idx, 3, out=room)
+    out = unsort_tokens(s.rows, s.slots, s.offsets, w)
+    gx = sort_tokens_backward(r.rows, r.slots)
+    gy, gw = unsort_tokens_backward(out, s.rows, s.slots, s.offsets, w)
+    into = unsort_tokens(s.rows, s.slots, s.offsets, w, out=torch.empty_like(x))
+    v, vs = quantize_rows(x)
+    y = int8_matmul(q, scale, weight, weight_scale)
+    return (*s[:1], *s[2:4], *t[:4], *r[:1], *r[2:4], out, gx, gy, gw, into, v, vs, y)
+
+
+CALLED = {"sorted_tokens": 2, "sort_tokens": 1, "unsort_tokens": 3, "unsort_tokens_backward": 1, "quantize_rows": 1, "int8_matmul": 1}
+
+
+def inputs_of_every_call(device, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    made = (torch.randn(6, 32, generator=gen), make_indices(6, 2, 3, gen, "mixed"),
+            torch.randint(-127, 128, (5, 48), generator=gen, dtype=torch.int8), torch.rand(5, generator=gen),
+            torch.randint(-127, 128, (7, 48), generator=gen, dtype=torch.int8), torch.rand(7, generator=gen),
+            torch.rand(6, 2, generator=gen))  # fmt: skip
+    return [t.to(device).view(torch.uint32) if i == 1 else t.to(device) for i, t in enumerate(made)]
+
+
+def ops_called(graph) -> dict:
+    names = [str(n.target).split(".")[1] for n in graph.graph.nodes if str(n.target).startswith("pplx_kernels.")]
+    return {name: names.count(name) for name in set(names)}
+
+
+def test_modes_and_traces_see_the_calls():
+    """Without a device: tensors that have none of their data, and a trace of a graph that needs no compiler."""
+    with FakeTensorMode():
+        args = [torch.empty(t.shape, dtype=t.dtype, device="cuda") for t in inputs_of_every_call("cpu")]
+        got = every_call(*args)
+        assert got[0].shape == (12, 32) and got[-1].shape == (5, 7) and got[-1].dtype == BF16
+        assert ops_called(make_fx(every_call)(*args)) == CALLED
+
+
+@gpu
+def test_traced_graphs_hold_the_calls(device):
+    """What make_fx traces on real tensors computes the same on others."""
+    graph = make_fx(every_call)(*inputs_of_every_call(device))
+    assert ops_called(graph) == CALLED
+    for seed in (1, 2):
+        args = inputs_of_every_call(device, seed)
+        want = every_call(*args)
+        torch.full((1 << 20,), float("nan"), device=device)  # (memory that the results may get)
+        got = graph(*args)
+        n = int(want[2][-1])
+        for i, (a, b) in enumerate(zip(got, want)):
+            assert torch.equal(a, b), i
+        assert n == int(got[2][-1])
+
+
+@gpu
+def test_a_mode_sees_the_calls(device):
+    seen = []
+
+    class Mode(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(func.name())
+            return func(*args, **(kwargs or {}))
+
+    args = inputs_of_every_call(device)
+    want = every_call(*args)
+    with Mode():
+        got = every_call(*args)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert {name: seen.count(f"pplx_kernels::{name}") for name in CALLED} == CALLED
 
 
 # ---------------------------------------------------------------------------
