@@ -512,7 +512,6 @@ struct SortFunction : torch::autograd::Function<SortFunction> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x,
                                                 const at::Tensor &indices, int64_t experts,
                                                 const std::optional<at::Tensor> &bound_m) {
-    TORCH_CHECK(x.dim() == 2 && x.sym_size(1) % 8 == 0, "x must have rows of a multiple of 8 elements for its gradient");
     auto [rows, scale, slots, offsets] = call_sorted_tokens(x, indices, experts, bound_m, false);
     ctx->save_for_backward({slots});
     ctx->mark_non_differentiable({scale, slots, offsets});
@@ -574,6 +573,9 @@ SortedTuple sorted_tokens_autograd(const at::Tensor &x, const at::Tensor &indice
                                    bool int8) {
   if (int8) return call_sorted_tokens(x, indices, experts, bound_m, true);
   check_no_tangent({&x});
+  if (at::GradMode::is_enabled() && x.requires_grad()) {
+    TORCH_CHECK(x.dim() == 2 && x.sym_size(1) % 8 == 0, "x must have rows of a multiple of 8 elements for its gradient");
+  }
   auto made = SortFunction::apply(x, indices, experts, bound_m);
   return {made[0], made[1], made[2], made[3]};
 }

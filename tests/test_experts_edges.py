@@ -218,6 +218,32 @@ def test_a_mode_sees_the_calls(device):
     assert {name: seen.count(f"pplx_kernels::{name}") for name in CALLED} == CALLED
 
 
+def test_rows_without_a_gradient_need_no_multiple_of_eight():
+    """Rows of 12 fp32 elements have a sort and no gradient of it: the registered op takes them unless one is recorded."""
+    def call(x):
+        return torch.ops.pplx_kernels.sorted_tokens(x, torch.empty(4, 2, dtype=torch.uint32, device="meta"), 3, None, False)
+
+    x = torch.empty(4, 12, device="meta")
+    assert call(x)[0].shape == (8, 12)
+    x.requires_grad_(True)
+    with torch.no_grad():
+        assert call(x)[0].shape == (8, 12)
+    with pytest.raises(RuntimeError, match="multiple of 8"):
+        call(x)
+
+
+@gpu
+def test_traced_rows_without_a_gradient_need_no_multiple_of_eight(device):
+    x, idx = torch.randn(4, 12, device=device), torch.zeros(4, 2, dtype=torch.uint32, device=device)
+    call = torch.compile(lambda a: sort_tokens(a, idx, 3).rows, backend="aot_eager", fullgraph=True)
+    assert torch.equal(call(x), sort_tokens(x, idx, 3).rows)
+    x.requires_grad_(True)
+    with torch.no_grad():
+        assert torch.equal(call(x), sort_tokens(x, idx, 3).rows)
+    with pytest.raises(Exception, match="multiple of 8"):
+        call(x)
+
+
 # ---------------------------------------------------------------------------
 # What the kernels take of a workgroup
 # ---------------------------------------------------------------------------
