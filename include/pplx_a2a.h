@@ -377,7 +377,7 @@ typedef struct pplx_a2a_unsort_args {
   int64_t y_rows;
   const int32_t *slots;      /* [m, K] contiguous */
   const float *weights;      /* [m, K] contiguous or NULL */
-  uint32_t m;
+  uint32_t m;                /* m * experts_per_token and m * ceil(hidden_dim / 512) are below 2^31 */
   uint32_t experts_per_token; /* 1..64 */
   uint64_t hidden_dim;       /* a multiple of 8 */
 } pplx_a2a_unsort_args_t;
@@ -401,7 +401,7 @@ typedef struct pplx_a2a_unsort_backward_args {
   const int32_t *slots;       /* [m, K] contiguous */
   const int32_t *num_rows;    /* device scalar: live rows, which is offsets + num_experts */
   const float *weights;       /* [m, K] contiguous or NULL (ones) */
-  uint32_t m;
+  uint32_t m;                 /* as above */
   uint32_t experts_per_token; /* 1..64 */
   uint64_t hidden_dim;        /* a multiple of 8 */
 } pplx_a2a_unsort_backward_args_t;

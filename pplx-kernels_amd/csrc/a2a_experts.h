@@ -50,6 +50,23 @@ template <class Fn> int with_type(int32_t dtype, Fn &&fn) {
   }
 }
 
+// A grid of any number of workgroups: a launch takes fewer than 2^32 threads along a dimension, so that more go out in several,
+// whose first argument's first_group is the number of the first one.  Those behind the first launch may be of another
+// kernel.
+template <typename A, typename... P, typename... R>
+int launch_groups(void (*kernel)(A, P...), void (*later)(A, P...), uint64_t groups, uint32_t threads, uint32_t lds, hipStream_t s,
+                  A a, const R &...rest) {
+  const uint64_t most = 0xffffffffu / threads;
+  for (uint64_t first = 0; first < groups; first += most) {
+    a.first_group = (uint32_t)first;
+    const uint64_t left = groups - first;
+    const int err =
+        launch_kernel(first ? later : kernel, dim3((uint32_t)(left < most ? left : most)), dim3(threads), lds, s, a, rest...);
+    if (err) return err;
+  }
+  return 0;
+}
+
 // ---------------------------------------------------------------------------
 // Eight consecutive elements as fp32 and back (rounded to nearest, ties to even)
 // ---------------------------------------------------------------------------

@@ -31,6 +31,7 @@ struct MatmulDev {
   const float *weight_scale;
   uint32_t n, k;
   uint32_t n_blocks;
+  uint32_t first_group;    // of the split forms
   uint32_t large_weights;  // more than the last-level cache is likely to hold until they are read again
 };
 
@@ -526,18 +527,18 @@ template <int RF, int CF, int AHEAD, class O> __global__ __launch_bounds__(kSpli
   extern __shared__ uint32_t upto[];
   __shared__ uint32_t of_wave[kSplitWaves];
   __shared__ int32_t sums[kSplitWaves][RF * CF * 4 * 64];
-  const uint32_t lane = lane_id(), wave = wave_id();
+  const uint32_t lane = lane_id(), wave = wave_id(), group = a.first_group + blockIdx.x;
   Tile t;
   if (a.rows.layout == PPLX_A2A_ROWS_DENSE) {
     t.e = t.begin = 0;
     t.count = a.rows.rows;
-    const uint32_t block = blockIdx.x / a.n_blocks;
+    const uint32_t block = group / a.n_blocks;
     t.m0 = block * kRows;
-    t.n0 = (blockIdx.x - block * a.n_blocks) * kColumns;
+    t.n0 = (group - block * a.n_blocks) * kColumns;
   } else {
     sum_blocks<kSplitWaves * 64, kRows>(a.rows, upto, of_wave);
-    if (blockIdx.x >= upto[a.rows.experts - 1] * a.n_blocks) return;
-    t = tile_of<kRows, kColumns>(a.rows, a.n_blocks, upto, blockIdx.x);
+    if (group >= upto[a.rows.experts - 1] * a.n_blocks) return;
+    t = tile_of<kRows, kColumns>(a.rows, a.n_blocks, upto, group);
     if (t.m0 >= t.count || t.n0 >= a.n) return;  // (offsets that do not ascend)
   }
   const int8_t *x_first = a.x + (int64_t)t.e * a.x_stride_expert + (int64_t)(t.begin + t.m0) * a.x_stride_row;
@@ -638,7 +639,8 @@ template <int RF, int CF, int AHEAD, class O> int launch_split(const MatmulDev &
   a.n_blocks = (a.n + 16 * CF - 1) / (16 * CF);
   const uint64_t tiles = most_blocks * a.n_blocks;
   if (tiles >= (1ull << 31)) return refuse(PPLX_A2A_UNSUPPORTED, "too many tiles");
-  PPLX_LAUNCH(launch_kernel(matmul_split<RF, CF, AHEAD, O>, dim3((uint32_t)tiles), dim3(kSplitWaves * 64), 4 * a.rows.experts, s, a));
+  auto kernel = matmul_split<RF, CF, AHEAD, O>;
+  PPLX_LAUNCH(launch_groups(kernel, kernel, tiles, kSplitWaves * 64, 4 * a.rows.experts, s, a));
   return PPLX_A2A_OK;
 }
 

@@ -15,6 +15,7 @@ struct QuantizeDev {
   const uint8_t *x;
   int64_t x_stride_row, x_stride_expert;
   uint32_t width;
+  uint32_t first_group;
 };
 
 // What one thread holds of a row: PIECES times eight elements, eight elements apart from the next thread's.
@@ -96,7 +97,8 @@ __global__ __launch_bounds__(256) void quantize_flat(QuantizeDev a) {
     const int32_t last = as_global(a.rows.starts_or_counts)[a.rows.experts];
     there = last < 0 ? 0 : (uint32_t)last < there ? (uint32_t)last : there;
   }
-  const uint32_t r = LANES == 64 ? blockIdx.x * 4 + wave_id() : blockIdx.x;
+  const uint32_t group = a.first_group + blockIdx.x;
+  const uint32_t r = LANES == 64 ? group * 4 + wave_id() : group;
   if (r < there) quantize_one<T, SWIGLU, LANES, PIECES, NT>(a, 0, r, threadIdx.x % LANES);
 }
 
@@ -152,7 +154,7 @@ template <class T, bool SWIGLU, int LANES, int PIECES> int launch_quantize(const
     // (253.5).
     const bool large = (uint64_t)a.rows.rows * a.width * sizeof(T) * (SWIGLU ? 2 : 1) > kStreamBytes && a.width <= 8 * PIECES * LANES;
     auto kernel = large ? quantize_flat<T, SWIGLU, LANES, PIECES, true> : quantize_flat<T, SWIGLU, LANES, PIECES, false>;
-    PPLX_LAUNCH(launch_kernel(kernel, dim3((a.rows.rows + kAtOnce - 1) / kAtOnce), dim3(256), 0, s, a));
+    PPLX_LAUNCH(launch_groups(kernel, kernel, (a.rows.rows + kAtOnce - 1) / kAtOnce, 256, 0, s, a));
   }
   return PPLX_A2A_OK;
 }

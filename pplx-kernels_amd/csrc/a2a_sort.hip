@@ -24,6 +24,7 @@ struct SortDev {
   uint32_t m, K, E, width;  // width: elements of a row
   uint32_t row_vecs;        // 16-byte vectors of a row of x
   uint32_t tile, tiles;     // picks of a tile, tiles
+  uint32_t first_group;
 };
 
 __device__ __forceinline__ uint32_t tokens_there(const SortDev &a) {
@@ -358,11 +359,13 @@ __global__ __launch_bounds__(WAVES * 64) void sort_slots(SortDev a, uint32_t id_
   }
 }
 
-// Third launch: the rows.
-template <int LANES, class T>
+// Third launch: the rows.  LATER: workgroups behind those of one launch.  (Two scalar instructions that add first_group, a
+// zero, to the number of the workgroup cost 8192 tokens x 8 rows of 14 KiB 6 of 195 us, in whatever way they are written.)
+template <int LANES, class T, bool LATER>
 __global__ __launch_bounds__(256) void sort_rows(SortDev a) {
   const uint32_t lane = lane_id();
-  const uint32_t t = LANES == 64 ? blockIdx.x * 4 + wave_id() : blockIdx.x;
+  const uint32_t group = LATER ? a.first_group + blockIdx.x : blockIdx.x;
+  const uint32_t t = LANES == 64 ? group * 4 + wave_id() : group;
   if (t >= a.m) return;  // (with 256 lanes to a row the grid has one workgroup a token)
   const uint32_t total = (uint32_t)as_global(a.offsets)[a.E];
   const int32_t slot = lane < a.K ? as_global(a.slots)[(size_t)t * a.K + lane] : -1;
@@ -405,7 +408,7 @@ template <int LANES, class T> int launch_sort(const SortDev &a, hipStream_t s) {
   if (waves == 16) PPLX_LAUNCH(launch_kernel(sort_slots<16>, grid, block, lds, s, a, bits));
   else if (waves == 8) PPLX_LAUNCH(launch_kernel(sort_slots<8>, grid, block, lds, s, a, bits));
   else PPLX_LAUNCH(launch_kernel(sort_slots<2>, grid, block, lds, s, a, bits));
-  PPLX_LAUNCH(launch_kernel(sort_rows<LANES, T>, dim3(LANES == 64 ? (a.m + 3) / 4 : a.m), dim3(256), 0, s, a));
+  PPLX_LAUNCH(launch_groups(sort_rows<LANES, T, false>, sort_rows<LANES, T, true>, LANES == 64 ? (a.m + 3) / 4 : a.m, 256, 0, s, a));
   return PPLX_A2A_OK;
 }
 

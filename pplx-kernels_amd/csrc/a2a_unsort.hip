@@ -17,6 +17,7 @@ struct UnsortDev {
   const int32_t *slots;
   const float *weights;
   uint32_t m, K, width;
+  uint32_t first_group;
 };
 
 // Where the eight elements of a lane lie in a piece of 512: together where they are 16 bytes, in two halves of the piece where
@@ -62,7 +63,7 @@ __device__ __forceinline__ void gather_some(const UnsortDev &a, int32_t slot, fl
 template <class Y, class O, bool NT>
 __global__ __launch_bounds__(256) void unsort_gather(UnsortDev a, uint32_t pieces, FastDiv by_pieces) {
   const uint32_t lane = lane_id();
-  const uint32_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + threadIdx.x / kWave);
+  const uint32_t wave = __builtin_amdgcn_readfirstlane((a.first_group + blockIdx.x) * 4 + threadIdx.x / kWave);
   const uint32_t t = fast_div(wave, by_pieces);
   if (t >= a.m) return;
   const uint32_t piece = (wave - t * pieces) * 512;
@@ -115,6 +116,7 @@ struct UnsortBackwardDev {
   const int32_t *num_rows;
   const float *weights;
   uint32_t m, K, width;
+  uint32_t first_group;
   uint32_t sweeps, sweep_rows;  // workgroups in front of the tokens', rows of grad_y that one looks at
 };
 
@@ -149,7 +151,7 @@ template <uint32_t AT_ONCE, class Fn> __device__ __forceinline__ void for_slots(
 
 template <class T> __device__ void clear_unnamed(const UnsortBackwardDev &a, uint32_t total, uint32_t *named) {
   const uint32_t rows = total < a.y_rows ? total : a.y_rows;
-  const uint32_t first = blockIdx.x * a.sweep_rows;
+  const uint32_t first = (a.first_group + blockIdx.x) * a.sweep_rows;
   if (first >= rows) return;
   const uint32_t count = rows - first < a.sweep_rows ? rows - first : a.sweep_rows;
   uint32_t own = 0;
@@ -192,12 +194,12 @@ __global__ __launch_bounds__(256) void unsort_backward(UnsortBackwardDev a) {
   constexpr int kPicks = 8;
   const uint32_t lane = lane_id(), wave = wave_id(), g = threadIdx.x % LANES;
   __shared__ uint32_t named[kMaxSweepRows / 32];
-  if (blockIdx.x < a.sweeps) {
+  if (a.first_group + blockIdx.x < a.sweeps) {
     const int32_t live_rows = *as_global(a.num_rows);
     clear_unnamed<T>(a, live_rows > 0 ? (uint32_t)live_rows : 0u, named);
     return;
   }
-  const uint32_t group = blockIdx.x - a.sweeps;
+  const uint32_t group = a.first_group + blockIdx.x - a.sweeps;
   const uint32_t t = LANES == 64 ? group * 4 + wave : group;
   if (t >= a.m) return;  // (with 256 lanes to a token the grid has one workgroup a token)
   int32_t slot = -1;
@@ -293,7 +295,7 @@ int check_unsort_size(uint64_t m, uint64_t K, uint64_t hidden_dim, int64_t y_row
   PPLX_REQUIRE(hidden_dim > 0 && hidden_dim < (1ull << 28) && hidden_dim % 8 == 0,
                "hidden_dim must be a multiple of 8 below 2^28");
   PPLX_REQUIRE(y_rows >= 0 && y_rows < (1ll << 31), "y must have fewer than 2^31 rows");
-  if (m * K >= (1ull << 31) || m * ((hidden_dim + 511) / 512) >= (1ull << 32))
+  if (m * K >= (1ull << 31) || m * ((hidden_dim + 511) / 512) >= (1ull << 31))
     return refuse(PPLX_A2A_UNSUPPORTED, "too many picks or elements");
   return PPLX_A2A_OK;
 }
@@ -333,7 +335,7 @@ extern "C" int pplx_a2a_unsort_tokens(int device, const pplx_a2a_unsort_args_t *
   a.K = p.experts_per_token;
   a.width = (uint32_t)p.hidden_dim;
   const uint32_t pieces = (a.width + 511) / 512;
-  const dim3 grid((uint32_t)(((uint64_t)a.m * pieces + 3) / 4));
+  const uint64_t groups = ((uint64_t)a.m * pieces + 3) / 4;
   return guarded(device, [&] {
     return with_type(p.y_dtype, [&](auto y) {
       return with_type(p.out_dtype, [&](auto out) {
@@ -345,7 +347,7 @@ extern "C" int pplx_a2a_unsort_tokens(int device, const pplx_a2a_unsort_args_t *
         // 8192 of 4096 (67 MB) 26.7 / 20.6 / 23.0, 1024 x 2 of 7168 8.6 / 8.2 / 8.9.  Large ones run at 6.0 TB/s.
         const uint64_t bytes = (uint64_t)a.m * a.K * a.width * sizeof(Y);
         auto kernel = bytes > kStreamRowsBytes ? unsort_gather<Y, O, true> : unsort_gather<Y, O, false>;
-        PPLX_LAUNCH(launch_kernel(kernel, grid, dim3(256), 0, (hipStream_t)stream, a, pieces, make_fast_div(pieces)));
+        PPLX_LAUNCH(launch_groups(kernel, kernel, groups, 256, 0, (hipStream_t)stream, a, pieces, make_fast_div(pieces)));
         return (int)PPLX_A2A_OK;
       });
     });
@@ -405,8 +407,8 @@ extern "C" int pplx_a2a_unsort_tokens_backward(int device, const pplx_a2a_unsort
         auto launch = [&](auto lanes) {
           constexpr int L = decltype(lanes)::value;
           auto kernel = large ? unsort_backward<Y, G, L, true> : unsort_backward<Y, G, L, false>;
-          const uint32_t groups = a.sweeps + (L == 64 ? (a.m + 3) / 4 : a.m);
-          PPLX_LAUNCH(launch_kernel(kernel, dim3(groups), dim3(256), 0, (hipStream_t)stream, a));
+          const uint64_t groups = (uint64_t)a.sweeps + (L == 64 ? (a.m + 3) / 4 : a.m);
+          PPLX_LAUNCH(launch_groups(kernel, kernel, groups, 256, 0, (hipStream_t)stream, a));
           return (int)PPLX_A2A_OK;
         };
         return a.width <= 1024 ? launch(std::integral_constant<int, 64>{}) : launch(std::integral_constant<int, 256>{});

@@ -245,6 +245,63 @@ def test_traced_rows_without_a_gradient_need_no_multiple_of_eight(device):
 
 
 # ---------------------------------------------------------------------------
+# More workgroups than a launch takes threads for along one dimension
+# ---------------------------------------------------------------------------
+@gpu
+def test_more_tokens_than_one_line_of_workgroups(device):
+    """2^26 tokens and a few, four to a workgroup of 256 threads: sorted, back again, and the gradient of that."""
+    m, experts = (1 << 26) + 5, 8
+    gen = torch.Generator(device).manual_seed(1)
+    x = torch.randint(-(1 << 15), 1 << 15, (m, 8), dtype=torch.int16, device=device, generator=gen).view(BF16)
+    idx = torch.randint(0, experts, (m, 1), dtype=torch.int32, device=device, generator=gen)
+    s = sort_tokens(x, idx.view(torch.uint32), experts)
+    order = torch.argsort(idx[:, 0], stable=True)
+    assert torch.equal(s.slots[:, 0][order], torch.arange(m, dtype=torch.int32, device=device))
+    # (in pieces: torch's own gather of 2^26 rows of 16 bytes at once leaves the last ones as zeros)
+    for rows, picked in zip(s.rows.view(torch.int16).split(1 << 22), order.split(1 << 22)):
+        assert torch.equal(rows, x.view(torch.int16)[picked])
+    del order, rows, picked
+    x = torch.randn(m, 8, dtype=F32, device=device, generator=gen).to(BF16)
+    sort_tokens(x, idx.view(torch.uint32), experts, out=s)
+    assert torch.equal(unsort_tokens(s.rows, s.slots, s.offsets), x)
+    grad_y, grad_w = torch.empty_like(s.rows), torch.empty(m, 1, device=device)
+    unsort_tokens_backward(x, s.rows, s.slots, s.offsets, out=(grad_y, grad_w))
+    assert torch.equal(grad_y, s.rows)
+    for a in (0, m - 1000):
+        size = (x[a : a + 1000].double() ** 2).sum(1, keepdim=True).cpu()
+        assert_within(grad_w[a : a + 1000], size, 9 * U32 * size)
+
+
+@gpu
+def test_more_tokens_than_one_line_of_workgroups_one_to_each(device):
+    """2^24 tokens and a few, one to a workgroup."""
+    m, hidden = (1 << 24) + 3, 1032
+    gen = torch.Generator().manual_seed(2)
+    y, grad = torch.randn(64, hidden, generator=gen).to(BF16).to(device), torch.randn(1, hidden, generator=gen).to(BF16).to(device)
+    slots = (torch.arange(m, dtype=torch.int32, device=device) % 64)[:, None]
+    offsets = torch.tensor([0, 64], dtype=torch.int32, device=device)
+    got, few = torch.empty(m, 1, device=device), torch.empty(64, 1, device=device)
+    unsort_tokens_backward(grad.expand(m, hidden), y, slots, offsets, out=(None, got))
+    unsort_tokens_backward(grad.expand(64, hidden), y, slots[:64], offsets, out=(None, few))
+    assert all(torch.equal(part, few.repeat(1 << 14, 1)[: part.shape[0]]) for part in got.split(64 << 14))
+    # the sort, of rows in 8 bits
+    wide = torch.randn(1, 2064, generator=gen).to(BF16).to(device)
+    s = sort_tokens(wide.expand(m, 2064), torch.zeros(m, 1, dtype=torch.uint32, device=device), 1, int8=True)
+    q, scale = quantize_rows(wide)
+    assert all(bool((part == q).all()) for part in s.rows.split(1 << 20)) and bool((s.scale == scale).all())
+
+
+@gpu
+def test_more_rows_than_one_line_of_workgroups(device):
+    rows = (1 << 26) + 7
+    x = torch.empty(rows, 16, dtype=BF16, device=device).normal_(generator=torch.Generator(device).manual_seed(3))
+    q, scale = quantize_rows(x)
+    for part, q_part, scale_part in zip(x.split(1 << 22), q.split(1 << 22), scale.split(1 << 22)):
+        want, want_scale = quantize_rows(part)
+        assert torch.equal(q_part, want) and torch.equal(scale_part, want_scale)
+
+
+# ---------------------------------------------------------------------------
 # What the kernels take of a workgroup
 # ---------------------------------------------------------------------------
 def test_product_tiles_begin_at_the_first_byte_of_lds():
