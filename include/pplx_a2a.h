@@ -465,6 +465,15 @@ typedef struct pplx_a2a_int8_matmul_args {
 } pplx_a2a_int8_matmul_args_t;
 int pplx_a2a_int8_matmul(int device, const pplx_a2a_int8_matmul_args_t *args, void *stream);
 
+/* Which form a product takes (rows->starts_or_counts is not looked at; no GPU needed). */
+typedef struct pplx_a2a_int8_matmul_plan {
+  uint32_t tile_rows, tile_columns; /* of the result, to a workgroup at a time; 0 where there is nothing to do */
+  int32_t split;                    /* the waves of a workgroup share out k, and it takes one tile */
+  uint32_t workgroups;
+  uint64_t tiles;                   /* at most: as the rows of the experts spread */
+} pplx_a2a_int8_matmul_plan_t;
+int pplx_a2a_int8_matmul_plan(const pplx_a2a_rows_t *rows, uint64_t n, uint64_t k, pplx_a2a_int8_matmul_plan_t *out);
+
 /* ---- misc -------------------------------------------------------------- */
 
 const char *pplx_a2a_last_error(void);

@@ -245,19 +245,24 @@ __device__ __forceinline__ Span span_of(const RowsDev &r, uint32_t e) {
   return Span{a, b > a ? b - a : 0};
 }
 
-inline int check_rows(const pplx_a2a_rows_t &r, RowsDev *out) {
+inline int check_row_numbers(const pplx_a2a_rows_t &r, RowsDev *out) {
   PPLX_REQUIRE(r.layout == PPLX_A2A_ROWS_DENSE || r.layout == PPLX_A2A_ROWS_SORTED || r.layout == PPLX_A2A_ROWS_PADDED,
                "unknown layout of rows");
   PPLX_REQUIRE(r.num_experts >= 1 && r.num_experts <= kMaxExperts, "num_experts must be in [1, %u]", kMaxExperts);
   PPLX_REQUIRE(r.layout != PPLX_A2A_ROWS_DENSE || r.num_experts == 1, "rows without offsets or counts have one expert");
-  PPLX_REQUIRE(r.layout == PPLX_A2A_ROWS_DENSE || (r.starts_or_counts && is_aligned(r.starts_or_counts, 4)),
-               "starts_or_counts is NULL or not aligned");
   const uint64_t per = r.layout == PPLX_A2A_ROWS_PADDED ? r.num_experts : 1;
   if (r.rows >= (1ull << 31) / per) return refuse(PPLX_A2A_UNSUPPORTED, "2^31 rows or more");
-  out->starts_or_counts = r.starts_or_counts;
   out->rows = (uint32_t)r.rows;
   out->experts = r.num_experts;
   out->layout = r.layout;
+  return PPLX_A2A_OK;
+}
+inline int check_rows(const pplx_a2a_rows_t &r, RowsDev *out) {
+  const int st = check_row_numbers(r, out);
+  if (st) return st;
+  PPLX_REQUIRE(r.layout == PPLX_A2A_ROWS_DENSE || (r.starts_or_counts && is_aligned(r.starts_or_counts, 4)),
+               "starts_or_counts is NULL or not aligned");
+  out->starts_or_counts = r.starts_or_counts;
   return PPLX_A2A_OK;
 }
 

@@ -495,8 +495,9 @@ __global__ __launch_bounds__(WM *WN * 64) void matmul_tiles(MatmulDev) {
 
 constexpr uint32_t kComputeUnits = 256;
 
+// Launches take a plan to fill instead, or NULL.
 template <int BM, int BN, int WM, int WN, int BK, int STAGES, class O>
-int launch_tiles(const MatmulDev &from, uint64_t most_blocks, hipStream_t s) {
+int launch_tiles(const MatmulDev &from, uint64_t most_blocks, hipStream_t s, pplx_a2a_int8_matmul_plan_t *plan) {
   MatmulDev a = from;
   constexpr uint32_t kTileLds = STAGES * (BM + BN) * BK;
   const uint32_t lds = kTileLds + 4 * (BM + BN) + 4 * a.rows.experts + 4 * WM * WN;
@@ -507,6 +508,10 @@ int launch_tiles(const MatmulDev &from, uint64_t most_blocks, hipStream_t s) {
   if (tiles >= (1ull << 31)) return refuse(PPLX_A2A_UNSUPPORTED, "too many tiles");
   uint64_t grid = per_unit * kComputeUnits;
   grid = tiles < grid ? (tiles + 7) / 8 * 8 : grid;  // (whole rounds of the XCDs)
+  if (plan) {
+    *plan = {BM, BN, 0, (uint32_t)grid, tiles};
+    return PPLX_A2A_OK;
+  }
   auto kernel = a.k % BK ? matmul_tiles<BM, BN, WM, WN, BK, STAGES, true, O> : matmul_tiles<BM, BN, WM, WN, BK, STAGES, false, O>;
   if (lds > 64 * 1024) {
     const hipError_t err =
@@ -634,11 +639,16 @@ template <int RF, int CF, int AHEAD, class O> __global__ __launch_bounds__(kSpli
   }
 }
 
-template <int RF, int CF, int AHEAD, class O> int launch_split(const MatmulDev &from, uint64_t most_blocks, hipStream_t s) {
+template <int RF, int CF, int AHEAD, class O>
+int launch_split(const MatmulDev &from, uint64_t most_blocks, hipStream_t s, pplx_a2a_int8_matmul_plan_t *plan) {
   MatmulDev a = from;
   a.n_blocks = (a.n + 16 * CF - 1) / (16 * CF);
   const uint64_t tiles = most_blocks * a.n_blocks;
   if (tiles >= (1ull << 31)) return refuse(PPLX_A2A_UNSUPPORTED, "too many tiles");
+  if (plan) {
+    *plan = {16 * RF, 16 * CF, 1, (uint32_t)tiles, tiles};
+    return PPLX_A2A_OK;
+  }
   auto kernel = matmul_split<RF, CF, AHEAD, O>;
   PPLX_LAUNCH(launch_groups(kernel, kernel, tiles, kSplitWaves * 64, 4 * a.rows.experts, s, a));
   return PPLX_A2A_OK;
@@ -698,7 +708,7 @@ int matmul_form(const MatmulDev &a) {
   return best;
 }
 
-template <class O> int launch_matmul(const MatmulDev &a, hipStream_t s) {
+template <class O> int launch_matmul(const MatmulDev &a, hipStream_t s, pplx_a2a_int8_matmul_plan_t *plan = nullptr) {
   const uint64_t E = a.rows.experts;
   auto most_blocks = [&](uint64_t bm) -> uint64_t {  // that the rows of all experts can make
     const uint64_t rows = a.rows.rows;
@@ -706,15 +716,15 @@ template <class O> int launch_matmul(const MatmulDev &a, hipStream_t s) {
     return (rows + bm - 1) / bm + (E < rows ? E : rows) - 1;
   };
   switch (matmul_form(a)) {
-    case 0: return launch_split<1, 1, 4, O>(a, most_blocks(16), s);
-    case 1: return launch_split<1, 2, 4, O>(a, most_blocks(16), s);
-    case 2: return launch_split<2, 2, 2, O>(a, most_blocks(32), s);
-    case 3: return launch_tiles<32, 128, 1, 4, 128, 3, O>(a, most_blocks(32), s);
-    case 4: return launch_tiles<64, 128, 1, 4, 128, 3, O>(a, most_blocks(64), s);
-    case 5: return launch_tiles<128, 128, 2, 2, 64, 4, O>(a, most_blocks(128), s);
-    case 6: return launch_tiles<128, 256, 2, 4, 64, 4, O>(a, most_blocks(128), s);
-    case 7: return launch_tiles<256, 256, 2, 4, 64, 4, O>(a, most_blocks(256), s);
-    default: return launch_tiles<64, 256, 1, 4, 128, 3, O>(a, most_blocks(64), s);
+    case 0: return launch_split<1, 1, 4, O>(a, most_blocks(16), s, plan);
+    case 1: return launch_split<1, 2, 4, O>(a, most_blocks(16), s, plan);
+    case 2: return launch_split<2, 2, 2, O>(a, most_blocks(32), s, plan);
+    case 3: return launch_tiles<32, 128, 1, 4, 128, 3, O>(a, most_blocks(32), s, plan);
+    case 4: return launch_tiles<64, 128, 1, 4, 128, 3, O>(a, most_blocks(64), s, plan);
+    case 5: return launch_tiles<128, 128, 2, 2, 64, 4, O>(a, most_blocks(128), s, plan);
+    case 6: return launch_tiles<128, 256, 2, 4, 64, 4, O>(a, most_blocks(128), s, plan);
+    case 7: return launch_tiles<256, 256, 2, 4, 64, 4, O>(a, most_blocks(256), s, plan);
+    default: return launch_tiles<64, 256, 1, 4, 128, 3, O>(a, most_blocks(64), s, plan);
   }
 }
 
@@ -723,15 +733,35 @@ template <class O> int launch_matmul(const MatmulDev &a, hipStream_t s) {
 
 using namespace pplx_amd;
 
+namespace {
+int check_matmul_size(uint64_t n, uint64_t k) {
+  PPLX_REQUIRE(n < (1ull << 31), "n must be below 2^31");
+  PPLX_REQUIRE(k > 0 && k % 16 == 0 && k <= 131056, "k must be a multiple of 16 in [16, 131056]");
+  return PPLX_A2A_OK;
+}
+}  // namespace
+
+extern "C" int pplx_a2a_int8_matmul_plan(const pplx_a2a_rows_t *rows, uint64_t n, uint64_t k, pplx_a2a_int8_matmul_plan_t *out) {
+  PPLX_REQUIRE(rows && out, "rows or out is NULL");
+  MatmulDev a{};
+  int st = check_row_numbers(*rows, &a.rows);
+  if (!st) st = check_matmul_size(n, k);
+  if (st) return st;
+  a.n = (uint32_t)n;
+  a.k = (uint32_t)k;
+  *out = {};
+  return a.rows.rows == 0 || n == 0 ? (int)PPLX_A2A_OK : launch_matmul<float>(a, nullptr, out);
+}
+
 extern "C" int pplx_a2a_int8_matmul(int device, const pplx_a2a_int8_matmul_args_t *args, void *stream) {
   PPLX_REQUIRE(args, "args is NULL");
   const pplx_a2a_int8_matmul_args_t &p = *args;
   MatmulDev a{};
-  const int st = check_rows(p.rows, &a.rows);
+  int st = check_rows(p.rows, &a.rows);
   if (st) return st;
   PPLX_REQUIRE(is_dtype(p.out_dtype), "unsupported dtype of out");
-  PPLX_REQUIRE(p.n < (1ull << 31), "n must be below 2^31");
-  PPLX_REQUIRE(p.k > 0 && p.k % 16 == 0 && p.k <= 131056, "k must be a multiple of 16 in [16, 131056]");
+  st = check_matmul_size(p.n, p.k);
+  if (st) return st;
   if (p.rows.rows == 0 || p.n == 0) return PPLX_A2A_OK;
   PPLX_REQUIRE(p.out && p.x && p.x_scale && p.weight && p.weight_scale, "out / x / x_scale / weight / weight_scale is NULL");
   PPLX_REQUIRE(is_aligned(p.x, 16) && p.x_stride_row % 16 == 0 && p.x_stride_expert % 16 == 0,

@@ -76,6 +76,7 @@ EXPORTED_SYMBOLS = (
     "pplx_a2a_unsort_tokens_backward",
     "pplx_a2a_quantize_rows",
     "pplx_a2a_int8_matmul",
+    "pplx_a2a_int8_matmul_plan",
     "pplx_a2a_last_error",
     "pplx_a2a_version",
     "pplx_a2a_build_id",
@@ -116,6 +117,29 @@ class CombinePlan(ctypes.Structure):
         ("picks", ctypes.c_uint32),
         ("pieces", ctypes.c_uint32),
         ("per_group", ctypes.c_int32),
+    ]
+
+
+class Rows(ctypes.Structure):
+    """pplx_a2a_rows_t"""
+
+    _fields_ = [
+        ("layout", ctypes.c_int32),
+        ("num_experts", ctypes.c_uint32),
+        ("rows", ctypes.c_uint64),
+        ("starts_or_counts", ctypes.c_void_p),
+    ]
+
+
+class ProductPlan(ctypes.Structure):
+    """pplx_a2a_int8_matmul_plan_t"""
+
+    _fields_ = [
+        ("tile_rows", ctypes.c_uint32),
+        ("tile_columns", ctypes.c_uint32),
+        ("split", ctypes.c_int32),
+        ("workgroups", ctypes.c_uint32),
+        ("tiles", ctypes.c_uint64),
     ]
 
 
@@ -207,6 +231,9 @@ def load_library() -> ctypes.CDLL:
         ]  # fmt: skip
         lib.pplx_a2a_combine_plan.argtypes = [ctypes.POINTER(Config), i32, ctypes.POINTER(CombinePlan)]
         lib.pplx_a2a_combine_stores.argtypes = [ctypes.POINTER(Config), ctypes.POINTER(i32)]
+        lib.pplx_a2a_int8_matmul_plan.argtypes = [
+            ctypes.POINTER(Rows), ctypes.c_uint64, ctypes.c_uint64, ctypes.POINTER(ProductPlan),
+        ]  # fmt: skip
         lib.pplx_a2a_world_of.argtypes = [vp]
         lib.pplx_a2a_world_of.restype = vp
         lib.pplx_a2a_world_recorded_calls.argtypes = [vp, i32, i32, ctypes.POINTER(u32)]
@@ -260,6 +287,14 @@ def combine_stores_plainly(config: Config) -> bool:
     plain = ctypes.c_int32()
     check_status(load_library().pplx_a2a_combine_stores(ctypes.byref(config), ctypes.byref(plain)))
     return bool(plain.value)
+
+
+def product_plan_of(rows: int, n: int, k: int, experts: int = 1, layout: str = "dense") -> ProductPlan:
+    """Which form ``int8_matmul`` takes for rows in a "dense", "sorted" or "padded" layout, which then has ``rows`` rows for
+    each of its experts (no GPU needed)."""
+    plan, where = ProductPlan(), Rows(("dense", "sorted", "padded").index(layout), experts, rows, None)
+    check_status(load_library().pplx_a2a_int8_matmul_plan(ctypes.byref(where), n, k, ctypes.byref(plan)))
+    return plan
 
 
 def check_status(status: int) -> None:

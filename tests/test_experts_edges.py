@@ -34,6 +34,7 @@ from tests.test_experts import (
     rounded,
     to_u32,
 )
+from tests.test_experts_path import product64, random_int8
 
 gpu = pytest.mark.gpu
 
@@ -299,6 +300,122 @@ def test_more_rows_than_one_line_of_workgroups(device):
     for part, q_part, scale_part in zip(x.split(1 << 22), q.split(1 << 22), scale.split(1 << 22)):
         want, want_scale = quantize_rows(part)
         assert torch.equal(q_part, want) and torch.equal(scale_part, want_scale)
+
+
+# ---------------------------------------------------------------------------
+# Products whose workgroups take several tiles
+# ---------------------------------------------------------------------------
+SEVERAL_TILES = [
+    # tile, layout, experts, rows (padded: of each expert), n, k: odd and even n, k that fills the steps of its form and k that does not
+    ((32, 128), "dense", 1, 9, 65544, 128),
+    ((32, 128), "dense", 1, 9, 65537, 64),
+    ((32, 128), "sorted", 32, 33, 2057, 128),
+    ((32, 128), "sorted", 32, 33, 2056, 64),
+    ((32, 128), "padded", 4, 40, 8201, 64),
+    ((64, 128), "sorted", 16, 33, 2056, 2064),
+    ((64, 128), "sorted", 16, 33, 2057, 2064),
+    ((64, 128), "sorted", 8, 700, 2056, 1024),
+    ((64, 128), "sorted", 8, 700, 2057, 1024),
+    ((64, 128), "padded", 32, 257, 520, 272),
+    ((64, 256), "sorted", 4, 200, 16392, 528),
+    ((64, 256), "sorted", 4, 200, 16385, 528),
+    ((64, 256), "sorted", 32, 1500, 2056, 1024),
+    ((64, 256), "sorted", 32, 1500, 2057, 1024),
+    ((64, 256), "padded", 32, 520, 1000, 528),
+    ((128, 128), "dense", 1, 70, 65544, 64),
+    ((128, 128), "dense", 1, 70, 65537, 80),
+    ((128, 128), "sorted", 32, 1500, 2056, 80),
+    ((128, 128), "sorted", 32, 1500, 2057, 64),
+    ((128, 128), "padded", 4, 2000, 2057, 64),
+    ((128, 256), "sorted", 4, 257, 16392, 528),
+    ((128, 256), "sorted", 4, 257, 16385, 528),
+    ((128, 256), "sorted", 32, 2049, 2056, 1024),
+    ((128, 256), "sorted", 32, 2049, 2057, 1024),
+    ((128, 256), "padded", 16, 520, 2057, 272),
+    ((256, 256), "dense", 1, 700, 32776, 272),
+    ((256, 256), "dense", 1, 700, 32777, 512),
+    ((256, 256), "sorted", 16, 4999, 2056, 512),
+    ((256, 256), "sorted", 16, 4999, 2057, 528),
+    ((256, 256), "padded", 8, 2000, 4104, 64),
+]
+
+
+def rows_of_experts(layout, experts, rows):
+    if layout == "padded":
+        return [rows - e % 5 for e in range(experts)]
+    return [rows // experts + (e < rows % experts) for e in range(experts)]
+
+
+@pytest.mark.parametrize("tile,layout,experts,rows,n,k", SEVERAL_TILES)
+def test_the_products_of_several_tiles_are_that(tile, layout, experts, rows, n, k):
+    """Each size of the test below takes the form that it is there for, and more of its tiles than there are workgroups."""
+    plan = ops.product_plan_of(rows, n, k, experts, layout)
+    assert (plan.tile_rows, plan.tile_columns) == tile and not plan.split
+    columns = -(-n // tile[1])
+    tiles = sum(-(-c // tile[0]) for c in rows_of_experts(layout, experts, rows)) * columns
+    assert plan.workgroups < tiles <= plan.tiles
+
+
+def test_plans_of_products():
+    assert ops.product_plan_of(1, 1408, 2048).split == 1
+    nothing = ops.product_plan_of(0, 8, 16)
+    assert (nothing.tile_rows, nothing.workgroups, nothing.tiles) == (0, 0, 0)
+    for bad, message in (
+        (dict(rows=4, n=8, k=24), "multiple of 16"),
+        (dict(rows=4, n=8, k=131072), "131056"),
+        (dict(rows=4, n=1 << 31, k=16), "2\\^31"),
+        (dict(rows=4, n=8, k=16, experts=0, layout="sorted"), "num_experts"),
+        (dict(rows=4, n=8, k=16, experts=2), "one expert"),
+        (dict(rows=1 << 30, n=8, k=16, experts=2, layout="padded"), "2\\^31"),
+    ):
+        with pytest.raises(RuntimeError, match=message):
+            ops.product_plan_of(**bad)
+    lib = ops.load_library()
+    assert lib.pplx_a2a_int8_matmul_plan(None, 8, 16, None) == 1
+
+
+def test_the_products_of_several_tiles_are_of_every_kind():
+    steps = {(32, 128): 128, (64, 128): 128, (64, 256): 128, (128, 128): 64, (128, 256): 64, (256, 256): 64}
+    for tile, step in steps.items():
+        here = [(n % 2, k % step == 0) for t, _, _, _, n, k in SEVERAL_TILES if t == tile]
+        assert {odd for odd, _ in here} == {0, 1} and {full for _, full in here} == {True, False}
+        assert any(t == tile and layout == "padded" for t, layout, *_ in SEVERAL_TILES)
+
+
+def assert_product(got, ref):
+    """The sum becomes fp32, the scales are multiplied, and their product with the sum; then the result is rounded to its type.
+    (fp16 has no more than multiples of 2^-24 below 2^-14: off by 2^-25 there, which `rounded` counts.)"""
+    off = (got.double() - ref).abs() - rounded(ref, got.dtype, 3 * U32 * ref.abs())
+    assert float(off.max()) <= 0
+
+
+@gpu
+@pytest.mark.parametrize("tile,layout,experts,rows,n,k", SEVERAL_TILES)
+def test_products_of_several_tiles(device, tile, layout, experts, rows, n, k):
+    """A workgroup's second tile, whose first loads go out in front of the stores of the tile before, in every form and type."""
+    gen = torch.Generator(device).manual_seed(rows + n + k)
+    counts = rows_of_experts(layout, experts, rows)
+    shape = (experts, rows) if layout == "padded" else (rows,)
+    x, xs = random_int8((*shape, k), gen, device), torch.rand(shape, generator=gen, device=device) * 1e-2
+    lead = () if layout == "dense" else (experts,)
+    w, ws = random_int8((*lead, n, k), gen, device), torch.rand((*lead, n), generator=gen, device=device) * 1e-2
+    where = {}
+    if layout == "padded":
+        where["num_tokens"] = torch.tensor(counts, dtype=torch.int32, device=device)
+    elif layout == "sorted":
+        where["offsets"] = torch.tensor([0, *torch.tensor(counts).cumsum(0).tolist()], dtype=torch.int32, device=device)
+    outs = [torch.full((*shape, n), 7.0, dtype=t, device=device) for t in (BF16, F16, F32)]
+    for out in outs:
+        int8_matmul(x, xs, w, ws, **where, out=out)
+    first = 0
+    for e, c in enumerate(counts):
+        at = (e, slice(0, c)) if layout == "padded" else (slice(first, first + c),)
+        first += c
+        ref = product64(x[at], xs[at], w[e] if lead else w, ws[e] if lead else ws)
+        for out in outs:
+            assert_product(out[at], ref)
+            if layout == "padded":
+                assert (out[e, c:] == 7).all()
 
 
 # ---------------------------------------------------------------------------
