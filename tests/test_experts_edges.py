@@ -22,6 +22,7 @@ from pplx_kernels import (
     unsort_tokens,
     unsort_tokens_backward,
 )
+from tests import test_experts
 from tests.test_capi_cpu import _gpu_kernels_of
 from tests.test_experts import (
     BF16,
@@ -31,6 +32,7 @@ from tests.test_experts import (
     assert_within,
     make_indices,
     make_sorted,
+    ref_unsort,
     rounded,
     to_u32,
 )
@@ -300,6 +302,73 @@ def test_more_rows_than_one_line_of_workgroups(device):
     for part, q_part, scale_part in zip(x.split(1 << 22), q.split(1 << 22), scale.split(1 << 22)):
         want, want_scale = quantize_rows(part)
         assert torch.equal(q_part, want) and torch.equal(scale_part, want_scale)
+
+
+# ---------------------------------------------------------------------------
+# Rows that go past the caches, and rows longer than registers hold
+# ---------------------------------------------------------------------------
+def large_step(device, m, k, hidden, y_dtype, grad_dtype):
+    gen = torch.Generator(device).manual_seed(m + hidden)
+    idx = torch.randint(0, 10, (m, k), dtype=torch.int32, generator=gen, device=device)  # (two of ten experts are elsewhere)
+    s = sort_tokens(torch.zeros(m, 8, dtype=BF16, device=device), idx.view(torch.uint32), 8)
+    y = torch.randn(m * k, hidden, generator=gen, device=device).to(y_dtype)
+    y[int(s.offsets[-1]) :] = float("nan")
+    weights = torch.where(s.slots >= 0, torch.rand(m, k, generator=gen, device=device), float("nan"))
+    grad = torch.randn(m, hidden, generator=gen, device=device).to(grad_dtype)
+    return s.slots, s.offsets, y, weights, grad
+
+
+@gpu
+@pytest.mark.parametrize("out_dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("m,k,hidden,y_dtype", [(9001, 6, 1000, BF16), (9001, 6, 1000, F16), (9001, 3, 1000, F32)])
+def test_large_gathers(device, m, k, hidden, y_dtype, out_dtype):
+    """More than the 96 MiB from which on rows are read past the caches: as in parts, which are read through them."""
+    assert m * k * hidden * y_dtype.itemsize > 96 << 20 > 3000 * k * hidden * y_dtype.itemsize
+    slots, offsets, y, weights, _ = large_step(device, m, k, hidden, y_dtype, F32)
+    got = unsort_tokens(y, slots, offsets, weights, out_dtype=out_dtype)
+    for a in range(0, m, 3000):
+        assert torch.equal(got[a : a + 3000], unsort_tokens(y, slots[a : a + 3000], offsets, weights[a : a + 3000], out_dtype=out_dtype))
+    few = slice(m - 40, m)
+    ref, size = ref_unsort(y.cpu(), slots[few].cpu(), weights[few].cpu())
+    assert_within(got[few], ref, rounded(ref, out_dtype, (k + 1) * U32 * size))
+
+
+@gpu
+@pytest.mark.parametrize("grad_dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("m,k,hidden,y_dtype", [
+    (9001, 4, 1000, BF16), (9001, 4, 1000, F16), (9001, 2, 1000, F32), (6001, 4, 1544, BF16), (6001, 4, 1544, F16), (6001, 2, 1544, F32),
+])  # fmt: skip
+def test_large_gradients(device, m, k, hidden, y_dtype, grad_dtype):
+    """The same of the gradient, from 56 MiB on, with a wave to a token and with a workgroup."""
+    part = 2500
+    assert m * k * hidden * y_dtype.itemsize > 56 << 20 > part * k * hidden * y_dtype.itemsize
+    slots, offsets, y, weights, grad = large_step(device, m, k, hidden, y_dtype, grad_dtype)
+    grad_y, grad_w = unsort_tokens_backward(grad, y, slots, offsets, weights)
+    assert (grad_y[int(offsets[-1]) :] == 0).all()
+    for a in range(0, m, part):
+        some = slots[a : a + part]
+        part_y, part_w = unsort_tokens_backward(grad[a : a + part], y, some, offsets, weights[a : a + part])
+        rows = some[some >= 0].long()
+        assert torch.equal(grad_y[rows], part_y[rows]) and torch.equal(grad_w[a : a + part], part_w)
+    few = torch.arange(m - 40, m)
+    live, at = slots[few].cpu() >= 0, slots[few].cpu().clamp_min(0).long()
+    picked = torch.where(live[:, :, None], y.cpu().double()[at], 0.0) * grad[few].cpu().double()[:, None]
+    assert_within(grad_w[few], picked.sum(2), (hidden + 1) * U32 * picked.abs().sum(2))
+    t, p = torch.nonzero(live, as_tuple=True)
+    ref = grad[few].cpu().double()[t] * weights[few].cpu().double()[t, p][:, None]
+    assert_within(grad_y[at[t, p].to(device)], ref, rounded(ref, y_dtype, U32 * ref.abs()))
+
+
+@gpu
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("m,k,experts,hidden,dtype,bound,routing", [
+    (33, 3, 7, 8208, BF16, 30, "mixed"), (40, 2, 5, 8208, F32, None, "any"), (40, 2, 5, 5000, F32, None, "mixed"), (7, 3, 4, 20000, F16, 6, "mixed"),
+    (4200, 2, 5, 8208, BF16, 4199, "mixed"), (2100, 4, 9, 8208, F32, None, "mixed"),
+])  # fmt: skip
+def test_sort_tokens_of_long_rows(device, m, k, experts, hidden, dtype, bound, routing, int8):
+    """Copies of more than 16 KiB and quantised rows of more than 8192 elements take more than one turn, in one launch and in
+    three."""
+    test_experts.test_sort_tokens(device, m, k, experts, hidden, dtype, bound, routing, int8)
 
 
 # ---------------------------------------------------------------------------
