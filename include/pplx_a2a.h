@@ -444,7 +444,8 @@ typedef struct pplx_a2a_quantize_args {
 int pplx_a2a_quantize_rows(int device, const pplx_a2a_quantize_args_t *args, void *stream);
 
 /* Rows times their experts' weights in 8-bit integers: out[r, n] = x_scale[r] * weight_scale[e, n] *
- * sum over k of x[r, k] * weight[e, n, k].  The sums are exact (int32), the scaling is fp32, rounded once to out_dtype.
+ * sum over k of x[r, k] * weight[e, n, k].  The sums are exact (int32); the sum, the product of the scales and the product
+ * of both are rounded to fp32, and the result to out_dtype.
  * Rows that are not there are neither read nor written. */
 typedef struct pplx_a2a_int8_matmul_args {
   pplx_a2a_rows_t rows;

@@ -207,7 +207,8 @@ def int8_matmul(
     out: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """``out[r, n] = x_scale[r] * weight_scale[e, n] * sum_k x[r, k] * weight[e, n, k]`` for the rows of each expert ``e``,
-    with exact int32 sums and one rounding.
+    with exact int32 sums.  The scaling is fp32: the sum, the product of the scales and their product are rounded to it, and the
+    result once more to its type.  Not differentiable, in the scales neither.
 
     ``x`` is int8 ``[rows, K]``, ``weight`` int8 ``[experts, N, K]`` and ``weight_scale`` float32 ``[experts, N]``; the rows
     of expert ``e`` are those from ``offsets[e]`` to ``offsets[e + 1]``.  Or ``x`` is ``[experts, rows, K]`` with

@@ -36,7 +36,7 @@ from tests.test_experts import (
     rounded,
     to_u32,
 )
-from tests.test_experts_path import product64, random_int8
+from tests.test_experts_path import make_layer, product64, random_int8, run_layer
 
 gpu = pytest.mark.gpu
 
@@ -247,6 +247,33 @@ def test_traced_rows_without_a_gradient_need_no_multiple_of_eight(device):
         call(x)
 
 
+@gpu
+def test_compiled_calls(device):
+    """torch.compile with its own backend, which turns what surrounds the calls into kernels of its own."""
+    pytest.importorskip("triton")
+    import torch._inductor.config as inductor
+
+    k, experts, hidden = 2, 4, 64
+
+    def layer(x, weights, indices):
+        s = sort_tokens(x, indices, experts)
+        return unsort_tokens(s.rows * 2.0, s.slots, s.offsets, weights)
+
+    gen = torch.Generator().manual_seed(9)
+    with inductor.patch(compile_threads=1):
+        compiled = torch.compile(layer, fullgraph=True, dynamic=True)
+        for m in (30, 41):
+            x = torch.randn(m, hidden, generator=gen).to(device).requires_grad_(True)
+            weights = torch.rand(m, k, generator=gen).to(device).requires_grad_(True)
+            indices = to_u32(make_indices(m, k, experts, gen, "mixed"), device)
+            want, got = layer(x, weights, indices), compiled(x, weights, indices)
+            assert torch.equal(got, want)
+            grads = [torch.autograd.grad(out.sum(), [x, weights]) for out in (want, got)]
+            assert all(torch.equal(a, b) for a, b in zip(*grads))
+        args = make_layer(device, gen, 40, 2, 4, 64, 48)
+        assert torch.equal(torch.compile(lambda *a: run_layer(a)[0], fullgraph=True)(*args), run_layer(args)[0])
+
+
 # ---------------------------------------------------------------------------
 # More workgroups than a launch takes threads for along one dimension
 # ---------------------------------------------------------------------------
@@ -423,6 +450,15 @@ def test_the_products_of_several_tiles_are_that(tile, layout, experts, rows, n, 
     columns = -(-n // tile[1])
     tiles = sum(-(-c // tile[0]) for c in rows_of_experts(layout, experts, rows)) * columns
     assert plan.workgroups < tiles <= plan.tiles
+
+
+@gpu
+def test_products_record_no_gradient(device):
+    """Neither the products nor the quantisation are differentiable: their results say so, whatever the scales require."""
+    q, scale = quantize_rows(torch.randn(4, 32, device=device, requires_grad=True))
+    assert not q.requires_grad and not scale.requires_grad
+    got = int8_matmul(q, scale.requires_grad_(True), q, scale)
+    assert not got.requires_grad
 
 
 def test_plans_of_products():
