@@ -424,8 +424,8 @@ typedef struct pplx_a2a_rows {
 } pplx_a2a_rows_t;
 
 /* Rows to 8 bits with one scale each, as sort_tokens does it: of x [.., width], or with swiglu of
- * silu(x[.., :width]) * x[.., width:2 * width] in fp32, silu(g) = g / (1 + exp(-g)).  Rows that are not there
- * are neither read nor written. */
+ * silu(x[.., :width]) * x[.., width:2 * width] in fp32, silu(g) = g / (1 + exp(-g)), which is -0 where exp(-g) is
+ * more than fp32 holds (g < -88.7).  Rows that are not there are neither read nor written. */
 typedef struct pplx_a2a_quantize_args {
   pplx_a2a_rows_t rows;
   void *out;                       /* int8 [.., width], 16-byte aligned */

@@ -45,8 +45,9 @@ template <class T, bool SWIGLU, int LANES, int PIECES, bool NT> struct Piece {
         const f32x8 u = Eight<T>::wide(up[i]);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          // (a reciprocal of one ulp: a quotient to the last bit is ten instructions more, which the rows' bytes do not hide)
-          v[i][k] = v[i][k] * __builtin_amdgcn_rcpf(1.f + __expf(-v[i][k])) * u[k];
+          // (A reciprocal of one ulp: a quotient to the last bit is ten instructions more, which the rows' bytes do not hide.  Of
+          // a sixteenth: that of 2^126 and more is subnormal, and comes as zero.)
+          v[i][k] = 0.0625f * v[i][k] * __builtin_amdgcn_rcpf(__builtin_fmaf(__expf(-v[i][k]), 0.0625f, 0.0625f)) * u[k];
         }
       }
     }

@@ -30,10 +30,12 @@ from tests.test_experts import (
     F32,
     U32,
     assert_within,
+    check_quantized,
     make_indices,
     make_sorted,
     ref_unsort,
     rounded,
+    swiglu64,
     to_u32,
 )
 from tests.test_experts_path import make_layer, product64, random_int8, run_layer
@@ -396,6 +398,17 @@ def test_sort_tokens_of_long_rows(device, m, k, experts, hidden, dtype, bound, r
     """Copies of more than 16 KiB and quantised rows of more than 8192 elements take more than one turn, in one launch and in
     three."""
     test_experts.test_sort_tokens(device, m, k, experts, hidden, dtype, bound, routing, int8)
+
+
+@gpu
+def test_the_activation_to_the_end_of_its_range(device):
+    """Gates down to -88.7, whose sigmoid is subnormal, with values that bring the result back to ordinary sizes."""
+    gate = torch.linspace(-88.7, -80.0, 256)[:, None].expand(256, 48)
+    x = torch.cat([gate, torch.full((256, 48), 1e36)], dim=1).contiguous()
+    q, scale = quantize_rows(x.to(device), swiglu=True)
+    v, off = swiglu64(x)
+    assert float(v.abs().min()) > 0.1
+    check_quantized(q, scale, v, off)
 
 
 # ---------------------------------------------------------------------------
