@@ -475,6 +475,160 @@ typedef struct pplx_a2a_int8_matmul_plan {
 } pplx_a2a_int8_matmul_plan_t;
 int pplx_a2a_int8_matmul_plan(const pplx_a2a_rows_t *rows, uint64_t n, uint64_t k, pplx_a2a_int8_matmul_plan_t *out);
 
+/* ---- before dispatch ------------------------------------------------------- */
+
+/* Operators on plain device buffers as above: what makes the rows that dispatch sends, and its picks and weights. */
+
+/* Root-mean-square norm of rows, with the addition of a residual in front and the rows in 8 bits behind it:
+ *   h = x + residual, rounded to dtype (h = x without residual)            -> sum
+ *   v = h * weight / sqrt(mean(h^2) + eps), in fp32, rounded to dtype      -> y
+ *   the quantised v, of which y is not a part                              -> q, scale
+ * PPLX_A2A_ROWS_INT8: one scale a row, as pplx_a2a_quantize_rows.  PPLX_A2A_ROWS_E4M3: one scale for each 128 columns, which
+ * is how dispatch carries fp8 rows: a = max(max |v|, 2^-100), scale = a / 448, q = v * (448 / a) rounded to e4m3.  A row that
+ * holds an infinity or a NaN becomes NaN: y and the scales are NaN, q is zeros.  y and sum may be x or residual themselves (same
+ * address and stride). */
+typedef enum pplx_a2a_row_format { PPLX_A2A_ROWS_PLAIN = 0, PPLX_A2A_ROWS_INT8 = 1, PPLX_A2A_ROWS_E4M3 = 2 } pplx_a2a_row_format;
+typedef struct pplx_a2a_rms_norm_args {
+  const void *x;               /* [m, hidden_dim] of dtype; all rows 16-byte aligned, strides in bytes, multiples of 16 */
+  int64_t x_stride_row;
+  const void *residual;        /* the same, or NULL */
+  int64_t residual_stride_row;
+  const void *weight;          /* [hidden_dim] of weight_dtype, 16-byte aligned */
+  int32_t dtype;               /* pplx_a2a_dtype */
+  int32_t weight_dtype;        /* dtype or F32 */
+  float eps;                   /* positive, a normal number */
+  uint32_t m;
+  uint64_t hidden_dim;         /* a multiple of 8, with q of 16; below 2^27 */
+  void *y;                     /* [m, hidden_dim] of dtype, or NULL */
+  int64_t y_stride_row;
+  void *sum;                   /* the same: with residual and only with it */
+  int64_t sum_stride_row;
+  void *q;                     /* [m, hidden_dim] bytes, or NULL */
+  int64_t q_stride_row;
+  float *scale;                /* [m], or [m, ceil(hidden_dim / 128)], with q */
+  int64_t scale_stride_row;    /* floats */
+  int64_t scale_stride_block;  /* floats (E4M3) */
+  int32_t format;              /* pplx_a2a_row_format */
+} pplx_a2a_rms_norm_args_t;
+int pplx_a2a_rms_norm(int device, const pplx_a2a_rms_norm_args_t *args, void *stream);
+
+/* Gradients of y = rms_norm(h) and of h itself, with r = 1 / sqrt(mean(h^2) + eps) and g = grad_y * weight:
+ *   grad_h = r * (g - h * r^2 * mean(g * h)) + grad_sum, rounded once: that of x and of residual
+ *   grad_weight = sum over rows of grad_y * h * r, in fp32, in an order that the sizes alone decide
+ * Either may be left out (NULL).  grad_h may be grad_y or grad_sum itself. */
+typedef struct pplx_a2a_rms_norm_backward_args {
+  const void *grad_y;          /* [m, hidden_dim] of dtype, as above */
+  int64_t grad_y_stride_row;
+  const void *grad_sum;        /* the same, or NULL (zeros) */
+  int64_t grad_sum_stride_row;
+  const void *h;               /* the same: x, or sum where there was a residual */
+  int64_t h_stride_row;
+  const void *weight;          /* [hidden_dim] of weight_dtype, 16-byte aligned */
+  int32_t dtype;               /* pplx_a2a_dtype */
+  int32_t weight_dtype;        /* dtype or F32 */
+  float eps;
+  uint32_t m;
+  uint64_t hidden_dim;         /* a multiple of 8 below 2^27 */
+  void *grad_h;                /* [m, hidden_dim] of dtype, or NULL */
+  int64_t grad_h_stride_row;
+  void *grad_weight;           /* [hidden_dim] of weight_dtype, 16-byte aligned, or NULL */
+  void *workspace;             /* pplx_a2a_rms_norm_workspace bytes, 16-byte aligned: with grad_weight */
+} pplx_a2a_rms_norm_backward_args_t;
+int pplx_a2a_rms_norm_workspace(uint32_t m, uint64_t hidden_dim, uint64_t *bytes);
+int pplx_a2a_rms_norm_backward(int device, const pplx_a2a_rms_norm_backward_args_t *args, void *stream);
+
+/* The router's product: logits[t, e] = sum over k of x[t, k] * weight[e, k], added up in fp32.  Products of 16-bit elements are
+ * exact; fp32 elements count to 24 bits (an infinity among them makes a NaN). */
+typedef struct pplx_a2a_router_logits_args {
+  const void *x;               /* [m, hidden_dim] of dtype; rows 16-byte aligned, strides in bytes, multiples of 16 */
+  int64_t x_stride_row;
+  const void *weight;          /* [num_experts, hidden_dim] of weight_dtype, the same */
+  int64_t weight_stride_row;
+  int32_t dtype;               /* pplx_a2a_dtype */
+  int32_t weight_dtype;        /* dtype or F32 */
+  uint32_t m;
+  uint32_t num_experts;        /* 1..5461 */
+  uint64_t hidden_dim;         /* a multiple of 8 below 2^27 */
+  float *logits;               /* [m, num_experts], 4-byte aligned */
+  int64_t logits_stride_row;   /* floats */
+  void *workspace;             /* pplx_a2a_router_workspace bytes, 16-byte aligned; may be NULL when that is 0 */
+} pplx_a2a_router_logits_args_t;
+/* backward: of pplx_a2a_router_logits_backward. */
+int pplx_a2a_router_workspace(uint32_t m, uint32_t num_experts, uint64_t hidden_dim, int32_t dtype, int32_t weight_dtype,
+                              int32_t backward, uint64_t *bytes);
+int pplx_a2a_router_logits(int device, const pplx_a2a_router_logits_args_t *args, void *stream);
+
+/* Its gradients: grad_x = grad_logits * weight and grad_weight = grad_logits^T * x, each rounded once.  Either may be left out
+ * (NULL). */
+typedef struct pplx_a2a_router_logits_backward_args {
+  const float *grad_logits;    /* [m, num_experts], 4-byte aligned */
+  int64_t grad_logits_stride_row; /* floats */
+  const void *x;               /* [m, hidden_dim] of dtype, as above: read for grad_weight */
+  int64_t x_stride_row;
+  const void *weight;          /* [num_experts, hidden_dim] of weight_dtype, as above: read for grad_x */
+  int64_t weight_stride_row;
+  int32_t dtype;
+  int32_t weight_dtype;
+  uint32_t m;
+  uint32_t num_experts;
+  uint64_t hidden_dim;
+  void *grad_x;                /* [m, hidden_dim] of dtype, as x, or NULL */
+  int64_t grad_x_stride_row;
+  void *grad_weight;           /* [num_experts, hidden_dim] of weight_dtype, as weight, or NULL */
+  int64_t grad_weight_stride_row;
+  void *workspace;             /* pplx_a2a_router_workspace bytes, 16-byte aligned */
+} pplx_a2a_router_logits_backward_args_t;
+int pplx_a2a_router_logits_backward(int device, const pplx_a2a_router_logits_backward_args_t *args, void *stream);
+
+/* Each token's experts and their weights.  With s the softmax of a token's logits, or the sigmoid of each:
+ *   key[e] = s[e] + bias[e], in an order as if computed in 64 bits; without a bias the logits' order
+ *   the experts are num_groups groups of consecutive ones, of which the top_groups take part whose group_top best keys
+ *   (s + bias) have the largest sums
+ *   indices = the experts_per_token experts of the largest keys, largest first; equal ones, and equal groups, by number
+ *   weights = weight_scale * s[indices], divided by the sum of the s[indices] with renormalize
+ * An expert whose logit or key is -inf is not there.  Picks that no expert is left for, and those of tokens from *bound_m on,
+ * have index num_experts and weight 0.  A token with a logit or key that is NaN or +inf gets the first experts and weights of
+ * NaN. */
+typedef enum pplx_a2a_scores { PPLX_A2A_SOFTMAX = 0, PPLX_A2A_SIGMOID = 1 } pplx_a2a_scores;
+typedef struct pplx_a2a_route_args {
+  const void *logits;          /* [m, num_experts] of dtype, aligned to its elements */
+  int64_t logits_stride_row;   /* elements */
+  int32_t dtype;               /* pplx_a2a_dtype */
+  uint32_t m;
+  uint32_t num_experts;        /* 1..5461 */
+  uint32_t experts_per_token;  /* 1..64, at most top_groups * num_experts / num_groups */
+  const float *bias;           /* [num_experts] or NULL */
+  const uint32_t *bound_m;     /* device scalar or NULL (= m) */
+  uint32_t num_groups;         /* divides num_experts; 1: no groups */
+  uint32_t top_groups;         /* 1..num_groups */
+  uint32_t group_top;          /* 1 or 2, at most num_experts / num_groups (where top_groups < num_groups) */
+  int32_t scores;              /* pplx_a2a_scores */
+  int32_t renormalize;
+  float weight_scale;          /* finite */
+  uint32_t *indices;           /* [m, experts_per_token] contiguous */
+  float *weights;              /* [m, experts_per_token] contiguous */
+} pplx_a2a_route_args_t;
+int pplx_a2a_route_tokens(int device, const pplx_a2a_route_args_t *args, void *stream);
+
+/* The gradient of the weights with respect to the logits, for the picks (distinct in each token) that route_tokens made;
+ * picks with an index of num_experts or more have none.  Every logit's gradient is written. */
+typedef struct pplx_a2a_route_backward_args {
+  const float *grad_weights;   /* [m, experts_per_token] contiguous */
+  const void *logits;          /* [m, num_experts] of dtype, as above */
+  int64_t logits_stride_row;
+  const uint32_t *indices;     /* [m, experts_per_token] contiguous */
+  int32_t dtype;
+  uint32_t m;
+  uint32_t num_experts;
+  uint32_t experts_per_token;
+  int32_t scores;
+  int32_t renormalize;
+  float weight_scale;
+  void *grad_logits;           /* [m, num_experts] of dtype, aligned to its elements */
+  int64_t grad_logits_stride_row; /* elements */
+} pplx_a2a_route_backward_args_t;
+int pplx_a2a_route_tokens_backward(int device, const pplx_a2a_route_backward_args_t *args, void *stream);
+
 /* ---- misc -------------------------------------------------------------- */
 
 const char *pplx_a2a_last_error(void);

@@ -1,0 +1,522 @@
+// Root-mean-square norm of rows with the residual's addition, the rows in 8 bits behind it, and the gradients.
+//
+//   h = x + residual      v = h * r * weight, r = 1 / sqrt(mean(h^2) + eps)
+//
+// Bound by the rows' bytes: a row stays in registers between the sum of its squares and what is made of it, so that each is
+// read once and each result written once.  Sums are fp32.
+#include <cfloat>
+#include <cmath>
+
+#include "a2a_experts.h"
+
+namespace pplx_amd {
+namespace {
+
+struct NormDev {
+  const uint8_t *x;
+  int64_t x_stride_row;
+  const uint8_t *residual;
+  int64_t residual_stride_row;
+  const uint8_t *weight;
+  uint8_t *y;
+  int64_t y_stride_row;
+  uint8_t *sum;
+  int64_t sum_stride_row;
+  uint8_t *q;
+  int64_t q_stride_row;
+  float *scale;
+  int64_t scale_stride_row, scale_stride_block;
+  float eps, inverse_width;
+  uint32_t m, width;
+  uint32_t first_group;
+};
+
+template <class T> __device__ __forceinline__ PPLX_GLOBAL T *row_at(uint8_t *base, int64_t stride, uint32_t r) {
+  return as_global(reinterpret_cast<T *>(base + (int64_t)r * stride));
+}
+template <class T> __device__ __forceinline__ const PPLX_GLOBAL T *row_at(const uint8_t *base, int64_t stride, uint32_t r) {
+  return as_global(reinterpret_cast<const T *>(base + (int64_t)r * stride));
+}
+
+// The sum over the LANES threads of a row (64, or all of a workgroup, which all call), the same in each.
+template <int LANES> __device__ __forceinline__ float row_sum(float v) {
+  v = wave_sum(v);
+  if constexpr (LANES > 64) {
+    __shared__ float of_wave[LANES / 64];
+    __syncthreads();  // (the row before has been read)
+    if (lane_id() == 0) of_wave[wave_id()] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int w = 0; w < LANES / 64; ++w) v += of_wave[w];
+  }
+  return v;
+}
+
+// 1 / sqrt(squares / width + eps).
+__device__ __forceinline__ float inverse_root(float squares, const float inverse_width, const float eps) {
+  return __builtin_amdgcn_rsqf(__builtin_fmaf(squares, inverse_width, eps));
+}
+// Squares that fp32 does not hold (of 1.8e19 and more) are added up once more of values 2^-70 times as large, beside which eps is
+// nothing.  What is an infinity or NaN even then makes the row NaN.
+constexpr float kSmall = 0x1p-70f;
+__device__ __forceinline__ float inverse_root_of_small(float squares, const float inverse_width) {
+  if (!(squares <= FLT_MAX)) return __uint_as_float(0x7fc00000u);
+  return __builtin_amdgcn_rsqf(squares * inverse_width) * kSmall;
+}
+__device__ __forceinline__ float squares_of(f32x8 v, float factor) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float f = v[i] * factor;
+    s = __builtin_fmaf(f, f, s);
+  }
+  return s;
+}
+
+// The largest value of the sixteen lanes around this one, which hold a block of 128 columns.
+__device__ __forceinline__ uint32_t block_max(uint32_t v) {
+#pragma unroll
+  for (int d = 8; d; d >>= 1) {
+    const uint32_t o = (uint32_t)__shfl_xor((int)v, d);
+    v = v > o ? v : o;
+  }
+  return v;
+}
+
+// A block's scale and its inverse: a / 448 and 448 / a.  |v| * (448 / a) is at most 448 (1 + 2^-23), which rounds to 448, the
+// largest e4m3.
+__device__ __forceinline__ RowScale block_scale(uint32_t max_bits) {
+  RowScale s;
+  if (max_bits >= 0x7f800000u) {
+    s.inverse = 0.f;
+    s.scale = __uint_as_float(0x7fc00000u);
+  } else {
+    const float a = __uint_as_float(max_bits > kTinyBits ? max_bits : kTinyBits);
+    s.inverse = 448.f / a;
+    s.scale = a / 448.f;
+  }
+  return s;
+}
+// Eight values as e4m3, rounded to nearest, ties to even (zeros where the inverse is 0).
+__device__ __forceinline__ u32x2 e4m3_eight(f32x8 v, float inverse) {
+  u32x2 out;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i] * inverse, v[4 * i + 1] * inverse, 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i + 2] * inverse, v[4 * i + 3] * inverse, w, true);
+    out[i] = inverse != 0.f ? (uint32_t)w : 0u;
+  }
+  return out;
+}
+
+// One row by LANES threads, each with PIECES times eight elements of it, eight elements apart from the next thread's.  Rows that
+// are longer than that are taken in several steps, twice: once for the sum of squares, and once or, for one scale a row, twice
+// more for the results.
+template <class T, class W, int FORMAT, int LANES, int PIECES>
+__device__ __forceinline__ void norm_one(const NormDev &a, uint32_t r, uint32_t g) {
+  constexpr uint32_t kStep = LANES * PIECES;
+  const uint32_t groups = a.width / 8;
+  const bool whole = groups <= kStep;  // the row stays in registers
+  const PPLX_GLOBAL T *x = row_at<T>(a.x, a.x_stride_row, r);
+  const PPLX_GLOBAL W *weight = as_global(reinterpret_cast<const W *>(a.weight));
+  f32x8 v[PIECES];
+  auto load = [&](uint32_t base, const PPLX_GLOBAL T *from) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const uint32_t j = base + i * LANES + g;
+      v[i] = j < groups ? Eight<T>::wide(load_eight<T>(from + 8ull * j)) : f32x8{};
+    }
+  };
+  // (x + residual, rounded: what the sum's reader and the gradient see is what the norm is of)
+  auto add = [&](uint32_t base) __attribute__((always_inline)) {
+    const PPLX_GLOBAL T *residual = row_at<T>(a.residual, a.residual_stride_row, r);
+    PPLX_GLOBAL T *sum = row_at<T>(a.sum, a.sum_stride_row, r);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const uint32_t j = base + i * LANES + g;
+      if (j >= groups) continue;
+      const f32x8 h = v[i] + Eight<T>::wide(load_eight<T>(residual + 8ull * j));
+      v[i] = Eight<T>::wide(Eight<T>::narrow(h));
+      store_eight<T>(sum + 8ull * j, v[i]);
+    }
+  };
+  float squares = 0.f;
+  for (uint32_t base = 0; base < groups; base += kStep) {
+    load(base, x);
+    if (a.residual) add(base);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) squares += squares_of(v[i], 1.f);
+  }
+  squares = row_sum<LANES>(squares);
+  const PPLX_GLOBAL T *again = a.residual ? row_at<T>(a.sum, a.sum_stride_row, r) : x;
+  float root;
+  if (squares <= FLT_MAX) {
+    root = inverse_root(squares, a.inverse_width, a.eps);
+  } else {
+    float small = 0.f;
+    for (uint32_t base = 0; base < groups; base += kStep) {
+      if (!whole) load(base, again);
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) small += squares_of(v[i], kSmall);
+    }
+    root = inverse_root_of_small(row_sum<LANES>(small), a.inverse_width);
+  }
+  auto norm = [&](uint32_t base) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const uint32_t j = base + i * LANES + g;
+      if (j >= groups) continue;
+      v[i] = v[i] * root * Eight<W>::wide(load_eight<W>(weight + 8ull * j));
+    }
+  };
+  PPLX_GLOBAL uint8_t *q = FORMAT == PPLX_A2A_ROWS_PLAIN ? nullptr : row_at<uint8_t>(a.q, a.q_stride_row, r);
+  float inverse = 0.f;
+  if constexpr (FORMAT == PPLX_A2A_ROWS_INT8) {
+    uint32_t bits = 0;
+    for (uint32_t base = 0; base < groups; base += kStep) {
+      if (!whole) load(base, again);
+      norm(base);
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        const uint32_t b = magnitude_bits(v[i]);
+        bits = bits > b ? bits : b;
+      }
+    }
+    const RowScale s = row_scale(row_max<LANES>(bits));
+    inverse = s.inverse;
+    if (g == 0) as_global(a.scale)[(int64_t)r * a.scale_stride_row] = s.scale;
+  }
+  for (uint32_t base = 0; base < groups; base += kStep) {
+    if (!whole) load(base, again);
+    if (!whole || FORMAT != PPLX_A2A_ROWS_INT8) norm(base);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const uint32_t j = base + i * LANES + g;
+      if constexpr (FORMAT == PPLX_A2A_ROWS_E4M3) {
+        // (all lanes of a block call; those behind the row hold zeros)
+        const RowScale s = block_scale(block_max(magnitude_bits(v[i])));
+        inverse = s.inverse;
+        if (j < groups && j % 16 == 0) as_global(a.scale)[(int64_t)r * a.scale_stride_row + (int64_t)(j / 16) * a.scale_stride_block] = s.scale;
+      }
+      if (j >= groups) continue;
+      if (a.y) store_eight<T>(row_at<T>(a.y, a.y_stride_row, r) + 8ull * j, v[i]);
+      if constexpr (FORMAT == PPLX_A2A_ROWS_INT8) *reinterpret_cast<PPLX_GLOBAL u32x2 *>(q + 8ull * j) = quantize_eight(v[i], inverse);
+      if constexpr (FORMAT == PPLX_A2A_ROWS_E4M3) *reinterpret_cast<PPLX_GLOBAL u32x2 *>(q + 8ull * j) = e4m3_eight(v[i], inverse);
+    }
+  }
+}
+
+template <class T, class W, int FORMAT, int LANES, int PIECES>
+__global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_rows(NormDev a) {
+  const uint32_t group = a.first_group + blockIdx.x;
+  const uint32_t r = LANES == 64 ? group * 4 + wave_id() : group;
+  if (r < a.m) norm_one<T, W, FORMAT, LANES, PIECES>(a, r, threadIdx.x % LANES);
+}
+
+// ---------------------------------------------------------------------------
+// Gradients
+// ---------------------------------------------------------------------------
+struct NormBackwardDev {
+  const uint8_t *grad_y;
+  int64_t grad_y_stride_row;
+  const uint8_t *grad_sum;
+  int64_t grad_sum_stride_row;
+  const uint8_t *h;
+  int64_t h_stride_row;
+  const uint8_t *weight;
+  uint8_t *grad_h;
+  int64_t grad_h_stride_row;
+  float *partial;  // [gridDim.x, width], or of long rows r of each row
+  float eps, inverse_width;
+  uint32_t m, width;
+};
+
+template <int LANES> __device__ __forceinline__ float gradient_root(const f32x8 *h, int pieces, float squares, const NormBackwardDev &a) {
+  if (squares <= FLT_MAX) return inverse_root(squares, a.inverse_width, a.eps);
+  float small = 0.f;
+#pragma unroll
+  for (int i = 0; i < pieces; ++i) small += squares_of(h[i], kSmall);
+  return inverse_root_of_small(row_sum<LANES>(small), a.inverse_width);
+}
+
+// Rows of up to 8 LANES PIECES elements, which stay in registers; a workgroup takes one row behind the other and holds its
+// share of the weight's gradient.
+template <class T, class W, int LANES, int PIECES>
+__global__ __launch_bounds__(LANES) void norm_backward_rows(NormBackwardDev a) {
+  const uint32_t g = threadIdx.x, groups = a.width / 8;
+  const PPLX_GLOBAL W *weight = as_global(reinterpret_cast<const W *>(a.weight));
+  f32x8 of_weight[PIECES] = {};
+  for (uint32_t r = blockIdx.x; r < a.m; r += gridDim.x) {
+    const PPLX_GLOBAL T *grad = row_at<T>(a.grad_y, a.grad_y_stride_row, r), *row = row_at<T>(a.h, a.h_stride_row, r);
+    f32x8 h[PIECES], d[PIECES];
+    float squares = 0.f;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const uint32_t j = i * LANES + g;
+      h[i] = j < groups ? Eight<T>::wide(load_eight<T>(row + 8ull * j)) : f32x8{};
+      d[i] = j < groups ? Eight<T>::wide(load_eight<T>(grad + 8ull * j)) : f32x8{};
+      squares += squares_of(h[i], 1.f);
+    }
+    const float root = gradient_root<LANES>(h, PIECES, row_sum<LANES>(squares), a);
+    float along = 0.f;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const uint32_t j = i * LANES + g;
+      if (j >= groups) continue;
+      h[i] = h[i] * root;
+      of_weight[i] += d[i] * h[i];
+      d[i] = d[i] * Eight<W>::wide(load_eight<W>(weight + 8ull * j));
+#pragma unroll
+      for (int k = 0; k < 8; ++k) along = __builtin_fmaf(d[i][k], h[i][k], along);
+    }
+    along = row_sum<LANES>(along) * a.inverse_width;
+    if (!a.grad_h) continue;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const uint32_t j = i * LANES + g;
+      if (j >= groups) continue;
+      f32x8 out = (d[i] - h[i] * along) * root;
+      if (a.grad_sum) out += Eight<T>::wide(load_eight<T>(row_at<T>(a.grad_sum, a.grad_sum_stride_row, r) + 8ull * j));
+      store_eight<T>(row_at<T>(a.grad_h, a.grad_h_stride_row, r) + 8ull * j, out);
+    }
+  }
+  if (!a.partial) return;
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    const uint32_t j = i * LANES + g;
+    if (j < groups) store_eight<float>(as_global(a.partial) + (uint64_t)blockIdx.x * a.width + 8ull * j, of_weight[i]);
+  }
+}
+
+// Longer rows, read twice; r of each row is left for the weight's gradient.
+constexpr int kLongLanes = 512;
+template <class T, class W> __global__ __launch_bounds__(kLongLanes) void norm_backward_long(NormBackwardDev a) {
+  const uint32_t g = threadIdx.x, groups = a.width / 8;
+  const PPLX_GLOBAL W *weight = as_global(reinterpret_cast<const W *>(a.weight));
+  for (uint32_t r = blockIdx.x; r < a.m; r += gridDim.x) {
+    const PPLX_GLOBAL T *grad = row_at<T>(a.grad_y, a.grad_y_stride_row, r), *row = row_at<T>(a.h, a.h_stride_row, r);
+    auto squares_times = [&](float factor) {
+      float s = 0.f;
+      for (uint32_t j = g; j < groups; j += kLongLanes) s += squares_of(Eight<T>::wide(load_eight<T>(row + 8ull * j)), factor);
+      return row_sum<kLongLanes>(s);
+    };
+    const float squares = squares_times(1.f);
+    const float root = squares <= FLT_MAX ? inverse_root(squares, a.inverse_width, a.eps)
+                                          : inverse_root_of_small(squares_times(kSmall), a.inverse_width);
+    if (a.partial && g == 0) as_global(a.partial)[r] = root;
+    if (!a.grad_h) continue;
+    float along = 0.f;
+    for (uint32_t j = g; j < groups; j += kLongLanes) {
+      const f32x8 h = Eight<T>::wide(load_eight<T>(row + 8ull * j)) * root;
+      const f32x8 d = Eight<T>::wide(load_eight<T>(grad + 8ull * j)) * Eight<W>::wide(load_eight<W>(weight + 8ull * j));
+#pragma unroll
+      for (int k = 0; k < 8; ++k) along = __builtin_fmaf(d[k], h[k], along);
+    }
+    along = row_sum<kLongLanes>(along) * a.inverse_width;
+    for (uint32_t j = g; j < groups; j += kLongLanes) {
+      const f32x8 h = Eight<T>::wide(load_eight<T>(row + 8ull * j)) * root;
+      const f32x8 d = Eight<T>::wide(load_eight<T>(grad + 8ull * j)) * Eight<W>::wide(load_eight<W>(weight + 8ull * j));
+      f32x8 out = (d - h * along) * root;
+      if (a.grad_sum) out += Eight<T>::wide(load_eight<T>(row_at<T>(a.grad_sum, a.grad_sum_stride_row, r) + 8ull * j));
+      store_eight<T>(row_at<T>(a.grad_h, a.grad_h_stride_row, r) + 8ull * j, out);
+    }
+  }
+}
+
+// The weight's gradient out of the workgroups' shares, or of long rows out of the rows: 64 threads to 512 columns each, eight
+// waves that take every eighth share or row.
+constexpr int kSumWaves = 8;
+template <class Fn> __device__ __forceinline__ f32x8 sum_of_waves(uint32_t count, Fn &&of) {
+  __shared__ float sums[kSumWaves][8][64];
+  f32x8 s = {};
+  for (uint32_t i = wave_id(); i < count; i += kSumWaves) s += of(i);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) sums[wave_id()][k][lane_id()] = s[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    s[k] = 0.f;
+#pragma unroll
+    for (int w = 0; w < kSumWaves; ++w) s[k] += sums[w][k][lane_id()];
+  }
+  return s;
+}
+template <class W> __global__ __launch_bounds__(kSumWaves * 64) void norm_weight_gradient(const float *partial, uint32_t count, uint32_t width, W *out) {
+  const uint32_t j = blockIdx.x * 64 + lane_id(), groups = width / 8;
+  const f32x8 s = sum_of_waves(count, [&](uint32_t i) {
+    return j < groups ? load_eight<float>(as_global(partial) + (uint64_t)i * width + 8ull * j) : f32x8{};
+  });
+  if (wave_id() == 0 && j < groups) store_eight<W>(as_global(out) + 8ull * j, s);
+}
+template <class T, class W> __global__ __launch_bounds__(kSumWaves * 64) void norm_weight_gradient_long(NormBackwardDev a, W *out) {
+  const uint32_t j = blockIdx.x * 64 + lane_id(), groups = a.width / 8;
+  const f32x8 s = sum_of_waves(a.m, [&](uint32_t r) {
+    if (j >= groups) return f32x8{};
+    const f32x8 h = Eight<T>::wide(load_eight<T>(row_at<T>(a.h, a.h_stride_row, r) + 8ull * j)) * as_global(a.partial)[r];
+    return h * Eight<T>::wide(load_eight<T>(row_at<T>(a.grad_y, a.grad_y_stride_row, r) + 8ull * j));
+  });
+  if (wave_id() == 0 && j < groups) store_eight<W>(as_global(out) + 8ull * j, s);
+}
+
+constexpr uint64_t kMostInRegisters = 8 * 4 * 512;  // elements of a row in the gradient's kernel
+constexpr uint32_t kBackwardGroups = 512;           // workgroups that share out the rows
+
+uint32_t backward_groups(uint32_t m) { return m < kBackwardGroups ? m : kBackwardGroups; }
+
+template <class Fn> int with_weight_type(int32_t dtype, int32_t weight_dtype, Fn &&fn) {
+  return with_type(dtype, [&](auto tag) {
+    typedef typename decltype(tag)::type T;
+    return weight_dtype == dtype ? fn(tag, TypeTag<T>{}) : fn(tag, TypeTag<float>{});
+  });
+}
+
+int check_rows_of(const void *p, int64_t stride, const char *name) {
+  PPLX_REQUIRE(is_aligned(p, 16) && stride % 16 == 0, "%s must be 16-byte aligned with 16-byte strides", name);
+  return PPLX_A2A_OK;
+}
+#define PPLX_ROWS(p, name)                                               \
+  do {                                                                   \
+    const int st_ = check_rows_of(p.name, p.name##_stride_row, #name);   \
+    if (st_) return st_;                                                 \
+  } while (0)
+
+template <class P> int check_norm_size(const P &p, uint64_t unit) {
+  PPLX_REQUIRE(is_dtype(p.dtype), "unsupported dtype of the rows");
+  PPLX_REQUIRE(p.weight_dtype == p.dtype || p.weight_dtype == PPLX_A2A_F32, "weight_dtype must be dtype or F32");
+  PPLX_REQUIRE(p.hidden_dim > 0 && p.hidden_dim < (1ull << 27) && p.hidden_dim % unit == 0,
+               "hidden_dim must be a multiple of %u below 2^27", (unsigned)unit);
+  PPLX_REQUIRE(p.eps >= FLT_MIN && p.eps <= FLT_MAX, "eps must be positive, finite and normal");
+  return PPLX_A2A_OK;
+}
+
+}  // namespace
+}  // namespace pplx_amd
+
+using namespace pplx_amd;
+
+extern "C" int pplx_a2a_rms_norm(int device, const pplx_a2a_rms_norm_args_t *args, void *stream) {
+  PPLX_REQUIRE(args, "args is NULL");
+  const pplx_a2a_rms_norm_args_t &p = *args;
+  PPLX_REQUIRE(p.format >= PPLX_A2A_ROWS_PLAIN && p.format <= PPLX_A2A_ROWS_E4M3, "unknown format of quantised rows");
+  const int st = check_norm_size(p, p.format == PPLX_A2A_ROWS_PLAIN ? 8 : 16);
+  if (st) return st;
+  if (p.m == 0) return PPLX_A2A_OK;
+  PPLX_REQUIRE(p.x && p.weight, "x / weight is NULL");
+  PPLX_REQUIRE((p.q != nullptr) == (p.format != PPLX_A2A_ROWS_PLAIN), "q goes with a format of quantised rows");
+  PPLX_REQUIRE(p.y || p.q, "neither y nor q is asked for");
+  PPLX_REQUIRE((p.residual != nullptr) == (p.sum != nullptr), "sum goes with residual");
+  PPLX_REQUIRE(!p.q || (p.scale && is_aligned(p.scale, 4)), "scale is NULL or not aligned");
+  PPLX_REQUIRE(is_aligned(p.weight, 16), "weight must be 16-byte aligned");
+  PPLX_ROWS(p, x);
+  if (p.residual) PPLX_ROWS(p, residual);
+  if (p.residual) PPLX_ROWS(p, sum);
+  if (p.y) PPLX_ROWS(p, y);
+  if (p.q) PPLX_ROWS(p, q);
+  NormDev a{};
+  a.x = static_cast<const uint8_t *>(p.x);
+  a.x_stride_row = p.x_stride_row;
+  a.residual = static_cast<const uint8_t *>(p.residual);
+  a.residual_stride_row = p.residual_stride_row;
+  a.weight = static_cast<const uint8_t *>(p.weight);
+  a.y = static_cast<uint8_t *>(p.y);
+  a.y_stride_row = p.y_stride_row;
+  a.sum = static_cast<uint8_t *>(p.sum);
+  a.sum_stride_row = p.sum_stride_row;
+  a.q = static_cast<uint8_t *>(p.q);
+  a.q_stride_row = p.q_stride_row;
+  a.scale = p.scale;
+  a.scale_stride_row = p.scale_stride_row;
+  a.scale_stride_block = p.scale_stride_block;
+  a.eps = p.eps;
+  a.inverse_width = (float)(1.0 / (double)p.hidden_dim);
+  a.m = p.m;
+  a.width = (uint32_t)p.hidden_dim;
+  return guarded(device, [&] {
+    return with_weight_type(p.dtype, p.weight_dtype, [&](auto tag, auto weight_tag) {
+      typedef typename decltype(tag)::type T;
+      typedef typename decltype(weight_tag)::type W;
+      auto launch = [&](auto format) {
+        constexpr int F = decltype(format)::value;
+        hipStream_t s = (hipStream_t)stream;
+        if (a.width <= 2048) {
+          auto kernel = norm_rows<T, W, F, 64, 4>;
+          PPLX_LAUNCH(launch_groups(kernel, kernel, ((uint64_t)a.m + 3) / 4, 256, 0, s, a));
+        } else if (a.width <= 8192) {
+          auto kernel = norm_rows<T, W, F, 256, 4>;
+          PPLX_LAUNCH(launch_groups(kernel, kernel, a.m, 256, 0, s, a));
+        } else {
+          auto kernel = norm_rows<T, W, F, 512, 4>;
+          PPLX_LAUNCH(launch_groups(kernel, kernel, a.m, 512, 0, s, a));
+        }
+        return (int)PPLX_A2A_OK;
+      };
+      switch (p.format) {
+        case PPLX_A2A_ROWS_INT8: return launch(std::integral_constant<int, PPLX_A2A_ROWS_INT8>{});
+        case PPLX_A2A_ROWS_E4M3: return launch(std::integral_constant<int, PPLX_A2A_ROWS_E4M3>{});
+        default: return launch(std::integral_constant<int, PPLX_A2A_ROWS_PLAIN>{});
+      }
+    });
+  });
+}
+
+extern "C" int pplx_a2a_rms_norm_workspace(uint32_t m, uint64_t hidden_dim, uint64_t *bytes) {
+  PPLX_REQUIRE(bytes, "bytes is NULL");
+  PPLX_REQUIRE(hidden_dim > 0 && hidden_dim < (1ull << 27) && hidden_dim % 8 == 0, "hidden_dim must be a multiple of 8 below 2^27");
+  *bytes = 4 * (hidden_dim > kMostInRegisters ? (uint64_t)m : backward_groups(m) * hidden_dim);
+  return PPLX_A2A_OK;
+}
+
+extern "C" int pplx_a2a_rms_norm_backward(int device, const pplx_a2a_rms_norm_backward_args_t *args, void *stream) {
+  PPLX_REQUIRE(args, "args is NULL");
+  const pplx_a2a_rms_norm_backward_args_t &p = *args;
+  const int st = check_norm_size(p, 8);
+  if (st) return st;
+  PPLX_REQUIRE(p.m > 0, "there are no tokens");
+  PPLX_REQUIRE(p.grad_y && p.h && p.weight, "grad_y / h / weight is NULL");
+  PPLX_REQUIRE(is_aligned(p.weight, 16), "weight must be 16-byte aligned");
+  PPLX_REQUIRE(is_aligned(p.grad_weight, 16), "grad_weight must be 16-byte aligned");
+  PPLX_REQUIRE(!p.grad_weight || (p.workspace && is_aligned(p.workspace, 16)), "workspace is NULL or not aligned");
+  PPLX_ROWS(p, grad_y);
+  if (p.grad_sum) PPLX_ROWS(p, grad_sum);
+  PPLX_ROWS(p, h);
+  if (p.grad_h) PPLX_ROWS(p, grad_h);
+  if (!p.grad_h && !p.grad_weight) return PPLX_A2A_OK;
+  NormBackwardDev a{};
+  a.grad_y = static_cast<const uint8_t *>(p.grad_y);
+  a.grad_y_stride_row = p.grad_y_stride_row;
+  a.grad_sum = static_cast<const uint8_t *>(p.grad_sum);
+  a.grad_sum_stride_row = p.grad_sum_stride_row;
+  a.h = static_cast<const uint8_t *>(p.h);
+  a.h_stride_row = p.h_stride_row;
+  a.weight = static_cast<const uint8_t *>(p.weight);
+  a.grad_h = static_cast<uint8_t *>(p.grad_h);
+  a.grad_h_stride_row = p.grad_h_stride_row;
+  a.partial = p.grad_weight ? static_cast<float *>(p.workspace) : nullptr;
+  a.eps = p.eps;
+  a.inverse_width = (float)(1.0 / (double)p.hidden_dim);
+  a.m = p.m;
+  a.width = (uint32_t)p.hidden_dim;
+  return guarded(device, [&] {
+    return with_weight_type(p.dtype, p.weight_dtype, [&](auto tag, auto weight_tag) {
+      typedef typename decltype(tag)::type T;
+      typedef typename decltype(weight_tag)::type W;
+      hipStream_t s = (hipStream_t)stream;
+      const uint32_t groups = backward_groups(a.m), columns = (a.width + 511) / 512;
+      W *out = static_cast<W *>(p.grad_weight);
+      if (a.width > kMostInRegisters) {
+        PPLX_LAUNCH(launch_kernel(norm_backward_long<T, W>, dim3(groups), dim3(kLongLanes), 0, s, a));
+        if (out) PPLX_LAUNCH(launch_kernel(norm_weight_gradient_long<T, W>, dim3(columns), dim3(kSumWaves * 64), 0, s, a, out));
+        return (int)PPLX_A2A_OK;
+      }
+      if (a.width <= 2048) PPLX_LAUNCH(launch_kernel(norm_backward_rows<T, W, 64, 4>, dim3(groups), dim3(64), 0, s, a));
+      else if (a.width <= 8192) PPLX_LAUNCH(launch_kernel(norm_backward_rows<T, W, 256, 4>, dim3(groups), dim3(256), 0, s, a));
+      else PPLX_LAUNCH(launch_kernel(norm_backward_rows<T, W, 512, 4>, dim3(groups), dim3(512), 0, s, a));
+      if (out) {
+        const float *partial = a.partial;
+        PPLX_LAUNCH(launch_kernel(norm_weight_gradient<W>, dim3(columns), dim3(kSumWaves * 64), 0, s, partial, groups, a.width, out));
+      }
+      return (int)PPLX_A2A_OK;
+    });
+  });
+}

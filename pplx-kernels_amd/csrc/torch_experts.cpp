@@ -1,74 +1,13 @@
 // The torch layer of the operators between dispatch and combine: ops of pplx_kernels that write tensors of the caller,
 // and the same as functions of pplx_kernels._C, which also make the tensors where they are asked to (pplx_kernels/experts.py).
-#include <Python.h>
-
-#include <ATen/MemoryOverlap.h>
-#include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
-#include <c10/core/AutogradState.h>
 #include <torch/csrc/Dtype.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/library.h>
 
-#include <string>
 #include <tuple>
 
-#include "pplx_a2a.h"
-#include "torch_common.h"
+#include "torch_tensors.h"
 
 namespace {
-
-// ---------------------------------------------------------------------------
-// Checks
-// ---------------------------------------------------------------------------
-void check_on(const at::Tensor &x, const at::Tensor &with, const char *name) {
-  TORCH_CHECK(x.is_cuda(), "Tensor ", name, " must be on GPU");
-  TORCH_CHECK(x.device() == with.device(), "Tensor ", name, " must be on ", with.device(), ", not on ", x.device());
-}
-
-// Rows of the last dimension that lie in one piece, at 16-byte boundaries.
-void check_rows_of(const at::Tensor &x, const char *name) {
-  const int64_t dims = x.dim(), bytes = (int64_t)x.element_size();
-  TORCH_CHECK(x.sizes()[dims - 1] <= 1 || x.strides()[dims - 1] == 1, "the rows of ", name, " must be contiguous");
-  for (int64_t d = 0; d + 1 < dims; ++d) {
-    TORCH_CHECK(x.sizes()[d] <= 1 || x.strides()[d] * bytes % 16 == 0, "the rows of ", name, " must be 16-byte aligned");
-  }
-  TORCH_CHECK(reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0, "Tensor ", name, " must be 16-byte aligned");
-}
-
-// Stride of dimension d (elements); where there is one entry it is not used, and 0.
-int64_t step_of(const at::Tensor &x, int64_t d) { return x.sizes()[d] <= 1 ? 0 : x.strides()[d]; }
-int64_t byte_step_of(const at::Tensor &x, int64_t d) { return step_of(x, d) * (int64_t)x.element_size(); }
-
-void check_dense(const at::Tensor &x, at::ScalarType type, int64_t dims, const at::Tensor &with, const char *name) {
-  check_on(x, with, name);
-  TORCH_CHECK(x.dim() == dims, "Tensor ", name, " must be ", dims, " dimensional");
-  TORCH_CHECK(x.scalar_type() == type, name, " must be of type ", type);
-  TORCH_CHECK(x.is_contiguous(), "Tensor ", name, " must be contiguous");
-}
-
-void check_float(const at::Tensor &x, const char *name) {
-  TORCH_CHECK(dtype_code(x.scalar_type()) >= 0, "Unsupported dtype for ", name);
-}
-
-// What is written holds no element twice and none of what is read.
-void check_written(const at::Tensor &out, const char *name, std::initializer_list<const at::Tensor *> read) {
-  TORCH_CHECK(at::has_internal_overlap(out) != at::MemOverlap::Yes, "Tensor ", name, " holds elements more than once");
-  for (const at::Tensor *x : read) {
-    if (!x || !out.is_alias_of(*x)) continue;
-    const at::MemOverlapStatus status = at::get_overlap_status(out, *x);
-    TORCH_CHECK(status != at::MemOverlapStatus::Full && status != at::MemOverlapStatus::Partial, "Tensor ", name,
-                " overlaps a tensor that is read or written too");
-  }
-}
-
-// The writes are seen by autograd's check of saved tensors.
-void written(const at::Tensor &x) {
-  if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
-}
-
-template <class T> T *data_of(const at::Tensor *x) { return x ? static_cast<T *>(x->data_ptr()) : nullptr; }
 
 uint64_t sort_workspace(int64_t m, int64_t k, int64_t experts) {
   TORCH_CHECK(m <= UINT32_MAX && k <= UINT32_MAX && experts >= 0 && experts <= UINT32_MAX,
@@ -357,8 +296,6 @@ void int8_matmul(const at::Tensor &out, const at::Tensor &x, const at::Tensor &x
 // ---------------------------------------------------------------------------
 // The registered ops
 // ---------------------------------------------------------------------------
-using opt_tensor = const std::optional<at::Tensor> &;
-
 void sort_tokens_op(at::Tensor &rows, opt_tensor scale, at::Tensor &slots, at::Tensor &offsets, opt_tensor workspace,
                     const at::Tensor &x, const at::Tensor &indices, opt_tensor bound_m) {
   sort_tokens(rows, opt(scale), slots, offsets, opt(workspace), x, indices, opt(bound_m));
@@ -386,15 +323,6 @@ int64_t sort_workspace_op(int64_t m, int64_t k, int64_t experts) {
 // ---------------------------------------------------------------------------
 // The differentiable ones, which make their results
 // ---------------------------------------------------------------------------
-at::Tensor fresh(at::IntArrayRef sizes, const at::Tensor &with, at::ScalarType type) {
-  return at::empty(sizes, at::TensorOptions(with.device()).dtype(type));
-}
-
-// The same of sizes that a trace may not know.
-at::Tensor fresh_traced(c10::SymIntArrayRef sizes, const at::Tensor &with, at::ScalarType type) {
-  return at::empty_symint(sizes, at::TensorOptions(with.device()).dtype(type));
-}
-
 struct Sorted {
   at::Tensor rows, scale, slots, offsets, workspace;
 };
@@ -412,8 +340,6 @@ Sorted new_sorted(const at::Tensor &x, const at::Tensor &indices, int64_t expert
   if (words) s.workspace = fresh({words}, x, at::kInt);
   return s;
 }
-
-const at::Tensor *defined(const at::Tensor &t) { return t.defined() ? &t : nullptr; }
 
 Sorted sort_new(const at::Tensor &x, const at::Tensor &indices, int64_t experts, const at::Tensor *bound_m, bool int8) {
   TORCH_CHECK(x.is_cuda(), "Tensor x must be on GPU");
@@ -456,50 +382,7 @@ at::Tensor unsorted_tokens_op(const at::Tensor &y, const at::Tensor &slots, cons
   return out;
 }
 
-// The ops above and those on tensors of the caller, through the dispatcher, so that a step can be traced.
-template <class Fn> auto op_handle(const char *name) {
-  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Fn>();
-}
-
-// Gradients come in any layout (that of a sum is one element, expanded).  Those of a traced step have no address, and sizes
-// that may not be known.
-at::Tensor as_rows(const at::Tensor &g) {
-  if (g.is_meta() || g.key_set().has(c10::DispatchKey::Python) || g.key_set().has(c10::DispatchKey::Functionalize)) return g.contiguous();
-  const int64_t bytes = (int64_t)g.element_size();
-  const bool fits =
-      g.strides()[1] == 1 && g.strides()[0] * bytes % 16 == 0 && reinterpret_cast<uintptr_t>(g.data_ptr()) % 16 == 0;
-  return fits ? g : g.clone(at::MemoryFormat::Contiguous);
-}
-
-// Gradients that are asked for their own (create_graph) say that they have none when they are.
-torch::autograd::variable_list differentiable_once(torch::autograd::variable_list grads) {
-  if (!at::GradMode::is_enabled()) return grads;
-  torch::autograd::variable_list made;
-  for (const at::Tensor &g : grads) {
-    if (g.defined()) made.push_back(g);
-  }
-  auto error = std::make_shared<torch::autograd::DelayedError>(
-      "pplx_kernels: the gradients of sort_tokens and unsort_tokens are differentiable once", (int64_t)made.size());
-  for (at::Tensor &g : made) {
-    g = g.detach();
-    g.requires_grad_(true);
-  }
-  made = (*error)(std::move(made));
-  size_t next = 0;
-  for (at::Tensor &g : grads) {
-    if (g.defined()) g = made[next++];
-  }
-  return grads;
-}
-
-// Tangents of forward-mode differentiation are refused, not dropped.
-void check_no_tangent(std::initializer_list<const at::Tensor *> read) {
-  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
-  for (const at::Tensor *x : read) {
-    TORCH_CHECK(!x || !x->defined() || !x->_fw_grad(0).defined(),
-                "pplx_kernels: sort_tokens, unsort_tokens and their gradients have no forward-mode derivatives");
-  }
-}
+constexpr char kDifferentiable[] = "sort_tokens and unsort_tokens";  // (in messages)
 
 SortedTuple call_sorted_tokens(const at::Tensor &x, const at::Tensor &indices, int64_t experts, opt_tensor bound_m, bool int8) {
   at::AutoDispatchBelowADInplaceOrView below;
@@ -521,7 +404,7 @@ struct SortFunction : torch::autograd::Function<SortFunction> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
                                                  torch::autograd::variable_list grads) {
     at::Tensor grad_x;
-    check_no_tangent({&grads[0]});
+    check_no_tangent({&grads[0]}, kDifferentiable);
     if (grads[0].defined()) {
       const at::Tensor slots = ctx->get_saved_variables()[0];
       at::NoGradGuard plain;
@@ -531,7 +414,7 @@ struct SortFunction : torch::autograd::Function<SortFunction> {
       grad_x = fresh_traced({slots.sym_size(0), g.sym_size(1)}, g, g.scalar_type());
       op.call(grad_x, g, slots, std::nullopt);
     }
-    return differentiable_once({grad_x, at::Tensor(), at::Tensor(), at::Tensor()});
+    return differentiable_once({grad_x, at::Tensor(), at::Tensor(), at::Tensor()}, kDifferentiable);
   }
 };
 
@@ -551,7 +434,7 @@ struct UnsortFunction : torch::autograd::Function<UnsortFunction> {
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &y = saved[0], &weights = saved[3];
     at::Tensor grad_y, grad_weights;
-    check_no_tangent({&grads[0], &y, &weights});
+    check_no_tangent({&grads[0], &y, &weights}, kDifferentiable);
     {
       at::NoGradGuard plain;
       static auto op = op_handle<void(opt_tensor, opt_tensor, const at::Tensor &, const at::Tensor &, const at::Tensor &,
@@ -565,14 +448,14 @@ struct UnsortFunction : torch::autograd::Function<UnsortFunction> {
         op.call(if_defined(grad_y), if_defined(grad_weights), as_rows(grads[0]), y, saved[1], saved[2], if_defined(weights));
       }
     }
-    return differentiable_once({grad_y, at::Tensor(), at::Tensor(), grad_weights, at::Tensor()});
+    return differentiable_once({grad_y, at::Tensor(), at::Tensor(), grad_weights, at::Tensor()}, kDifferentiable);
   }
 };
 
 SortedTuple sorted_tokens_autograd(const at::Tensor &x, const at::Tensor &indices, int64_t experts, opt_tensor bound_m,
                                    bool int8) {
   if (int8) return call_sorted_tokens(x, indices, experts, bound_m, true);
-  check_no_tangent({&x});
+  check_no_tangent({&x}, kDifferentiable);
   if (at::GradMode::is_enabled() && x.requires_grad()) {
     TORCH_CHECK(x.dim() == 2 && x.sym_size(1) % 8 == 0, "x must have rows of a multiple of 8 elements for its gradient");
   }
@@ -581,20 +464,8 @@ SortedTuple sorted_tokens_autograd(const at::Tensor &x, const at::Tensor &indice
 }
 at::Tensor unsorted_tokens_autograd(const at::Tensor &y, const at::Tensor &slots, const at::Tensor &offsets,
                                     opt_tensor weights, std::optional<at::ScalarType> out_dtype) {
-  check_no_tangent({&y, opt(weights)});
+  check_no_tangent({&y, opt(weights)}, kDifferentiable);
   return UnsortFunction::apply(y, slots, offsets, weights, out_dtype);
-}
-
-// Meta kernels: a traced call does nothing.
-template <class Fn> struct Nothing;
-template <class... A> struct Nothing<void (*)(A...)> {
-  static void run(A...) {}
-};
-
-template <class Fn> void define(torch::Library &m, const char *name, const char *schema, Fn fn) {
-  m.def((std::string(name) + schema).c_str());
-  m.impl(name, c10::kCUDA, fn);
-  m.impl(name, c10::kMeta, &Nothing<Fn>::run);
 }
 
 }  // namespace
@@ -630,29 +501,6 @@ TORCH_LIBRARY_FRAGMENT(pplx_kernels, m) {
 // Functions of pplx_kernels._C
 // ---------------------------------------------------------------------------
 namespace {
-
-// Whether the dispatcher would go straight to the kernel (or to autograd, which the functions see to).  A tracer, a mode, a
-// transform or a tensor that is more than its data has to see the registered op: behind its back the results would be taken for
-// what `empty` made.
-bool straight(std::initializer_list<const at::Tensor *> tensors) {
-  static const uint64_t usual =
-      c10::full_backend_mask | c10::autocast_dispatch_keyset.raw_repr() |
-      c10::DispatchKeySet({c10::DispatchKey::Dense, c10::DispatchKey::BackendSelect, c10::DispatchKey::ADInplaceOrView,
-                           c10::DispatchKey::AutogradFunctionality}).raw_repr();
-  const auto local = c10::impl::tls_local_dispatch_key_set();
-  c10::DispatchKeySet keys = local.included_;
-  for (const at::Tensor *x : tensors) {
-    if (x) keys = keys | x->key_set();
-  }
-  return ((keys - local.excluded_).raw_repr() & ~usual) == 0;
-}
-
-std::optional<at::Tensor> maybe(const at::Tensor *x) { return x ? std::optional<at::Tensor>(*x) : std::nullopt; }
-
-PyObject *wrap_or_none(const at::Tensor &t) {
-  if (!t.defined()) Py_RETURN_NONE;
-  return THPVariable_Wrap(t);
-}
 
 // sort_tokens(x, indices, num_experts, bound_m, int8) -> (rows, scale, slots, offsets, workspace): on new tensors
 PyObject *py_sort_tokens(PyObject *, PyObject *const *args, Py_ssize_t nargs) {

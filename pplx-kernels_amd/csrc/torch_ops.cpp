@@ -38,6 +38,7 @@
 #include "torch_common.h"
 
 PyMethodDef *experts_methods();  // the functions of torch_experts.cpp
+PyMethodDef *router_methods();   // the functions of torch_router.cpp
 
 namespace {
 
@@ -978,5 +979,6 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_C", "torch operator layer of ppl
 PyMODINIT_FUNC PyInit__C(void) {
   PyObject *module = PyModule_Create(&kModule);
   if (module && PyModule_AddFunctions(module, experts_methods()) != 0) Py_CLEAR(module);
+  if (module && PyModule_AddFunctions(module, router_methods()) != 0) Py_CLEAR(module);
   return module;
 }

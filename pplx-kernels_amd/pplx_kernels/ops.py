@@ -77,6 +77,14 @@ EXPORTED_SYMBOLS = (
     "pplx_a2a_quantize_rows",
     "pplx_a2a_int8_matmul",
     "pplx_a2a_int8_matmul_plan",
+    "pplx_a2a_rms_norm",
+    "pplx_a2a_rms_norm_workspace",
+    "pplx_a2a_rms_norm_backward",
+    "pplx_a2a_router_workspace",
+    "pplx_a2a_router_logits",
+    "pplx_a2a_router_logits_backward",
+    "pplx_a2a_route_tokens",
+    "pplx_a2a_route_tokens_backward",
     "pplx_a2a_last_error",
     "pplx_a2a_version",
     "pplx_a2a_build_id",
