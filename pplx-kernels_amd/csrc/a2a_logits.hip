@@ -6,10 +6,15 @@
 // first.  The matrix cores take 16-bit elements.  What has more bits is a sum of bf16 pieces, each the part of a value
 // that the pieces before leave: two hold an fp16 value, three an fp32 one.  Of the products of pieces those below 2^-24 of the
 // largest are left out.
+#include <cmath>
+
 #include "a2a_experts.h"
+#include "a2a_tiles.h"
 
 namespace pplx_amd {
 namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 struct ProductDev {
   const uint8_t *a;
@@ -23,27 +28,31 @@ struct ProductDev {
   uint32_t first_group;
 };
 
-template <class T> struct Pieces;
-template <> struct Pieces<__bf16> {
-  static constexpr int count = 1;
-  static __device__ __forceinline__ void of(bf16x8 v, bf16x8 *p) { p[0] = v; }
-};
-template <> struct Pieces<_Float16> {
-  static constexpr int count = 2;
-  static __device__ __forceinline__ void of(f16x8 v, bf16x8 *p) {
-    const f32x8 w = __builtin_convertvector(v, f32x8);
-    p[0] = __builtin_convertvector(w, bf16x8);
-    p[1] = __builtin_convertvector(w - __builtin_convertvector(p[0], f32x8), bf16x8);
+// N pieces of eight values, each rounded to nearest; two fp32 words to a pair of bf16 and back take one instruction each way.
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+template <int N> __device__ __forceinline__ void cut(f32x8 v, bf16x8 *p) {
+  typedef uint32_t words __attribute__((ext_vector_type(4)));
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    words w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{v[2 * i], v[2 * i + 1]}, bf16x2));
+      if (n + 1 == N) continue;
+      v[2 * i] -= __uint_as_float(w[i] << 16);
+      v[2 * i + 1] -= __uint_as_float(w[i] & 0xffff0000u);
+    }
+    p[n] = __builtin_bit_cast(bf16x8, w);
   }
-};
-template <> struct Pieces<float> {
-  static constexpr int count = 3;
-  static __device__ __forceinline__ void of(f32x8 v, bf16x8 *p) {
-    p[0] = __builtin_convertvector(v, bf16x8);
-    f32x8 left = v - __builtin_convertvector(p[0], f32x8);
-    p[1] = __builtin_convertvector(left, bf16x8);
-    left -= __builtin_convertvector(p[1], f32x8);
-    p[2] = __builtin_convertvector(left, bf16x8);
+}
+// Pieces that hold a value in full, or the first ORDER + 1 of them.
+template <class T, int ORDER = 2> struct Pieces {
+  static constexpr int kFull = std::is_same_v<T, __bf16> ? 1 : std::is_same_v<T, _Float16> ? 2 : 3;
+  static constexpr int count = kFull < ORDER + 1 ? kFull : ORDER + 1;
+  static __device__ __forceinline__ void of(typename Eight<T>::raw v, bf16x8 *p) {
+    if constexpr (std::is_same_v<T, __bf16>) p[0] = v;
+    else cut<count>(Eight<T>::wide(v), p);
   }
 };
 
@@ -75,8 +84,8 @@ template <class A, class B> __device__ __forceinline__ f32x4 multiply_add(const 
 // A workgroup to 16 RF rows by 16 CF columns, whose eight waves share out k, 32 elements at a time, and add their sums in
 // LDS, in the order of the waves.  Operands go straight to registers.
 constexpr int kProductWaves = 8;
-template <class TA, class TB, class O, int RF, int CF, int AHEAD>
-__global__ __launch_bounds__(kProductWaves * 64) void product_split(ProductDev a) {
+template <class TA, class TB, class O> __global__ __launch_bounds__(kProductWaves * 64) void product_split(ProductDev a) {
+  constexpr int RF = 1, CF = 1, AHEAD = 2;
   __shared__ float sums[kProductWaves][RF * CF * 4 * 64];
   const uint32_t lane = lane_id(), wave = wave_id(), group = a.first_group + blockIdx.x;
   const uint32_t block = group / a.column_blocks;
@@ -99,9 +108,10 @@ __global__ __launch_bounds__(kProductWaves * 64) void product_split(ProductDev a
     typename Eight<TB>::raw b[CF];
   };
   Unit u[AHEAD];
+  // (units behind the last are loads of the first elements, which are taken for zeros: a branch would wait for all loads)
   auto load = [&](Unit &to, uint32_t unit) __attribute__((always_inline)) {
     const uint32_t k = unit * 32 + own;
-    const uint32_t at = k < a.k ? k : 0;  // (elements behind k are taken for zeros)
+    const uint32_t at = k < a.k ? k : 0;
 #pragma unroll
     for (int i = 0; i < CF; ++i) to.b[i] = load_eight<TB>(column[i] + at);
 #pragma unroll
@@ -109,14 +119,11 @@ __global__ __launch_bounds__(kProductWaves * 64) void product_split(ProductDev a
   };
   f32x4 acc[RF][CF] = {};
 #pragma unroll
-  for (int i = 0; i < AHEAD; ++i) {
-    if (wave + i * kProductWaves < units) load(u[i], wave + i * kProductWaves);
-  }
+  for (int i = 0; i < AHEAD; ++i) load(u[i], wave + i * kProductWaves);
   for (uint32_t first = wave; first < units; first += AHEAD * kProductWaves) {
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       const uint32_t unit = first + i * kProductWaves;
-      if (unit >= units) break;
       const bool there = unit * 32 + own < a.k;
       Operand<TB, TA> fb[CF];
 #pragma unroll
@@ -128,7 +135,7 @@ __global__ __launch_bounds__(kProductWaves * 64) void product_split(ProductDev a
 #pragma unroll
         for (int c = 0; c < CF; ++c) acc[r][c] = multiply_add(fb[c], fa, acc[r][c]);
       }
-      if (unit + AHEAD * kProductWaves < units) load(u[i], unit + AHEAD * kProductWaves);
+      load(u[i], unit + AHEAD * kProductWaves);
     }
   }
 #pragma unroll
@@ -155,67 +162,475 @@ __global__ __launch_bounds__(kProductWaves * 64) void product_split(ProductDev a
   }
 }
 
-template <class TA, class TB, class O> int launch_product(const ProductDev &from, hipStream_t s) {
-  ProductDev a = from;
-  a.column_blocks = (a.columns + 31) / 32;
-  auto kernel = product_split<TA, TB, O, 2, 2, 2>;
-  return launch_groups(kernel, kernel, ((uint64_t)a.rows + 31) / 32 * a.column_blocks, kProductWaves * 64, 0, s, a);
+// ---------------------------------------------------------------------------
+// Tiles of BM rows by BN columns through LDS, which loads write directly
+// ---------------------------------------------------------------------------
+struct TilesDev {
+  const int8_t *a, *b;
+  int64_t a_stride, b_stride;  // bytes
+  float *out;
+  int64_t out_stride;  // elements
+  uint64_t out_split;  // elements from one split's sums to the next's
+  uint32_t rows, columns, k;
+  uint32_t row_blocks, column_blocks, splits, steps_per_split;
+};
+
+__device__ __forceinline__ f32x16 multiply_32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 multiply_32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+// Lines of 64 elements of a row: of 128 bytes, or 256.  Chunk c of line r lies at c ^ exchange(r): sixteen consecutive lines hold a
+// chunk at sixteen places of 256 bytes, which is what LDS reads at a time.
+template <class T> struct Lines {
+  static constexpr uint32_t kBytes = 64 * sizeof(T), kChunks = kBytes / 16, kPerLoad = 64 / kChunks;
+  static __device__ __forceinline__ uint32_t exchange(uint32_t line) { return kChunks == 8 ? (line >> 1) & 7 : line & 15; }
+};
+
+// WM by WN waves, each BM / WM rows by BN / WN columns in fragments of 32 by 32; STAGES steps of 64 elements of k in LDS.  A wave
+// reads the fragments of the next sixteen k before it multiplies those at hand, over the border between two steps too: there it
+// waits for the next step's loads, and behind the barrier this step's place takes those of a step to come.  What is cut into pieces
+// is cut between LDS and the matrix cores.  TAIL: k is no multiple of 64.
+template <class TA, class TB, int BM, int BN, int WM, int WN, int STAGES, bool TAIL>
+__global__ __launch_bounds__(WM *WN * 64) void logits_tiles(TilesDev a) {
+  typedef Lines<TA> LA;
+  typedef Lines<TB> LB;
+  constexpr int kWaves = WM * WN;
+  constexpr int kRows = BM / WM, kColumns = BN / WN, MF = kRows / 32, NF = kColumns / 32;
+  constexpr int kLoadsA = BM / (int)LA::kPerLoad / kWaves, kLoadsB = BN / (int)LB::kPerLoad / kWaves, kLoads = kLoadsA + kLoadsB;
+  static_assert(kLoadsA * LA::kPerLoad * kWaves == BM && kLoadsB * LB::kPerLoad * kWaves == BN, "whole loads");
+  static_assert(MF >= 1 && NF >= 1 && kRows % 32 == 0 && kColumns % 32 == 0, "whole fragments");
+  static_assert((STAGES - 1) * kLoads < 63, "loads that can be counted");
+  constexpr uint32_t kPlaceB = BM * LA::kBytes, kStage = kPlaceB + BN * LB::kBytes;
+  static_assert(STAGES * kStage <= kLdsBytes, "loads to LDS stay in front of kLdsBytes");
+  extern __shared__ __align__(128) uint8_t lds[];  // [STAGES][BM lines of the rows, BN of the columns]
+  const uint32_t lane = lane_id(), wave = wave_id();
+  const uint32_t wm = wave % WM, wn = wave / WM;
+  // (blockIdx goes round the eight XCDs: one of them takes tiles of one split, whose part of the columns' operand its L2 holds, and all
+  // tiles of a block of rows)
+  const uint32_t id = (blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;
+  const uint32_t block = id / a.column_blocks, split = block / a.row_blocks;
+  if (split >= a.splits) return;
+  const uint32_t m0 = __builtin_amdgcn_readfirstlane((block - split * a.row_blocks) * BM);
+  const uint32_t n0 = __builtin_amdgcn_readfirstlane((id - block * a.column_blocks) * BN);
+  const uint32_t all_steps = (a.k + 63) / 64;
+  const uint32_t begin = __builtin_amdgcn_readfirstlane(split * a.steps_per_split);
+  const uint32_t end = begin + a.steps_per_split < all_steps ? begin + a.steps_per_split : all_steps;
+  const uint32_t lds0 = lds_address(lds);
+
+  const int8_t *first_a = a.a + (int64_t)m0 * a.a_stride, *first_b = a.b + (int64_t)n0 * a.b_stride;
+  const uint32_t rows_left = a.rows - m0, columns_left = a.columns - n0;
+  uint32_t offset[kLoads], chunk[kLoads];  // (the chunks are the same for all loads of an operand, or alternate)
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const bool of_a = i < kLoadsA;
+    const uint32_t chunks = of_a ? LA::kChunks : LB::kChunks, per_load = 64 / chunks;
+    const uint32_t line = ((of_a ? i : i - kLoadsA) * kWaves + wave) * per_load + lane / chunks;
+    chunk[i] = (lane % chunks) ^ (of_a ? LA::exchange(line) : LB::exchange(line));
+    offset[i] = chunk[i] * 16 + (of_a ? (line < rows_left ? line : rows_left - 1) * (uint32_t)a.a_stride
+                                      : (line < columns_left ? line : columns_left - 1) * (uint32_t)a.b_stride);
+  }
+  // Load number i of a step.  Behind k a lane fetches the first chunk of its line; what it brings is taken for zeros.  Loads of
+  // steps that do not exist bring nothing, and count.
+  auto fetch = [&](int i, uint32_t step, uint32_t stage) __attribute__((always_inline)) {
+    const bool of_a = i < kLoadsA;
+    const uint32_t bytes = of_a ? LA::kBytes : LB::kBytes, size = of_a ? sizeof(TA) : sizeof(TB);
+    const int8_t *base = (of_a ? first_a : first_b) + (uint64_t)step * bytes;
+    const bool behind = TAIL && step * 64 + chunk[i] * (16 / size) >= a.k;
+    const uint32_t place = of_a ? i * kWaves + wave : (i - kLoadsA) * kWaves + wave;
+    load_to_lds(base, behind ? offset[i] - chunk[i] * 16 : offset[i], lds0 + stage * kStage + (of_a ? 0 : kPlaceB) + place * 1024,
+                step < end ? ~0u : 0u);
+  };
+  typename Eight<TA>::raw ra[2][MF];
+  typename Eight<TB>::raw rb[2][NF];
+  constexpr int kReads = MF + NF;
+  auto read_line = [&](auto &to, auto lines, const uint8_t *line, int kk, uint32_t step) __attribute__((always_inline)) {
+    typedef decltype(lines) L;
+    u32x4 v[L::kChunks / 8];
+#pragma unroll
+    for (uint32_t h = 0; h < L::kChunks / 8; ++h) {
+      const uint32_t c = (2 * kk + lane / 32) * (L::kChunks / 8) + h;
+      v[h] = *reinterpret_cast<const u32x4 *>(line + (c ^ L::exchange(lane % 32)) * 16);
+      if constexpr (TAIL) v[h] &= step * 64 + kk * 16 + lane / 32 * 8 < a.k ? ~0u : 0u;
+    }
+    __builtin_memcpy(&to, v, sizeof(v));
+  };
+  auto read = [&](int i, int to, int kk, uint32_t step, uint32_t stage) __attribute__((always_inline)) {
+    const uint8_t *lines = lds + stage * kStage;
+    if (i < MF) read_line(ra[to][i], LA{}, lines + (wm * kRows + i * 32 + lane % 32) * LA::kBytes, kk, step);
+    else read_line(rb[to][i - MF], LB{}, lines + kPlaceB + (wn * kColumns + (i - MF) * 32 + lane % 32) * LB::kBytes, kk, step);
+  };
+  f32x16 acc[NF][MF] = {};
+#pragma unroll
+  for (int s = 0; s < STAGES; ++s) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) fetch(i, begin + s, s);
+  }
+  wait_loads<(STAGES - 1) * kLoads>();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < kReads; ++i) read(i, 0, 0, begin, 0);
+  typedef Operand<TA, TB> OA;
+  typedef Operand<TB, TA> OB;
+  constexpr int kMost = OA::count + OB::count - 2 < 2 ? OA::count + OB::count - 2 : 2;
+  constexpr int kPairs = OA::count + OB::count < 4 || OA::count == 1 || OB::count == 1 ? OA::count * OB::count
+                         : OA::count + OB::count == 6                                  ? 6
+                                                                                       : 5;
+  constexpr int kProducts = MF * NF * kPairs;
+  // The products of sixteen k, between which the reads of the next sixteen and the loads of a step go out: a wave issues in order, and
+  // one that hands over all its reads or loads at once waits for them to be taken.
+  auto multiply = [&](int from, auto read_next, auto fetch_next) __attribute__((always_inline)) {
+    OA fa[MF];
+    OB fb[NF];
+#pragma unroll
+    for (int i = 0; i < MF; ++i) fa[i].set(ra[from][i]);
+#pragma unroll
+    for (int j = 0; j < NF; ++j) fb[j].set(rb[from][j]);
+    int q = 0;
+#pragma unroll
+    for (int order = kMost; order >= 0; --order) {
+#pragma unroll
+      for (int pa = 0; pa < OA::count; ++pa) {
+        const int pb = order - pa;
+        if (pb < 0 || pb >= OB::count) continue;
+#pragma unroll
+        for (int j = 0; j < NF; ++j) {
+#pragma unroll
+          for (int i = 0; i < MF; ++i) {
+            acc[j][i] = multiply_32(fb[j].p[pb], fa[i].p[pa], acc[j][i]);
+#pragma unroll
+            for (int r = q * kReads / kProducts; r < (q + 1) * kReads / kProducts; ++r) read_next(r);
+#pragma unroll
+            for (int l = q * kLoads / kProducts; l < (q + 1) * kLoads / kProducts; ++l) fetch_next(l);
+            __builtin_amdgcn_sched_barrier(0);
+            ++q;
+          }
+        }
+      }
+    }
+  };
+  uint32_t stage = 0;
+  for (uint32_t step = begin; step < end; ++step) {
+    const uint32_t next = stage + 1 == STAGES ? 0 : stage + 1;
+#pragma unroll
+    for (int kk = 0; kk < 3; ++kk) {
+      multiply(kk % 2, [&](int r) { read(r, (kk + 1) % 2, kk + 1, step, stage); }, [](int) {});
+    }
+    // Loads under way are those of steps step + 1 .. step + STAGES - 1; this step's place is free behind the barrier.
+    wait_loads<(STAGES - 2) * kLoads, true>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    multiply(1, [&](int r) { read(r, 0, 0, step + 1, next); }, [&](int l) { fetch(l, step + STAGES, stage); });
+    stage = next;
+  }
+  wait_loads<0, true>();
+  // Lane l holds row l % 32 of each fragment and columns 4 (l / 32) .. + 3 of every eight.
+  typedef float four __attribute__((ext_vector_type(4), aligned(4)));
+#pragma unroll
+  for (int i = 0; i < MF; ++i) {
+    const uint32_t row = m0 + wm * kRows + i * 32 + lane % 32;
+    if (row >= a.rows) continue;
+    PPLX_GLOBAL float *out = as_global(a.out) + split * a.out_split + (int64_t)row * a.out_stride;
+#pragma unroll
+    for (int j = 0; j < NF; ++j) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t n = n0 + wn * kColumns + j * 32 + q * 8 + 4 * (lane / 32);
+        if (n + 4 <= a.columns) {
+          *reinterpret_cast<PPLX_GLOBAL four *>(out + n) = four{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
+        } else {
+#pragma unroll
+          for (uint32_t u = 0; u < 3; ++u) {
+            if (n + u < a.columns) out[n + u] = acc[j][i][4 * q + u];
+          }
+        }
+      }
+    }
+  }
 }
 
-// out[c, r] = in[r, c], zeros for r from rows up to the next multiple of eight; a workgroup to 64 by 64.
-struct TurnDev {
-  const uint8_t *in;
-  int64_t in_stride;  // bytes
+// The sums of the splits as results: eight threads to four columns, each with every eighth split, whose sums are added in order.
+// Rows of the sums are `columns` long, a multiple of four, of which `width` are there.
+struct SumDev {
+  const float *sums;
+  uint64_t split;  // elements
   uint8_t *out;
-  int64_t out_stride;  // bytes
-  uint32_t rows, columns;
-  uint32_t column_blocks;
+  int64_t out_stride;  // elements
+  uint32_t rows, columns, width, splits;
   uint32_t first_group;
 };
-template <class T> __global__ __launch_bounds__(256) void turn(TurnDev a) {
-  __shared__ T tile[64][65];
-  const uint32_t group = a.first_group + blockIdx.x, block = group / a.column_blocks;
-  const uint32_t r0 = block * 64, c0 = (group - block * a.column_blocks) * 64;
-  const uint32_t x = threadIdx.x % 64;
-  for (uint32_t y = threadIdx.x / 64; y < 64; y += 4) {
-    const uint32_t r = r0 + y, c = c0 + x;
-    tile[y][x] = r < a.rows && c < a.columns ? as_global(reinterpret_cast<const T *>(a.in + (int64_t)r * a.in_stride))[c] : (T)0;
+template <class O, int SHARES> __global__ __launch_bounds__(256) void sum_splits(SumDev a) {
+  __shared__ f32x4 shares[SHARES > 1 ? 256 : 1];
+  constexpr uint32_t kPer = 256 / SHARES;  // results of a workgroup
+  const uint32_t per_row = a.columns / 4, share = threadIdx.x / kPer;
+  const uint64_t i = (uint64_t)(a.first_group + blockIdx.x) * kPer + threadIdx.x % kPer;
+  const uint32_t r = i >> 32 ? (uint32_t)(i / per_row) : (uint32_t)i / per_row, c = (uint32_t)(i - (uint64_t)r * per_row) * 4;
+  f32x4 s = {};
+  if (r < a.rows) {
+    const PPLX_GLOBAL float *p = as_global(a.sums) + (uint64_t)r * a.columns + c;
+#pragma unroll 4
+    for (uint32_t k = share; k < a.splits; k += SHARES) s += *reinterpret_cast<const PPLX_GLOBAL f32x4 *>(p + k * a.split);
+  }
+  if constexpr (SHARES > 1) {
+    shares[threadIdx.x] = s;
+    __syncthreads();
+    if (share) return;
+#pragma unroll
+    for (int k = 1; k < SHARES; ++k) s += shares[k * kPer + threadIdx.x];
+  }
+  if (r >= a.rows) return;
+  PPLX_GLOBAL O *out = as_global(reinterpret_cast<O *>(a.out)) + (int64_t)r * a.out_stride + c;
+  typedef O four __attribute__((ext_vector_type(4), aligned(sizeof(O))));
+  if (c + 4 <= a.width) {
+    *reinterpret_cast<PPLX_GLOBAL four *>(out) = four{(O)s[0], (O)s[1], (O)s[2], (O)s[3]};
+  } else {
+#pragma unroll
+    for (uint32_t u = 0; u < 3; ++u) {
+      if (c + u < a.width) out[u] = (O)s[u];
+    }
+  }
+}
+template <class O> int launch_sum(const SumDev &a, hipStream_t s) {
+  const uint64_t results = (uint64_t)a.rows * (a.columns / 4);
+  if (a.splits <= 8) return launch_groups(sum_splits<O, 1>, sum_splits<O, 1>, (results + 255) / 256, 256, 0, s, a);
+  return launch_groups(sum_splits<O, 8>, sum_splits<O, 8>, (results + 31) / 32, 256, 0, s, a);
+}
+
+// ---------------------------------------------------------------------------
+// Gradients: sums over k of a[i, k] * b[k, n], where the rows of b lie along n
+// ---------------------------------------------------------------------------
+// The matrix cores want eight consecutive k of a column in a lane.  A lane fetches NV consecutive columns of eight rows of b, and the
+// vectors are turned in its registers: fragment f has the columns f, NV + f, 2 NV + f .. of a block of 32 NV, and the sums of a lane,
+// one for each fragment, are consecutive columns again.  Fragments go to LDS, from where all waves of a workgroup take them.
+// The other operand, grad_logits, is cut into pieces once, by split_gradient, and lies in the order in which lanes take them.
+struct GradientDev {
+  const uint8_t *a;  // [blocks of 32 rows][sixteens of k][pieces][64 lanes] of 16 bytes
+  const uint8_t *b;
+  int64_t b_stride;  // bytes
+  uint8_t *out;
+  int64_t out_stride;  // elements
+  uint64_t out_split;  // elements
+  uint32_t rows, columns, k;
+  uint32_t column_blocks, parts;  // (parts: of the rows, or of k)
+  uint32_t first_group;
+};
+
+template <class TB, int NV, int ORDER> struct Turned {
+  typedef Pieces<TB, ORDER> Cut;
+  static constexpr int kPieces = Cut::count;
+  static constexpr int kBytes = kPieces * NV * 1024;  // of sixteen k in LDS
+  typedef TB vec __attribute__((ext_vector_type(NV)));
+  vec row[8];
+
+  // Columns `column` .. + NV of rows k .. k + 7.  What lies behind the last k is zeros.
+  __device__ __forceinline__ void load(const GradientDev &a, uint32_t column, uint32_t k) {
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const uint32_t at = k + r < a.k ? k + r : a.k - 1;
+      row[r] = *reinterpret_cast<const PPLX_GLOBAL vec *>(as_global(reinterpret_cast<const TB *>(a.b + (int64_t)at * a.b_stride)) + column);
+    }
+  }
+  __device__ __forceinline__ void store(uint8_t *to, uint32_t left, uint32_t lane) const {  // (left: k that are there)
+#pragma unroll
+    for (int f = 0; f < NV; ++f) {
+      typename Eight<TB>::raw v;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) v[r] = (uint32_t)r < left ? row[r][f] : (TB)0;
+      bf16x8 p[kPieces];
+      Cut::of(v, p);
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) *reinterpret_cast<bf16x8 *>(to + ((i * NV + f) * 64 + lane) * 16) = p[i];
+    }
+  }
+};
+
+typedef const PPLX_GLOBAL bf16x8 *FragmentPtr;
+template <int ORDER> struct Fragments {  // of 32 rows and sixteen k
+  bf16x8 p[ORDER + 1];
+  // Number i of those at `from`, the first where there are not so many.
+  __device__ __forceinline__ void load(FragmentPtr from, uint32_t i, uint32_t all) {
+    from += (uint64_t)(i < all ? i : 0) * (64 * (ORDER + 1));
+#pragma unroll
+    for (int n = 0; n <= ORDER; ++n) p[n] = from[n * 64];
+  }
+};
+// Their products with the columns' fragments at `from`.
+template <int PIECES, int NV, int ORDER>
+__device__ __forceinline__ void multiply_turned(const Fragments<ORDER> &fa, const uint8_t *from, uint32_t lane, f32x16 *acc) {
+#pragma unroll
+  for (int pb = PIECES - 1; pb >= 0; --pb) {
+    bf16x8 fb[NV];
+#pragma unroll
+    for (int f = 0; f < NV; ++f) fb[f] = *reinterpret_cast<const bf16x8 *>(from + ((pb * NV + f) * 64 + lane) * 16);
+#pragma unroll
+    for (int pa = ORDER - pb; pa >= 0; --pa) {
+#pragma unroll
+      for (int f = 0; f < NV; ++f) acc[f] = multiply_32(fa.p[pa], fb[f], acc[f]);
+    }
+  }
+}
+
+// Pieces of grad_logits [rows, columns] as fragments of its rows, and of its columns (either may be left out).
+struct PiecesDev {
+  const float *in;
+  int64_t in_stride;  // elements
+  uint32_t rows, columns;
+  uint8_t *by_rows, *by_columns;
+  uint32_t pieces_by_rows, pieces_by_columns;
+  uint32_t first_group;
+};
+// A workgroup to 32 rows by 32 columns, of which a wave each takes half a block of rows, and of columns.
+__global__ __launch_bounds__(128) void split_gradient(PiecesDev a) {
+  __shared__ float tile[32][33];
+  const uint32_t lane = lane_id(), wave = wave_id();
+  const uint32_t column_blocks = (a.columns + 31) / 32, group = a.first_group + blockIdx.x;
+  const uint32_t block = group / column_blocks, column_block = group - block * column_blocks;
+  const uint32_t r0 = block * 32, c0 = column_block * 32;
+#pragma unroll
+  for (uint32_t y = 0; y < 32; y += 4) {
+    const uint32_t r = r0 + y + threadIdx.x / 32, c = c0 + threadIdx.x % 32;
+    tile[y + threadIdx.x / 32][threadIdx.x % 32] = r < a.rows && c < a.columns ? as_global(a.in)[(int64_t)r * a.in_stride + c] : 0.f;
   }
   __syncthreads();
-  const uint32_t most = (a.rows + 7) / 8 * 8;
-  for (uint32_t y = threadIdx.x / 64; y < 64; y += 4) {
-    const uint32_t r = r0 + x, c = c0 + y;
-    if (r < most && c < a.columns) as_global(reinterpret_cast<T *>(a.out + (int64_t)c * a.out_stride))[r] = tile[x][y];
+  auto write = [&](uint8_t *to, uint64_t fragment, uint32_t pieces, auto at) {
+    f32x8 v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = at(lane % 32, wave * 16 + lane / 32 * 8 + i);
+    bf16x8 p[3];
+    cut<3>(v, p);
+    PPLX_GLOBAL bf16x8 *out = as_global(reinterpret_cast<bf16x8 *>(to)) + fragment * pieces * 64 + lane;
+#pragma unroll
+    for (uint32_t i = 0; i < 3; ++i) {
+      if (i < pieces) out[i * 64] = p[i];
+    }
+  };
+  const uint32_t row_sixteens = (a.rows + 15) / 16, column_sixteens = (a.columns + 15) / 16;
+  if (a.by_rows && column_block * 2 + wave < column_sixteens) {
+    write(a.by_rows, (uint64_t)block * column_sixteens + column_block * 2 + wave, a.pieces_by_rows,
+          [&](uint32_t r, uint32_t k) { return tile[r][k]; });
+  }
+  if (a.by_columns && block * 2 + wave < row_sixteens) {
+    write(a.by_columns, (uint64_t)column_block * row_sixteens + block * 2 + wave, a.pieces_by_columns,
+          [&](uint32_t c, uint32_t k) { return tile[k][c]; });
   }
 }
-template <class T> int launch_turn(const void *in, int64_t in_stride, void *out, int64_t out_stride, uint32_t rows, uint32_t columns, hipStream_t s) {
-  TurnDev a{static_cast<const uint8_t *>(in), in_stride, static_cast<uint8_t *>(out), out_stride, rows, columns, (columns + 63) / 64, 0};
-  return launch_groups(turn<T>, turn<T>, (uint64_t)((rows + 63) / 64) * a.column_blocks, 256, 0, s, a);
+uint64_t fragment_bytes(uint64_t rows, uint64_t k, int pieces) { return (rows + 31) / 32 * ((k + 15) / 16) * (1024 * pieces); }
+int launch_split(const PiecesDev &a, hipStream_t s) {
+  return launch_groups(split_gradient, split_gradient, ((uint64_t)a.rows + 31) / 32 * ((a.columns + 31) / 32), 128, 0, s, a);
 }
 
-// out[r, c] = in[r, c], zeros for c from columns up to the next multiple of eight.
-template <class T> __global__ __launch_bounds__(256) void fill_out(TurnDev a) {
-  const uint64_t width = (a.columns + 7) / 8 * 8, i = (uint64_t)(a.first_group + blockIdx.x) * 256 + threadIdx.x;
-  const uint32_t r = (uint32_t)(i / width), c = (uint32_t)(i - r * width);
-  if (r >= a.rows) return;
-  as_global(reinterpret_cast<T *>(a.out + (int64_t)r * a.out_stride))[c] =
-      c < a.columns ? as_global(reinterpret_cast<const T *>(a.in + (int64_t)r * a.in_stride))[c] : (T)0;
+// Lane l holds NV columns of rows 8 i + 4 (l / 32) .. + 3.
+template <class O, int NV>
+__device__ __forceinline__ void store_turned(const GradientDev &a, uint64_t first, uint32_t m0, uint32_t column, uint32_t lane, const f32x16 *acc) {
+  typedef O vec __attribute__((ext_vector_type(NV)));
+#pragma unroll
+  for (int q = 0; q < 16; ++q) {
+    const uint32_t r = m0 + q / 4 * 8 + 4 * (lane / 32) + q % 4;
+    if (r >= a.rows) continue;
+    vec v;
+#pragma unroll
+    for (int f = 0; f < NV; ++f) v[f] = (O)acc[f][q];
+    *reinterpret_cast<PPLX_GLOBAL vec *>(as_global(reinterpret_cast<O *>(a.out)) + first + (int64_t)r * a.out_stride + column) = v;
+  }
 }
 
-uint64_t in_eights(uint64_t n) { return (n + 7) / 8 * 8; }
+// Of x: a workgroup keeps the fragments of 32 NV columns of the weight in LDS, CHUNK k of them at a time, and its waves take 32 rows
+// of grad_logits each, a round after the other.
+constexpr int kGradientWaves = 8;
+template <class TB, class O, int NV, int ORDER>
+__global__ __launch_bounds__(kGradientWaves * 64) void gradient_of_rows(GradientDev a, uint32_t chunk) {
+  typedef Turned<TB, NV, ORDER> B;
+  extern __shared__ __align__(16) uint8_t lds[];  // [chunk / 16][pieces][NV][64 lanes]
+  const uint32_t lane = lane_id(), wave = wave_id(), half = lane / 32 * 8;
+  const uint32_t group = a.first_group + blockIdx.x;
+  const uint32_t part = group / a.column_blocks, n0 = (group - part * a.column_blocks) * 32 * NV;
+  const uint32_t column = n0 + lane % 32 * NV;
+  const bool there = column < a.columns;
+  const uint32_t rounds = (a.rows + 32 * kGradientWaves - 1) / (32 * kGradientWaves);
+  const uint32_t chunks = (a.k + chunk - 1) / chunk;
+  auto fill = [&](uint32_t first) {
+    const uint32_t sixteens = ((a.k - first < chunk ? a.k - first : chunk) + 15) / 16;
+    for (uint32_t i = wave; i < sixteens; i += kGradientWaves) {
+      const uint32_t k = first + i * 16 + half;
+      B b;
+      b.load(a, there ? column : 0, k);
+      b.store(lds + i * B::kBytes, k < a.k ? a.k - k : 0, lane);
+    }
+  };
+  if (chunks == 1) {
+    fill(0);
+    __syncthreads();
+  }
+  const uint32_t all = (a.k + 15) / 16;
+  for (uint32_t round = part; round < rounds; round += a.parts) {
+    const uint32_t block = round * kGradientWaves + wave, m0 = block * 32;
+    const FragmentPtr from = as_global(reinterpret_cast<const bf16x8 *>(a.a)) + (uint64_t)(m0 < a.rows ? block : 0) * all * (64 * (ORDER + 1)) + lane;
+    constexpr int kAhead = 4;  // fragments under way
+    Fragments<ORDER> fa[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) fa[i].load(from, i, all);
+    f32x16 acc[NV] = {};
+    for (uint32_t c = 0; c < chunks; ++c) {
+      const uint32_t first = c * chunk / 16, count = all - first < chunk / 16 ? all - first : chunk / 16;
+      if (chunks > 1) {
+        __syncthreads();  // (the chunk before has been read)
+        fill(c * chunk);
+        __syncthreads();
+      }
+      if (m0 >= a.rows) continue;
+      for (uint32_t i = 0; i < count; i += kAhead) {  // (a chunk that is not the last is a multiple of 16 kAhead)
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          if (i + u >= count) break;
+          multiply_turned<B::kPieces, NV>(fa[u], lds + (i + u) * B::kBytes, lane, acc);
+          fa[u].load(from, first + i + u + kAhead, all);
+        }
+      }
+    }
+    if (there) store_turned<O, NV>(a, 0, m0, column, lane, acc);
+  }
+}
 
-// The workspace of the gradients: grad_logits with rows of whole eights, the same turned, and the weight and x turned.
-struct BackwardSpace {
-  uint64_t grad, grad_turned, weight_turned, x_turned, bytes;
-};
-BackwardSpace backward_space(uint64_t m, uint64_t experts, uint64_t hidden, int64_t size, int64_t weight_size) {
-  BackwardSpace s{};
-  s.grad = 0;
-  s.grad_turned = s.grad + 4 * m * in_eights(experts);
-  s.weight_turned = s.grad_turned + 4 * experts * in_eights(m);
-  s.x_turned = s.weight_turned + (hidden * in_eights(experts) * weight_size + 15) / 16 * 16;
-  s.bytes = s.x_turned + hidden * in_eights(m) * size;
-  return s;
+// Of the weight: waves take 32 experts each, a workgroup all of a block of them, and go through the tokens sixteen for each wave at a
+// time: every wave turns sixteen of x, and all multiply with what the others turned.  Parts of the tokens add up in sum_splits.
+template <class TB, class O, int NV, int ORDER>
+__global__ __launch_bounds__(512) void gradient_of_weight(GradientDev a, uint32_t tokens_per_part, uint32_t row_blocks) {
+  typedef Turned<TB, NV, ORDER> B;
+  extern __shared__ __align__(16) uint8_t lds[];  // [2][waves][pieces][NV][64 lanes]
+  const uint32_t lane = lane_id(), wave = wave_id(), waves = blockDim.x / 64, half = lane / 32 * 8;
+  const uint32_t group = a.first_group + blockIdx.x;
+  const uint32_t block = group / a.column_blocks, n0 = (group - block * a.column_blocks) * 32 * NV;
+  const uint32_t part = block / row_blocks, m0 = ((block - part * row_blocks) * waves + wave) * 32;
+  const uint32_t column = n0 + lane % 32 * NV;
+  const bool there = column < a.columns;
+  const uint32_t begin = part * tokens_per_part, end = a.k - begin < tokens_per_part ? a.k : begin + tokens_per_part;
+  const uint32_t step = 16 * waves, size = waves * B::kBytes;
+  const uint32_t all = (a.k + 15) / 16, first = begin / 16;
+  const FragmentPtr from = as_global(reinterpret_cast<const bf16x8 *>(a.a)) + (uint64_t)(m0 < a.rows ? m0 / 32 : 0) * all * (64 * (ORDER + 1)) + lane;
+  auto left_at = [&](uint32_t k) { return k < end ? end - k : 0u; };
+  B b;
+  f32x16 acc[NV] = {};
+  b.load(a, there ? column : 0, begin + wave * 16 + half);
+  constexpr uint32_t kAhead = 4;  // fragments under way
+  Fragments<ORDER> fa[kAhead];
+#pragma unroll
+  for (uint32_t i = 0; i < kAhead; ++i) fa[i].load(from, first + i, all);
+  uint32_t buffer = 0;
+  for (uint32_t at = begin; at < end; at += step) {
+    b.store(lds + buffer * size + wave * B::kBytes, left_at(at + wave * 16 + half), lane);
+    __syncthreads();
+    if (at + step < end) b.load(a, there ? column : 0, at + step + wave * 16 + half);
+    // (waves are a multiple of kAhead, so that a fragment's place is known)
+    for (uint32_t i = 0; i < waves; i += kAhead) {
+#pragma unroll
+      for (uint32_t u = 0; u < kAhead; ++u) {
+        const uint32_t now = at / 16 + i + u;
+        if (now < all && m0 < a.rows) multiply_turned<B::kPieces, NV>(fa[u], lds + buffer * size + (i + u) * B::kBytes, lane, acc);
+        fa[u].load(from, now + kAhead, all);
+      }
+    }
+    buffer ^= 1;
+  }
+  if (there && m0 < a.rows) store_turned<O, NV>(a, part * a.out_split, m0, column, lane, acc);
 }
 
 template <class Fn> int with_weight_type(int32_t dtype, int32_t weight_dtype, Fn &&fn) {
@@ -225,11 +640,194 @@ template <class Fn> int with_weight_type(int32_t dtype, int32_t weight_dtype, Fn
   });
 }
 
-int check_router_size(uint32_t experts, uint64_t hidden, int32_t dtype, int32_t weight_dtype) {
+uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
+
+// Kernels that take more than 64 KiB of LDS say so.
+template <class K> void allow_lds(K *kernel, uint32_t bytes) {
+  if (bytes <= 64 * 1024) return;
+  const hipError_t err =
+      hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (err != hipSuccess) (void)hipGetLastError();  // (the launch says so if it matters)
+}
+
+// ---------------------------------------------------------------------------
+// Which form a product takes, and in how many splits of k
+// ---------------------------------------------------------------------------
+struct LogitsForm {
+  uint32_t bm, bn;
+  double per_step[4];  // us for 64 k: 16-bit operands; bf16 and fp32; fp16 and fp32; fp32
+};
+constexpr LogitsForm kForms[] = {
+    {32, 128, {0.27, 0.60, 0.80, 1.00}},
+    {64, 64, {0.25, 0.60, 0.80, 1.00}},
+    {64, 128, {0.36, 0.90, 1.30, 1.70}},
+    {128, 128, {0.58, 1.75, 2.50, 3.20}},
+};
+struct LogitsPlan {
+  int form = -1;  // -1: product_split
+  uint32_t splits = 1, steps_per_split = 0;
+  uint64_t bytes = 0;  // of workspace
+};
+uint64_t sums_width(uint64_t columns) { return (columns + 3) / 4 * 4; }
+LogitsPlan plan_logits(uint64_t m, uint64_t experts, uint64_t hidden, int32_t dtype, int32_t weight_dtype, bool far_apart) {
+  LogitsPlan best;
+  const int kind = dtype == PPLX_A2A_F32 ? 3 : weight_dtype != PPLX_A2A_F32 ? 0 : dtype == PPLX_A2A_BF16 ? 1 : 2;
+  const uint64_t steps = ceil_div(hidden, 64);
+  const double tiles16 = (double)(ceil_div(m, 16) * ceil_div(experts, 16));
+  double least = 2.6 + std::ceil(tiles16 / 1024) * (double)steps * (kind == 0 ? 0.05 : kind == 3 ? 0.12 : 0.085) *
+                           (tiles16 > 256 ? std::ceil(tiles16 / 256) / std::ceil(tiles16 / 1024) * 0.6 : 1.0);
+  if (far_apart) return best;
+  for (int f = 0; f < (int)(sizeof(kForms) / sizeof(kForms[0])); ++f) {
+    const LogitsForm &form = kForms[f];
+    const uint64_t tiles = ceil_div(m, form.bm) * ceil_div(experts, form.bn);
+    if (tiles >= (1ull << 28)) continue;
+    for (uint64_t per = steps; per >= 1; per = per > 16 ? per * 3 / 4 : per - 1) {
+      const uint64_t splits = ceil_div(steps, per), bytes = splits > 1 ? 4 * splits * m * sums_width(experts) : 0;
+      if (splits > 64 || bytes > (512ull << 20)) break;
+      const double rounds = std::ceil((double)(tiles * splits) / kComputeUnits);
+      const double cost = 2.5 + rounds * ((double)per * form.per_step[kind] + 0.4) + (splits > 1 ? 2.0 + (double)bytes / 5e6 : 0.0);
+      if (cost < least) {
+        least = cost;
+        best.form = f;
+        best.splits = (uint32_t)splits;
+        best.steps_per_split = (uint32_t)per;
+        best.bytes = bytes;
+      }
+    }
+  }
+  return best;
+}
+
+template <class T, class W, int BM, int BN, int WM, int WN, int STAGES> int launch_tiles(const TilesDev &from, hipStream_t s) {
+  TilesDev a = from;
+  a.row_blocks = (uint32_t)ceil_div(a.rows, BM);
+  a.column_blocks = (uint32_t)ceil_div(a.columns, BN);
+  constexpr uint32_t lds = STAGES * 64 * (BM * sizeof(T) + BN * sizeof(W));
+  auto kernel = a.k % 64 ? logits_tiles<T, W, BM, BN, WM, WN, STAGES, true> : logits_tiles<T, W, BM, BN, WM, WN, STAGES, false>;
+  allow_lds(kernel, lds);
+  // (a launch takes fewer than 2^32 threads: more rows go out in several, which steps of few rows, the only ones that are split, never
+  // come to)
+  const uint32_t most = (1u << 22) / a.column_blocks;
+  const int8_t *first = a.a;
+  float *out = a.out;
+  for (uint64_t block = 0, blocks = a.row_blocks; block < blocks; block += most) {
+    a.a = first + (int64_t)block * BM * a.a_stride;
+    a.out = out + (int64_t)block * BM * a.out_stride;
+    a.rows = from.rows - (uint32_t)(block * BM);
+    a.row_blocks = (uint32_t)(blocks - block);
+    if (blocks - block > most) {
+      a.row_blocks = most;
+      a.rows = most * BM;
+    }
+    const uint64_t grid = ceil_div((uint64_t)a.row_blocks * a.column_blocks * a.splits, 8) * 8;
+    const int err = launch_kernel(kernel, dim3((uint32_t)grid), dim3(WM * WN * 64), lds, s, a);
+    if (err) return err;
+  }
+  return 0;
+}
+template <class T, class W> int launch_form(int form, const TilesDev &a, hipStream_t s) {
+  // (stages of 128 KiB and less; waves that share out the columns cut fewer pieces twice)
+  switch (form) {
+    case 0: return launch_tiles<T, W, 32, 128, 1, 4, 3>(a, s);
+    case 1: return launch_tiles<T, W, 64, 64, 2, 2, 4>(a, s);
+    case 2: return launch_tiles<T, W, 64, 128, 1, 4, sizeof(T) == 4 ? 2 : 3>(a, s);
+    default: return sizeof(W) == 2 ? launch_tiles<T, W, 128, 128, 2, sizeof(W) == 2 ? 4 : 2, sizeof(W) == 2 ? 4 : 2>(a, s)
+                                   : launch_tiles<T, W, 128, 128, 2, sizeof(W) == 2 ? 4 : 2, sizeof(W) == 2 ? 4 : 2>(a, s);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The gradients' shares
+// ---------------------------------------------------------------------------
+// Results of 16 bits are sums of operands that count to two pieces, 2^-18 of each value, a hundredth of what the result is rounded by
+// and less: with three, 3001 x 7168 of 256 takes 33 us and not 26.
+template <class O> constexpr int kOrder = sizeof(O) == 4 ? 2 : 1;
+// Columns of a lane: four where their pieces fit LDS.
+template <class TB, int ORDER> constexpr int kColumnsOfLane = Pieces<TB, ORDER>::count <= 2 ? 4 : 2;
+
+struct WeightShares {
+  uint32_t waves, row_blocks, parts, tokens_per_part;
+};
+WeightShares weight_shares(uint64_t m, uint64_t experts, uint64_t hidden, uint32_t columns) {
+  WeightShares w{};
+  w.waves = experts > 128 ? 8 : 4;
+  w.row_blocks = (uint32_t)ceil_div(experts, 32 * w.waves);
+  const uint64_t step = 16 * w.waves, steps = ceil_div(m, step), blocks = ceil_div(hidden, columns) * w.row_blocks;
+  double least = 0;
+  for (uint64_t per = steps; per >= 1; per = per > 8 ? per * 7 / 8 : per - 1) {
+    const uint64_t parts = ceil_div(steps, per);
+    if (parts > 32) break;
+    const double rounds = std::ceil((double)(blocks * parts) / kComputeUnits);
+    const double cost = rounds * ((double)per * (w.waves == 8 ? 3.2 : 1.2) + 2.0) + (parts > 1 ? 2.0 + (double)(parts * experts * hidden) * 8 / 6e6 : 0.0);
+    if (w.parts == 0 || cost < least) {
+      least = cost;
+      w.parts = (uint32_t)parts;
+      w.tokens_per_part = (uint32_t)(per * step);
+    }
+  }
+  return w;
+}
+
+struct BackwardSpace {
+  WeightShares shares;
+  uint64_t by_columns, sums, bytes;  // (fragments of the rows come first)
+};
+template <class T, class W> BackwardSpace backward_space(uint64_t m, uint64_t experts, uint64_t hidden) {
+  BackwardSpace s{};
+  s.shares = weight_shares(m, experts, hidden, 32 * kColumnsOfLane<T, kOrder<W>>);
+  s.by_columns = fragment_bytes(m, experts, kOrder<T> + 1);
+  s.sums = s.by_columns + fragment_bytes(experts, m, kOrder<W> + 1);
+  s.bytes = s.sums + (s.shares.parts > 1 ? 4 * s.shares.parts * experts * hidden : 0);
+  return s;
+}
+
+template <class T, class W> int launch_gradient_of_rows(GradientDev a, hipStream_t s) {
+  constexpr int kOrd = kOrder<T>, kNV = kColumnsOfLane<W, kOrd>;
+  typedef Turned<W, kNV, kOrd> B;
+  constexpr uint32_t kMost = kLdsBytes / B::kBytes / 4 * 64;  // k of a chunk
+  const uint32_t whole = (a.k + 15) / 16 * 16, chunk = whole < kMost ? whole : kMost;
+  a.column_blocks = (uint32_t)ceil_div(a.columns, 32 * kNV);
+  // Workgroups keep the weight's columns for as many rounds of rows as leaves no compute unit idle for long.
+  const uint64_t rounds = ceil_div(a.rows, 32 * kGradientWaves);
+  uint64_t least = 0;
+  for (uint64_t per = rounds; per >= 1; per = per > 8 ? per * 7 / 8 : per - 1) {
+    const uint64_t parts = ceil_div(rounds, per), cost = ceil_div(a.column_blocks * parts, kComputeUnits) * (per + 1);
+    if (a.parts == 0 || cost < least) {
+      least = cost;
+      a.parts = (uint32_t)parts;
+    }
+  }
+  auto kernel = gradient_of_rows<W, T, kNV, kOrd>;
+  const uint32_t lds = chunk / 16 * B::kBytes;
+  allow_lds(kernel, lds);
+  return launch_groups(kernel, kernel, (uint64_t)a.column_blocks * a.parts, kGradientWaves * 64, lds, s, a, chunk);
+}
+
+template <class T, class W> int launch_gradient_of_weight(GradientDev a, const WeightShares &w, float *sums, hipStream_t s) {
+  constexpr int kOrd = kOrder<W>, kNV = kColumnsOfLane<T, kOrd>;
+  a.column_blocks = (uint32_t)ceil_div(a.columns, 32 * kNV);
+  a.parts = w.parts;
+  const uint64_t groups = (uint64_t)a.column_blocks * w.row_blocks * w.parts;
+  const uint32_t lds = 2 * w.waves * Turned<T, kNV, kOrd>::kBytes;
+  auto launch = [&](auto kernel) {
+    allow_lds(kernel, lds);
+    return launch_groups(kernel, kernel, groups, w.waves * 64, lds, s, a, w.tokens_per_part, w.row_blocks);
+  };
+  if (w.parts == 1) return launch(gradient_of_weight<T, W, kNV, kOrd>);
+  const SumDev sum{sums, (uint64_t)a.rows * a.columns, a.out, a.out_stride, a.rows, a.columns, a.columns, w.parts, 0};
+  a.out = reinterpret_cast<uint8_t *>(sums);
+  a.out_stride = a.columns;
+  a.out_split = sum.split;
+  const int err = launch(gradient_of_weight<T, float, kNV, kOrd>);
+  return err ? err : launch_sum<W>(sum, s);
+}
+
+int check_router_size(uint64_t m, uint32_t experts, uint64_t hidden, int32_t dtype, int32_t weight_dtype) {
   PPLX_REQUIRE(is_dtype(dtype), "unsupported dtype of the rows");
   PPLX_REQUIRE(weight_dtype == dtype || weight_dtype == PPLX_A2A_F32, "weight_dtype must be dtype or F32");
   PPLX_REQUIRE(experts >= 1 && experts <= kMaxExperts, "num_experts must be in [1, %u]", kMaxExperts);
   PPLX_REQUIRE(hidden > 0 && hidden < (1ull << 27) && hidden % 8 == 0, "hidden_dim must be a multiple of 8 below 2^27");
+  if (m >= (1ull << 31)) return refuse(PPLX_A2A_UNSUPPORTED, "2^31 tokens or more");
   return PPLX_A2A_OK;
 }
 int check_rows_of(const void *p, int64_t stride, const char *name) {
@@ -243,6 +841,9 @@ int check_rows_of(const void *p, int64_t stride, const char *name) {
     if (st_) return st_;                                                 \
   } while (0)
 
+// A tile's rows are reached by 32-bit offsets.
+bool is_far(int64_t stride) { return stride < 0 || stride >= (1 << 23); }
+
 }  // namespace
 }  // namespace pplx_amd
 
@@ -251,36 +852,70 @@ using namespace pplx_amd;
 extern "C" int pplx_a2a_router_workspace(uint32_t m, uint32_t num_experts, uint64_t hidden_dim, int32_t dtype,
                                          int32_t weight_dtype, int32_t backward, uint64_t *bytes) {
   PPLX_REQUIRE(bytes, "bytes is NULL");
-  const int st = check_router_size(num_experts, hidden_dim, dtype, weight_dtype);
+  const int st = check_router_size(m, num_experts, hidden_dim, dtype, weight_dtype);
   if (st) return st;
-  *bytes = backward ? backward_space(m, num_experts, hidden_dim, dtype_bytes(dtype), dtype_bytes(weight_dtype)).bytes : 0;
-  return PPLX_A2A_OK;
+  if (!backward) {
+    *bytes = plan_logits(m, num_experts, hidden_dim, dtype, weight_dtype, false).bytes;
+    return PPLX_A2A_OK;
+  }
+  return with_weight_type(dtype, weight_dtype, [&](auto tag, auto weight_tag) {
+    *bytes = backward_space<typename decltype(tag)::type, typename decltype(weight_tag)::type>(m, num_experts, hidden_dim).bytes;
+    return (int)PPLX_A2A_OK;
+  });
 }
 
 extern "C" int pplx_a2a_router_logits(int device, const pplx_a2a_router_logits_args_t *args, void *stream) {
   PPLX_REQUIRE(args, "args is NULL");
   const pplx_a2a_router_logits_args_t &p = *args;
-  const int st = check_router_size(p.num_experts, p.hidden_dim, p.dtype, p.weight_dtype);
+  const int st = check_router_size(p.m, p.num_experts, p.hidden_dim, p.dtype, p.weight_dtype);
   if (st) return st;
   if (p.m == 0) return PPLX_A2A_OK;
   PPLX_ROWS(p, x);
   PPLX_ROWS(p, weight);
   PPLX_REQUIRE(p.logits && is_aligned(p.logits, 4), "logits is NULL or not aligned");
-  ProductDev a{};
-  a.a = static_cast<const uint8_t *>(p.x);
-  a.a_stride = p.x_stride_row;
-  a.b = static_cast<const uint8_t *>(p.weight);
-  a.b_stride = p.weight_stride_row;
-  a.out = reinterpret_cast<uint8_t *>(p.logits);
-  a.out_stride = p.logits_stride_row;
-  a.rows = p.m;
-  a.columns = p.num_experts;
-  a.k = (uint32_t)p.hidden_dim;
+  const LogitsPlan plan =
+      plan_logits(p.m, p.num_experts, p.hidden_dim, p.dtype, p.weight_dtype, is_far(p.x_stride_row) || is_far(p.weight_stride_row));
+  PPLX_REQUIRE(plan.bytes == 0 || (p.workspace && is_aligned(p.workspace, 16)), "workspace is NULL or not aligned");
   return guarded(device, [&] {
     return with_weight_type(p.dtype, p.weight_dtype, [&](auto tag, auto weight_tag) {
       typedef typename decltype(tag)::type T;
       typedef typename decltype(weight_tag)::type W;
-      PPLX_LAUNCH((launch_product<T, W, float>(a, (hipStream_t)stream)));
+      hipStream_t s = (hipStream_t)stream;
+      if (plan.form < 0) {
+        ProductDev a{};
+        a.a = static_cast<const uint8_t *>(p.x);
+        a.a_stride = p.x_stride_row;
+        a.b = static_cast<const uint8_t *>(p.weight);
+        a.b_stride = p.weight_stride_row;
+        a.out = reinterpret_cast<uint8_t *>(p.logits);
+        a.out_stride = p.logits_stride_row;
+        a.rows = p.m;
+        a.columns = p.num_experts;
+        a.k = (uint32_t)p.hidden_dim;
+        a.column_blocks = (uint32_t)ceil_div(a.columns, 16);
+        auto kernel = product_split<T, W, float>;
+        PPLX_LAUNCH(launch_groups(kernel, kernel, ceil_div(a.rows, 16) * a.column_blocks, kProductWaves * 64, 0, s, a));
+        return (int)PPLX_A2A_OK;
+      }
+      const uint64_t width = sums_width(p.num_experts);
+      TilesDev a{};
+      a.a = static_cast<const int8_t *>(p.x);
+      a.a_stride = p.x_stride_row;
+      a.b = static_cast<const int8_t *>(p.weight);
+      a.b_stride = p.weight_stride_row;
+      a.rows = p.m;
+      a.columns = p.num_experts;
+      a.k = (uint32_t)p.hidden_dim;
+      a.splits = plan.splits;
+      a.steps_per_split = plan.steps_per_split;
+      a.out = plan.splits > 1 ? static_cast<float *>(p.workspace) : p.logits;
+      a.out_stride = plan.splits > 1 ? (int64_t)width : p.logits_stride_row;
+      a.out_split = (uint64_t)p.m * width;
+      PPLX_LAUNCH((launch_form<T, W>(plan.form, a, s)));
+      if (plan.splits > 1) {
+        const SumDev sum{a.out, a.out_split, reinterpret_cast<uint8_t *>(p.logits), p.logits_stride_row, p.m, (uint32_t)width, p.num_experts, plan.splits, 0};
+        PPLX_LAUNCH(launch_sum<float>(sum, s));
+      }
       return (int)PPLX_A2A_OK;
     });
   });
@@ -289,7 +924,7 @@ extern "C" int pplx_a2a_router_logits(int device, const pplx_a2a_router_logits_a
 extern "C" int pplx_a2a_router_logits_backward(int device, const pplx_a2a_router_logits_backward_args_t *args, void *stream) {
   PPLX_REQUIRE(args, "args is NULL");
   const pplx_a2a_router_logits_backward_args_t &p = *args;
-  const int st = check_router_size(p.num_experts, p.hidden_dim, p.dtype, p.weight_dtype);
+  const int st = check_router_size(p.m, p.num_experts, p.hidden_dim, p.dtype, p.weight_dtype);
   if (st) return st;
   PPLX_REQUIRE(p.m > 0, "there are no tokens");
   PPLX_REQUIRE(p.grad_logits && is_aligned(p.grad_logits, 4), "grad_logits is NULL or not aligned");
@@ -303,48 +938,46 @@ extern "C" int pplx_a2a_router_logits_backward(int device, const pplx_a2a_router
   }
   if (!p.grad_x && !p.grad_weight) return PPLX_A2A_OK;
   PPLX_REQUIRE(p.workspace && is_aligned(p.workspace, 16), "workspace is NULL or not aligned");
-  const uint32_t m = p.m, experts = p.num_experts, hidden = (uint32_t)p.hidden_dim;
-  const BackwardSpace space = backward_space(m, experts, hidden, dtype_bytes(p.dtype), dtype_bytes(p.weight_dtype));
-  uint8_t *work = static_cast<uint8_t *>(p.workspace);
-  const int64_t by_experts = (int64_t)in_eights(experts), by_tokens = (int64_t)in_eights(m);
   return guarded(device, [&] {
     return with_weight_type(p.dtype, p.weight_dtype, [&](auto tag, auto weight_tag) {
       typedef typename decltype(tag)::type T;
       typedef typename decltype(weight_tag)::type W;
       hipStream_t s = (hipStream_t)stream;
+      const BackwardSpace space = backward_space<T, W>(p.m, p.num_experts, p.hidden_dim);
+      uint8_t *work = static_cast<uint8_t *>(p.workspace);
+      PiecesDev pieces{};
+      pieces.in = p.grad_logits;
+      pieces.in_stride = p.grad_logits_stride_row;
+      pieces.rows = p.m;
+      pieces.columns = p.num_experts;
+      pieces.by_rows = p.grad_x ? work : nullptr;
+      pieces.by_columns = p.grad_weight ? work + space.by_columns : nullptr;
+      pieces.pieces_by_rows = kOrder<T> + 1;
+      pieces.pieces_by_columns = kOrder<W> + 1;
+      PPLX_LAUNCH(launch_split(pieces, s));
       if (p.grad_x) {
-        const TurnDev fill{reinterpret_cast<const uint8_t *>(p.grad_logits), 4 * p.grad_logits_stride_row, work + space.grad,
-                           4 * by_experts, m, experts, 0, 0};
-        PPLX_LAUNCH(launch_groups(fill_out<float>, fill_out<float>, ((uint64_t)m * by_experts + 255) / 256, 256, 0, s, fill));
-        PPLX_LAUNCH(launch_turn<W>(p.weight, p.weight_stride_row, work + space.weight_turned, by_experts * (int64_t)sizeof(W),
-                                   experts, hidden, s));
-        ProductDev a{};
-        a.a = work + space.grad;
-        a.a_stride = 4 * by_experts;
-        a.b = work + space.weight_turned;
-        a.b_stride = by_experts * (int64_t)sizeof(W);
+        GradientDev a{};
+        a.a = pieces.by_rows;
+        a.b = static_cast<const uint8_t *>(p.weight);
+        a.b_stride = p.weight_stride_row;
         a.out = static_cast<uint8_t *>(p.grad_x);
         a.out_stride = p.grad_x_stride_row / (int64_t)sizeof(T);
-        a.rows = m;
-        a.columns = hidden;
-        a.k = (uint32_t)by_experts;
-        PPLX_LAUNCH((launch_product<float, W, T>(a, s)));
+        a.rows = p.m;
+        a.columns = (uint32_t)p.hidden_dim;
+        a.k = p.num_experts;
+        PPLX_LAUNCH((launch_gradient_of_rows<T, W>(a, s)));
       }
       if (p.grad_weight) {
-        PPLX_LAUNCH(launch_turn<float>(p.grad_logits, 4 * p.grad_logits_stride_row, work + space.grad_turned, 4 * by_tokens, m,
-                                       experts, s));
-        PPLX_LAUNCH(launch_turn<T>(p.x, p.x_stride_row, work + space.x_turned, by_tokens * (int64_t)sizeof(T), m, hidden, s));
-        ProductDev a{};
-        a.a = work + space.grad_turned;
-        a.a_stride = 4 * by_tokens;
-        a.b = work + space.x_turned;
-        a.b_stride = by_tokens * (int64_t)sizeof(T);
+        GradientDev a{};
+        a.a = pieces.by_columns;
+        a.b = static_cast<const uint8_t *>(p.x);
+        a.b_stride = p.x_stride_row;
         a.out = static_cast<uint8_t *>(p.grad_weight);
         a.out_stride = p.grad_weight_stride_row / (int64_t)sizeof(W);
-        a.rows = experts;
-        a.columns = hidden;
-        a.k = (uint32_t)by_tokens;
-        PPLX_LAUNCH((launch_product<float, T, W>(a, s)));
+        a.rows = p.num_experts;
+        a.columns = (uint32_t)p.hidden_dim;
+        a.k = p.m;
+        PPLX_LAUNCH((launch_gradient_of_weight<T, W>(a, space.shares, reinterpret_cast<float *>(work + space.sums), s)));
       }
       return (int)PPLX_A2A_OK;
     });

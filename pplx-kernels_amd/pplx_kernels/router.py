@@ -157,7 +157,8 @@ def router_logits_backward(
     out: tuple[torch.Tensor | None, torch.Tensor | None] | None = None,
 ) -> tuple[torch.Tensor | None, torch.Tensor | None]:
     """The gradients of :func:`router_logits`: ``grad_logits @ weight`` and ``grad_logits.T @ x``, added up in float32 and rounded
-    once.  In ``out`` either may be None, which leaves it out."""
+    once.  For 16-bit results ``grad_logits`` (and the other operand, unless it is bfloat16) counts to 2**-18 of each value, for
+    float32 to 24 bits.  In ``out`` either may be None, which leaves it out."""
     if out is None:
         out = (
             torch.empty_like(x, memory_format=torch.contiguous_format),

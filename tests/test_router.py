@@ -332,6 +332,17 @@ def product(a, b, chain):
     return a.double() @ b.double(), (a.double().abs() @ b.double().abs()) * (2 * (chain + 8) * U32)
 
 
+def gradient(a, b, chain, dtype):
+    """The same of gradients, whose 16-bit results are sums of operands that count to two pieces of eight bits.  A value less its
+    nearest piece p is at most 2^-9 of it, and that less its own nearest piece at most 2^-9 of the rest: two pieces leave out 2^-18
+    of a value.  bf16 is one piece; where both operands are cut, both leave that out, and the product of the two second pieces,
+    2^-9 of each value, is left out too."""
+    want, off = product(a, b, chain)
+    if dtype != F32:
+        off = off + (a.double().abs() @ b.double().abs()) * 2.0**-18 * (1 if b.dtype == BF16 else 3)
+    return want, off
+
+
 @gpu
 @pytest.mark.parametrize("m,experts,hidden,dtype,weight_dtype", LOGITS)
 def test_router_logits(device, m, experts, hidden, dtype, weight_dtype):
@@ -398,8 +409,8 @@ def test_gradients_of_router_logits(device, m, experts, hidden, dtype, weight_dt
     grad = 1e-2 * torch.randn(m, experts, generator=gen)
     leaves = [t.to(device).requires_grad_(True) for t in (x, weight)]
     gx, gw = torch.autograd.grad(router_logits(*leaves), leaves, grad.to(device))
-    want, off = product(grad, weight, experts)
-    want_w, off_w = product(grad.t(), x, m)
+    want, off = gradient(grad, weight, experts, dtype)
+    want_w, off_w = gradient(grad.t(), x, m, weight_dtype)
     assert_within(gx, want, rounded(want, dtype, off))
     assert_within(gw, want_w, rounded(want_w, weight_dtype, off_w))
     # the call itself, with rows that lie apart, and each of the two alone
