@@ -653,16 +653,20 @@ template <class K> void allow_lds(K *kernel, uint32_t bytes) {
 // ---------------------------------------------------------------------------
 // Which form a product takes, and in how many splits of k
 // ---------------------------------------------------------------------------
+// What a product costs in microseconds: a start, `per_step` for every 64 k of a tile and every round of the compute units, and where k is
+// split the sums' launch and bytes.  Measured with rows that come from HBM, forms 64 x 64 / 128 x 128 with their best splits, us:
+//   both bf16       8192 x 256 x 7168  65 (1) / 47.8 (2)     3001 x 256 x 7168  32.9 (4) / 27.2 (4)   1024 x 256 x 7168  15.0 (4) / 17.2 (12)
+//                   16384 x 64 x 4096  32.0 (1) / 37.5 (4)   256 x 256 x 7168  9.4 (16) / 11.9 (16)   64 x 256 x 7168   7.6 (28) / 9.0 (28)
+//   bf16, fp32      8192 x 256 x 7168  199 (2) / 97.7 (2)    64 x 256 x 7168   9.9 (56) / 11.1 (56)
+//   both fp32       4096 x 256 x 7168  144 (4) / 101 (4)     64 x 256 x 7168  10.9 (56) / 14.5 (56)
+// Tiles of 64 x 128, 64 x 256, 32 x 64 and 32 x 128 were within 5 % of the better of the two, or slower, in all of twenty products.
+// product_split, which is one launch: 4 x 64 x 2048 4.3 (tiles 5.8), 1 x 256 x 7168 9.5 (6.5), 64 x 256 x 7168 14.2, with fp32
+// weights 20.9: its loads take a cycle for each row of 64 bytes, whatever else is under way.
 struct LogitsForm {
   uint32_t bm, bn;
-  double per_step[4];  // us for 64 k: 16-bit operands; bf16 and fp32; fp16 and fp32; fp32
+  double per_step[4];  // 16-bit operands; bf16 and fp32; fp16 and fp32; fp32
 };
-constexpr LogitsForm kForms[] = {
-    {32, 128, {0.27, 0.60, 0.80, 1.00}},
-    {64, 64, {0.25, 0.60, 0.80, 1.00}},
-    {64, 128, {0.36, 0.90, 1.30, 1.70}},
-    {128, 128, {0.58, 1.75, 2.50, 3.20}},
-};
+constexpr LogitsForm kForms[] = {{64, 64, {0.25, 0.87, 1.1, 1.3}}, {128, 128, {0.66, 1.6, 2.55, 3.3}}};
 struct LogitsPlan {
   int form = -1;  // -1: product_split
   uint32_t splits = 1, steps_per_split = 0;
@@ -673,9 +677,9 @@ LogitsPlan plan_logits(uint64_t m, uint64_t experts, uint64_t hidden, int32_t dt
   LogitsPlan best;
   const int kind = dtype == PPLX_A2A_F32 ? 3 : weight_dtype != PPLX_A2A_F32 ? 0 : dtype == PPLX_A2A_BF16 ? 1 : 2;
   const uint64_t steps = ceil_div(hidden, 64);
-  const double tiles16 = (double)(ceil_div(m, 16) * ceil_div(experts, 16));
-  double least = 2.6 + std::ceil(tiles16 / 1024) * (double)steps * (kind == 0 ? 0.05 : kind == 3 ? 0.12 : 0.085) *
-                           (tiles16 > 256 ? std::ceil(tiles16 / 256) / std::ceil(tiles16 / 1024) * 0.6 : 1.0);
+  const double of_rows = (m < 16 ? (double)m : 16.0) * (dtype == PPLX_A2A_F32 ? 8 : 4), of_columns = weight_dtype == PPLX_A2A_F32 ? 128 : 64;
+  double least = 2.2 + std::ceil((double)ceil_div(m, 16) * (double)ceil_div(experts, 16) / kComputeUnits) * (double)steps * 2 *
+                           (of_rows + of_columns) / 2400;
   if (far_apart) return best;
   for (int f = 0; f < (int)(sizeof(kForms) / sizeof(kForms[0])); ++f) {
     const LogitsForm &form = kForms[f];
@@ -685,7 +689,8 @@ LogitsPlan plan_logits(uint64_t m, uint64_t experts, uint64_t hidden, int32_t dt
       const uint64_t splits = ceil_div(steps, per), bytes = splits > 1 ? 4 * splits * m * sums_width(experts) : 0;
       if (splits > 64 || bytes > (512ull << 20)) break;
       const double rounds = std::ceil((double)(tiles * splits) / kComputeUnits);
-      const double cost = 2.5 + rounds * ((double)per * form.per_step[kind] + 0.4) + (splits > 1 ? 2.0 + (double)bytes / 5e6 : 0.0);
+      const double cost = (kind == 0 ? 3.0 : 3.6) + rounds * (double)per * form.per_step[kind] +
+                          (splits > 1 ? 2.2 + 0.02 * (double)splits + (double)bytes / 5.5e6 : 0.0);
       if (cost < least) {
         least = cost;
         best.form = f;
@@ -726,14 +731,8 @@ template <class T, class W, int BM, int BN, int WM, int WN, int STAGES> int laun
   return 0;
 }
 template <class T, class W> int launch_form(int form, const TilesDev &a, hipStream_t s) {
-  // (stages of 128 KiB and less; waves that share out the columns cut fewer pieces twice)
-  switch (form) {
-    case 0: return launch_tiles<T, W, 32, 128, 1, 4, 3>(a, s);
-    case 1: return launch_tiles<T, W, 64, 64, 2, 2, 4>(a, s);
-    case 2: return launch_tiles<T, W, 64, 128, 1, 4, sizeof(T) == 4 ? 2 : 3>(a, s);
-    default: return sizeof(W) == 2 ? launch_tiles<T, W, 128, 128, 2, sizeof(W) == 2 ? 4 : 2, sizeof(W) == 2 ? 4 : 2>(a, s)
-                                   : launch_tiles<T, W, 128, 128, 2, sizeof(W) == 2 ? 4 : 2, sizeof(W) == 2 ? 4 : 2>(a, s);
-  }
+  if (form == 0) return launch_tiles<T, W, 64, 64, 2, 2, 4>(a, s);
+  return launch_tiles<T, W, 128, 128, 2, 4, sizeof(W) == 2 ? 4 : 2>(a, s);
 }
 
 // ---------------------------------------------------------------------------
