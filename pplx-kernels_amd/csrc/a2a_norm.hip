@@ -110,108 +110,134 @@ __device__ __forceinline__ u32x2 e4m3_eight(f32x8 v, float inverse) {
   return out;
 }
 
-// One row by LANES threads, each with PIECES times eight elements of it, eight elements apart from the next thread's.  Rows that
-// are longer than that are taken in several steps, twice: once for the sum of squares, and once or, for one scale a row, twice
-// more for the results.
+// What a thread makes of eight elements of a normed row, whose scale has been found.
+template <class T, int FORMAT> __device__ __forceinline__ void store_normed(const NormDev &a, uint32_t r, uint32_t j, f32x8 v, float inverse) {
+  if (a.y) store_eight<T>(row_at<T>(a.y, a.y_stride_row, r) + 8ull * j, v);
+  if constexpr (FORMAT == PPLX_A2A_ROWS_INT8) *reinterpret_cast<PPLX_GLOBAL u32x2 *>(row_at<uint8_t>(a.q, a.q_stride_row, r) + 8ull * j) = quantize_eight(v, inverse);
+  if constexpr (FORMAT == PPLX_A2A_ROWS_E4M3) *reinterpret_cast<PPLX_GLOBAL u32x2 *>(row_at<uint8_t>(a.q, a.q_stride_row, r) + 8ull * j) = e4m3_eight(v, inverse);
+}
+// The scale of the block of 128 columns around these eight, by sixteen lanes; those behind the row bring zeros.
+__device__ __forceinline__ float block_inverse(const NormDev &a, uint32_t r, uint32_t j, bool there, f32x8 v) {
+  const RowScale s = block_scale(block_max(magnitude_bits(v)));
+  if (there && j % 16 == 0) as_global(a.scale)[(int64_t)r * a.scale_stride_row + (int64_t)(j / 16) * a.scale_stride_block] = s.scale;
+  return s.inverse;
+}
+
+// Rows of up to 8 LANES PIECES elements, LANES threads to one, which stay in registers; eight elements apart from the next thread's.  All of
+// a row's loads, and the weight's, are under way before the first is used.
 template <class T, class W, int FORMAT, int LANES, int PIECES>
-__device__ __forceinline__ void norm_one(const NormDev &a, uint32_t r, uint32_t g) {
-  constexpr uint32_t kStep = LANES * PIECES;
-  const uint32_t groups = a.width / 8;
-  const bool whole = groups <= kStep;  // the row stays in registers
-  const PPLX_GLOBAL T *x = row_at<T>(a.x, a.x_stride_row, r);
+__global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_rows(NormDev a) {
+  const uint32_t g = threadIdx.x % LANES, groups = a.width / 8, group = a.first_group + blockIdx.x;
+  const uint32_t r = LANES == 64 ? group * 4 + wave_id() : group;
+  if (r >= a.m) return;
   const PPLX_GLOBAL W *weight = as_global(reinterpret_cast<const W *>(a.weight));
+  typename Eight<W>::raw w[PIECES];
+  typename Eight<T>::raw x[PIECES], residual[PIECES];
+  // (a thread without elements reads the row's first, which count for nothing)
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    const uint32_t j = i * LANES + g, at = j < groups ? j : 0;
+    x[i] = load_eight<T>(row_at<T>(a.x, a.x_stride_row, r) + 8ull * at);
+    if (a.residual) residual[i] = load_eight<T>(row_at<T>(a.residual, a.residual_stride_row, r) + 8ull * at);
+  }
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    const uint32_t j = i * LANES + g;
+    w[i] = load_eight<W>(weight + 8ull * (j < groups ? j : 0));
+  }
   f32x8 v[PIECES];
-  auto load = [&](uint32_t base, const PPLX_GLOBAL T *from) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-      const uint32_t j = base + i * LANES + g;
-      v[i] = j < groups ? Eight<T>::wide(load_eight<T>(from + 8ull * j)) : f32x8{};
-    }
-  };
-  // (x + residual, rounded: what the sum's reader and the gradient see is what the norm is of)
-  auto add = [&](uint32_t base) __attribute__((always_inline)) {
-    const PPLX_GLOBAL T *residual = row_at<T>(a.residual, a.residual_stride_row, r);
-    PPLX_GLOBAL T *sum = row_at<T>(a.sum, a.sum_stride_row, r);
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-      const uint32_t j = base + i * LANES + g;
-      if (j >= groups) continue;
-      const f32x8 h = v[i] + Eight<T>::wide(load_eight<T>(residual + 8ull * j));
-      v[i] = Eight<T>::wide(Eight<T>::narrow(h));
-      store_eight<T>(sum + 8ull * j, v[i]);
-    }
-  };
   float squares = 0.f;
-  for (uint32_t base = 0; base < groups; base += kStep) {
-    load(base, x);
-    if (a.residual) add(base);
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) squares += squares_of(v[i], 1.f);
+  for (int i = 0; i < PIECES; ++i) {
+    const uint32_t j = i * LANES + g;
+    v[i] = Eight<T>::wide(x[i]);
+    if (a.residual) {
+      // (rounded: what the sum's reader and the gradient see is what the norm is of)
+      v[i] = Eight<T>::wide(Eight<T>::narrow(v[i] + Eight<T>::wide(residual[i])));
+      if (j < groups) store_eight<T>(row_at<T>(a.sum, a.sum_stride_row, r) + 8ull * j, v[i]);
+    }
+    if (j >= groups) v[i] = f32x8{};
+    squares += squares_of(v[i], 1.f);
   }
   squares = row_sum<LANES>(squares);
+  float root;
+  if (squares <= FLT_MAX) {
+    root = inverse_root(squares, a.inverse_width, a.eps);
+  } else {
+    float small = 0.f;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) small += squares_of(v[i], kSmall);
+    root = inverse_root_of_small(row_sum<LANES>(small), a.inverse_width);
+  }
+  uint32_t bits = 0;
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    v[i] = v[i] * root * Eight<W>::wide(w[i]);
+    if constexpr (FORMAT == PPLX_A2A_ROWS_INT8) {
+      const uint32_t b = magnitude_bits(i * LANES + g < groups ? v[i] : f32x8{});
+      bits = bits > b ? bits : b;
+    }
+  }
+  float inverse = 0.f;
+  if constexpr (FORMAT == PPLX_A2A_ROWS_INT8) {
+    const RowScale s = row_scale(row_max<LANES>(bits));
+    inverse = s.inverse;
+    if (g == 0) as_global(a.scale)[(int64_t)r * a.scale_stride_row] = s.scale;
+  }
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    const uint32_t j = i * LANES + g;
+    if constexpr (FORMAT == PPLX_A2A_ROWS_E4M3) inverse = block_inverse(a, r, j, j < groups, j < groups ? v[i] : f32x8{});
+    if (j < groups) store_normed<T, FORMAT>(a, r, j, v[i], inverse);
+  }
+}
+
+// Longer rows, of which a workgroup reads one twice, or for one scale a row three times.
+constexpr int kLongLanes = 512;
+template <class T, class W, int FORMAT> __global__ __launch_bounds__(kLongLanes) void norm_long_rows(NormDev a) {
+  const uint32_t g = threadIdx.x, groups = a.width / 8, turns = (groups + kLongLanes - 1) / kLongLanes;
+  const PPLX_GLOBAL W *weight = as_global(reinterpret_cast<const W *>(a.weight));
+  const uint32_t r = a.first_group + blockIdx.x;
+  const PPLX_GLOBAL T *x = row_at<T>(a.x, a.x_stride_row, r);
+  float squares = 0.f;
+  for (uint32_t j = g; j < groups; j += kLongLanes) {
+    f32x8 v = Eight<T>::wide(load_eight<T>(x + 8ull * j));
+    if (a.residual) {
+      v += Eight<T>::wide(load_eight<T>(row_at<T>(a.residual, a.residual_stride_row, r) + 8ull * j));
+      v = Eight<T>::wide(Eight<T>::narrow(v));
+      store_eight<T>(row_at<T>(a.sum, a.sum_stride_row, r) + 8ull * j, v);
+    }
+    squares += squares_of(v, 1.f);
+  }
+  squares = row_sum<kLongLanes>(squares);
+  // (a thread reads again what it has written itself)
   const PPLX_GLOBAL T *again = a.residual ? row_at<T>(a.sum, a.sum_stride_row, r) : x;
   float root;
   if (squares <= FLT_MAX) {
     root = inverse_root(squares, a.inverse_width, a.eps);
   } else {
     float small = 0.f;
-    for (uint32_t base = 0; base < groups; base += kStep) {
-      if (!whole) load(base, again);
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i) small += squares_of(v[i], kSmall);
-    }
-    root = inverse_root_of_small(row_sum<LANES>(small), a.inverse_width);
+    for (uint32_t j = g; j < groups; j += kLongLanes) small += squares_of(Eight<T>::wide(load_eight<T>(again + 8ull * j)), kSmall);
+    root = inverse_root_of_small(row_sum<kLongLanes>(small), a.inverse_width);
   }
-  auto norm = [&](uint32_t base) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-      const uint32_t j = base + i * LANES + g;
-      if (j >= groups) continue;
-      v[i] = v[i] * root * Eight<W>::wide(load_eight<W>(weight + 8ull * j));
-    }
-  };
-  PPLX_GLOBAL uint8_t *q = FORMAT == PPLX_A2A_ROWS_PLAIN ? nullptr : row_at<uint8_t>(a.q, a.q_stride_row, r);
+  auto normed = [&](uint32_t j) { return Eight<T>::wide(load_eight<T>(again + 8ull * j)) * root * Eight<W>::wide(load_eight<W>(weight + 8ull * j)); };
   float inverse = 0.f;
   if constexpr (FORMAT == PPLX_A2A_ROWS_INT8) {
     uint32_t bits = 0;
-    for (uint32_t base = 0; base < groups; base += kStep) {
-      if (!whole) load(base, again);
-      norm(base);
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i) {
-        const uint32_t b = magnitude_bits(v[i]);
-        bits = bits > b ? bits : b;
-      }
+    for (uint32_t j = g; j < groups; j += kLongLanes) {
+      const uint32_t b = magnitude_bits(normed(j));
+      bits = bits > b ? bits : b;
     }
-    const RowScale s = row_scale(row_max<LANES>(bits));
+    const RowScale s = row_scale(row_max<kLongLanes>(bits));
     inverse = s.inverse;
     if (g == 0) as_global(a.scale)[(int64_t)r * a.scale_stride_row] = s.scale;
   }
-  for (uint32_t base = 0; base < groups; base += kStep) {
-    if (!whole) load(base, again);
-    if (!whole || FORMAT != PPLX_A2A_ROWS_INT8) norm(base);
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-      const uint32_t j = base + i * LANES + g;
-      if constexpr (FORMAT == PPLX_A2A_ROWS_E4M3) {
-        // (all lanes of a block call; those behind the row hold zeros)
-        const RowScale s = block_scale(block_max(magnitude_bits(v[i])));
-        inverse = s.inverse;
-        if (j < groups && j % 16 == 0) as_global(a.scale)[(int64_t)r * a.scale_stride_row + (int64_t)(j / 16) * a.scale_stride_block] = s.scale;
-      }
-      if (j >= groups) continue;
-      if (a.y) store_eight<T>(row_at<T>(a.y, a.y_stride_row, r) + 8ull * j, v[i]);
-      if constexpr (FORMAT == PPLX_A2A_ROWS_INT8) *reinterpret_cast<PPLX_GLOBAL u32x2 *>(q + 8ull * j) = quantize_eight(v[i], inverse);
-      if constexpr (FORMAT == PPLX_A2A_ROWS_E4M3) *reinterpret_cast<PPLX_GLOBAL u32x2 *>(q + 8ull * j) = e4m3_eight(v[i], inverse);
-    }
+  for (uint32_t t = 0; t < turns; ++t) {
+    const uint32_t j = t * kLongLanes + g;
+    const f32x8 v = j < groups ? normed(j) : f32x8{};
+    if constexpr (FORMAT == PPLX_A2A_ROWS_E4M3) inverse = block_inverse(a, r, j, j < groups, v);
+    if (j < groups) store_normed<T, FORMAT>(a, r, j, v, inverse);
   }
-}
-
-template <class T, class W, int FORMAT, int LANES, int PIECES>
-__global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_rows(NormDev a) {
-  const uint32_t group = a.first_group + blockIdx.x;
-  const uint32_t r = LANES == 64 ? group * 4 + wave_id() : group;
-  if (r < a.m) norm_one<T, W, FORMAT, LANES, PIECES>(a, r, threadIdx.x % LANES);
 }
 
 // ---------------------------------------------------------------------------
@@ -232,56 +258,124 @@ struct NormBackwardDev {
   uint32_t m, width;
 };
 
-template <int LANES> __device__ __forceinline__ float gradient_root(const f32x8 *h, int pieces, float squares, const NormBackwardDev &a) {
-  if (squares <= FLT_MAX) return inverse_root(squares, a.inverse_width, a.eps);
-  float small = 0.f;
-#pragma unroll
-  for (int i = 0; i < pieces; ++i) small += squares_of(h[i], kSmall);
-  return inverse_root_of_small(row_sum<LANES>(small), a.inverse_width);
-}
-
-// Rows of up to 8 LANES PIECES elements, which stay in registers; a workgroup takes one row behind the other and holds its
-// share of the weight's gradient.
-template <class T, class W, int LANES, int PIECES>
-__global__ __launch_bounds__(LANES) void norm_backward_rows(NormBackwardDev a) {
-  const uint32_t g = threadIdx.x, groups = a.width / 8;
-  const PPLX_GLOBAL W *weight = as_global(reinterpret_cast<const W *>(a.weight));
-  f32x8 of_weight[PIECES] = {};
-  for (uint32_t r = blockIdx.x; r < a.m; r += gridDim.x) {
-    const PPLX_GLOBAL T *grad = row_at<T>(a.grad_y, a.grad_y_stride_row, r), *row = row_at<T>(a.h, a.h_stride_row, r);
-    f32x8 h[PIECES], d[PIECES];
-    float squares = 0.f;
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-      const uint32_t j = i * LANES + g;
-      h[i] = j < groups ? Eight<T>::wide(load_eight<T>(row + 8ull * j)) : f32x8{};
-      d[i] = j < groups ? Eight<T>::wide(load_eight<T>(grad + 8ull * j)) : f32x8{};
-      squares += squares_of(h[i], 1.f);
+// Two sums over the threads of a workgroup.  `buffer` alternates from call to call, so that one barrier is enough.
+template <int LANES> __device__ __forceinline__ void row_sums(float &a, float &b, uint32_t buffer) {
+  a = wave_sum(a);
+  b = wave_sum(b);
+  if constexpr (LANES > 64) {
+    __shared__ float of_wave[2][LANES / 64][2];
+    if (lane_id() == 0) {
+      of_wave[buffer][wave_id()][0] = a;
+      of_wave[buffer][wave_id()][1] = b;
     }
-    const float root = gradient_root<LANES>(h, PIECES, row_sum<LANES>(squares), a);
-    float along = 0.f;
+    __syncthreads();
+    a = b = 0.f;
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-      const uint32_t j = i * LANES + g;
-      if (j >= groups) continue;
-      h[i] = h[i] * root;
-      of_weight[i] += d[i] * h[i];
-      d[i] = d[i] * Eight<W>::wide(load_eight<W>(weight + 8ull * j));
-#pragma unroll
-      for (int k = 0; k < 8; ++k) along = __builtin_fmaf(d[i][k], h[i][k], along);
-    }
-    along = row_sum<LANES>(along) * a.inverse_width;
-    if (!a.grad_h) continue;
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-      const uint32_t j = i * LANES + g;
-      if (j >= groups) continue;
-      f32x8 out = (d[i] - h[i] * along) * root;
-      if (a.grad_sum) out += Eight<T>::wide(load_eight<T>(row_at<T>(a.grad_sum, a.grad_sum_stride_row, r) + 8ull * j));
-      store_eight<T>(row_at<T>(a.grad_h, a.grad_h_stride_row, r) + 8ull * j, out);
+    for (int w = 0; w < LANES / 64; ++w) {
+      a += of_wave[buffer][w][0];
+      b += of_wave[buffer][w][1];
     }
   }
+}
+
+// Rows of up to 8 LANES PIECES elements, which stay in registers; a workgroup takes one row behind the other, with the loads of the next
+// one under way (AHEAD: registers allow it), and holds its share of the weight's gradient.
+template <class T, class W, int LANES, int PIECES, bool AHEAD>
+__global__ __launch_bounds__(LANES == 64 ? 256 : LANES) void norm_backward_rows(NormBackwardDev a) {
+  constexpr uint32_t kAtOnce = LANES == 64 ? 4 : 1;  // rows: a wave to a short one
+  const uint32_t g = threadIdx.x % LANES, groups = a.width / 8, step = gridDim.x * kAtOnce;
+  const PPLX_GLOBAL W *weight = as_global(reinterpret_cast<const W *>(a.weight));
+  struct Rows {
+    typename Eight<T>::raw h[PIECES], d[PIECES], s[PIECES];
+  };
+  // (a thread without elements reads the rows' first, which count for nothing)
+  auto load = [&](Rows &to, uint32_t r) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const uint32_t j = i * LANES + g, at = j < groups ? j : 0;
+      to.h[i] = load_eight<T>(row_at<T>(a.h, a.h_stride_row, r) + 8ull * at);
+      to.d[i] = load_eight<T>(row_at<T>(a.grad_y, a.grad_y_stride_row, r) + 8ull * at);
+      if (a.grad_sum && a.grad_h) to.s[i] = load_eight<T>(row_at<T>(a.grad_sum, a.grad_sum_stride_row, r) + 8ull * at);
+    }
+  };
+  typename Eight<W>::raw w[PIECES];
+  Rows now, next;
+  uint32_t r = blockIdx.x * kAtOnce + (LANES == 64 ? wave_id() : 0);
+  bool here = r < a.m;  // (without short rows there are no more workgroups than rows)
+  if (AHEAD) load(next, here ? r : 0);
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    const uint32_t j = i * LANES + g;
+    w[i] = load_eight<W>(weight + 8ull * (j < groups ? j : 0));
+  }
+  f32x8 of_weight[PIECES] = {};
+  for (uint32_t buffer = 0; here; buffer ^= 1) {
+    const bool more = a.m - r > step;
+    if (AHEAD) {
+      now = next;
+      if (more) load(next, r + step);
+    } else {
+      load(now, r);
+    }
+    float squares = 0.f, along = 0.f;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      if (i * LANES + g >= groups) continue;
+      const f32x8 h = Eight<T>::wide(now.h[i]), d = Eight<T>::wide(now.d[i]) * Eight<W>::wide(w[i]);
+      squares += squares_of(h, 1.f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) along = __builtin_fmaf(d[k], h[k], along);
+    }
+    row_sums<LANES>(squares, along, buffer);
+    float root = inverse_root(squares, a.inverse_width, a.eps);
+    if (!(squares <= FLT_MAX)) {
+      // (values whose squares fp32 does not hold: both sums of values 2^-70 times as large)
+      squares = along = 0.f;
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        if (i * LANES + g >= groups) continue;
+        const f32x8 h = Eight<T>::wide(now.h[i]) * kSmall, d = Eight<T>::wide(now.d[i]) * Eight<W>::wide(w[i]);
+        squares += squares_of(h, 1.f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) along = __builtin_fmaf(d[k], h[k], along);
+      }
+      if (LANES > 64) __syncthreads();  // (the sums have been read)
+      row_sums<LANES>(squares, along, buffer);
+      if (LANES > 64) __syncthreads();
+      root = inverse_root_of_small(squares, a.inverse_width);
+      along *= root * (1.f / kSmall);
+    } else {
+      along *= root;
+    }
+    along *= a.inverse_width;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const uint32_t j = i * LANES + g;
+      if (j >= groups) continue;
+      const f32x8 d = Eight<T>::wide(now.d[i]), h = Eight<T>::wide(now.h[i]) * root;
+      of_weight[i] += d * h;
+      if (!a.grad_h) continue;
+      f32x8 out = (d * Eight<W>::wide(w[i]) - h * along) * root;
+      if (a.grad_sum) out += Eight<T>::wide(now.s[i]);
+      store_eight<T>(row_at<T>(a.grad_h, a.grad_h_stride_row, r) + 8ull * j, out);
+    }
+    here = more;
+    r += step;
+  }
   if (!a.partial) return;
+  if constexpr (LANES == 64) {
+    // The four waves' shares are one.
+    __shared__ f32x8 shares[PIECES][256];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) shares[i][threadIdx.x] = of_weight[i];
+    __syncthreads();
+    if (wave_id()) return;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+#pragma unroll
+      for (int w = 1; w < 4; ++w) of_weight[i] += shares[i][w * 64 + g];
+    }
+  }
 #pragma unroll
   for (int i = 0; i < PIECES; ++i) {
     const uint32_t j = i * LANES + g;
@@ -290,11 +384,10 @@ __global__ __launch_bounds__(LANES) void norm_backward_rows(NormBackwardDev a) {
 }
 
 // Longer rows, read twice; r of each row is left for the weight's gradient.
-constexpr int kLongLanes = 512;
 template <class T, class W> __global__ __launch_bounds__(kLongLanes) void norm_backward_long(NormBackwardDev a) {
   const uint32_t g = threadIdx.x, groups = a.width / 8;
   const PPLX_GLOBAL W *weight = as_global(reinterpret_cast<const W *>(a.weight));
-  for (uint32_t r = blockIdx.x; r < a.m; r += gridDim.x) {
+  for (uint32_t r = blockIdx.x;;) {
     const PPLX_GLOBAL T *grad = row_at<T>(a.grad_y, a.grad_y_stride_row, r), *row = row_at<T>(a.h, a.h_stride_row, r);
     auto squares_times = [&](float factor) {
       float s = 0.f;
@@ -305,64 +398,65 @@ template <class T, class W> __global__ __launch_bounds__(kLongLanes) void norm_b
     const float root = squares <= FLT_MAX ? inverse_root(squares, a.inverse_width, a.eps)
                                           : inverse_root_of_small(squares_times(kSmall), a.inverse_width);
     if (a.partial && g == 0) as_global(a.partial)[r] = root;
-    if (!a.grad_h) continue;
-    float along = 0.f;
-    for (uint32_t j = g; j < groups; j += kLongLanes) {
-      const f32x8 h = Eight<T>::wide(load_eight<T>(row + 8ull * j)) * root;
-      const f32x8 d = Eight<T>::wide(load_eight<T>(grad + 8ull * j)) * Eight<W>::wide(load_eight<W>(weight + 8ull * j));
+    if (a.grad_h) {
+      float along = 0.f;
+      for (uint32_t j = g; j < groups; j += kLongLanes) {
+        const f32x8 h = Eight<T>::wide(load_eight<T>(row + 8ull * j)) * root;
+        const f32x8 d = Eight<T>::wide(load_eight<T>(grad + 8ull * j)) * Eight<W>::wide(load_eight<W>(weight + 8ull * j));
 #pragma unroll
-      for (int k = 0; k < 8; ++k) along = __builtin_fmaf(d[k], h[k], along);
+        for (int k = 0; k < 8; ++k) along = __builtin_fmaf(d[k], h[k], along);
+      }
+      along = row_sum<kLongLanes>(along) * a.inverse_width;
+      for (uint32_t j = g; j < groups; j += kLongLanes) {
+        const f32x8 h = Eight<T>::wide(load_eight<T>(row + 8ull * j)) * root;
+        const f32x8 d = Eight<T>::wide(load_eight<T>(grad + 8ull * j)) * Eight<W>::wide(load_eight<W>(weight + 8ull * j));
+        f32x8 out = (d - h * along) * root;
+        if (a.grad_sum) out += Eight<T>::wide(load_eight<T>(row_at<T>(a.grad_sum, a.grad_sum_stride_row, r) + 8ull * j));
+        store_eight<T>(row_at<T>(a.grad_h, a.grad_h_stride_row, r) + 8ull * j, out);
+      }
     }
-    along = row_sum<kLongLanes>(along) * a.inverse_width;
-    for (uint32_t j = g; j < groups; j += kLongLanes) {
-      const f32x8 h = Eight<T>::wide(load_eight<T>(row + 8ull * j)) * root;
-      const f32x8 d = Eight<T>::wide(load_eight<T>(grad + 8ull * j)) * Eight<W>::wide(load_eight<W>(weight + 8ull * j));
-      f32x8 out = (d - h * along) * root;
-      if (a.grad_sum) out += Eight<T>::wide(load_eight<T>(row_at<T>(a.grad_sum, a.grad_sum_stride_row, r) + 8ull * j));
-      store_eight<T>(row_at<T>(a.grad_h, a.grad_h_stride_row, r) + 8ull * j, out);
-    }
+    if (a.m - r <= gridDim.x) break;
+    r += gridDim.x;
   }
 }
 
-// The weight's gradient out of the workgroups' shares, or of long rows out of the rows: 64 threads to 512 columns each, eight
-// waves that take every eighth share or row.
-constexpr int kSumWaves = 8;
-template <class Fn> __device__ __forceinline__ f32x8 sum_of_waves(uint32_t count, Fn &&of) {
-  __shared__ float sums[kSumWaves][8][64];
+// The weight's gradient out of the workgroups' shares, or of long rows out of the rows: a workgroup to 32 columns, four threads to a
+// share or row, whose sums are added in LDS in their order.
+constexpr int kSumThreads = 256, kSumSlots = kSumThreads / 4;
+template <class W, class Fn> __device__ __forceinline__ void sum_columns(uint32_t count, uint32_t width, W *out, Fn &&of) {
+  __shared__ float sums[kSumSlots][33];
+  const uint32_t slot = threadIdx.x / 4, j = blockIdx.x * 4 + threadIdx.x % 4;
   f32x8 s = {};
-  for (uint32_t i = wave_id(); i < count; i += kSumWaves) s += of(i);
-#pragma unroll
-  for (int k = 0; k < 8; ++k) sums[wave_id()][k][lane_id()] = s[k];
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    s[k] = 0.f;
-#pragma unroll
-    for (int w = 0; w < kSumWaves; ++w) s[k] += sums[w][k][lane_id()];
+  if (j < width / 8) {
+    for (uint32_t i = slot; i < count; i += kSumSlots) s += of(i, j);
   }
-  return s;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) sums[slot][threadIdx.x % 4 * 8 + k] = s[k];
+  __syncthreads();
+  const uint32_t column = blockIdx.x * 32 + threadIdx.x;
+  if (threadIdx.x >= 32 || column >= width) return;
+  float sum = 0.f;
+#pragma unroll 8
+  for (int k = 0; k < kSumSlots; ++k) sum += sums[k][threadIdx.x];
+  as_global(out)[column] = (W)sum;
 }
-template <class W> __global__ __launch_bounds__(kSumWaves * 64) void norm_weight_gradient(const float *partial, uint32_t count, uint32_t width, W *out) {
-  const uint32_t j = blockIdx.x * 64 + lane_id(), groups = width / 8;
-  const f32x8 s = sum_of_waves(count, [&](uint32_t i) {
-    return j < groups ? load_eight<float>(as_global(partial) + (uint64_t)i * width + 8ull * j) : f32x8{};
-  });
-  if (wave_id() == 0 && j < groups) store_eight<W>(as_global(out) + 8ull * j, s);
+template <class W> __global__ __launch_bounds__(kSumThreads) void norm_weight_gradient(const float *partial, uint32_t count, uint32_t width, W *out) {
+  sum_columns(count, width, out, [&](uint32_t i, uint32_t j) { return load_eight<float>(as_global(partial) + (uint64_t)i * width + 8ull * j); });
 }
-template <class T, class W> __global__ __launch_bounds__(kSumWaves * 64) void norm_weight_gradient_long(NormBackwardDev a, W *out) {
-  const uint32_t j = blockIdx.x * 64 + lane_id(), groups = a.width / 8;
-  const f32x8 s = sum_of_waves(a.m, [&](uint32_t r) {
-    if (j >= groups) return f32x8{};
+template <class T, class W> __global__ __launch_bounds__(kSumThreads) void norm_weight_gradient_long(NormBackwardDev a, W *out) {
+  sum_columns(a.m, a.width, out, [&](uint32_t r, uint32_t j) {
     const f32x8 h = Eight<T>::wide(load_eight<T>(row_at<T>(a.h, a.h_stride_row, r) + 8ull * j)) * as_global(a.partial)[r];
     return h * Eight<T>::wide(load_eight<T>(row_at<T>(a.grad_y, a.grad_y_stride_row, r) + 8ull * j));
   });
-  if (wave_id() == 0 && j < groups) store_eight<W>(as_global(out) + 8ull * j, s);
 }
 
 constexpr uint64_t kMostInRegisters = 8 * 4 * 512;  // elements of a row in the gradient's kernel
 constexpr uint32_t kBackwardGroups = 512;           // workgroups that share out the rows
 
-uint32_t backward_groups(uint32_t m) { return m < kBackwardGroups ? m : kBackwardGroups; }
+uint32_t backward_groups(uint32_t m, uint64_t width) {
+  const uint64_t rows = width <= 2048 ? ((uint64_t)m + 3) / 4 : m, most = width <= 8192 ? kBackwardGroups : kBackwardGroups / 2;
+  return (uint32_t)(rows < most ? rows : most);
+}
 
 template <class Fn> int with_weight_type(int32_t dtype, int32_t weight_dtype, Fn &&fn) {
   return with_type(dtype, [&](auto tag) {
@@ -439,16 +533,13 @@ extern "C" int pplx_a2a_rms_norm(int device, const pplx_a2a_rms_norm_args_t *arg
       auto launch = [&](auto format) {
         constexpr int F = decltype(format)::value;
         hipStream_t s = (hipStream_t)stream;
-        if (a.width <= 2048) {
-          auto kernel = norm_rows<T, W, F, 64, 4>;
-          PPLX_LAUNCH(launch_groups(kernel, kernel, ((uint64_t)a.m + 3) / 4, 256, 0, s, a));
-        } else if (a.width <= 8192) {
-          auto kernel = norm_rows<T, W, F, 256, 4>;
-          PPLX_LAUNCH(launch_groups(kernel, kernel, a.m, 256, 0, s, a));
-        } else {
-          auto kernel = norm_rows<T, W, F, 512, 4>;
-          PPLX_LAUNCH(launch_groups(kernel, kernel, a.m, 512, 0, s, a));
-        }
+        auto rows = [&](auto kernel, uint32_t threads, uint32_t at_once) {
+          return launch_groups(kernel, kernel, ((uint64_t)a.m + at_once - 1) / at_once, threads, 0, s, a);
+        };
+        if (a.width <= 2048) PPLX_LAUNCH(rows(norm_rows<T, W, F, 64, 4>, 256, 4));
+        else if (a.width <= 8192) PPLX_LAUNCH(rows(norm_rows<T, W, F, 256, 4>, 256, 1));
+        else if (a.width <= kMostInRegisters) PPLX_LAUNCH(rows(norm_rows<T, W, F, 512, 4>, 512, 1));
+        else PPLX_LAUNCH(rows(norm_long_rows<T, W, F>, kLongLanes, 1));
         return (int)PPLX_A2A_OK;
       };
       switch (p.format) {
@@ -463,7 +554,7 @@ extern "C" int pplx_a2a_rms_norm(int device, const pplx_a2a_rms_norm_args_t *arg
 extern "C" int pplx_a2a_rms_norm_workspace(uint32_t m, uint64_t hidden_dim, uint64_t *bytes) {
   PPLX_REQUIRE(bytes, "bytes is NULL");
   PPLX_REQUIRE(hidden_dim > 0 && hidden_dim < (1ull << 27) && hidden_dim % 8 == 0, "hidden_dim must be a multiple of 8 below 2^27");
-  *bytes = 4 * (hidden_dim > kMostInRegisters ? (uint64_t)m : backward_groups(m) * hidden_dim);
+  *bytes = 4 * (hidden_dim > kMostInRegisters ? (uint64_t)m : backward_groups(m, hidden_dim) * hidden_dim);
   return PPLX_A2A_OK;
 }
 
@@ -502,19 +593,21 @@ extern "C" int pplx_a2a_rms_norm_backward(int device, const pplx_a2a_rms_norm_ba
       typedef typename decltype(tag)::type T;
       typedef typename decltype(weight_tag)::type W;
       hipStream_t s = (hipStream_t)stream;
-      const uint32_t groups = backward_groups(a.m), columns = (a.width + 511) / 512;
+      const uint32_t groups = backward_groups(a.m, a.width), columns = (a.width + 31) / 32;
+      constexpr bool kAhead = sizeof(T) == 2;  // (rows of fp32 that are longer than 2048 fill the registers once)
       W *out = static_cast<W *>(p.grad_weight);
       if (a.width > kMostInRegisters) {
         PPLX_LAUNCH(launch_kernel(norm_backward_long<T, W>, dim3(groups), dim3(kLongLanes), 0, s, a));
-        if (out) PPLX_LAUNCH(launch_kernel(norm_weight_gradient_long<T, W>, dim3(columns), dim3(kSumWaves * 64), 0, s, a, out));
+        if (out) PPLX_LAUNCH(launch_kernel(norm_weight_gradient_long<T, W>, dim3(columns), dim3(kSumThreads), 0, s, a, out));
         return (int)PPLX_A2A_OK;
       }
-      if (a.width <= 2048) PPLX_LAUNCH(launch_kernel(norm_backward_rows<T, W, 64, 4>, dim3(groups), dim3(64), 0, s, a));
-      else if (a.width <= 8192) PPLX_LAUNCH(launch_kernel(norm_backward_rows<T, W, 256, 4>, dim3(groups), dim3(256), 0, s, a));
-      else PPLX_LAUNCH(launch_kernel(norm_backward_rows<T, W, 512, 4>, dim3(groups), dim3(512), 0, s, a));
+      if (a.width <= 2048) PPLX_LAUNCH(launch_kernel(norm_backward_rows<T, W, 64, 4, kAhead>, dim3(groups), dim3(256), 0, s, a));
+      else if (a.width <= 4096) PPLX_LAUNCH(launch_kernel(norm_backward_rows<T, W, 256, 2, true>, dim3(groups), dim3(256), 0, s, a));
+      else if (a.width <= 8192) PPLX_LAUNCH(launch_kernel(norm_backward_rows<T, W, 256, 4, kAhead>, dim3(groups), dim3(256), 0, s, a));
+      else PPLX_LAUNCH(launch_kernel(norm_backward_rows<T, W, 512, 4, kAhead>, dim3(groups), dim3(512), 0, s, a));
       if (out) {
         const float *partial = a.partial;
-        PPLX_LAUNCH(launch_kernel(norm_weight_gradient<W>, dim3(columns), dim3(kSumWaves * 64), 0, s, partial, groups, a.width, out));
+        PPLX_LAUNCH(launch_kernel(norm_weight_gradient<W>, dim3(columns), dim3(kSumThreads), 0, s, partial, groups, a.width, out));
       }
       return (int)PPLX_A2A_OK;
     });

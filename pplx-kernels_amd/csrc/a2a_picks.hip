@@ -1,7 +1,10 @@
 // Each token's experts and their weights out of the router's logits, and the gradient of the weights.
 //
 // Experts are put in order as if everything were computed in 64 bits: two whose scores with bias are closer than fp32 tells
-// apart come out in the same order everywhere.
+// apart come out in the same order everywhere.  Without a bias the logits themselves have that order.  Otherwise fp32 makes the
+// choice and watches how near its keys come: a token with two of them closer than their errors is done once more in 64 bits.
+// A wave takes a token, whose logits it reads once; what bounds it is the instructions of the choice, a reduction over the wave for
+// each pick.
 #include <cfloat>
 #include <cmath>
 
@@ -25,17 +28,75 @@ struct PicksDev {
 };
 
 constexpr double kNone = -HUGE_VAL;
+constexpr float kNoLogit = -HUGE_VALF;
 
-template <class Op> __device__ __forceinline__ double wave_all(double v, Op &&op) {
+// What a wave's lanes wrote to LDS is there for its other lanes.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+template <class F, class Op> __device__ __forceinline__ F wave_all(F v, Op &&op) {
 #pragma unroll
   for (int d = 32; d; d >>= 1) v = op(v, __shfl_xor(v, d));
   return v;
 }
-__device__ __forceinline__ double wave_max_of(double v) {
-  return wave_all(v, [](double a, double b) { return a > b ? a : b; });
+template <class F> __device__ __forceinline__ F wave_max_of(F v) {
+  return wave_all(v, [](F a, F b) { return a > b ? a : b; });
 }
-__device__ __forceinline__ double wave_sum_of(double v) {
-  return wave_all(v, [](double a, double b) { return a + b; });
+template <class F> __device__ __forceinline__ F wave_sum_of(F v) {
+  return wave_all(v, [](F a, F b) { return a + b; });
+}
+__device__ __forceinline__ uint32_t wave_min_of(uint32_t v) {
+  return wave_all(v, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+}
+
+// The largest of the lanes' values (none is NaN), in a scalar register: lanes pass theirs on inside rows of sixteen, then from row
+// to row, without LDS.
+template <int CONTROL, int ROWS> __device__ __forceinline__ float larger_of_lanes(float v) {
+  const float o = __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), CONTROL, ROWS, 0xf, false));
+  return v > o ? v : o;
+}
+__device__ __forceinline__ float wave_largest(float v) {
+  v = larger_of_lanes<0x111, 0xf>(v);  // from the lane 1, 2, 4, 8 below
+  v = larger_of_lanes<0x112, 0xf>(v);
+  v = larger_of_lanes<0x114, 0xf>(v);
+  v = larger_of_lanes<0x118, 0xf>(v);
+  v = larger_of_lanes<0x142, 0xa>(v);  // from the last lane of the row before, of the first two rows
+  v = larger_of_lanes<0x143, 0xc>(v);
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+
+// exp(x) to two ulps, of x <= 88 (of more, exp(88)): 2^p for the rounded product p = x log2(e), times 1 + what the rounding left, in two
+// steps where the result is subnormal (the instruction has none).
+__device__ __forceinline__ float exp_of(float x) {
+  x = x < 88.f ? x : 88.f;
+  constexpr float kLog2e = 1.44269504088896340736f, kRest = 1.925963033500865e-8f;  // (their sum is log2(e))
+  const float p = x * kLog2e;
+  const float left = __builtin_fmaf(x, kLog2e, -p) + x * kRest;
+  const float shift = p < -100.f ? 64.f : 0.f;
+  float v = __builtin_amdgcn_exp2f(p + shift);
+  v = __builtin_fmaf(v, left * 0.69314718055994530942f, v);
+  return p < -1000.f ? 0.f : p < -100.f ? v * 0x1p-64f : v;  // (-inf brings a NaN from `left`)
+}
+__device__ __forceinline__ double exp_of(double x) { return exp(x); }
+template <class F> __device__ __forceinline__ F sigmoid_of(F l) { return (F)1 / ((F)1 + exp_of(-l)); }
+
+// The weights of a wave's picks, lane k's of pick k with logit l: their scores, or their shares of the sum.
+template <class F> __device__ __forceinline__ F weight_of_pick(bool picked, F l, bool softmax, bool renormalize, F most, F total) {
+  if (renormalize) {
+    // (scores over the largest of them: none of them is 0 because its type does not hold it)
+    const F top = wave_max_of(picked ? l : (F)kNone), up = top < 0 ? -top : (F)0;
+    F w = !picked ? (F)0 : softmax ? exp_of(l - top) : (F)1 / (exp_of(-up) + exp_of(-l - up));
+    const F sum = wave_sum_of(w);
+    return picked ? w / sum : (F)0;
+  }
+  return !picked ? (F)0 : softmax ? exp_of(l - most) / total : sigmoid_of(l);
+}
+// Whether fp32 holds what weight_of_pick comes to: the distances from the largest logit, and from 0.
+__device__ __forceinline__ bool picks_are_near(bool picked, float l, float most) {
+  return __ballot(picked && !(l - most > -80.f && l > -80.f && l < 80.f)) == 0;
 }
 
 // The number of the largest key of `keys`, the first of several (count where all are -inf).  Called by a wave.
@@ -49,30 +110,22 @@ __device__ __forceinline__ uint32_t first_of_largest(const double *keys, uint32_
     }
   }
   const double most = wave_max_of(best);
-  at = best == most && most > kNone ? at : count;
-#pragma unroll
-  for (int d = 32; d; d >>= 1) {
-    const uint32_t o = (uint32_t)__shfl_xor((int)at, d);
-    at = at < o ? at : o;
-  }
-  return at;
+  return wave_min_of(best == most && most > kNone ? at : count);
 }
 
-// A wave to a token, whose keys are in LDS.
-template <class T> __global__ __launch_bounds__(64) void pick_experts(PicksDev a) {
-  extern __shared__ double keys[];  // of the experts, then the sums of the groups
-  const uint32_t t = a.first_group + blockIdx.x, lane = lane_id(), E = a.experts;
-  uint32_t there = a.m;
-  if (a.bound_m) there = *as_global(a.bound_m) < there ? *as_global(a.bound_m) : there;
-  PPLX_GLOBAL uint32_t *indices = as_global(a.indices) + (uint64_t)t * a.picks;
-  PPLX_GLOBAL float *weights = as_global(a.weights) + (uint64_t)t * a.picks;
-  if (t >= there) {
-    if (lane < a.picks) {
-      indices[lane] = E;
-      weights[lane] = 0.f;
-    }
-    return;
-  }
+__device__ __forceinline__ void store_pick(const PicksDev &a, uint32_t t, uint32_t lane, uint32_t expert, float weight) {
+  if (lane >= a.picks) return;
+  as_global(a.indices)[(uint64_t)t * a.picks + lane] = expert;
+  as_global(a.weights)[(uint64_t)t * a.picks + lane] = weight;
+}
+// A token with a logit or key that is no number, or +inf.
+__device__ __forceinline__ void store_bad(const PicksDev &a, uint32_t t, uint32_t lane) {
+  store_pick(a, t, lane, lane, __uint_as_float(0x7fc00000u));
+}
+
+// A token's choice in 64 bits by a wave, with keys in LDS: of the experts, then the sums of the groups.
+template <class T> __device__ __forceinline__ void pick_exactly(const PicksDev &a, uint32_t t, double *keys) {
+  const uint32_t lane = lane_id(), E = a.experts;
   const PPLX_GLOBAL T *logits = as_global(reinterpret_cast<const T *>(a.logits)) + (int64_t)t * a.logits_stride_row;
   const PPLX_GLOBAL float *bias = as_global(a.bias);
   bool bad = false;
@@ -88,25 +141,19 @@ template <class T> __global__ __launch_bounds__(64) void pick_experts(PicksDev a
     for (uint32_t e = lane; e < E; e += 64) total += exp((double)(float)logits[e] - most);
     total = wave_sum_of(total);
   }
-  auto score = [&](double l) { return softmax ? exp(l - most) / total : 1.0 / (1.0 + exp(-l)); };
   // An expert's chance beside the others' of its group; -inf where it is not there.
   auto chance = [&](uint32_t e) {
     const double l = (float)logits[e];
-    return l > kNone ? score(l) + (a.bias ? (double)bias[e] : 0.0) : kNone;
+    const double s = softmax ? exp(l - most) / total : sigmoid_of(l);
+    return l > kNone ? s + (a.bias ? (double)bias[e] : 0.0) : kNone;
   };
   for (uint32_t e = lane; e < E; e += 64) {
     const double key = a.bias ? chance(e) : (double)(float)logits[e];
     keys[e] = key;
     bad |= !(key < HUGE_VAL);
   }
-  if (__ballot(bad)) {
-    if (lane < a.picks) {
-      indices[lane] = lane;
-      weights[lane] = __uint_as_float(0x7fc00000u);
-    }
-    return;
-  }
-  __syncthreads();
+  if (__ballot(bad)) return store_bad(a, t, lane);
+  wave_sync();
   if (grouped) {
     double *sums = keys + E;
     const uint32_t size = E / a.groups;
@@ -119,49 +166,209 @@ template <class T> __global__ __launch_bounds__(64) void pick_experts(PicksDev a
       }
       sums[g] = a.group_top == 1 ? first : first + second;
     }
-    __syncthreads();
-    // (groups that are taken have a sum of NaN; one whose sum is -inf comes after all others, by number)
+    wave_sync();
+    // (groups that are taken have a sum of NaN; those whose sum is -inf come after all others, by number)
     for (uint32_t i = 0; i < a.top_groups; ++i) {
       uint32_t g = first_of_largest(sums, a.groups);
       if (g == a.groups) {
         for (uint32_t j = lane; j < a.groups; j += 64) g = j < g && sums[j] == kNone ? j : g;
-#pragma unroll
-        for (int d = 32; d; d >>= 1) {
-          const uint32_t o = (uint32_t)__shfl_xor((int)g, d);
-          g = g < o ? g : o;
-        }
+        g = wave_min_of(g);
       }
-      __syncthreads();
+      wave_sync();
       if (lane == 0) sums[g] = __longlong_as_double(0x7ff8000000000000ll);
-      __syncthreads();
+      wave_sync();
     }
     for (uint32_t e = lane; e < E; e += 64) keys[e] = sums[e / size] != sums[e / size] ? keys[e] : kNone;
-    __syncthreads();
+    wave_sync();
   }
   uint32_t own = E;  // lane k: pick k
   for (uint32_t k = 0; k < a.picks; ++k) {
     const uint32_t e = first_of_largest(keys, E);
     if (e == E) break;
     own = lane == k ? e : own;
-    __syncthreads();
+    wave_sync();
     if (lane == 0) keys[e] = kNone;
-    __syncthreads();
+    wave_sync();
   }
   const bool picked = own < E;
   const double l = picked ? (double)(float)logits[own] : kNone;
-  double w;
-  if (a.renormalize) {
-    // The scores over the largest of them: none of them is 0 because 64 bits do not hold it.
-    const double top = wave_max_of(l), up = top < 0 ? -top : 0;
-    w = !picked ? 0 : softmax ? exp(l - top) : 1.0 / (exp(-up) + exp(-l - up));
-    w /= wave_sum_of(w);
+  const double w = weight_of_pick(picked, l, softmax, a.renormalize, most, total);
+  store_pick(a, t, lane, own, (float)(w * (double)a.weight_scale));
+}
+
+constexpr uint32_t kTokensAtOnce = 4;  // of a workgroup, a wave to each
+// The token of a wave; tokens from bound_m on are done here.
+__device__ __forceinline__ bool has_token(const PicksDev &a, uint32_t t, uint32_t lane) {
+  if (t >= a.m) return false;
+  if (!a.bound_m || t < *as_global(a.bound_m)) return true;
+  store_pick(a, t, lane, a.experts, 0.f);
+  return false;
+}
+
+template <class T> __global__ __launch_bounds__(64) void pick_experts_exactly(PicksDev a) {
+  extern __shared__ double keys[];
+  const uint32_t t = a.first_group + blockIdx.x;
+  if (has_token(a, t, lane_id())) pick_exactly<T>(a, t, keys);
+}
+
+// PER consecutive elements from `base` on, of which those behind the last of `count` are -inf.
+template <class T, int PER> __device__ __forceinline__ void load_logits(const PPLX_GLOBAL T *row, uint32_t base, uint32_t count, float *l) {
+  typedef T vec __attribute__((ext_vector_type(PER), aligned(sizeof(T))));
+  if (base + PER <= count) {
+    if constexpr (PER == 1) {
+      l[0] = (float)row[base];
+    } else {
+      const vec v = *reinterpret_cast<const PPLX_GLOBAL vec *>(row + base);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) l[j] = (float)v[j];
+    }
   } else {
-    w = score(l);
+#pragma unroll
+    for (int j = 0; j < PER; ++j) l[j] = base + j < count ? (float)row[base + j] : kNoLogit;
   }
-  if (lane < a.picks) {
-    indices[lane] = own;
-    weights[lane] = picked ? (float)(w * (double)a.weight_scale) : 0.f;
+}
+
+// Up to 64 PER experts, PER consecutive ones in a lane, so that the first of equal keys is that of the first lane.  SCORED: keys
+// or the groups' sums are fp32 scores.
+template <class T, int PER, bool SCORED> __global__ __launch_bounds__(64 * kTokensAtOnce) void pick_experts(PicksDev a) {
+  extern __shared__ double room[];  // SCORED: of each wave, for a choice in 64 bits; of the groups, two words for each lane
+  const uint32_t lane = lane_id(), wave = wave_id(), E = a.experts;
+  const uint32_t t = (a.first_group + blockIdx.x) * kTokensAtOnce + wave;
+  if (!has_token(a, t, lane)) return;
+  double *keys = room + wave * (SCORED && E + a.groups > 64 ? E + a.groups : 64);
+  const PPLX_GLOBAL T *logits = as_global(reinterpret_cast<const T *>(a.logits)) + (int64_t)t * a.logits_stride_row;
+  const uint32_t base = lane * PER;
+  float l[PER], key[PER];
+  load_logits<T, PER>(logits, base, E, l);
+  bool bad = false;
+  float most = kNoLogit, total = 0.f;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    bad |= !(l[j] < HUGE_VALF);
+    most = l[j] > most ? l[j] : most;
   }
+  if (__ballot(bad)) return store_bad(a, t, lane);
+  const bool softmax = a.scores == PPLX_A2A_SOFTMAX, grouped = a.top_groups < a.groups;
+  most = wave_largest(most);
+  if (softmax && (SCORED || !a.renormalize)) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      key[j] = l[j] > kNoLogit ? exp_of(l[j] - most) : 0.f;
+      total += key[j];
+    }
+    total = wave_sum_of(total);
+  }
+  if constexpr (SCORED) {
+    // Scores with their biases.
+    const float share = 1.f / total;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const float s = softmax ? key[j] * share : sigmoid_of(l[j]);
+      const float b = a.bias && base + j < E ? as_global(a.bias)[base + j] : 0.f;
+      key[j] = l[j] > kNoLogit ? s + b : kNoLogit;
+      bad |= !(key[j] < HUGE_VALF);
+    }
+    if (__ballot(bad)) return store_bad(a, t, lane);
+  } else {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) key[j] = l[j];
+  }
+  // How far a key may be from its value in 64 bits: a score is within 2^-20 of it, relative, and of 1, and the sum with the bias is rounded
+  // once.  Two keys further apart than twice that are in order.
+  auto is_near = [](float larger, float smaller) {
+    return larger - smaller <= 0x1p-18f + 0x1p-21f * (__builtin_fabsf(larger) + __builtin_fabsf(smaller));
+  };
+  bool near = false;
+  if (grouped) {
+    // A lane's experts are of one group, a group's of `lanes` lanes (as the launch sees to).
+    const uint32_t lanes = E / a.groups / PER, group = lane / lanes;
+    float *best = reinterpret_cast<float *>(keys);
+    float first = kNoLogit, second = kNoLogit;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      second = key[j] > first ? first : key[j] > second ? key[j] : second;
+      first = key[j] > first ? key[j] : first;
+    }
+    best[2 * lane] = first;
+    best[2 * lane + 1] = second;
+    wave_sync();
+    first = second = kNoLogit;
+    if (group < a.groups) {
+      for (uint32_t i = 0; i < lanes; ++i) {
+        const float c = best[2 * (group * lanes + i)], d = best[2 * (group * lanes + i) + 1];
+        const float low = c > first ? first : c;
+        first = c > first ? c : first;
+        second = second > low ? second : low;
+        second = second > d ? second : d;
+      }
+    }
+    const float sum = a.group_top == 1 ? first : first + second;
+    uint32_t before = 0;  // groups in front of this one
+    for (uint32_t g = 0; g < a.groups; ++g) {
+      const float other = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sum), (int)(g * lanes)));
+      before += other > sum || (other == sum && g < group) ? 1 : 0;
+      if (SCORED) near |= g != group && group < a.groups && other > kNoLogit && sum > kNoLogit && (other > sum ? is_near(other, sum) : is_near(sum, other));
+    }
+    if (before >= a.top_groups) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) key[j] = kNoLogit;
+    }
+    wave_sync();
+  }
+  // The largest key of each lane; the largest of all is taken, and its lane looks for its next one.
+  float head, head_logit;
+  uint32_t head_at;
+  auto find_head = [&]() __attribute__((always_inline)) {
+    head = key[0];
+    head_logit = l[0];
+    head_at = 0;
+#pragma unroll
+    for (int j = 1; j < PER; ++j) {
+      const bool more = key[j] > head;
+      head = more ? key[j] : head;
+      head_logit = more ? l[j] : head_logit;
+      head_at = more ? j : head_at;
+    }
+  };
+  find_head();
+  uint32_t own = E, last_expert = 0;  // lane k: pick k and its logit
+  float own_logit = kNoLogit, last = 0.f, last_logit = 0.f;
+  for (uint32_t k = 0; k < a.picks + (SCORED ? 1 : 0); ++k) {
+    const float largest = wave_largest(head);
+    if (largest == kNoLogit) break;
+    const int winner = __builtin_ctzll(__ballot(head == largest));
+    const uint32_t expert = (uint32_t)winner * PER + (PER > 1 ? (uint32_t)__builtin_amdgcn_readlane((int)head_at, winner) : 0);
+    const float logit = SCORED ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(head_logit), winner)) : largest;
+    if constexpr (SCORED) {
+      // (equal logits with equal biases are equal in any arithmetic)
+      if (k && is_near(last, largest)) {
+        near |= !(logit == last_logit && (!a.bias || as_global(a.bias)[expert] == as_global(a.bias)[last_expert]));
+      }
+      last = largest;
+      last_logit = logit;
+      last_expert = expert;
+    }
+    if (lane == k && k < a.picks) {
+      own = expert;
+      own_logit = logit;
+    }
+    if ((int)lane == winner) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) key[j] = (uint32_t)j == head_at ? kNoLogit : key[j];
+      find_head();
+    }
+  }
+  if constexpr (SCORED) {
+    if (__ballot(near)) return pick_exactly<T>(a, t, keys);
+  }
+  const bool picked = own < E;
+  float w;
+  if (picks_are_near(picked, own_logit, most)) {
+    w = weight_of_pick(picked, own_logit, softmax, a.renormalize, most, total) * a.weight_scale;
+  } else {
+    w = (float)(weight_of_pick<double>(picked, own_logit, softmax, a.renormalize, most, total) * (double)a.weight_scale);
+  }
+  store_pick(a, t, lane, own, w);
 }
 
 struct PicksBackwardDev {
@@ -177,52 +384,86 @@ struct PicksBackwardDev {
   uint32_t first_group;
 };
 
-// A wave to a token.  Without renormalisation the gradient of a softmax has a part for every expert, p_e times the sum of
-// g_k w_k; everything else is that of the picks alone.
-template <class T> __global__ __launch_bounds__(64) void pick_gradient(PicksBackwardDev a) {
-  extern __shared__ float of_picks[];  // an expert's own part
-  const uint32_t t = a.first_group + blockIdx.x, lane = lane_id(), E = a.experts;
+// The parts of a token's gradient that are its picks' own, lane k's of pick k, and what all experts' scores are multiplied with: without
+// renormalisation the gradient of a softmax has a part for every expert, p_e times the sum of g_k w_k.
+template <class F>
+__device__ __forceinline__ F gradient_of_pick(const PicksBackwardDev &a, bool picked, F g, F l, F most, F total, F *inner) {
+  const bool softmax = a.scores == PPLX_A2A_SOFTMAX;
+  const F w = weight_of_pick(picked, l, softmax, a.renormalize, most, total);
+  const F sum = wave_sum_of(picked ? g * w : (F)0);
+  F part = picked ? w * g : (F)0;
+  if (a.renormalize) part = picked ? w * (g - sum) : (F)0;
+  if (!softmax) part *= sigmoid_of(-l);  // 1 - s
+  *inner = softmax && !a.renormalize ? sum * (F)a.weight_scale : (F)0;
+  return picked ? part * (F)a.weight_scale : (F)0;
+}
+
+// A wave to a token, PER consecutive experts in a lane and 64 PER at a time; rows of up to that are read once.
+template <class T, int PER> __global__ __launch_bounds__(64 * kTokensAtOnce) void pick_gradient(PicksBackwardDev a) {
+  extern __shared__ float of_picks[];  // [waves][experts]: an expert's own part
+  const uint32_t lane = lane_id(), wave = wave_id(), E = a.experts;
+  const uint32_t t = (a.first_group + blockIdx.x) * kTokensAtOnce + wave;
+  if (t >= a.m) return;
+  float *own_parts = of_picks + wave * E;
   const PPLX_GLOBAL T *logits = as_global(reinterpret_cast<const T *>(a.logits)) + (int64_t)t * a.logits_stride_row;
   PPLX_GLOBAL T *out = as_global(reinterpret_cast<T *>(a.grad_logits)) + (int64_t)t * a.grad_logits_stride_row;
-  const bool softmax = a.scores == PPLX_A2A_SOFTMAX;
   const uint32_t own = lane < a.picks ? as_global(a.indices)[(uint64_t)t * a.picks + lane] : E;
   const bool picked = own < E;
-  const double g = picked ? (double)as_global(a.grad_weights)[(uint64_t)t * a.picks + lane] : 0.0;
-  const double l = picked ? (double)(float)logits[own] : kNone;
-  for (uint32_t e = lane; e < E; e += 64) of_picks[e] = 0.f;
-  double most = kNone, total = 0, inner = 0, part = 0;
-  const bool dense = softmax && !a.renormalize;
+  const float g = picked ? as_global(a.grad_weights)[(uint64_t)t * a.picks + lane] : 0.f;
+  const bool dense = a.scores == PPLX_A2A_SOFTMAX && !a.renormalize, once = E <= 64 * PER;
+  float l[PER];
+  float most = kNoLogit, total = 0.f;
   if (dense) {
-    for (uint32_t e = lane; e < E; e += 64) {
-      const double x = (float)logits[e];
-      most = x > most ? x : most;
+    for (uint32_t first = 0; first < E; first += 64 * PER) {
+      load_logits<T, PER>(logits, first + lane * PER, E, l);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) most = l[j] > most ? l[j] : most;
     }
     most = wave_max_of(most);
-    for (uint32_t e = lane; e < E; e += 64) total += exp((double)(float)logits[e] - most);
-    total = wave_sum_of(total);
-    const double w = picked ? exp(l - most) / total * a.weight_scale : 0.0;
-    inner = wave_sum_of(g * w);
-    part = g * w;
-  } else {
-    const double s = picked ? 1.0 / (1.0 + exp(-l)) : 0.0;
-    double w = s;
-    if (a.renormalize) {
-      const double top = wave_max_of(l), up = top < 0 ? -top : 0;
-      w = !picked ? 0 : softmax ? exp(l - top) : 1.0 / (exp(-up) + exp(-l - up));
-      w /= wave_sum_of(w);
-      part = w * a.weight_scale * (g - wave_sum_of(g * w));
-    } else {
-      part = g * w * a.weight_scale;
+    for (uint32_t first = 0; first < E; first += 64 * PER) {
+      if (!once) load_logits<T, PER>(logits, first + lane * PER, E, l);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) total += l[j] == kNoLogit ? 0.f : exp_of(l[j] - most);
     }
-    if (!softmax) part *= 1.0 - s;
+    total = wave_sum_of(total);
   }
-  __syncthreads();
-  if (picked) of_picks[own] = (float)part;
-  __syncthreads();
-  for (uint32_t e = lane; e < E; e += 64) {
-    double d = of_picks[e];
-    if (dense && inner != 0) d -= exp((double)(float)logits[e] - most) / total * inner;
-    out[e] = (T)(float)d;
+  for (uint32_t e = lane; e < E; e += 64) own_parts[e] = 0.f;
+  const float own_logit = picked ? (float)logits[own] : kNoLogit;
+  float inner, part;
+  if (picks_are_near(picked, own_logit, dense ? most : own_logit)) {
+    part = gradient_of_pick<float>(a, picked, g, own_logit, most, total, &inner);
+  } else {
+    double sum;
+    part = (float)gradient_of_pick<double>(a, picked, g, own_logit, most, total, &sum);
+    inner = (float)sum;
+  }
+  wave_sync();
+  if (picked) own_parts[own] = part;
+  wave_sync();
+  const float share = inner / total;
+  for (uint32_t first = 0; first < E; first += 64 * PER) {
+    const uint32_t base = first + lane * PER;
+    if (dense && !once) load_logits<T, PER>(logits, base, E, l);
+    float d[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      d[j] = base + j < E ? own_parts[base + j] : 0.f;
+      if (dense && inner != 0.f) d[j] -= l[j] == kNoLogit ? 0.f : exp_of(l[j] - most) * share;
+    }
+    if constexpr (PER > 1) {
+      typedef T vec __attribute__((ext_vector_type(PER), aligned(sizeof(T))));
+      if (base + PER <= E) {
+        vec v;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) v[j] = (T)d[j];
+        *reinterpret_cast<PPLX_GLOBAL vec *>(out + base) = v;
+        continue;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      if (base + j < E) out[base + j] = (T)d[j];
+    }
   }
 }
 
@@ -274,16 +515,37 @@ extern "C" int pplx_a2a_route_tokens(int device, const pplx_a2a_route_args_t *ar
   a.weight_scale = p.weight_scale;
   return guarded(device, [&] {
     return with_type(p.dtype, [&](auto tag) {
-      auto kernel = pick_experts<typename decltype(tag)::type>;
-      // (5461 experts in as many groups take 85 KiB)
-      const uint32_t lds = 8 * (a.experts + (a.top_groups < a.groups ? a.groups : 0));
-      if (lds > 64 * 1024) {
-        const hipError_t err =
-            hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-        if (err != hipSuccess) (void)hipGetLastError();  // (the launch says so if it matters)
+      typedef typename decltype(tag)::type T;
+      const bool grouped = a.top_groups < a.groups, scored = a.bias || (grouped && a.group_top > 1);
+      // Experts of a lane: as few as hold all of them, where no lane has some of two groups.
+      const uint32_t per = a.experts <= 64 ? 1 : a.experts <= 128 ? 2 : a.experts <= 256 ? 4 : a.experts <= 512 ? 8 : 16;
+      if (a.experts > 1024 || (grouped && (size % per || a.groups > 64))) {
+        // (5461 experts in as many groups take 85 KiB)
+        const uint32_t lds = 8 * (a.experts + (grouped ? a.groups : 0));
+        auto kernel = pick_experts_exactly<T>;
+        if (lds > 64 * 1024) {
+          const hipError_t err =
+              hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+          if (err != hipSuccess) (void)hipGetLastError();  // (the launch says so if it matters)
+        }
+        PPLX_LAUNCH(launch_groups(kernel, kernel, a.m, 64, lds, (hipStream_t)stream, a));
+        return (int)PPLX_A2A_OK;
       }
-      PPLX_LAUNCH(launch_groups(kernel, kernel, a.m, 64, lds, (hipStream_t)stream, a));
-      return (int)PPLX_A2A_OK;
+      auto launch = [&](auto count) {
+        constexpr int PER = decltype(count)::value;
+        auto kernel = scored ? pick_experts<T, PER, true> : pick_experts<T, PER, false>;
+        const uint32_t lds = 8 * kTokensAtOnce * (scored ? a.experts + a.groups < 64 ? 64 : a.experts + a.groups : 64);
+        PPLX_LAUNCH(launch_groups(kernel, kernel, ((uint64_t)a.m + kTokensAtOnce - 1) / kTokensAtOnce, 64 * kTokensAtOnce, lds,
+                                  (hipStream_t)stream, a));
+        return (int)PPLX_A2A_OK;
+      };
+      switch (per) {
+        case 1: return launch(std::integral_constant<int, 1>{});
+        case 2: return launch(std::integral_constant<int, 2>{});
+        case 4: return launch(std::integral_constant<int, 4>{});
+        case 8: return launch(std::integral_constant<int, 8>{});
+        default: return launch(std::integral_constant<int, 16>{});
+      }
     });
   });
 }
@@ -313,8 +575,16 @@ extern "C" int pplx_a2a_route_tokens_backward(int device, const pplx_a2a_route_b
   a.weight_scale = p.weight_scale;
   return guarded(device, [&] {
     return with_type(p.dtype, [&](auto tag) {
-      auto kernel = pick_gradient<typename decltype(tag)::type>;
-      PPLX_LAUNCH(launch_groups(kernel, kernel, a.m, 64, 4 * a.experts, (hipStream_t)stream, a));
+      typedef typename decltype(tag)::type T;
+      auto kernel = a.experts <= 64 ? pick_gradient<T, 1> : a.experts <= 256 ? pick_gradient<T, 4> : pick_gradient<T, 8>;
+      const uint32_t lds = 4 * kTokensAtOnce * a.experts;
+      if (lds > 64 * 1024) {
+        const hipError_t err =
+            hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (err != hipSuccess) (void)hipGetLastError();  // (the launch says so if it matters)
+      }
+      PPLX_LAUNCH(launch_groups(kernel, kernel, ((uint64_t)a.m + kTokensAtOnce - 1) / kTokensAtOnce, 64 * kTokensAtOnce, lds,
+                                (hipStream_t)stream, a));
       return (int)PPLX_A2A_OK;
     });
   });
