@@ -6,6 +6,7 @@
 // A wave takes a token, whose logits it reads once; what bounds it is the instructions of the choice, a reduction over the wave for
 // each pick.
 #include <cfloat>
+#include <climits>
 #include <cmath>
 
 #include "a2a_experts.h"
@@ -52,21 +53,40 @@ __device__ __forceinline__ uint32_t wave_min_of(uint32_t v) {
   return wave_all(v, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
 }
 
-// The largest of the lanes' values (none is NaN), in a scalar register: lanes pass theirs on inside rows of sixteen, then from row
-// to row, without LDS.
-template <int CONTROL, int ROWS> __device__ __forceinline__ float larger_of_lanes(float v) {
-  const float o = __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), CONTROL, ROWS, 0xf, false));
-  return v > o ? v : o;
+// Reductions without LDS, whose results are in scalar registers: lanes pass theirs on inside rows of sixteen, to the lane 1, 2, 4 and 8
+// above, then the last lane of a row to the next row, and that of the second to the last two.
+template <int CONTROL, int ROWS> __device__ __forceinline__ int from_lane(int otherwise, int v) {
+  return __builtin_amdgcn_update_dpp(otherwise, v, CONTROL, ROWS, 0xf, false);
 }
-__device__ __forceinline__ float wave_largest(float v) {
-  v = larger_of_lanes<0x111, 0xf>(v);  // from the lane 1, 2, 4, 8 below
-  v = larger_of_lanes<0x112, 0xf>(v);
-  v = larger_of_lanes<0x114, 0xf>(v);
-  v = larger_of_lanes<0x118, 0xf>(v);
-  v = larger_of_lanes<0x142, 0xa>(v);  // from the last lane of the row before, of the first two rows
-  v = larger_of_lanes<0x143, 0xc>(v);
-  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+template <class Fn> __device__ __forceinline__ int over_lanes(int v, Fn &&step) {
+  v = step(v, std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});
+  v = step(v, std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});
+  v = step(v, std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});
+  v = step(v, std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});
+  v = step(v, std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});
+  v = step(v, std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
+  return __builtin_amdgcn_readlane(v, 63);
 }
+__device__ __forceinline__ int wave_largest(int v) {
+  return over_lanes(v, [](int x, auto control, auto rows) {
+    const int o = from_lane<decltype(control)::value, decltype(rows)::value>(INT_MIN, x);
+    return o > x ? o : x;
+  });
+}
+__device__ __forceinline__ float wave_total(float v) {
+  return __int_as_float(over_lanes(__float_as_int(v), [](int x, auto control, auto rows) {
+    return __float_as_int(__int_as_float(x) + __int_as_float(from_lane<decltype(control)::value, decltype(rows)::value>(0, x)));
+  }));
+}
+// Numbers, none of them NaN, as integers of the same order, and back; 0 and -0 are one.
+__device__ __forceinline__ int order_of(float v) {
+  const int b = __float_as_int(v + 0.f);
+  return b ^ ((b >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float number_of(int order) { return __int_as_float(order ^ ((order >> 31) & 0x7fffffff)); }
+__device__ __forceinline__ float wave_max_of_lanes(float v) { return number_of(wave_largest(order_of(v))); }
+__device__ __forceinline__ double wave_max_of_lanes(double v) { return wave_max_of(v); }
+__device__ __forceinline__ double wave_total(double v) { return wave_sum_of(v); }
 
 // exp(x) to two ulps, of x <= 88 (of more, exp(88)): 2^p for the rounded product p = x log2(e), times 1 + what the rounding left, in two
 // steps where the result is subnormal (the instruction has none).
@@ -87,9 +107,9 @@ template <class F> __device__ __forceinline__ F sigmoid_of(F l) { return (F)1 / 
 template <class F> __device__ __forceinline__ F weight_of_pick(bool picked, F l, bool softmax, bool renormalize, F most, F total) {
   if (renormalize) {
     // (scores over the largest of them: none of them is 0 because its type does not hold it)
-    const F top = wave_max_of(picked ? l : (F)kNone), up = top < 0 ? -top : (F)0;
+    const F top = wave_max_of_lanes(picked ? l : (F)kNone), up = top < 0 ? -top : (F)0;
     F w = !picked ? (F)0 : softmax ? exp_of(l - top) : (F)1 / (exp_of(-up) + exp_of(-l - up));
-    const F sum = wave_sum_of(w);
+    const F sum = wave_total(w);
     return picked ? w / sum : (F)0;
   }
   return !picked ? (F)0 : softmax ? exp_of(l - most) / total : sigmoid_of(l);
@@ -197,9 +217,8 @@ template <class T> __device__ __forceinline__ void pick_exactly(const PicksDev &
 }
 
 constexpr uint32_t kTokensAtOnce = 4;  // of a workgroup, a wave to each
-// The token of a wave; tokens from bound_m on are done here.
-__device__ __forceinline__ bool has_token(const PicksDev &a, uint32_t t, uint32_t lane) {
-  if (t >= a.m) return false;
+// Whether a token is there; those from bound_m on are done here.
+__device__ __forceinline__ bool is_there(const PicksDev &a, uint32_t t, uint32_t lane) {
   if (!a.bound_m || t < *as_global(a.bound_m)) return true;
   store_pick(a, t, lane, a.experts, 0.f);
   return false;
@@ -208,7 +227,7 @@ __device__ __forceinline__ bool has_token(const PicksDev &a, uint32_t t, uint32_
 template <class T> __global__ __launch_bounds__(64) void pick_experts_exactly(PicksDev a) {
   extern __shared__ double keys[];
   const uint32_t t = a.first_group + blockIdx.x;
-  if (has_token(a, t, lane_id())) pick_exactly<T>(a, t, keys);
+  if (is_there(a, t, lane_id())) pick_exactly<T>(a, t, keys);
 }
 
 // PER consecutive elements from `base` on, of which those behind the last of `count` are -inf.
@@ -234,12 +253,13 @@ template <class T, int PER, bool SCORED> __global__ __launch_bounds__(64 * kToke
   extern __shared__ double room[];  // SCORED: of each wave, for a choice in 64 bits; of the groups, two words for each lane
   const uint32_t lane = lane_id(), wave = wave_id(), E = a.experts;
   const uint32_t t = (a.first_group + blockIdx.x) * kTokensAtOnce + wave;
-  if (!has_token(a, t, lane)) return;
+  if (t >= a.m) return;
   double *keys = room + wave * (SCORED && E + a.groups > 64 ? E + a.groups : 64);
   const PPLX_GLOBAL T *logits = as_global(reinterpret_cast<const T *>(a.logits)) + (int64_t)t * a.logits_stride_row;
   const uint32_t base = lane * PER;
-  float l[PER], key[PER];
+  float l[PER];
   load_logits<T, PER>(logits, base, E, l);
+  if (!is_there(a, t, lane)) return;
   bool bad = false;
   float most = kNoLogit, total = 0.f;
 #pragma unroll
@@ -249,34 +269,41 @@ template <class T, int PER, bool SCORED> __global__ __launch_bounds__(64 * kToke
   }
   if (__ballot(bad)) return store_bad(a, t, lane);
   const bool softmax = a.scores == PPLX_A2A_SOFTMAX, grouped = a.top_groups < a.groups;
-  most = wave_largest(most);
+  most = wave_max_of_lanes(most);
+  float score[PER];
   if (softmax && (SCORED || !a.renormalize)) {
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      key[j] = l[j] > kNoLogit ? exp_of(l[j] - most) : 0.f;
-      total += key[j];
+      score[j] = l[j] > kNoLogit ? exp_of(l[j] - most) : 0.f;
+      total += score[j];
     }
-    total = wave_sum_of(total);
+    total = wave_total(total);
   }
+  int key[PER];  // in order_of's order
+  const int none = order_of(kNoLogit);
   if constexpr (SCORED) {
     // Scores with their biases.
     const float share = 1.f / total;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      const float s = softmax ? key[j] * share : sigmoid_of(l[j]);
+      const float s = softmax ? score[j] * share : sigmoid_of(l[j]);
       const float b = a.bias && base + j < E ? as_global(a.bias)[base + j] : 0.f;
-      key[j] = l[j] > kNoLogit ? s + b : kNoLogit;
-      bad |= !(key[j] < HUGE_VALF);
+      const float sum = l[j] > kNoLogit ? s + b : kNoLogit;
+      key[j] = order_of(sum);
+      bad |= !(sum < HUGE_VALF);
     }
     if (__ballot(bad)) return store_bad(a, t, lane);
   } else {
 #pragma unroll
-    for (int j = 0; j < PER; ++j) key[j] = l[j];
+    for (int j = 0; j < PER; ++j) key[j] = order_of(l[j]);
   }
-  // How far a key may be from its value in 64 bits: a score is within 2^-20 of it, relative, and of 1, and the sum with the bias is rounded
-  // once.  Two keys further apart than twice that are in order.
-  auto is_near = [](float larger, float smaller) {
-    return larger - smaller <= 0x1p-18f + 0x1p-21f * (__builtin_fabsf(larger) + __builtin_fabsf(smaller));
+  // How far keys may be from their values in 64 bits.  An exponential is off by two ulps, 2^-22 of it.  The sigmoid moves by at most a
+  // quarter of that, and its sum and quotient round: 3 * 2^-24.  A softmax divides by a sum of PER + 6 roundings, 2^-19 of a
+  // score that is at most `share`.  Two keys are off by twice as much, the sums of two groups by four times; the sums with the bias and of
+  // two scores round by 2^-24 of what they come to.
+  const float off = softmax ? 0x1p-18f / total : 0x1p-21f;
+  auto is_near = [](float larger, float smaller, float off) {
+    return larger - smaller <= off + 0x1p-22f * (__builtin_fabsf(larger) + __builtin_fabsf(smaller));
   };
   bool near = false;
   if (grouped) {
@@ -286,8 +313,9 @@ template <class T, int PER, bool SCORED> __global__ __launch_bounds__(64 * kToke
     float first = kNoLogit, second = kNoLogit;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      second = key[j] > first ? first : key[j] > second ? key[j] : second;
-      first = key[j] > first ? key[j] : first;
+      const float c = number_of(key[j]);
+      second = __builtin_fmaxf(second, __builtin_fminf(first, c));
+      first = __builtin_fmaxf(first, c);
     }
     best[2 * lane] = first;
     best[2 * lane + 1] = second;
@@ -296,10 +324,8 @@ template <class T, int PER, bool SCORED> __global__ __launch_bounds__(64 * kToke
     if (group < a.groups) {
       for (uint32_t i = 0; i < lanes; ++i) {
         const float c = best[2 * (group * lanes + i)], d = best[2 * (group * lanes + i) + 1];
-        const float low = c > first ? first : c;
-        first = c > first ? c : first;
-        second = second > low ? second : low;
-        second = second > d ? second : d;
+        second = __builtin_fmaxf(__builtin_fmaxf(second, d), __builtin_fminf(first, c));
+        first = __builtin_fmaxf(first, c);
       }
     }
     const float sum = a.group_top == 1 ? first : first + second;
@@ -307,16 +333,17 @@ template <class T, int PER, bool SCORED> __global__ __launch_bounds__(64 * kToke
     for (uint32_t g = 0; g < a.groups; ++g) {
       const float other = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sum), (int)(g * lanes)));
       before += other > sum || (other == sum && g < group) ? 1 : 0;
-      if (SCORED) near |= g != group && group < a.groups && other > kNoLogit && sum > kNoLogit && (other > sum ? is_near(other, sum) : is_near(sum, other));
+      if (SCORED) near |= g != group && group < a.groups && other > kNoLogit && sum > kNoLogit && (other > sum ? is_near(other, sum, 2 * off) : is_near(sum, other, 2 * off));
     }
     if (before >= a.top_groups) {
 #pragma unroll
-      for (int j = 0; j < PER; ++j) key[j] = kNoLogit;
+      for (int j = 0; j < PER; ++j) key[j] = none;
     }
     wave_sync();
   }
   // The largest key of each lane; the largest of all is taken, and its lane looks for its next one.
-  float head, head_logit;
+  int head;
+  float head_logit;
   uint32_t head_at;
   auto find_head = [&]() __attribute__((always_inline)) {
     head = key[0];
@@ -334,14 +361,15 @@ template <class T, int PER, bool SCORED> __global__ __launch_bounds__(64 * kToke
   uint32_t own = E, last_expert = 0;  // lane k: pick k and its logit
   float own_logit = kNoLogit, last = 0.f, last_logit = 0.f;
   for (uint32_t k = 0; k < a.picks + (SCORED ? 1 : 0); ++k) {
-    const float largest = wave_largest(head);
-    if (largest == kNoLogit) break;
-    const int winner = __builtin_ctzll(__ballot(head == largest));
+    const int order = wave_largest(head);
+    if (order == none) break;
+    const float largest = number_of(order);
+    const int winner = __builtin_ctzll(__ballot(head == order));
     const uint32_t expert = (uint32_t)winner * PER + (PER > 1 ? (uint32_t)__builtin_amdgcn_readlane((int)head_at, winner) : 0);
     const float logit = SCORED ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(head_logit), winner)) : largest;
     if constexpr (SCORED) {
       // (equal logits with equal biases are equal in any arithmetic)
-      if (k && is_near(last, largest)) {
+      if (k && is_near(last, largest, off)) {
         near |= !(logit == last_logit && (!a.bias || as_global(a.bias)[expert] == as_global(a.bias)[last_expert]));
       }
       last = largest;
@@ -354,7 +382,7 @@ template <class T, int PER, bool SCORED> __global__ __launch_bounds__(64 * kToke
     }
     if ((int)lane == winner) {
 #pragma unroll
-      for (int j = 0; j < PER; ++j) key[j] = (uint32_t)j == head_at ? kNoLogit : key[j];
+      for (int j = 0; j < PER; ++j) key[j] = (uint32_t)j == head_at ? none : key[j];
       find_head();
     }
   }
@@ -390,7 +418,7 @@ template <class F>
 __device__ __forceinline__ F gradient_of_pick(const PicksBackwardDev &a, bool picked, F g, F l, F most, F total, F *inner) {
   const bool softmax = a.scores == PPLX_A2A_SOFTMAX;
   const F w = weight_of_pick(picked, l, softmax, a.renormalize, most, total);
-  const F sum = wave_sum_of(picked ? g * w : (F)0);
+  const F sum = wave_total(picked ? g * w : (F)0);
   F part = picked ? w * g : (F)0;
   if (a.renormalize) part = picked ? w * (g - sum) : (F)0;
   if (!softmax) part *= sigmoid_of(-l);  // 1 - s
@@ -419,13 +447,13 @@ template <class T, int PER> __global__ __launch_bounds__(64 * kTokensAtOnce) voi
 #pragma unroll
       for (int j = 0; j < PER; ++j) most = l[j] > most ? l[j] : most;
     }
-    most = wave_max_of(most);
+    most = wave_max_of_lanes(most);
     for (uint32_t first = 0; first < E; first += 64 * PER) {
       if (!once) load_logits<T, PER>(logits, first + lane * PER, E, l);
 #pragma unroll
       for (int j = 0; j < PER; ++j) total += l[j] == kNoLogit ? 0.f : exp_of(l[j] - most);
     }
-    total = wave_sum_of(total);
+    total = wave_total(total);
   }
   for (uint32_t e = lane; e < E; e += 64) own_parts[e] = 0.f;
   const float own_logit = picked ? (float)logits[own] : kNoLogit;
