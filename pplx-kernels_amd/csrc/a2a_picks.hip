@@ -2,7 +2,8 @@
 //
 // Experts are put in order as if everything were computed in 64 bits: two whose scores with bias are closer than fp32 tells
 // apart come out in the same order everywhere.  Without a bias the logits themselves have that order.  Otherwise fp32 makes the
-// choice and watches how near its keys come: a token with two of them closer than their errors is done once more in 64 bits.
+// choice and watches how near its keys come: a token with two of them closer than their errors is chosen for once more in 64 bits, out of
+// the registers that hold its logits.
 // A wave takes a token, whose logits it reads once; what bounds it is the instructions of the choice, a reduction over the wave for
 // each pick.
 #include <cfloat>
@@ -25,6 +26,7 @@ struct PicksDev {
   uint32_t groups, top_groups, group_top;
   int32_t scores, renormalize;
   float weight_scale;
+  uint32_t group_lanes, lanes_shift;  // lanes that hold a group's experts, a power of two
   uint32_t first_group;
 };
 
@@ -78,14 +80,56 @@ __device__ __forceinline__ float wave_total(float v) {
     return __float_as_int(__int_as_float(x) + __int_as_float(from_lane<decltype(control)::value, decltype(rows)::value>(0, x)));
   }));
 }
+__device__ __forceinline__ int of_lane(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ float of_lane(float v, int lane) { return __int_as_float(of_lane(__float_as_int(v), lane)); }
+__device__ __forceinline__ double of_lane(double v, int lane) {
+  return __hiloint2double(of_lane(__double2hiint(v), lane), of_lane(__double2loint(v), lane));
+}
+// The upper halves' largest, then of the lower halves that come with it.
+__device__ __forceinline__ int64_t wave_largest(int64_t v) {
+  const int high = (int)(v >> 32), most = wave_largest(high);
+  const int low = wave_largest(high == most ? (int)((uint32_t)v ^ 0x80000000u) : INT_MIN);
+  return (int64_t)((uint64_t)(uint32_t)most << 32 | ((uint32_t)low ^ 0x80000000u));
+}
+// What the lanes of a group of `lanes` (1, 2, 4, ... 64) hold, joined by `join`, in all of them; where the lanes next to each other hold the
+// same already, a mirrored row is as good as an exchange.
+__device__ __forceinline__ float of_partner(float v, int control) {
+  const int x = __float_as_int(v);
+  switch (control) {
+    case 1: return __int_as_float(__builtin_amdgcn_mov_dpp(x, 0xb1, 0xf, 0xf, true));
+    case 2: return __int_as_float(__builtin_amdgcn_mov_dpp(x, 0x4e, 0xf, 0xf, true));
+    case 4: return __int_as_float(__builtin_amdgcn_mov_dpp(x, 0x141, 0xf, 0xf, true));
+    case 8: return __int_as_float(__builtin_amdgcn_mov_dpp(x, 0x140, 0xf, 0xf, true));
+    default: return __shfl_xor(v, control);
+  }
+}
+__device__ __forceinline__ double of_partner(double v, int control) {
+  return __hiloint2double(__float_as_int(of_partner(__int_as_float(__double2hiint(v)), control)),
+                          __float_as_int(of_partner(__int_as_float(__double2loint(v)), control)));
+}
+template <class Join> __device__ __forceinline__ void over_group(uint32_t lanes, Join &&join) {
+  if (lanes > 1) join(std::integral_constant<int, 1>{});
+  if (lanes > 2) join(std::integral_constant<int, 2>{});
+  if (lanes > 4) join(std::integral_constant<int, 4>{});
+  if (lanes > 8) join(std::integral_constant<int, 8>{});
+  if (lanes > 16) join(std::integral_constant<int, 16>{});
+  if (lanes > 32) join(std::integral_constant<int, 32>{});
+}
 // Numbers, none of them NaN, as integers of the same order, and back; 0 and -0 are one.
 __device__ __forceinline__ int order_of(float v) {
   const int b = __float_as_int(v + 0.f);
   return b ^ ((b >> 31) & 0x7fffffff);
 }
+__device__ __forceinline__ int64_t order_of(double v) {
+  const int64_t b = __double_as_longlong(v + 0.0);
+  return b ^ ((b >> 63) & 0x7fffffffffffffffll);
+}
 __device__ __forceinline__ float number_of(int order) { return __int_as_float(order ^ ((order >> 31) & 0x7fffffff)); }
+__device__ __forceinline__ double number_of(int64_t order) {
+  return __longlong_as_double(order ^ ((order >> 63) & 0x7fffffffffffffffll));
+}
 __device__ __forceinline__ float wave_max_of_lanes(float v) { return number_of(wave_largest(order_of(v))); }
-__device__ __forceinline__ double wave_max_of_lanes(double v) { return wave_max_of(v); }
+__device__ __forceinline__ double wave_max_of_lanes(double v) { return number_of(wave_largest(order_of(v))); }
 __device__ __forceinline__ double wave_total(double v) { return wave_sum_of(v); }
 
 // exp(x) to two ulps, of x <= 88 (of more, exp(88)): 2^p for the rounded product p = x log2(e), times 1 + what the rounding left, in two
@@ -102,6 +146,20 @@ __device__ __forceinline__ float exp_of(float x) {
 }
 __device__ __forceinline__ double exp_of(double x) { return exp(x); }
 template <class F> __device__ __forceinline__ F sigmoid_of(F l) { return (F)1 / ((F)1 + exp_of(-l)); }
+// The same for keys, where an absolute error counts: in a few instructions and without branches.  exp(x) of x <= 0 to 2^-22 of it, or 2^-100.
+__device__ __forceinline__ float key_exp(float x) {
+  constexpr float kLog2e = 1.44269504088896340736f, kRest = 1.925963033500865e-8f;
+  x = __builtin_fmaxf(x, -100.f);
+  const float p = x * kLog2e, left = __builtin_fmaf(x, kLog2e, -p) + x * kRest, v = __builtin_amdgcn_exp2f(p);
+  return __builtin_fmaf(v, left * 0.69314718055994530942f, v);
+}
+__device__ __forceinline__ double key_exp(double x) { return exp(x); }
+// Off by 2^-22 at most.  The product rounds: |x| s (1 - s) <= 0.23 times 1.5 * 2^-24; the exponential: 2^-23 s (1 - s); the sum: 2^-24; the
+// reciprocal: 2^-23.
+__device__ __forceinline__ float key_sigmoid(float x) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.44269504088896340736f));
+}
+__device__ __forceinline__ double key_sigmoid(double x) { return sigmoid_of(x); }
 
 // The weights of a wave's picks, lane k's of pick k with logit l: their scores, or their shares of the sum.
 template <class F> __device__ __forceinline__ F weight_of_pick(bool picked, F l, bool softmax, bool renormalize, F most, F total) {
@@ -230,10 +288,11 @@ template <class T> __global__ __launch_bounds__(64) void pick_experts_exactly(Pi
   if (is_there(a, t, lane_id())) pick_exactly<T>(a, t, keys);
 }
 
-// PER consecutive elements from `base` on, of which those behind the last of `count` are -inf.
-template <class T, int PER> __device__ __forceinline__ void load_logits(const PPLX_GLOBAL T *row, uint32_t base, uint32_t count, float *l) {
+// PER consecutive elements from `base` on, of which those from `end` on are `otherwise`.
+template <class T, int PER>
+__device__ __forceinline__ void load_some(const PPLX_GLOBAL T *row, uint32_t base, uint32_t end, float otherwise, float *l) {
   typedef T vec __attribute__((ext_vector_type(PER), aligned(sizeof(T))));
-  if (base + PER <= count) {
+  if (base + PER <= end) {
     if constexpr (PER == 1) {
       l[0] = (float)row[base];
     } else {
@@ -243,106 +302,85 @@ template <class T, int PER> __device__ __forceinline__ void load_logits(const PP
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < PER; ++j) l[j] = base + j < count ? (float)row[base + j] : kNoLogit;
+    for (int j = 0; j < PER; ++j) l[j] = base + j < end ? (float)row[base + j] : otherwise;
   }
 }
 
-// Up to 64 PER experts, PER consecutive ones in a lane, so that the first of equal keys is that of the first lane.  SCORED: keys
-// or the groups' sums are fp32 scores.
-template <class T, int PER, bool SCORED> __global__ __launch_bounds__(64 * kTokensAtOnce) void pick_experts(PicksDev a) {
-  extern __shared__ double room[];  // SCORED: of each wave, for a choice in 64 bits; of the groups, two words for each lane
-  const uint32_t lane = lane_id(), wave = wave_id(), E = a.experts;
-  const uint32_t t = (a.first_group + blockIdx.x) * kTokensAtOnce + wave;
-  if (t >= a.m) return;
-  double *keys = room + wave * (SCORED && E + a.groups > 64 ? E + a.groups : 64);
-  const PPLX_GLOBAL T *logits = as_global(reinterpret_cast<const T *>(a.logits)) + (int64_t)t * a.logits_stride_row;
-  const uint32_t base = lane * PER;
-  float l[PER];
-  load_logits<T, PER>(logits, base, E, l);
-  if (!is_there(a, t, lane)) return;
-  bool bad = false;
-  float most = kNoLogit, total = 0.f;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    bad |= !(l[j] < HUGE_VALF);
-    most = l[j] > most ? l[j] : most;
-  }
-  if (__ballot(bad)) return store_bad(a, t, lane);
+// A token's choice in F, with its logits and biases in registers: of experts `base` on in this lane, which are of `group`.  False,
+// with nothing stored, if fp32 doesn't tell.  SCORED: keys or the groups' sums are scores, not logits.
+template <class F, int PER, bool SCORED>
+__device__ __forceinline__ bool choose(const PicksDev &a, uint32_t t, uint32_t lane, uint32_t group, uint32_t base, const float *l,
+                                       const float *bias, float most) {
+  constexpr bool kWatched = SCORED && sizeof(F) == 4;
+  typedef decltype(order_of(F())) Order;
   const bool softmax = a.scores == PPLX_A2A_SOFTMAX, grouped = a.top_groups < a.groups;
-  most = wave_max_of_lanes(most);
-  float score[PER];
+  const Order none = order_of((F)kNone);
+  F score[PER], total = 0;
   if (softmax && (SCORED || !a.renormalize)) {
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      score[j] = l[j] > kNoLogit ? exp_of(l[j] - most) : 0.f;
+      score[j] = key_exp((F)l[j] - (F)most);
+      score[j] = l[j] > kNoLogit ? score[j] : (F)0;
       total += score[j];
     }
     total = wave_total(total);
-  }
-  int key[PER];  // in order_of's order
-  const int none = order_of(kNoLogit);
-  if constexpr (SCORED) {
-    // Scores with their biases.
-    const float share = 1.f / total;
+    const F share = (F)1 / total;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const float s = softmax ? score[j] * share : sigmoid_of(l[j]);
-      const float b = a.bias && base + j < E ? as_global(a.bias)[base + j] : 0.f;
-      const float sum = l[j] > kNoLogit ? s + b : kNoLogit;
-      key[j] = order_of(sum);
-      bad |= !(sum < HUGE_VALF);
-    }
-    if (__ballot(bad)) return store_bad(a, t, lane);
-  } else {
+    for (int j = 0; j < PER; ++j) score[j] *= share;
+  } else if (SCORED) {
 #pragma unroll
-    for (int j = 0; j < PER; ++j) key[j] = order_of(l[j]);
+    for (int j = 0; j < PER; ++j) score[j] = key_sigmoid((F)l[j]);
   }
-  // How far keys may be from their values in 64 bits.  An exponential is off by two ulps, 2^-22 of it.  The sigmoid moves by at most a
-  // quarter of that, and its sum and quotient round: 3 * 2^-24.  A softmax divides by a sum of PER + 6 roundings, 2^-19 of a
-  // score that is at most `share`.  Two keys are off by twice as much, the sums of two groups by four times; the sums with the bias and of
-  // two scores round by 2^-24 of what they come to.
-  const float off = softmax ? 0x1p-18f / total : 0x1p-21f;
-  auto is_near = [](float larger, float smaller, float off) {
-    return larger - smaller <= off + 0x1p-22f * (__builtin_fabsf(larger) + __builtin_fabsf(smaller));
+  Order key[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    F k = l[j];
+    if (SCORED) k = l[j] > kNoLogit ? score[j] + (F)bias[j] : (F)kNone;
+    key[j] = order_of(k);
+  }
+  // How far keys may be from their values in 64 bits: a sigmoid by 2^-22.  A softmax by 2^-22 for its exponential, and it is divided by a
+  // sum of as much and PER + 6 roundings: 2^-19 of a score that is 1 / total at most.  Two keys are off by twice as much, the sums
+  // of two groups by four times; the sums with the bias and of two scores round by 2^-24 of what they come to.
+  const float off = !kWatched ? 0.f : softmax ? 0x1p-18f / (float)total : 0x1p-21f;
+  auto are_near = [](float larger, float smaller, float off) {
+    return larger - smaller <= __builtin_fmaf(0x1p-22f, __builtin_fabsf(larger) + __builtin_fabsf(smaller), off);
   };
   bool near = false;
   if (grouped) {
-    // A lane's experts are of one group, a group's of `lanes` lanes (as the launch sees to).
-    const uint32_t lanes = E / a.groups / PER, group = lane / lanes;
-    float *best = reinterpret_cast<float *>(keys);
-    float first = kNoLogit, second = kNoLogit;
+    auto larger_of = [](F x, F y) { return x > y ? x : y; };
+    auto smaller_of = [](F x, F y) { return x > y ? y : x; };
+    F first = kNone, second = kNone;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      const float c = number_of(key[j]);
-      second = __builtin_fmaxf(second, __builtin_fminf(first, c));
-      first = __builtin_fmaxf(first, c);
+      const F c = number_of(key[j]);
+      second = larger_of(second, smaller_of(first, c));
+      first = larger_of(first, c);
     }
-    best[2 * lane] = first;
-    best[2 * lane + 1] = second;
-    wave_sync();
-    first = second = kNoLogit;
-    if (group < a.groups) {
-      for (uint32_t i = 0; i < lanes; ++i) {
-        const float c = best[2 * (group * lanes + i)], d = best[2 * (group * lanes + i) + 1];
-        second = __builtin_fmaxf(__builtin_fmaxf(second, d), __builtin_fminf(first, c));
-        first = __builtin_fmaxf(first, c);
-      }
-    }
-    const float sum = a.group_top == 1 ? first : first + second;
+    over_group(a.group_lanes, [&](auto distance) {
+      const F c = of_partner(first, distance), d = of_partner(second, distance);
+      second = larger_of(larger_of(second, d), smaller_of(first, c));
+      first = larger_of(first, c);
+    });
+    const F sum = a.group_top == 1 ? first : first + second;
     uint32_t before = 0;  // groups in front of this one
     for (uint32_t g = 0; g < a.groups; ++g) {
-      const float other = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sum), (int)(g * lanes)));
+      const F other = of_lane(sum, (int)(g * a.group_lanes));
       before += other > sum || (other == sum && g < group) ? 1 : 0;
-      if (SCORED) near |= g != group && group < a.groups && other > kNoLogit && sum > kNoLogit && (other > sum ? is_near(other, sum, 2 * off) : is_near(sum, other, 2 * off));
     }
-    if (before >= a.top_groups) {
+    const bool taken = before < a.top_groups;
+    if (kWatched) {
+      // Of the groups that are taken the last, and the first of the others.
+      const float last = -wave_max_of_lanes(taken ? -(float)sum : kNoLogit);
+      const float next = wave_max_of_lanes(taken || group >= a.groups ? kNoLogit : (float)sum);
+      near |= next > kNoLogit && are_near(last, next, 2 * off);
+    }
+    if (!taken) {
 #pragma unroll
       for (int j = 0; j < PER; ++j) key[j] = none;
     }
-    wave_sync();
   }
   // The largest key of each lane; the largest of all is taken, and its lane looks for its next one.
-  int head;
+  Order head;
   float head_logit;
   uint32_t head_at;
   auto find_head = [&]() __attribute__((always_inline)) {
@@ -358,26 +396,17 @@ template <class T, int PER, bool SCORED> __global__ __launch_bounds__(64 * kToke
     }
   };
   find_head();
-  uint32_t own = E, last_expert = 0;  // lane k: pick k and its logit
-  float own_logit = kNoLogit, last = 0.f, last_logit = 0.f;
-  for (uint32_t k = 0; k < a.picks + (SCORED ? 1 : 0); ++k) {
-    const int order = wave_largest(head);
+  uint32_t own = a.experts;  // lane k: pick k, its key and logit
+  float own_key = kNoLogit, own_logit = kNoLogit;
+  for (uint32_t k = 0; k < a.picks; ++k) {
+    const Order order = wave_largest(head);
     if (order == none) break;
-    const float largest = number_of(order);
     const int winner = __builtin_ctzll(__ballot(head == order));
-    const uint32_t expert = (uint32_t)winner * PER + (PER > 1 ? (uint32_t)__builtin_amdgcn_readlane((int)head_at, winner) : 0);
-    const float logit = SCORED ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(head_logit), winner)) : largest;
-    if constexpr (SCORED) {
-      // (equal logits with equal biases are equal in any arithmetic)
-      if (k && is_near(last, largest, off)) {
-        near |= !(logit == last_logit && (!a.bias || as_global(a.bias)[expert] == as_global(a.bias)[last_expert]));
-      }
-      last = largest;
-      last_logit = logit;
-      last_expert = expert;
-    }
-    if (lane == k && k < a.picks) {
+    const uint32_t expert = (uint32_t)of_lane((int)(base + head_at), winner);
+    const float number = (float)number_of(order), logit = SCORED ? of_lane(head_logit, winner) : number;
+    if (lane == k) {
       own = expert;
+      own_key = number;
       own_logit = logit;
     }
     if ((int)lane == winner) {
@@ -386,17 +415,71 @@ template <class T, int PER, bool SCORED> __global__ __launch_bounds__(64 * kToke
       find_head();
     }
   }
-  if constexpr (SCORED) {
-    if (__ballot(near)) return pick_exactly<T>(a, t, keys);
+  const bool picked = own < a.experts;
+  if constexpr (kWatched) {
+    // Each pick beside the next, the last one beside all that are left.  Equal logits with equal biases are equal in any arithmetic.
+    const PPLX_GLOBAL float *biases = as_global(a.bias);
+    const float next_key = __shfl(own_key, (int)(lane + 1));
+    const bool close = lane + 1 < a.picks && next_key > kNoLogit && are_near(own_key, next_key, off);
+    if (__ballot(close)) {
+      const float next_logit = __shfl(own_logit, (int)(lane + 1));
+      const uint32_t next = __shfl(own, (int)(lane + 1));
+      if (close) near |= !(own_logit == next_logit && (!a.bias || biases[own] == biases[next]));
+    }
+    const Order order = wave_largest(head);
+    const float last_key = of_lane(own_key, (int)a.picks - 1), last_logit = of_lane(own_logit, (int)a.picks - 1);
+    const int last = of_lane((int)own, (int)a.picks - 1);
+    if (order != none && are_near(last_key, number_of(order), off)) {
+      const float last_bias = a.bias ? biases[last] : 0.f;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        near |= key[j] != none && are_near(last_key, number_of(key[j]), off) && !(l[j] == last_logit && bias[j] == last_bias);
+      }
+    }
+    if (__ballot(near)) return false;
   }
-  const bool picked = own < E;
   float w;
-  if (picks_are_near(picked, own_logit, most)) {
-    w = weight_of_pick(picked, own_logit, softmax, a.renormalize, most, total) * a.weight_scale;
+  if (sizeof(F) == 4 && picks_are_near(picked, own_logit, most)) {
+    w = (float)weight_of_pick<F>(picked, own_logit, softmax, a.renormalize, most, total) * a.weight_scale;
   } else {
     w = (float)(weight_of_pick<double>(picked, own_logit, softmax, a.renormalize, most, total) * (double)a.weight_scale);
   }
   store_pick(a, t, lane, own, w);
+  return true;
+}
+
+// Up to 64 PER experts, PER consecutive ones in a lane, so that the first of equal keys is that of the first lane; where groups are
+// chosen, no lane has experts of two.
+template <class T, int PER, bool SCORED> __global__ __launch_bounds__(64 * kTokensAtOnce) void pick_experts(PicksDev a) {
+  const uint32_t lane = lane_id(), wave = wave_id(), E = a.experts;
+  const uint32_t t = (a.first_group + blockIdx.x) * kTokensAtOnce + wave;
+  if (t >= a.m) return;
+  const PPLX_GLOBAL T *logits = as_global(reinterpret_cast<const T *>(a.logits)) + (int64_t)t * a.logits_stride_row;
+  uint32_t group = 0, base = lane * PER, end = E;
+  if (a.top_groups < a.groups) {
+    const uint32_t size = E / a.groups;
+    group = lane >> a.lanes_shift;
+    base = group * size + (lane - group * a.group_lanes) * PER;
+    end = group < a.groups ? (group + 1) * size : 0;
+  }
+  float l[PER], bias[PER];
+  load_some<T, PER>(logits, base, end, kNoLogit, l);
+#pragma unroll
+  for (int j = 0; j < PER; ++j) bias[j] = 0.f;
+  if (SCORED && a.bias) load_some<float, PER>(as_global(a.bias), base, end, 0.f, bias);
+  if (!is_there(a, t, lane)) return;
+  bool bad = false;
+  float most = kNoLogit;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    bad |= !(l[j] < HUGE_VALF);
+    if (SCORED) bad |= l[j] > kNoLogit && !(bias[j] < HUGE_VALF);
+    most = l[j] > most ? l[j] : most;
+  }
+  if (__ballot(bad)) return store_bad(a, t, lane);
+  most = wave_max_of_lanes(most);
+  if (choose<float, PER, SCORED>(a, t, lane, group, base, l, bias, most)) return;
+  if constexpr (SCORED) choose<double, PER, true>(a, t, lane, group, base, l, bias, most);
 }
 
 struct PicksBackwardDev {
@@ -443,13 +526,13 @@ template <class T, int PER> __global__ __launch_bounds__(64 * kTokensAtOnce) voi
   float most = kNoLogit, total = 0.f;
   if (dense) {
     for (uint32_t first = 0; first < E; first += 64 * PER) {
-      load_logits<T, PER>(logits, first + lane * PER, E, l);
+      load_some<T, PER>(logits, first + lane * PER, E, kNoLogit, l);
 #pragma unroll
       for (int j = 0; j < PER; ++j) most = l[j] > most ? l[j] : most;
     }
     most = wave_max_of_lanes(most);
     for (uint32_t first = 0; first < E; first += 64 * PER) {
-      if (!once) load_logits<T, PER>(logits, first + lane * PER, E, l);
+      if (!once) load_some<T, PER>(logits, first + lane * PER, E, kNoLogit, l);
 #pragma unroll
       for (int j = 0; j < PER; ++j) total += l[j] == kNoLogit ? 0.f : exp_of(l[j] - most);
     }
@@ -471,7 +554,7 @@ template <class T, int PER> __global__ __launch_bounds__(64 * kTokensAtOnce) voi
   const float share = inner / total;
   for (uint32_t first = 0; first < E; first += 64 * PER) {
     const uint32_t base = first + lane * PER;
-    if (dense && !once) load_logits<T, PER>(logits, base, E, l);
+    if (dense && !once) load_some<T, PER>(logits, base, E, kNoLogit, l);
     float d[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
@@ -546,8 +629,18 @@ extern "C" int pplx_a2a_route_tokens(int device, const pplx_a2a_route_args_t *ar
       typedef typename decltype(tag)::type T;
       const bool grouped = a.top_groups < a.groups, scored = a.bias || (grouped && a.group_top > 1);
       // Experts of a lane: as few as hold all of them, where no lane has some of two groups.
-      const uint32_t per = a.experts <= 64 ? 1 : a.experts <= 128 ? 2 : a.experts <= 256 ? 4 : a.experts <= 512 ? 8 : 16;
-      if (a.experts > 1024 || (grouped && (size % per || a.groups > 64))) {
+      // A group's lanes are a power of two.
+      const uint32_t size = a.experts / a.groups;
+      uint32_t per = 1;
+      auto lanes_of_group = [&] {
+        uint32_t lanes = 1;
+        while (lanes * per < size) lanes *= 2;
+        return lanes;
+      };
+      while (per <= 16 && (grouped ? (uint64_t)a.groups * lanes_of_group() > 64 : a.experts > 64 * per)) per *= 2;
+      a.group_lanes = grouped ? lanes_of_group() : 64;
+      a.lanes_shift = (uint32_t)__builtin_ctz(a.group_lanes);
+      if (per > 16) {
         // (5461 experts in as many groups take 85 KiB)
         const uint32_t lds = 8 * (a.experts + (grouped ? a.groups : 0));
         auto kernel = pick_experts_exactly<T>;
@@ -562,8 +655,7 @@ extern "C" int pplx_a2a_route_tokens(int device, const pplx_a2a_route_args_t *ar
       auto launch = [&](auto count) {
         constexpr int PER = decltype(count)::value;
         auto kernel = scored ? pick_experts<T, PER, true> : pick_experts<T, PER, false>;
-        const uint32_t lds = 8 * kTokensAtOnce * (scored ? a.experts + a.groups < 64 ? 64 : a.experts + a.groups : 64);
-        PPLX_LAUNCH(launch_groups(kernel, kernel, ((uint64_t)a.m + kTokensAtOnce - 1) / kTokensAtOnce, 64 * kTokensAtOnce, lds,
+        PPLX_LAUNCH(launch_groups(kernel, kernel, ((uint64_t)a.m + kTokensAtOnce - 1) / kTokensAtOnce, 64 * kTokensAtOnce, 0,
                                   (hipStream_t)stream, a));
         return (int)PPLX_A2A_OK;
       };

@@ -594,6 +594,23 @@ def test_route_tokens_tells_close_experts_apart(device, scores, groups):
 
 
 @gpu
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts,groups", [(64, 1), (66, 2), (104, 8), (128, 1), (256, 8), (500, 4), (500, 1), (520, 40), (1000, 1), (1200, 6)])
+def test_route_tokens_tells_picks_from_runners_up(device, scores, experts, groups):
+    """Every pick is close to the next one and the last to what comes after it, in each layout of experts over lanes.  Logits are a few
+    last bits apart, by the marks of a ruler on which no two distances are alike: sums of two differ unless their logits are the same."""
+    gen = torch.Generator().manual_seed(experts)
+    marks = torch.tensor([0.0, 1, 4, 9, 15, 22, 32, 34])
+    for k in (1, 7, 8):
+        logits = 2 + marks[torch.randint(0, 8, (200, experts), generator=gen)] * 2.0**-22
+        bias = torch.full((experts,), 0.25)
+        more = dict(scores=scores, num_groups=groups, top_groups=max(1, groups // 2))
+        got, _ = route_tokens(logits.to(device), k, bias=bias.to(device), **more)
+        want, _ = ref_route(logits, k, bias, **more)
+        assert torch.equal(got.view(torch.int32).cpu(), want)
+
+
+@gpu
 @pytest.mark.parametrize("bad", [float("inf"), float("nan")])
 @pytest.mark.parametrize("bias", [False, True])
 def test_route_tokens_of_logits_that_are_no_numbers(device, bad, bias):
