@@ -477,7 +477,8 @@ int pplx_a2a_int8_matmul_plan(const pplx_a2a_rows_t *rows, uint64_t n, uint64_t 
 
 /* ---- before dispatch ------------------------------------------------------- */
 
-/* Operators on plain device buffers as above: what makes the rows that dispatch sends, and its picks and weights. */
+/* Operators on plain device buffers as above: what makes the rows that dispatch sends, and its picks and weights.  Fewer than 2^31
+ * tokens. */
 
 /* Root-mean-square norm of rows, with the addition of a residual in front and the rows in 8 bits behind it:
  *   h = x + residual, rounded to dtype (h = x without residual)            -> sum

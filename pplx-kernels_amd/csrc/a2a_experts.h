@@ -49,6 +49,26 @@ template <class Fn> int with_type(int32_t dtype, Fn &&fn) {
     default: return fn(TypeTag<float>{});
   }
 }
+// The same with that of the weights, which is the rows' or fp32.
+template <class Fn> int with_weight_type(int32_t dtype, int32_t weight_dtype, Fn &&fn) {
+  return with_type(dtype, [&](auto tag) {
+    typedef typename decltype(tag)::type T;
+    return weight_dtype == dtype ? fn(tag, TypeTag<T>{}) : fn(tag, TypeTag<float>{});
+  });
+}
+
+// Rows that are there, 16-byte aligned.
+inline int check_rows_of(const void *p, int64_t stride, const char *name) {
+  PPLX_REQUIRE(p, "%s is NULL", name);
+  PPLX_REQUIRE(is_aligned(p, 16) && stride % 16 == 0, "%s must be 16-byte aligned with 16-byte strides", name);
+  return PPLX_A2A_OK;
+}
+#define PPLX_ROWS(p, name)                                               \
+  do {                                                                   \
+    const int st_ = check_rows_of(p.name, p.name##_stride_row, #name);   \
+    if (st_) return st_;                                                 \
+  } while (0)
+constexpr uint32_t kMaxTokens = (1u << 31) - 1;
 
 // A grid of any number of workgroups: a launch takes fewer than 2^32 threads along a dimension, so that more go out in several,
 // whose first argument's first_group is the number of the first one.  Those behind the first launch may be of another

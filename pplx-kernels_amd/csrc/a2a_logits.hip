@@ -485,11 +485,15 @@ __global__ __launch_bounds__(128) void split_gradient(PiecesDev a) {
   const uint32_t column_blocks = (a.columns + 31) / 32, group = a.first_group + blockIdx.x;
   const uint32_t block = group / column_blocks, column_block = group - block * column_blocks;
   const uint32_t r0 = block * 32, c0 = column_block * 32;
+  const uint32_t y = threadIdx.x / 32, x = threadIdx.x % 32, c = c0 + x < a.columns ? c0 + x : a.columns - 1;
+  float in[8];
 #pragma unroll
-  for (uint32_t y = 0; y < 32; y += 4) {
-    const uint32_t r = r0 + y + threadIdx.x / 32, c = c0 + threadIdx.x % 32;
-    tile[y + threadIdx.x / 32][threadIdx.x % 32] = r < a.rows && c < a.columns ? as_global(a.in)[(int64_t)r * a.in_stride + c] : 0.f;
+  for (uint32_t i = 0; i < 8; ++i) {
+    const uint32_t r = r0 + i * 4 + y;
+    in[i] = as_global(a.in)[(int64_t)(r < a.rows ? r : a.rows - 1) * a.in_stride + c];
   }
+#pragma unroll
+  for (uint32_t i = 0; i < 8; ++i) tile[i * 4 + y][x] = r0 + i * 4 + y < a.rows && c0 + x < a.columns ? in[i] : 0.f;
   __syncthreads();
   auto write = [&](uint8_t *to, uint64_t fragment, uint32_t pieces, auto at) {
     f32x8 v;
@@ -631,13 +635,6 @@ __global__ __launch_bounds__(512) void gradient_of_weight(GradientDev a, uint32_
     buffer ^= 1;
   }
   if (there && m0 < a.rows) store_turned<O, NV>(a, part * a.out_split, m0, column, lane, acc);
-}
-
-template <class Fn> int with_weight_type(int32_t dtype, int32_t weight_dtype, Fn &&fn) {
-  return with_type(dtype, [&](auto tag) {
-    typedef typename decltype(tag)::type T;
-    return weight_dtype == dtype ? fn(tag, TypeTag<T>{}) : fn(tag, TypeTag<float>{});
-  });
 }
 
 uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
@@ -826,20 +823,9 @@ int check_router_size(uint64_t m, uint32_t experts, uint64_t hidden, int32_t dty
   PPLX_REQUIRE(weight_dtype == dtype || weight_dtype == PPLX_A2A_F32, "weight_dtype must be dtype or F32");
   PPLX_REQUIRE(experts >= 1 && experts <= kMaxExperts, "num_experts must be in [1, %u]", kMaxExperts);
   PPLX_REQUIRE(hidden > 0 && hidden < (1ull << 27) && hidden % 8 == 0, "hidden_dim must be a multiple of 8 below 2^27");
-  if (m >= (1ull << 31)) return refuse(PPLX_A2A_UNSUPPORTED, "2^31 tokens or more");
+  if (m > kMaxTokens) return refuse(PPLX_A2A_UNSUPPORTED, "2^31 tokens or more");
   return PPLX_A2A_OK;
 }
-int check_rows_of(const void *p, int64_t stride, const char *name) {
-  PPLX_REQUIRE(p, "%s is NULL", name);
-  PPLX_REQUIRE(is_aligned(p, 16) && stride % 16 == 0, "%s must be 16-byte aligned with 16-byte strides", name);
-  return PPLX_A2A_OK;
-}
-#define PPLX_ROWS(p, name)                                               \
-  do {                                                                   \
-    const int st_ = check_rows_of(p.name, p.name##_stride_row, #name);   \
-    if (st_) return st_;                                                 \
-  } while (0)
-
 // A tile's rows are reached by 32-bit offsets.
 bool is_far(int64_t stride) { return stride < 0 || stride >= (1 << 23); }
 

@@ -458,29 +458,13 @@ uint32_t backward_groups(uint32_t m, uint64_t width) {
   return (uint32_t)(rows < most ? rows : most);
 }
 
-template <class Fn> int with_weight_type(int32_t dtype, int32_t weight_dtype, Fn &&fn) {
-  return with_type(dtype, [&](auto tag) {
-    typedef typename decltype(tag)::type T;
-    return weight_dtype == dtype ? fn(tag, TypeTag<T>{}) : fn(tag, TypeTag<float>{});
-  });
-}
-
-int check_rows_of(const void *p, int64_t stride, const char *name) {
-  PPLX_REQUIRE(is_aligned(p, 16) && stride % 16 == 0, "%s must be 16-byte aligned with 16-byte strides", name);
-  return PPLX_A2A_OK;
-}
-#define PPLX_ROWS(p, name)                                               \
-  do {                                                                   \
-    const int st_ = check_rows_of(p.name, p.name##_stride_row, #name);   \
-    if (st_) return st_;                                                 \
-  } while (0)
-
 template <class P> int check_norm_size(const P &p, uint64_t unit) {
   PPLX_REQUIRE(is_dtype(p.dtype), "unsupported dtype of the rows");
   PPLX_REQUIRE(p.weight_dtype == p.dtype || p.weight_dtype == PPLX_A2A_F32, "weight_dtype must be dtype or F32");
   PPLX_REQUIRE(p.hidden_dim > 0 && p.hidden_dim < (1ull << 27) && p.hidden_dim % unit == 0,
                "hidden_dim must be a multiple of %u below 2^27", (unsigned)unit);
   PPLX_REQUIRE(p.eps >= FLT_MIN && p.eps <= FLT_MAX, "eps must be positive, finite and normal");
+  if (p.m > kMaxTokens) return refuse(PPLX_A2A_UNSUPPORTED, "2^31 tokens or more");
   return PPLX_A2A_OK;
 }
 
@@ -496,12 +480,11 @@ extern "C" int pplx_a2a_rms_norm(int device, const pplx_a2a_rms_norm_args_t *arg
   const int st = check_norm_size(p, p.format == PPLX_A2A_ROWS_PLAIN ? 8 : 16);
   if (st) return st;
   if (p.m == 0) return PPLX_A2A_OK;
-  PPLX_REQUIRE(p.x && p.weight, "x / weight is NULL");
   PPLX_REQUIRE((p.q != nullptr) == (p.format != PPLX_A2A_ROWS_PLAIN), "q goes with a format of quantised rows");
   PPLX_REQUIRE(p.y || p.q, "neither y nor q is asked for");
   PPLX_REQUIRE((p.residual != nullptr) == (p.sum != nullptr), "sum goes with residual");
   PPLX_REQUIRE(!p.q || (p.scale && is_aligned(p.scale, 4)), "scale is NULL or not aligned");
-  PPLX_REQUIRE(is_aligned(p.weight, 16), "weight must be 16-byte aligned");
+  PPLX_REQUIRE(p.weight && is_aligned(p.weight, 16), "weight is NULL or not 16-byte aligned");
   PPLX_ROWS(p, x);
   if (p.residual) PPLX_ROWS(p, residual);
   if (p.residual) PPLX_ROWS(p, sum);
@@ -554,6 +537,7 @@ extern "C" int pplx_a2a_rms_norm(int device, const pplx_a2a_rms_norm_args_t *arg
 extern "C" int pplx_a2a_rms_norm_workspace(uint32_t m, uint64_t hidden_dim, uint64_t *bytes) {
   PPLX_REQUIRE(bytes, "bytes is NULL");
   PPLX_REQUIRE(hidden_dim > 0 && hidden_dim < (1ull << 27) && hidden_dim % 8 == 0, "hidden_dim must be a multiple of 8 below 2^27");
+  if (m > kMaxTokens) return refuse(PPLX_A2A_UNSUPPORTED, "2^31 tokens or more");
   *bytes = 4 * (hidden_dim > kMostInRegisters ? (uint64_t)m : backward_groups(m, hidden_dim) * hidden_dim);
   return PPLX_A2A_OK;
 }
@@ -564,8 +548,7 @@ extern "C" int pplx_a2a_rms_norm_backward(int device, const pplx_a2a_rms_norm_ba
   const int st = check_norm_size(p, 8);
   if (st) return st;
   PPLX_REQUIRE(p.m > 0, "there are no tokens");
-  PPLX_REQUIRE(p.grad_y && p.h && p.weight, "grad_y / h / weight is NULL");
-  PPLX_REQUIRE(is_aligned(p.weight, 16), "weight must be 16-byte aligned");
+  PPLX_REQUIRE(p.weight && is_aligned(p.weight, 16), "weight is NULL or not 16-byte aligned");
   PPLX_REQUIRE(is_aligned(p.grad_weight, 16), "grad_weight must be 16-byte aligned");
   PPLX_REQUIRE(!p.grad_weight || (p.workspace && is_aligned(p.workspace, 16)), "workspace is NULL or not aligned");
   PPLX_ROWS(p, grad_y);

@@ -578,12 +578,13 @@ template <class T, int PER> __global__ __launch_bounds__(64 * kTokensAtOnce) voi
   }
 }
 
-int check_picks(int32_t dtype, uint32_t experts, uint32_t picks, int32_t scores, float scale) {
+int check_picks(int32_t dtype, uint32_t m, uint32_t experts, uint32_t picks, int32_t scores, float scale) {
   PPLX_REQUIRE(is_dtype(dtype), "unsupported dtype of the logits");
   PPLX_REQUIRE(experts >= 1 && experts <= kMaxExperts, "num_experts must be in [1, %u]", kMaxExperts);
   PPLX_REQUIRE(picks >= 1 && picks <= 64 && picks <= experts, "experts_per_token must be in [1, 64] and at most num_experts");
   PPLX_REQUIRE(scores == PPLX_A2A_SOFTMAX || scores == PPLX_A2A_SIGMOID, "unknown scores");
   PPLX_REQUIRE(std::isfinite(scale), "weight_scale must be finite");
+  if (m > kMaxTokens) return refuse(PPLX_A2A_UNSUPPORTED, "2^31 tokens or more");
   return PPLX_A2A_OK;
 }
 
@@ -595,7 +596,7 @@ using namespace pplx_amd;
 extern "C" int pplx_a2a_route_tokens(int device, const pplx_a2a_route_args_t *args, void *stream) {
   PPLX_REQUIRE(args, "args is NULL");
   const pplx_a2a_route_args_t &p = *args;
-  const int st = check_picks(p.dtype, p.num_experts, p.experts_per_token, p.scores, p.weight_scale);
+  const int st = check_picks(p.dtype, p.m, p.num_experts, p.experts_per_token, p.scores, p.weight_scale);
   if (st) return st;
   PPLX_REQUIRE(p.num_groups >= 1 && p.num_experts % p.num_groups == 0, "num_groups must divide num_experts");
   PPLX_REQUIRE(p.top_groups >= 1 && p.top_groups <= p.num_groups, "top_groups must be in [1, num_groups]");
@@ -673,7 +674,7 @@ extern "C" int pplx_a2a_route_tokens(int device, const pplx_a2a_route_args_t *ar
 extern "C" int pplx_a2a_route_tokens_backward(int device, const pplx_a2a_route_backward_args_t *args, void *stream) {
   PPLX_REQUIRE(args, "args is NULL");
   const pplx_a2a_route_backward_args_t &p = *args;
-  const int st = check_picks(p.dtype, p.num_experts, p.experts_per_token, p.scores, p.weight_scale);
+  const int st = check_picks(p.dtype, p.m, p.num_experts, p.experts_per_token, p.scores, p.weight_scale);
   if (st) return st;
   if (p.m == 0) return PPLX_A2A_OK;
   PPLX_REQUIRE(p.grad_weights && p.logits && p.indices && p.grad_logits, "grad_weights / logits / indices / grad_logits is NULL");

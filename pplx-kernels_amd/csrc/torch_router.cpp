@@ -48,7 +48,15 @@ float as_float(double v) { return (float)v; }
 
 // Bytes for a call's own use, which go back to torch's allocator with the call: a later one on the same stream may have them,
 // and a captured one has them to itself.
-at::Tensor space(uint64_t bytes, const at::Tensor &with) { return fresh({(int64_t)bytes}, with, at::kByte); }
+// `given`, or memory of torch's allocator, which a capture by torch keeps in its graph's pool.
+at::Tensor space(uint64_t bytes, const at::Tensor &with, const at::Tensor *given, std::initializer_list<const at::Tensor *> others) {
+  if (!given) return fresh({(int64_t)bytes}, with, at::kByte);
+  check_dense(*given, at::kByte, 1, with, "workspace");
+  TORCH_CHECK((uint64_t)given->numel() >= bytes, "the workspace has fewer than ", bytes, " bytes");
+  TORCH_CHECK(bytes == 0 || reinterpret_cast<uintptr_t>(given->data_ptr()) % 16 == 0, "workspace must be 16-byte aligned");
+  if (bytes) check_written(*given, "workspace", others);
+  return *given;
+}
 
 // ---------------------------------------------------------------------------
 // The operators on tensors of the caller
@@ -121,7 +129,7 @@ void rms_norm(const at::Tensor *y, const at::Tensor *sum, const at::Tensor *q, c
 }
 
 void rms_norm_backward(const at::Tensor *grad_h, const at::Tensor *grad_weight, const at::Tensor &grad_y, const at::Tensor *grad_sum,
-                       const at::Tensor &h, const at::Tensor &weight, double eps) {
+                       const at::Tensor &h, const at::Tensor &weight, double eps, const at::Tensor *workspace) {
   check_matrix(h, "h");
   check_weight_type(weight, h);
   check_dense(weight, weight.scalar_type(), 1, h, "weight");
@@ -165,7 +173,7 @@ void rms_norm_backward(const at::Tensor *grad_h, const at::Tensor *grad_weight, 
   if (grad_weight) {
     uint64_t bytes = 0;
     A2A_CHECK(pplx_a2a_rms_norm_workspace(m, a.hidden_dim, &bytes));
-    work = space(bytes, h);
+    work = space(bytes, h, workspace, {&grad_y, grad_sum, &h, &weight, grad_h, grad_weight});
     a.grad_weight = grad_weight->data_ptr();
     a.workspace = work.data_ptr();
   }
@@ -183,7 +191,7 @@ void check_router(const at::Tensor &x, const at::Tensor &weight) {
   TORCH_CHECK(weight.sizes()[0] <= UINT32_MAX, "pplx_kernels: invalid argument: number of experts");
 }
 
-void router_logits(const at::Tensor &logits, const at::Tensor &x, const at::Tensor &weight) {
+void router_logits(const at::Tensor &logits, const at::Tensor &x, const at::Tensor &weight, const at::Tensor *workspace) {
   check_router(x, weight);
   check_on(logits, x, "logits");
   check_lines(logits, "logits");
@@ -207,7 +215,7 @@ void router_logits(const at::Tensor &logits, const at::Tensor &x, const at::Tens
   A2A_CHECK(pplx_a2a_router_workspace(a.m, a.num_experts, a.hidden_dim, a.dtype, a.weight_dtype, 0, &bytes));
   at::Tensor work;
   if (bytes) {
-    work = space(bytes, x);
+    work = space(bytes, x, workspace, {&x, &weight, &logits});
     a.workspace = work.data_ptr();
   }
   A2A_CHECK(pplx_a2a_router_logits(x.device().index(), &a, current_stream_of(x)));
@@ -215,7 +223,7 @@ void router_logits(const at::Tensor &logits, const at::Tensor &x, const at::Tens
 }
 
 void router_logits_backward(const at::Tensor *grad_x, const at::Tensor *grad_weight, const at::Tensor &grad_logits,
-                            const at::Tensor &x, const at::Tensor &weight) {
+                            const at::Tensor &x, const at::Tensor &weight, const at::Tensor *workspace) {
   check_router(x, weight);
   check_on(grad_logits, x, "grad_logits");
   check_lines(grad_logits, "grad_logits");
@@ -257,7 +265,7 @@ void router_logits_backward(const at::Tensor *grad_x, const at::Tensor *grad_wei
   }
   uint64_t bytes = 0;
   A2A_CHECK(pplx_a2a_router_workspace(m, a.num_experts, a.hidden_dim, a.dtype, a.weight_dtype, 1, &bytes));
-  const at::Tensor work = space(bytes, x);
+  const at::Tensor work = space(bytes, x, workspace, {&grad_logits, &x, &weight, grad_x, grad_weight});
   a.workspace = work.data_ptr();
   A2A_CHECK(pplx_a2a_router_logits_backward(x.device().index(), &a, current_stream_of(x)));
   if (grad_x) written(*grad_x);
@@ -352,13 +360,15 @@ void rms_norm_op(opt_tensor y, opt_tensor sum, opt_tensor q, opt_tensor scale, c
   rms_norm(opt(y), opt(sum), opt(q), opt(scale), x, weight, opt(residual), eps);
 }
 void rms_norm_backward_op(opt_tensor grad_h, opt_tensor grad_weight, const at::Tensor &grad_y, opt_tensor grad_sum,
-                          const at::Tensor &h, const at::Tensor &weight, double eps) {
-  rms_norm_backward(opt(grad_h), opt(grad_weight), grad_y, opt(grad_sum), h, weight, eps);
+                          const at::Tensor &h, const at::Tensor &weight, double eps, opt_tensor workspace) {
+  rms_norm_backward(opt(grad_h), opt(grad_weight), grad_y, opt(grad_sum), h, weight, eps, opt(workspace));
 }
-void router_logits_op(at::Tensor &logits, const at::Tensor &x, const at::Tensor &weight) { router_logits(logits, x, weight); }
+void router_logits_op(at::Tensor &logits, const at::Tensor &x, const at::Tensor &weight, opt_tensor workspace) {
+  router_logits(logits, x, weight, opt(workspace));
+}
 void router_logits_backward_op(opt_tensor grad_x, opt_tensor grad_weight, const at::Tensor &grad_logits, const at::Tensor &x,
-                               const at::Tensor &weight) {
-  router_logits_backward(opt(grad_x), opt(grad_weight), grad_logits, x, weight);
+                               const at::Tensor &weight, opt_tensor workspace) {
+  router_logits_backward(opt(grad_x), opt(grad_weight), grad_logits, x, weight, opt(workspace));
 }
 void route_tokens_op(at::Tensor &indices, at::Tensor &weights, const at::Tensor &logits, opt_tensor bias, opt_tensor bound_m,
                      int64_t num_groups, int64_t top_groups, int64_t group_top, bool sigmoid, bool renormalize, double scale) {
@@ -418,7 +428,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
       if (ctx->needs_input_grad(1)) grad_weight = fresh_traced(weight.sym_sizes(), weight, weight.scalar_type());
       op.call(if_defined(grad_h), if_defined(grad_weight), as_rows(grads[0]),
               grads[1].defined() ? std::optional<at::Tensor>(as_rows(grads[1])) : std::nullopt, h, weight,
-              ctx->saved_data["eps"].toDouble());
+              ctx->saved_data["eps"].toDouble(), std::nullopt);
     } else if (grads[1].defined()) {
       grad_h = grads[1];  // (of the sum alone)
     }
@@ -437,7 +447,7 @@ at::Tensor new_logits_op(const at::Tensor &x, const at::Tensor &weight) {
   TORCH_CHECK(x.dim() == 2, "Tensor x must be 2 dimensional");
   TORCH_CHECK(weight.dim() == 2, "Tensor weight must be 2 dimensional");
   const at::Tensor logits = fresh({x.sizes()[0], weight.sizes()[0]}, x, at::kFloat);
-  router_logits(logits, x, weight);
+  router_logits(logits, x, weight, nullptr);
   return logits;
 }
 at::Tensor new_logits_meta(const at::Tensor &x, const at::Tensor &weight) {
@@ -470,7 +480,7 @@ struct LogitsFunction : torch::autograd::Function<LogitsFunction> {
       static auto op = op_handle<decltype(router_logits_backward_op)>("pplx_kernels::router_logits_backward");
       if (ctx->needs_input_grad(0)) grad_x = fresh_traced(x.sym_sizes(), x, x.scalar_type());
       if (ctx->needs_input_grad(1)) grad_weight = fresh_traced(weight.sym_sizes(), weight, weight.scalar_type());
-      op.call(if_defined(grad_x), if_defined(grad_weight), as_lines(grads[0]), x, weight);
+      op.call(if_defined(grad_x), if_defined(grad_weight), as_lines(grads[0]), x, weight, std::nullopt);
     }
     return differentiable_once({grad_x, grad_weight}, kDifferentiable);
   }
@@ -556,11 +566,13 @@ TORCH_LIBRARY_FRAGMENT(pplx_kernels, m) {
          "(Tensor!? y, Tensor!? sum, Tensor!? q, Tensor!? scale, Tensor x, Tensor weight, Tensor? residual, float eps) -> ()",
          &rms_norm_op);
   define(m, "rms_norm_backward",
-         "(Tensor!? grad_h, Tensor!? grad_weight, Tensor grad_y, Tensor? grad_sum, Tensor h, Tensor weight, float eps) -> ()",
+         "(Tensor!? grad_h, Tensor!? grad_weight, Tensor grad_y, Tensor? grad_sum, Tensor h, Tensor weight, float eps, "
+         "Tensor!? workspace) -> ()",
          &rms_norm_backward_op);
-  define(m, "router_logits", "(Tensor! logits, Tensor x, Tensor weight) -> ()", &router_logits_op);
+  define(m, "router_logits", "(Tensor! logits, Tensor x, Tensor weight, Tensor!? workspace) -> ()", &router_logits_op);
   define(m, "router_logits_backward",
-         "(Tensor!? grad_x, Tensor!? grad_weight, Tensor grad_logits, Tensor x, Tensor weight) -> ()", &router_logits_backward_op);
+         "(Tensor!? grad_x, Tensor!? grad_weight, Tensor grad_logits, Tensor x, Tensor weight, Tensor!? workspace) -> ()",
+         &router_logits_backward_op);
   define(m, "route_tokens",
          "(Tensor! indices, Tensor! weights, Tensor logits, Tensor? bias, Tensor? bound_m, int num_groups, int top_groups, "
          "int group_top, bool sigmoid, bool renormalize, float scale) -> ()",
@@ -590,6 +602,11 @@ double float_arg(PyObject *obj, const char *name) {
     TORCH_CHECK_TYPE(false, name, " must be a float, not ", Py_TYPE(obj)->tp_name);
   }
   return v;
+}
+uint64_t count_arg(PyObject *obj, const char *name) {
+  const int64_t v = int_arg(obj, name);
+  TORCH_CHECK(v >= 0 && v < (1ll << 31), "pplx_kernels: invalid argument: ", name, " out of range");
+  return (uint64_t)v;
 }
 bool bool_arg(PyObject *obj) { return PyObject_IsTrue(obj) == 1; }
 
@@ -640,35 +657,66 @@ PyObject *py_normed_rows(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// rms_norm_backward(grad_h, grad_weight, grad_y, grad_sum, h, weight, eps)
+// quantized_rows(x, weight, residual, eps, int8) -> (y, sum, q, scale): rows in int8, or else e4m3
+PyObject *py_quantized_rows(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  arity("quantized_rows", nargs, 5);
+  const at::Tensor &x = tensor_arg(args[0], "x"), &weight = tensor_arg(args[1], "weight");
+  const at::Tensor *residual = optional_tensor_arg(args[2], "residual");
+  const double eps = float_arg(args[3], "eps");
+  const bool int8 = bool_arg(args[4]);
+  TORCH_CHECK(x.dim() == 2, "Tensor x must be 2 dimensional");
+  const c10::SymInt m = x.sym_size(0), h = x.sym_size(1);
+  const at::Tensor y = fresh_traced({m, h}, x, x.scalar_type());
+  const at::Tensor sum = residual ? fresh_traced({m, h}, x, x.scalar_type()) : at::Tensor();
+  const at::Tensor q = fresh_traced({m, h}, x, int8 ? at::kChar : at::kFloat8_e4m3fn);
+  const at::Tensor scale = int8 ? fresh_traced({m}, x, at::kFloat) : fresh_traced({m, (h + (kBlock - 1)) / kBlock}, x, at::kFloat);
+  if (straight({&x, &weight, residual})) {
+    rms_norm(&y, defined(sum), &q, &scale, x, weight, residual, eps);
+  } else {
+    static auto op = op_handle<decltype(rms_norm_op)>("pplx_kernels::rms_norm");
+    op.call(y, if_defined(sum), q, scale, x, weight, maybe(residual), eps);
+  }
+  PyObject *out = PyTuple_New(4);
+  if (!out) throw python_error();
+  PyTuple_SET_ITEM(out, 0, wrap_or_none(y));
+  PyTuple_SET_ITEM(out, 1, wrap_or_none(sum));
+  PyTuple_SET_ITEM(out, 2, wrap_or_none(q));
+  PyTuple_SET_ITEM(out, 3, wrap_or_none(scale));
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
+// rms_norm_backward(grad_h, grad_weight, grad_y, grad_sum, h, weight, eps, workspace)
 PyObject *py_rms_norm_backward(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  arity("rms_norm_backward", nargs, 7);
+  arity("rms_norm_backward", nargs, 8);
   const at::Tensor *grad_h = optional_tensor_arg(args[0], "grad_h"), *grad_weight = optional_tensor_arg(args[1], "grad_weight"),
-                   *grad_sum = optional_tensor_arg(args[3], "grad_sum");
+                   *grad_sum = optional_tensor_arg(args[3], "grad_sum"), *workspace = optional_tensor_arg(args[7], "workspace");
   const at::Tensor &grad_y = tensor_arg(args[2], "grad_y"), &h = tensor_arg(args[4], "h"), &weight = tensor_arg(args[5], "weight");
   const double eps = float_arg(args[6], "eps");
-  if (straight({grad_h, grad_weight, &grad_y, grad_sum, &h, &weight})) {
-    rms_norm_backward(grad_h, grad_weight, grad_y, grad_sum, h, weight, eps);
+  if (straight({grad_h, grad_weight, &grad_y, grad_sum, &h, &weight, workspace})) {
+    rms_norm_backward(grad_h, grad_weight, grad_y, grad_sum, h, weight, eps, workspace);
   } else {
     static auto op = op_handle<decltype(rms_norm_backward_op)>("pplx_kernels::rms_norm_backward");
-    op.call(maybe(grad_h), maybe(grad_weight), grad_y, maybe(grad_sum), h, weight, eps);
+    op.call(maybe(grad_h), maybe(grad_weight), grad_y, maybe(grad_sum), h, weight, eps, maybe(workspace));
   }
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
 
-// router_logits(logits, x, weight)
+// router_logits(logits, x, weight, workspace)
 PyObject *py_router_logits(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  arity("router_logits", nargs, 3);
+  arity("router_logits", nargs, 4);
   const at::Tensor &logits = tensor_arg(args[0], "logits"), &x = tensor_arg(args[1], "x"), &weight = tensor_arg(args[2], "weight");
-  if (straight({&logits, &x, &weight})) {
-    router_logits(logits, x, weight);
+  const at::Tensor *workspace = optional_tensor_arg(args[3], "workspace");
+  if (straight({&logits, &x, &weight, workspace})) {
+    router_logits(logits, x, weight, workspace);
   } else {
     static auto op = op_handle<decltype(router_logits_op)>("pplx_kernels::router_logits");
     at::Tensor to = logits;
-    op.call(to, x, weight);
+    op.call(to, x, weight, maybe(workspace));
   }
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
@@ -686,19 +734,43 @@ PyObject *py_new_logits(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// router_logits_backward(grad_x, grad_weight, grad_logits, x, weight)
+// router_logits_backward(grad_x, grad_weight, grad_logits, x, weight, workspace)
 PyObject *py_router_logits_backward(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  arity("router_logits_backward", nargs, 5);
-  const at::Tensor *grad_x = optional_tensor_arg(args[0], "grad_x"), *grad_weight = optional_tensor_arg(args[1], "grad_weight");
+  arity("router_logits_backward", nargs, 6);
+  const at::Tensor *grad_x = optional_tensor_arg(args[0], "grad_x"), *grad_weight = optional_tensor_arg(args[1], "grad_weight"),
+                   *workspace = optional_tensor_arg(args[5], "workspace");
   const at::Tensor &grad_logits = tensor_arg(args[2], "grad_logits"), &x = tensor_arg(args[3], "x"), &weight = tensor_arg(args[4], "weight");
-  if (straight({grad_x, grad_weight, &grad_logits, &x, &weight})) {
-    router_logits_backward(grad_x, grad_weight, grad_logits, x, weight);
+  if (straight({grad_x, grad_weight, &grad_logits, &x, &weight, workspace})) {
+    router_logits_backward(grad_x, grad_weight, grad_logits, x, weight, workspace);
   } else {
     static auto op = op_handle<decltype(router_logits_backward_op)>("pplx_kernels::router_logits_backward");
-    op.call(maybe(grad_x), maybe(grad_weight), grad_logits, x, weight);
+    op.call(maybe(grad_x), maybe(grad_weight), grad_logits, x, weight, maybe(workspace));
   }
   Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+// rms_norm_workspace(tokens, width) -> bytes that its gradients take
+PyObject *py_rms_norm_workspace(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  arity("rms_norm_workspace", nargs, 2);
+  uint64_t bytes = 0;
+  A2A_CHECK(pplx_a2a_rms_norm_workspace((uint32_t)count_arg(args[0], "tokens"), count_arg(args[1], "width"), &bytes));
+  return PyLong_FromUnsignedLongLong(bytes);
+  END_HANDLE_TH_ERRORS
+}
+
+// router_workspace(x, weight, backward) -> bytes
+PyObject *py_router_workspace(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  arity("router_workspace", nargs, 3);
+  const at::Tensor &x = tensor_arg(args[0], "x"), &weight = tensor_arg(args[1], "weight");
+  check_router(x, weight);
+  uint64_t bytes = 0;
+  A2A_CHECK(pplx_a2a_router_workspace(tokens_of(x), (uint32_t)weight.sizes()[0], (uint64_t)x.sizes()[1], dtype_code(x.scalar_type()),
+                                      dtype_code(weight.scalar_type()), bool_arg(args[2]), &bytes));
+  return PyLong_FromUnsignedLongLong(bytes);
   END_HANDLE_TH_ERRORS
 }
 
@@ -775,12 +847,15 @@ PyObject *py_router_build_id(PyObject *, PyObject *) { return PyUnicode_FromStri
 PyMethodDef kRouterMethods[] = {
     {"rms_norm", PPLX_FASTCALL(py_rms_norm), "rms_norm(y, sum, q, scale, x, weight, residual, eps)"},
     {"normed_rows", PPLX_FASTCALL(py_normed_rows), "normed_rows(x, weight, residual, eps, record) -> (y, sum)"},
+    {"quantized_rows", PPLX_FASTCALL(py_quantized_rows), "quantized_rows(x, weight, residual, eps, int8) -> (y, sum, q, scale)"},
     {"rms_norm_backward", PPLX_FASTCALL(py_rms_norm_backward),
-     "rms_norm_backward(grad_h, grad_weight, grad_y, grad_sum, h, weight, eps)"},
-    {"router_logits", PPLX_FASTCALL(py_router_logits), "router_logits(logits, x, weight)"},
+     "rms_norm_backward(grad_h, grad_weight, grad_y, grad_sum, h, weight, eps, workspace)"},
+    {"rms_norm_workspace", PPLX_FASTCALL(py_rms_norm_workspace), "rms_norm_workspace(tokens, width) -> bytes that its gradients take"},
+    {"router_logits", PPLX_FASTCALL(py_router_logits), "router_logits(logits, x, weight, workspace)"},
     {"new_logits", PPLX_FASTCALL(py_new_logits), "new_logits(x, weight, record) -> logits"},
     {"router_logits_backward", PPLX_FASTCALL(py_router_logits_backward),
-     "router_logits_backward(grad_x, grad_weight, grad_logits, x, weight)"},
+     "router_logits_backward(grad_x, grad_weight, grad_logits, x, weight, workspace)"},
+    {"router_workspace", PPLX_FASTCALL(py_router_workspace), "router_workspace(x, weight, backward) -> bytes"},
     {"route_tokens", PPLX_FASTCALL(py_route_tokens),
      "route_tokens(indices, weights, logits, bias, bound_m, num_groups, top_groups, group_top, sigmoid, renormalize, scale)"},
     {"routed_tokens", PPLX_FASTCALL(py_routed_tokens),

@@ -17,7 +17,9 @@ from .loopback import LoopbackWorld as LoopbackWorld
 from .router import NormedRows as NormedRows
 from .router import rms_norm as rms_norm
 from .router import rms_norm_backward as rms_norm_backward
+from .router import rms_norm_workspace as rms_norm_workspace
 from .router import route_tokens as route_tokens
 from .router import route_tokens_backward as route_tokens_backward
 from .router import router_logits as router_logits
 from .router import router_logits_backward as router_logits_backward
+from .router import router_workspace as router_workspace

@@ -73,8 +73,7 @@ def _wants_grad(*tensors: torch.Tensor | None) -> bool:
 def _check_recording(x: torch.Tensor) -> None:
     if x.is_cuda and torch.cuda.is_current_stream_capturing():
         raise RuntimeError(
-            "pplx_kernels: gradients are not recorded under stream capture: capture sort_tokens_backward and "
-            "unsort_tokens_backward, under torch.no_grad()"
+            "pplx_kernels: gradients are not recorded under stream capture: capture the _backward functions, under torch.no_grad()"
         )
 
 

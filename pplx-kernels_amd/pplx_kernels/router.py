@@ -8,9 +8,9 @@ experts with its weights, with the gradients of all three.
 
 A rank that holds its experts itself gives ``indices`` and ``weights`` to ``sort_tokens`` and ``unsort_tokens``; all of it is
 differentiable, so the same calls make a training step.  Calls run on the current stream of the tensors' device and keep nothing
-between calls.  With ``out=`` a call makes no results and can be captured as it is; the gradients of :func:`rms_norm` and
-:func:`router_logits`, and products of large batches, take workspace from torch's allocator.  Gradients are those of reverse mode;
-under capture they go through the ``_backward`` functions.
+between calls.  With ``out=``, and ``workspace=`` where there is one, a call allocates nothing and can be captured as it is; without
+``workspace`` it takes that from torch's allocator, which keeps it for a graph that torch captures, not for one that
+``LoopbackWorld.capture`` does.  Gradients are those of reverse mode; under capture they go through the ``_backward`` functions.
 """
 
 from __future__ import annotations
@@ -55,11 +55,15 @@ class NormedRows(NamedTuple):
         )
 
 
+def _check_quantize(quantize):
+    if quantize not in (torch.int8, torch.float8_e4m3fn):
+        raise RuntimeError("pplx_kernels: quantize must be torch.int8 or torch.float8_e4m3fn")
+
+
 def _quantized(shape, device, quantize):
     if quantize is None:
         return None, None
-    if quantize not in (torch.int8, torch.float8_e4m3fn):
-        raise RuntimeError("pplx_kernels: quantize must be torch.int8 or torch.float8_e4m3fn")
+    _check_quantize(quantize)
     of_scale = shape[:1] if quantize == torch.int8 else (shape[0], (shape[1] + BLOCK - 1) // BLOCK)
     return (
         torch.empty(shape, dtype=quantize, device=device),
@@ -93,16 +97,13 @@ def rms_norm(
         fn(out.y, out.sum, out.q, out.scale, x, weight, residual, eps)
         return out
     if quantize is not None:
+        _check_quantize(quantize)
         x, weight, residual = (t if t is None or not t.requires_grad else t.detach() for t in (x, weight, residual))
+        if not _is_compiling():
+            return NormedRows._make(_C.quantized_rows(x, weight, residual, eps, quantize == torch.int8))
         if x.dim() != 2:
             raise RuntimeError("Tensor x must be 2 dimensional")
-        q, scale = _quantized(x.shape, x.device, quantize)
-        made = NormedRows(
-            torch.empty_like(x, memory_format=torch.contiguous_format),
-            None if residual is None else torch.empty_like(x, memory_format=torch.contiguous_format),
-            q,
-            scale,
-        )
+        made = NormedRows.empty(*x.shape, x.dtype, x.device, residual=residual is not None, quantize=quantize)
         return rms_norm(x, weight, residual, eps=eps, out=made)
     if _is_compiling():
         y, total = _ops.normed_rows(x, weight, residual, eps)
@@ -121,26 +122,38 @@ def rms_norm_backward(
     grad_sum: torch.Tensor | None = None,
     eps: float = 1e-6,
     out: tuple[torch.Tensor | None, torch.Tensor | None] | None = None,
+    workspace: torch.Tensor | None = None,
 ) -> tuple[torch.Tensor | None, torch.Tensor | None]:
     """The gradients of :func:`rms_norm`: that of ``h`` (``NormedRows.sum``, or ``x`` where there was no residual), which is that of
     ``x`` and of ``residual``, and that of ``weight``.  ``grad_sum`` is the gradient that came for ``sum`` itself.  In ``out`` either
-    may be None, which leaves it out; the first may be ``grad_y`` or ``grad_sum`` itself."""
+    may be None, which leaves it out; the first may be ``grad_y`` or ``grad_sum`` itself.  ``workspace`` is of
+    :func:`rms_norm_workspace`."""
     if out is None:
         out = torch.empty_like(h, memory_format=torch.contiguous_format), torch.empty_like(weight)
     fn = _ops.rms_norm_backward if _is_compiling() else _C.rms_norm_backward
-    fn(out[0], out[1], grad_y, grad_sum, h, weight, eps)
+    fn(out[0], out[1], grad_y, grad_sum, h, weight, eps, workspace)
     return out
 
 
-def router_logits(x: torch.Tensor, weight: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
+def rms_norm_workspace(h: torch.Tensor) -> torch.Tensor:
+    """What :func:`rms_norm_backward` of ``h`` writes besides its results: for one call at a time."""
+    return torch.empty(_C.rms_norm_workspace(*h.shape), dtype=torch.uint8, device=h.device)
+
+
+def router_logits(
+    x: torch.Tensor, weight: torch.Tensor, *, out: torch.Tensor | None = None, workspace: torch.Tensor | None = None
+) -> torch.Tensor:
     """``x @ weight.T`` in float32: products of 16-bit elements are exact, those of float32 count to 24 bits, and sums are float32.
 
     ``x`` is ``[m, H]`` of float32, bfloat16 or float16 and ``weight`` ``[experts, H]`` of its type or float32, both with rows that
-    are 16-byte aligned and ``H`` a multiple of 8.  Differentiable in both unless ``out`` is given."""
+    are 16-byte aligned and ``H`` a multiple of 8.  Differentiable in both unless ``out`` is given, with which ``workspace`` may be
+    given too, of :func:`router_workspace`."""
     if out is not None:
         fn = _ops.router_logits if _is_compiling() else _C.router_logits
-        fn(out, x, weight)
+        fn(out, x, weight, workspace)
         return out
+    if workspace is not None:
+        raise RuntimeError("pplx_kernels: workspace goes with out")
     if _is_compiling():
         return _ops.new_logits(x, weight)
     record = _wants_grad(x, weight)
@@ -155,18 +168,24 @@ def router_logits_backward(
     weight: torch.Tensor,
     *,
     out: tuple[torch.Tensor | None, torch.Tensor | None] | None = None,
+    workspace: torch.Tensor | None = None,
 ) -> tuple[torch.Tensor | None, torch.Tensor | None]:
     """The gradients of :func:`router_logits`: ``grad_logits @ weight`` and ``grad_logits.T @ x``, added up in float32 and rounded
     once.  For 16-bit results ``grad_logits`` (and the other operand, unless it is bfloat16) counts to 2**-18 of each value, for
-    float32 to 24 bits.  In ``out`` either may be None, which leaves it out."""
+    float32 to 24 bits.  In ``out`` either may be None, which leaves it out.  ``workspace`` is of :func:`router_workspace`."""
     if out is None:
         out = (
             torch.empty_like(x, memory_format=torch.contiguous_format),
             torch.empty_like(weight, memory_format=torch.contiguous_format),
         )
     fn = _ops.router_logits_backward if _is_compiling() else _C.router_logits_backward
-    fn(out[0], out[1], grad_logits, x, weight)
+    fn(out[0], out[1], grad_logits, x, weight, workspace)
     return out
+
+
+def router_workspace(x: torch.Tensor, weight: torch.Tensor, *, backward: bool = False) -> torch.Tensor:
+    """What :func:`router_logits`, or its gradients, write besides their results (nothing for some sizes): for one call at a time."""
+    return torch.empty(_C.router_workspace(x, weight, backward), dtype=torch.uint8, device=x.device)
 
 
 def _is_sigmoid(scores: str) -> bool:
@@ -227,8 +246,8 @@ def route_tokens_backward(
     scale: float = 1.0,
     out: torch.Tensor | None = None,
 ) -> torch.Tensor:
-    """The gradient of the weights of :func:`route_tokens` with respect to ``logits``, for the picks in ``indices`` that it made.  Every
-    logit's is written, zeros where there is none."""
+    """The gradient of the weights of :func:`route_tokens` with respect to ``logits``, for the picks in ``indices`` that it made (no
+    expert twice in a token).  Every logit's is written, zeros where there is none."""
     if out is None:
         out = torch.empty_like(logits, memory_format=torch.contiguous_format)
     fn = _ops.route_tokens_backward if _is_compiling() else _C.route_tokens_backward
