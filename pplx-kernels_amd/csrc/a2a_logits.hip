@@ -656,14 +656,23 @@ template <class K> void allow_lds(K *kernel, uint32_t bytes) {
 //                   16384 x 64 x 4096  32.0 (1) / 37.5 (4)   256 x 256 x 7168  9.4 (16) / 11.9 (16)   64 x 256 x 7168   7.6 (28) / 9.0 (28)
 //   bf16, fp32      8192 x 256 x 7168  199 (2) / 97.7 (2)    64 x 256 x 7168   9.9 (56) / 11.1 (56)
 //   both fp32       4096 x 256 x 7168  144 (4) / 101 (4)     64 x 256 x 7168  10.9 (56) / 14.5 (56)
-// Tiles of 64 x 128, 64 x 256, 32 x 64 and 32 x 128 were within 5 % of the better of the two, or slower, in all of twenty products.
+// and 128 x 192, for 16-bit operands, beside 128 x 128:
+//   both bf16       16384 x 384 x 7168  91 (1) / 143 (1)     8192 x 384 x 7168  57.6 (2) / 72.2 (1)   4096 x 384 x 7168  36.2 (4) / 42.2 (2)   1024 x 384 x 7168  21.4 (14) / 19.7 (8)
+//                   3001 x 384 x 7168  32.2 (4) / 32.8 (3)
+// What bounds a tile of 128 x 128 is what a compute unit fetches into its LDS, 31 bytes a cycle: 0.43 us a step with rows in L2, and
+// 0.63 with rows out of HBM, whose latency its four steps do not cover.  Larger tiles fetch less and hold fewer steps: 128 x 256 and
+// 256 x 128 take 1.1 us a step, 256 x 256 1.4.  Tiles of 64 x 128, 64 x 256, 32 x 64 and 32 x 128 were within 5 % of the better of the
+// first two, or slower, in all of twenty products.
 // product_split, which is one launch: 4 x 64 x 2048 4.3 (tiles 5.8), 1 x 256 x 7168 9.5 (6.5), 64 x 256 x 7168 14.2, with fp32
 // weights 20.9: its loads take a cycle for each row of 64 bytes, whatever else is under way.
 struct LogitsForm {
   uint32_t bm, bn;
+  double start;        // beside the others' 3 us
   double per_step[4];  // 16-bit operands; bf16 and fp32; fp16 and fp32; fp32
 };
-constexpr LogitsForm kForms[] = {{64, 64, {0.25, 0.87, 1.1, 1.3}}, {128, 128, {0.66, 1.6, 2.55, 3.3}}};
+constexpr double kNever = 1e9;
+constexpr LogitsForm kForms[] = {
+    {64, 64, 0, {0.25, 0.87, 1.1, 1.3}}, {128, 128, 0, {0.66, 1.6, 2.55, 3.3}}, {128, 192, 1.5, {0.85, kNever, kNever, kNever}}};
 struct LogitsPlan {
   int form = -1;  // -1: product_split
   uint32_t splits = 1, steps_per_split = 0;
@@ -682,11 +691,11 @@ LogitsPlan plan_logits(uint64_t m, uint64_t experts, uint64_t hidden, int32_t dt
     const LogitsForm &form = kForms[f];
     const uint64_t tiles = ceil_div(m, form.bm) * ceil_div(experts, form.bn);
     if (tiles >= (1ull << 28)) continue;
-    for (uint64_t per = steps; per >= 1; per = per > 16 ? per * 3 / 4 : per - 1) {
-      const uint64_t splits = ceil_div(steps, per), bytes = splits > 1 ? 4 * splits * m * sums_width(experts) : 0;
+    for (uint64_t most = steps; most >= 1; most = most > 16 ? most * 3 / 4 : most - 1) {
+      const uint64_t splits = ceil_div(steps, most), per = ceil_div(steps, splits), bytes = splits > 1 ? 4 * splits * m * sums_width(experts) : 0;
       if (splits > 64 || bytes > (512ull << 20)) break;
       const double rounds = std::ceil((double)(tiles * splits) / kComputeUnits);
-      const double cost = (kind == 0 ? 3.0 : 3.6) + rounds * (double)per * form.per_step[kind] +
+      const double cost = (kind == 0 ? 3.0 : 3.6) + form.start + rounds * (double)per * form.per_step[kind] +
                           (splits > 1 ? 2.2 + 0.02 * (double)splits + (double)bytes / 5.5e6 : 0.0);
       if (cost < least) {
         least = cost;
@@ -729,6 +738,9 @@ template <class T, class W, int BM, int BN, int WM, int WN, int STAGES> int laun
 }
 template <class T, class W> int launch_form(int form, const TilesDev &a, hipStream_t s) {
   if (form == 0) return launch_tiles<T, W, 64, 64, 2, 2, 4>(a, s);
+  if constexpr (sizeof(W) == 2) {
+    if (form == 2) return launch_tiles<T, W, 128, 192, 2, 2, 3>(a, s);
+  }
   return launch_tiles<T, W, 128, 128, 2, 4, sizeof(W) == 2 ? 4 : 2>(a, s);
 }
 
@@ -750,8 +762,8 @@ WeightShares weight_shares(uint64_t m, uint64_t experts, uint64_t hidden, uint32
   w.row_blocks = (uint32_t)ceil_div(experts, 32 * w.waves);
   const uint64_t step = 16 * w.waves, steps = ceil_div(m, step), blocks = ceil_div(hidden, columns) * w.row_blocks;
   double least = 0;
-  for (uint64_t per = steps; per >= 1; per = per > 8 ? per * 7 / 8 : per - 1) {
-    const uint64_t parts = ceil_div(steps, per);
+  for (uint64_t most = steps; most >= 1; most = most > 8 ? most * 7 / 8 : most - 1) {
+    const uint64_t parts = ceil_div(steps, most), per = ceil_div(steps, parts);
     if (parts > 32) break;
     const double rounds = std::ceil((double)(blocks * parts) / kComputeUnits);
     const double cost = rounds * ((double)per * (w.waves == 8 ? 3.2 : 1.2) + 2.0) + (parts > 1 ? 2.0 + (double)(parts * experts * hidden) * 8 / 6e6 : 0.0);
@@ -786,8 +798,8 @@ template <class T, class W> int launch_gradient_of_rows(GradientDev a, hipStream
   // Workgroups keep the weight's columns for as many rounds of rows as leaves no compute unit idle for long.
   const uint64_t rounds = ceil_div(a.rows, 32 * kGradientWaves);
   uint64_t least = 0;
-  for (uint64_t per = rounds; per >= 1; per = per > 8 ? per * 7 / 8 : per - 1) {
-    const uint64_t parts = ceil_div(rounds, per), cost = ceil_div(a.column_blocks * parts, kComputeUnits) * (per + 1);
+  for (uint64_t most = rounds; most >= 1; most = most > 8 ? most * 7 / 8 : most - 1) {
+    const uint64_t parts = ceil_div(rounds, most), per = ceil_div(rounds, parts), cost = ceil_div(a.column_blocks * parts, kComputeUnits) * (per + 1);
     if (a.parts == 0 || cost < least) {
       least = cost;
       a.parts = (uint32_t)parts;

@@ -317,6 +317,9 @@ LOGITS = [
     (515, 128, 328, BF16, BF16),
     (2050, 72, 136, F16, F16),
     (4100, 256, 200, BF16, BF16),
+    (16400, 300, 200, F16, F16),
+    (3001, 384, 7168, BF16, BF16),
+    (8200, 300, 2048, BF16, BF16),
     (1000, 300, 1024, BF16, F32),
     (0, 8, 64, BF16, BF16),
 ]
