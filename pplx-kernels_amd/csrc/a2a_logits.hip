@@ -596,44 +596,45 @@ __global__ __launch_bounds__(kGradientWaves * 64) void gradient_of_rows(Gradient
 
 // Of the weight: waves take 32 experts each, a workgroup all of a block of them, and go through the tokens sixteen for each wave at a
 // time: every wave turns sixteen of x, and all multiply with what the others turned.  Parts of the tokens add up in sum_splits.
-template <class TB, class O, int NV, int ORDER>
-__global__ __launch_bounds__(512) void gradient_of_weight(GradientDev a, uint32_t tokens_per_part, uint32_t row_blocks) {
+// Memory answers a wave in order: the fragments of a step are all under way before the rows of x that come after it.
+template <class TB, class O, int NV, int ORDER, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void gradient_of_weight(GradientDev a, uint32_t tokens_per_part, uint32_t row_blocks) {
   typedef Turned<TB, NV, ORDER> B;
   extern __shared__ __align__(16) uint8_t lds[];  // [2][waves][pieces][NV][64 lanes]
-  const uint32_t lane = lane_id(), wave = wave_id(), waves = blockDim.x / 64, half = lane / 32 * 8;
+  const uint32_t lane = lane_id(), wave = wave_id(), half = lane / 32 * 8;
   const uint32_t group = a.first_group + blockIdx.x;
   const uint32_t block = group / a.column_blocks, n0 = (group - block * a.column_blocks) * 32 * NV;
-  const uint32_t part = block / row_blocks, m0 = ((block - part * row_blocks) * waves + wave) * 32;
+  const uint32_t part = block / row_blocks, m0 = ((block - part * row_blocks) * WAVES + wave) * 32;
   const uint32_t column = n0 + lane % 32 * NV;
   const bool there = column < a.columns;
   const uint32_t begin = part * tokens_per_part, end = a.k - begin < tokens_per_part ? a.k : begin + tokens_per_part;
-  const uint32_t step = 16 * waves, size = waves * B::kBytes;
+  constexpr uint32_t step = 16 * WAVES, size = WAVES * B::kBytes;
   const uint32_t all = (a.k + 15) / 16, first = begin / 16;
   const FragmentPtr from = as_global(reinterpret_cast<const bf16x8 *>(a.a)) + (uint64_t)(m0 < a.rows ? m0 / 32 : 0) * all * (64 * (ORDER + 1)) + lane;
   auto left_at = [&](uint32_t k) { return k < end ? end - k : 0u; };
   B b;
   f32x16 acc[NV] = {};
   b.load(a, there ? column : 0, begin + wave * 16 + half);
-  constexpr uint32_t kAhead = 4;  // fragments under way
-  Fragments<ORDER> fa[kAhead];
+  Fragments<ORDER> fa[WAVES];
 #pragma unroll
-  for (uint32_t i = 0; i < kAhead; ++i) fa[i].load(from, first + i, all);
-  uint32_t buffer = 0;
-  for (uint32_t at = begin; at < end; at += step) {
+  for (uint32_t i = 0; i < WAVES; ++i) fa[i].load(from, first + i, all);
+  uint32_t buffer = 0, at = begin;
+  auto take = [&](auto last) __attribute__((always_inline)) {
+    constexpr bool kLast = decltype(last)::value;
     b.store(lds + buffer * size + wave * B::kBytes, left_at(at + wave * 16 + half), lane);
     __syncthreads();
-    if (at + step < end) b.load(a, there ? column : 0, at + step + wave * 16 + half);
-    // (waves are a multiple of kAhead, so that a fragment's place is known)
-    for (uint32_t i = 0; i < waves; i += kAhead) {
+    if constexpr (!kLast) b.load(a, there ? column : 0, at + step + wave * 16 + half);
 #pragma unroll
-      for (uint32_t u = 0; u < kAhead; ++u) {
-        const uint32_t now = at / 16 + i + u;
-        if (now < all && m0 < a.rows) multiply_turned<B::kPieces, NV>(fa[u], lds + buffer * size + (i + u) * B::kBytes, lane, acc);
-        fa[u].load(from, now + kAhead, all);
-      }
+    for (uint32_t u = 0; u < WAVES; ++u) {
+      const uint32_t now = at / 16 + u;
+      if (!kLast || now < all) multiply_turned<B::kPieces, NV>(fa[u], lds + buffer * size + u * B::kBytes, lane, acc);
+      if constexpr (!kLast) fa[u].load(from, now + WAVES, all);
     }
     buffer ^= 1;
-  }
+    at += step;
+  };
+  while (at + step < end) take(std::false_type{});
+  take(std::true_type{});
   if (there && m0 < a.rows) store_turned<O, NV>(a, part * a.out_split, m0, column, lane, acc);
 }
 
@@ -821,12 +822,12 @@ template <class T, class W> int launch_gradient_of_weight(GradientDev a, const W
     allow_lds(kernel, lds);
     return launch_groups(kernel, kernel, groups, w.waves * 64, lds, s, a, w.tokens_per_part, w.row_blocks);
   };
-  if (w.parts == 1) return launch(gradient_of_weight<T, W, kNV, kOrd>);
+  if (w.parts == 1) return w.waves == 8 ? launch(gradient_of_weight<T, W, kNV, kOrd, 8>) : launch(gradient_of_weight<T, W, kNV, kOrd, 4>);
   const SumDev sum{sums, (uint64_t)a.rows * a.columns, a.out, a.out_stride, a.rows, a.columns, a.columns, w.parts, 0};
   a.out = reinterpret_cast<uint8_t *>(sums);
   a.out_stride = a.columns;
   a.out_split = sum.split;
-  const int err = launch(gradient_of_weight<T, float, kNV, kOrd>);
+  const int err = w.waves == 8 ? launch(gradient_of_weight<T, float, kNV, kOrd, 8>) : launch(gradient_of_weight<T, float, kNV, kOrd, 4>);
   return err ? err : launch_sum<W>(sum, s);
 }
 
