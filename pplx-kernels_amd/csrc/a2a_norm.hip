@@ -450,11 +450,22 @@ template <class T, class W> __global__ __launch_bounds__(kSumThreads) void norm_
   });
 }
 
-constexpr uint64_t kMostInRegisters = 8 * 4 * 512;  // elements of a row in the gradient's kernel
-constexpr uint32_t kBackwardGroups = 512;           // workgroups that share out the rows
+// How many threads a row has, in us of bf16 rows with a residual, out of HBM (16384 x 4096 and longer move at 5.7 TB/s):
+//   up to 512         a wave, 8 elements a thread   16384 x 512  13.8 (256 threads 17.4)   262144 x 128  73 (192)
+//   up to 2048        256 threads, 8 elements       256 x 2048  3.4 (a wave with 32: 4.4)  8192 x 2048 to e4m3  27.8 (31.8)   16384 x 2048  47.5 (47.5)
+//   up to 4096, 8192  512 threads, 8 and 16         512 x 4096  4.8 (256 with 16: 5.7)     8192 x 7168 to e4m3  93 (256 with 32: 98)
+//   up to 16384       512 threads, 32               4096 x 16384  94.6 (1024 with 16: 94.9)
+// The gradients' workgroups take a row after the other: a wave with 32 elements takes rows of up to 2048 faster than 256 threads do, 16384 x
+// 1024  31 (45), since it needs no barrier; longer rows have the same threads as above.
+constexpr uint64_t kMostInRegisters = 8 * 4 * 512;
 
+// The gradients' workgroups, each with a share of the weight's gradient to add up: as few as keep memory busy.  One of them has 8192
+// elements of each operand under way, or 4096 of rows of up to that, 2048 of short ones.  With the sum, us:
+//   8192 x 7168  256: 89, 512: 96, 1024: 102       8192 x 4096 with weights in fp32  256: 62, 512: 57     4096 x 2048  256: 18.2, 512: 19.2
+//   16384 x 512  256: 19.7, 512: 18.8, 1024: 21.5   262144 x 128  256: 177, 512: 113, 1024: 83
 uint32_t backward_groups(uint32_t m, uint64_t width) {
-  const uint64_t rows = width <= 2048 ? ((uint64_t)m + 3) / 4 : m, most = width <= 8192 ? kBackwardGroups : kBackwardGroups / 2;
+  const uint64_t rows = width <= 2048 ? ((uint64_t)m + 3) / 4 : m;
+  const uint64_t most = width <= 128 ? 1024 : width <= 512 || (width > 2048 && width <= 4096) ? 512 : 256;
   return (uint32_t)(rows < most ? rows : most);
 }
 
@@ -519,8 +530,10 @@ extern "C" int pplx_a2a_rms_norm(int device, const pplx_a2a_rms_norm_args_t *arg
         auto rows = [&](auto kernel, uint32_t threads, uint32_t at_once) {
           return launch_groups(kernel, kernel, ((uint64_t)a.m + at_once - 1) / at_once, threads, 0, s, a);
         };
-        if (a.width <= 2048) PPLX_LAUNCH(rows(norm_rows<T, W, F, 64, 4>, 256, 4));
-        else if (a.width <= 8192) PPLX_LAUNCH(rows(norm_rows<T, W, F, 256, 4>, 256, 1));
+        if (a.width <= 512) PPLX_LAUNCH(rows(norm_rows<T, W, F, 64, 1>, 256, 4));
+        else if (a.width <= 2048) PPLX_LAUNCH(rows(norm_rows<T, W, F, 256, 1>, 256, 1));
+        else if (a.width <= 4096) PPLX_LAUNCH(rows(norm_rows<T, W, F, 512, 1>, 512, 1));
+        else if (a.width <= 8192) PPLX_LAUNCH(rows(norm_rows<T, W, F, 512, 2>, 512, 1));
         else if (a.width <= kMostInRegisters) PPLX_LAUNCH(rows(norm_rows<T, W, F, 512, 4>, 512, 1));
         else PPLX_LAUNCH(rows(norm_long_rows<T, W, F>, kLongLanes, 1));
         return (int)PPLX_A2A_OK;
@@ -577,16 +590,17 @@ extern "C" int pplx_a2a_rms_norm_backward(int device, const pplx_a2a_rms_norm_ba
       typedef typename decltype(weight_tag)::type W;
       hipStream_t s = (hipStream_t)stream;
       const uint32_t groups = backward_groups(a.m, a.width), columns = (a.width + 31) / 32;
-      constexpr bool kAhead = sizeof(T) == 2;  // (rows of fp32 that are longer than 2048 fill the registers once)
+      constexpr bool kAhead = sizeof(T) == 2;  // (32 elements of fp32 in a thread fill its registers once)
       W *out = static_cast<W *>(p.grad_weight);
       if (a.width > kMostInRegisters) {
         PPLX_LAUNCH(launch_kernel(norm_backward_long<T, W>, dim3(groups), dim3(kLongLanes), 0, s, a));
         if (out) PPLX_LAUNCH(launch_kernel(norm_weight_gradient_long<T, W>, dim3(columns), dim3(kSumThreads), 0, s, a, out));
         return (int)PPLX_A2A_OK;
       }
-      if (a.width <= 2048) PPLX_LAUNCH(launch_kernel(norm_backward_rows<T, W, 64, 4, kAhead>, dim3(groups), dim3(256), 0, s, a));
-      else if (a.width <= 4096) PPLX_LAUNCH(launch_kernel(norm_backward_rows<T, W, 256, 2, true>, dim3(groups), dim3(256), 0, s, a));
-      else if (a.width <= 8192) PPLX_LAUNCH(launch_kernel(norm_backward_rows<T, W, 256, 4, kAhead>, dim3(groups), dim3(256), 0, s, a));
+      if (a.width <= 512) PPLX_LAUNCH(launch_kernel(norm_backward_rows<T, W, 64, 1, true>, dim3(groups), dim3(256), 0, s, a));
+      else if (a.width <= 2048) PPLX_LAUNCH(launch_kernel(norm_backward_rows<T, W, 64, 4, kAhead>, dim3(groups), dim3(256), 0, s, a));
+      else if (a.width <= 4096) PPLX_LAUNCH(launch_kernel(norm_backward_rows<T, W, 512, 1, true>, dim3(groups), dim3(512), 0, s, a));
+      else if (a.width <= 8192) PPLX_LAUNCH(launch_kernel(norm_backward_rows<T, W, 512, 2, true>, dim3(groups), dim3(512), 0, s, a));
       else PPLX_LAUNCH(launch_kernel(norm_backward_rows<T, W, 512, 4, kAhead>, dim3(groups), dim3(512), 0, s, a));
       if (out) {
         const float *partial = a.partial;

@@ -84,6 +84,11 @@ NORMS = [
     (2, 20000, BF16, BF16),
     (2, 40016, F32, F32),
     (9, 528, F16, F32),
+    (7, 512, BF16, BF16),
+    (6, 4096, F32, F32),
+    (5, 4112, BF16, F32),
+    (4, 8192, F16, F16),
+    (2051, 128, BF16, BF16),
     (0, 64, BF16, BF16),
 ]
 
@@ -204,6 +209,12 @@ def test_rms_norm_in_place_and_into_strided_buffers(device, hidden, quantize):
 NORM_GRADIENTS = [
     (1, 8, F32, F32), (1, 2048, BF16, BF16), (33, 520, F16, F16), (600, 264, F32, F32), (1100, 64, BF16, F32), (40, 7168, BF16, F32),
     (7, 16384, BF16, BF16), (5, 20000, F16, F32), (3, 17000, F32, F32),
+    (4100, 128, BF16, F32),
+    (2100, 512, F16, F16),
+    (300, 4096, F32, F32),
+    (513, 4104, BF16, BF16),
+    (261, 8192, F32, F32),
+    (30, 8200, F16, F32),
 ]  # fmt: skip
 
 
