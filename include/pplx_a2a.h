@@ -539,7 +539,7 @@ int pplx_a2a_rms_norm_workspace(uint32_t m, uint64_t hidden_dim, uint64_t *bytes
 int pplx_a2a_rms_norm_backward(int device, const pplx_a2a_rms_norm_backward_args_t *args, void *stream);
 
 /* The router's product: logits[t, e] = sum over k of x[t, k] * weight[e, k], added up in fp32.  Products of 16-bit elements are
- * exact; fp32 elements count to 24 bits (an infinity among them makes a NaN). */
+ * exact; fp32 elements count to 24 bits (an infinity among them, or a value above 3.38e38, makes a NaN). */
 typedef struct pplx_a2a_router_logits_args {
   const void *x;               /* [m, hidden_dim] of dtype; rows 16-byte aligned, strides in bytes, multiples of 16 */
   int64_t x_stride_row;

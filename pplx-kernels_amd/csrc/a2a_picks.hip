@@ -4,8 +4,10 @@
 // apart come out in the same order everywhere.  Without a bias the logits themselves have that order.  Otherwise fp32 makes the
 // choice and watches how near its keys come: a token with two of them closer than their errors is chosen for once more in 64 bits, out of
 // the registers that hold its logits.
-// A wave takes a token, whose logits it reads once; what bounds it is the instructions of the choice, a reduction over the wave for
-// each pick.
+// A wave takes a token, whose logits it reads once.  What bounds it is the instructions of the choice, six dependent steps over the wave for
+// each pick, 0.16 us of a wave: 256 experts in fp32, a pick and eight, us in a graph: 64 tokens 2.4 and 3.5, with scores and biases
+// 3.0 and 4.3, with groups too 3.8 and 5.0; 8192 tokens 3.7 and 6.9 (1.2 TB/s of logits), with scores and biases 5.6 and 11.6, with
+// groups too 7.8 and 14.2, of which some tokens' second choice is 2 to 4.
 #include <cfloat>
 #include <climits>
 #include <cmath>
@@ -274,7 +276,7 @@ template <class T> __device__ __forceinline__ void pick_exactly(const PicksDev &
   store_pick(a, t, lane, own, (float)(w * (double)a.weight_scale));
 }
 
-constexpr uint32_t kTokensAtOnce = 4;  // of a workgroup, a wave to each
+constexpr uint32_t kTokensAtOnce = 4;  // of a workgroup, a wave to each (no wave waits for another)
 // Whether a token is there; those from bound_m on are done here.
 __device__ __forceinline__ bool is_there(const PicksDev &a, uint32_t t, uint32_t lane) {
   if (!a.bound_m || t < *as_global(a.bound_m)) return true;
@@ -509,7 +511,8 @@ __device__ __forceinline__ F gradient_of_pick(const PicksBackwardDev &a, bool pi
   return picked ? part * (F)a.weight_scale : (F)0;
 }
 
-// A wave to a token, PER consecutive experts in a lane and 64 PER at a time; rows of up to that are read once.
+// A wave to a token, PER consecutive experts in a lane and 64 PER at a time; rows of up to that are read once.  An expert's own part goes
+// through LDS to the lane that writes it.  16384 tokens of 256 experts, softmax without renormalisation: 11.9 us, 2.8 TB/s.
 template <class T, int PER> __global__ __launch_bounds__(64 * kTokensAtOnce) void pick_gradient(PicksBackwardDev a) {
   extern __shared__ float of_picks[];  // [waves][experts]: an expert's own part
   const uint32_t lane = lane_id(), wave = wave_id(), E = a.experts;
@@ -629,8 +632,9 @@ extern "C" int pplx_a2a_route_tokens(int device, const pplx_a2a_route_args_t *ar
     return with_type(p.dtype, [&](auto tag) {
       typedef typename decltype(tag)::type T;
       const bool grouped = a.top_groups < a.groups, scored = a.bias || (grouped && a.group_top > 1);
-      // Experts of a lane: as few as hold all of them, where no lane has some of two groups.
-      // A group's lanes are a power of two.
+      // Experts of a lane: as few as hold all of them, where no lane has some of two groups, whose lanes are a power of two.  (More
+      // experts in a lane make its choice of the next one longer: 64 tokens of 256 experts 5.0 us, of 512 in 64 groups 8.0.)  What sixteen to
+      // a lane do not hold is chosen for in LDS in 64 bits.
       const uint32_t size = a.experts / a.groups;
       uint32_t per = 1;
       auto lanes_of_group = [&] {
