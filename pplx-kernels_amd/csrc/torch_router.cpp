@@ -637,23 +637,37 @@ PyObject *py_rms_norm(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// normed_rows(x, weight, residual, eps, record) -> (y, sum): differentiable if `record`
+// The four fields of NormedRows.
+PyObject *normed(const at::Tensor &y, const at::Tensor &sum, const at::Tensor &q, const at::Tensor &scale) {
+  PyObject *out = PyTuple_New(4);
+  if (!out) throw python_error();
+  PyTuple_SET_ITEM(out, 0, wrap_or_none(y));
+  PyTuple_SET_ITEM(out, 1, wrap_or_none(sum));
+  PyTuple_SET_ITEM(out, 2, wrap_or_none(q));
+  PyTuple_SET_ITEM(out, 3, wrap_or_none(scale));
+  return out;
+}
+
+// normed_rows(x, weight, residual, eps, record) -> (y, sum, None, None): differentiable if `record`
 PyObject *py_normed_rows(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   arity("normed_rows", nargs, 5);
   const at::Tensor &x = tensor_arg(args[0], "x"), &weight = tensor_arg(args[1], "weight");
-  const std::optional<at::Tensor> residual = maybe(optional_tensor_arg(args[2], "residual"));
+  const at::Tensor *residual = optional_tensor_arg(args[2], "residual");
   const double eps = float_arg(args[3], "eps");
   Normed made;
   if (bool_arg(args[4])) {
-    made = normed_rows_autograd(x, weight, residual, eps);
-  } else if (straight({&x, &weight, opt(residual)})) {
-    made = normed_rows_op(x, weight, residual, eps);
+    made = normed_rows_autograd(x, weight, maybe(residual), eps);
+  } else if (straight({&x, &weight, residual})) {
+    check_matrix(x, "x");
+    const at::Tensor y = fresh(x.sizes(), x, x.scalar_type()), sum = residual ? fresh(x.sizes(), x, x.scalar_type()) : at::Tensor();
+    rms_norm(&y, defined(sum), nullptr, nullptr, x, weight, residual, eps);
+    return normed(y, sum, at::Tensor(), at::Tensor());
   } else {
     static auto op = op_handle<decltype(normed_rows_op)>("pplx_kernels::normed_rows");
-    made = op.call(x, weight, residual, eps);
+    made = op.call(x, weight, maybe(residual), eps);
   }
-  return pair(std::get<0>(made), residual ? std::get<1>(made) : at::Tensor());
+  return normed(std::get<0>(made), residual ? std::get<1>(made) : at::Tensor(), at::Tensor(), at::Tensor());
   END_HANDLE_TH_ERRORS
 }
 
@@ -677,13 +691,7 @@ PyObject *py_quantized_rows(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     static auto op = op_handle<decltype(rms_norm_op)>("pplx_kernels::rms_norm");
     op.call(y, if_defined(sum), q, scale, x, weight, maybe(residual), eps);
   }
-  PyObject *out = PyTuple_New(4);
-  if (!out) throw python_error();
-  PyTuple_SET_ITEM(out, 0, wrap_or_none(y));
-  PyTuple_SET_ITEM(out, 1, wrap_or_none(sum));
-  PyTuple_SET_ITEM(out, 2, wrap_or_none(q));
-  PyTuple_SET_ITEM(out, 3, wrap_or_none(scale));
-  return out;
+  return normed(y, sum, q, scale);
   END_HANDLE_TH_ERRORS
 }
 
@@ -846,7 +854,7 @@ PyObject *py_router_build_id(PyObject *, PyObject *) { return PyUnicode_FromStri
 #define PPLX_FASTCALL(fn) (PyCFunction)(void (*)(void))fn, METH_FASTCALL
 PyMethodDef kRouterMethods[] = {
     {"rms_norm", PPLX_FASTCALL(py_rms_norm), "rms_norm(y, sum, q, scale, x, weight, residual, eps)"},
-    {"normed_rows", PPLX_FASTCALL(py_normed_rows), "normed_rows(x, weight, residual, eps, record) -> (y, sum)"},
+    {"normed_rows", PPLX_FASTCALL(py_normed_rows), "normed_rows(x, weight, residual, eps, record) -> (y, sum, None, None)"},
     {"quantized_rows", PPLX_FASTCALL(py_quantized_rows), "quantized_rows(x, weight, residual, eps, int8) -> (y, sum, q, scale)"},
     {"rms_norm_backward", PPLX_FASTCALL(py_rms_norm_backward),
      "rms_norm_backward(grad_h, grad_weight, grad_y, grad_sum, h, weight, eps, workspace)"},

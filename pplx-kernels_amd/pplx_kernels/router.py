@@ -111,7 +111,7 @@ def rms_norm(
     record = _wants_grad(x, weight, residual)
     if record:
         _check_recording(x)
-    return NormedRows._make((*_C.normed_rows(x, weight, residual, eps, record), None, None))
+    return NormedRows._make(_C.normed_rows(x, weight, residual, eps, record))
 
 
 def rms_norm_backward(
