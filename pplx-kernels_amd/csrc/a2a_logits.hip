@@ -632,8 +632,8 @@ template <class K> void allow_lds(K *kernel, uint32_t bytes) {
 // split the sums' launch and bytes.  Measured with rows that come from HBM, forms 64 x 64 / 128 x 128 with their best splits, us:
 //   both bf16       8192 x 256 x 7168  65 (1) / 47.8 (2)     3001 x 256 x 7168  32.9 (4) / 27.2 (4)   1024 x 256 x 7168  15.0 (4) / 17.2 (12)
 //                   16384 x 64 x 4096  32.0 (1) / 37.5 (4)   256 x 256 x 7168  9.4 (16) / 11.9 (16)   64 x 256 x 7168   7.6 (28) / 9.0 (28)
-//   bf16, fp32      8192 x 256 x 7168  199 (2) / 97.7 (2)    64 x 256 x 7168   9.9 (56) / 11.1 (56)
-//   both fp32       4096 x 256 x 7168  144 (4) / 101 (4)     64 x 256 x 7168  10.9 (56) / 14.5 (56)
+//   bf16, fp32      8192 x 256 x 7168  199 (2) / 97.7 (2)    256 x 256 x 7168  14.1 (16) / 16.1 (28)   64 x 256 x 7168   9.9 (56) / 11.1 (56)
+//   both fp32       4096 x 256 x 7168  144 (4) / 101 (4)     256 x 256 x 7168  17.2 (16) / 21.3 (38)   64 x 256 x 7168  10.9 (56) / 14.5 (56)
 // and 128 x 192, for 16-bit operands, beside 128 x 128:
 //   both bf16       16384 x 384 x 7168  91 (1) / 143 (1)     8192 x 384 x 7168  57.6 (2) / 72.2 (1)   4096 x 384 x 7168  36.2 (4) / 42.2 (2)   1024 x 384 x 7168  21.4 (14) / 19.7 (8)
 //                   3001 x 384 x 7168  32.2 (4) / 32.8 (3)
@@ -645,12 +645,12 @@ template <class K> void allow_lds(K *kernel, uint32_t bytes) {
 // weights 20.9: its loads take a cycle for each row of 64 bytes, whatever else is under way.
 struct LogitsForm {
   uint32_t bm, bn;
-  double start;        // beside the others' 3 us
-  double per_step[4];  // 16-bit operands; bf16 and fp32; fp16 and fp32; fp32
+  double start[4], per_step[4];  // 16-bit operands; bf16 and fp32; fp16 and fp32; fp32
 };
 constexpr double kNever = 1e9;
-constexpr LogitsForm kForms[] = {
-    {64, 64, 0, {0.25, 0.87, 1.1, 1.3}}, {128, 128, 0, {0.66, 1.6, 2.55, 3.3}}, {128, 192, 1.5, {0.85, kNever, kNever, kNever}}};
+constexpr LogitsForm kForms[] = {{64, 64, {3.0, 4.7, 5.0, 5.4}, {0.25, 0.8, 1.0, 1.08}},
+                                 {128, 128, {3.0, 6.0, 6.5, 7.0}, {0.66, 1.5, 2.4, 3.0}},
+                                 {128, 192, {4.5, kNever, kNever, kNever}, {0.85, kNever, kNever, kNever}}};
 struct LogitsPlan {
   int form = -1;  // -1: product_split
   uint32_t splits = 1, steps_per_split = 0;
@@ -668,7 +668,7 @@ LogitsPlan plan_logits(uint64_t m, uint64_t experts, uint64_t hidden, int32_t dt
   for (int f = 0; f < (int)(sizeof(kForms) / sizeof(kForms[0])); ++f) {
     const LogitsForm &form = kForms[f];
     const uint64_t tiles = ((m + form.bm - 1) / form.bm) * ((experts + form.bn - 1) / form.bn);
-    const double per_step = form.per_step[kind], start = (kind == 0 ? 3.0 : 3.6) + form.start;
+    const double per_step = form.per_step[kind], start = form.start[kind];
     if (tiles >= (1ull << 28) || start + per_step * rounds(tiles) >= least) continue;  // (no split of k is faster than one step)
     // As many splits as go into one, two or three rounds of the compute units, fewer where their sums cost more than they gain, and some
     // that make the last of a few rounds a short one: 1 % of products have a plan that costs 3 % more than the best of all splits.
