@@ -637,6 +637,9 @@ template <class K> void allow_lds(K *kernel, uint32_t bytes) {
 // and 128 x 192, for 16-bit operands, beside 128 x 128:
 //   both bf16       16384 x 384 x 7168  91 (1) / 143 (1)     8192 x 384 x 7168  57.6 (2) / 72.2 (1)   4096 x 384 x 7168  36.2 (4) / 42.2 (2)   1024 x 384 x 7168  21.4 (14) / 19.7 (8)
 //                   3001 x 384 x 7168  32.2 (4) / 32.8 (3)
+// and 128 x 32, where operands are cut into pieces (what a wave cuts of the rows is not cut by a second one), beside 64 x 64:
+//   bf16, fp32      16384 x 8 x 4096  38.4 (4) / 60.4 (1)    4096 x 32 x 2048  12.8 (8) / 13.6 (4)   64 x 8 x 4096  7.9 (32) / 8.7 (16)
+//   both fp32       16384 x 8 x 4096  63.5 (2) / 89.0 (2)    4096 x 32 x 2048  14.4 (8) / 17.8 (4)   both bf16, 16384 x 8 x 4096  30.4 (4) / 29.1 (4)
 // What bounds a tile of 128 x 128 is what a compute unit fetches into its LDS, 31 bytes a cycle: 0.43 us a step with rows in L2, and
 // 0.63 with rows out of HBM, whose latency its four steps do not cover.  Larger tiles fetch less and hold fewer steps: 128 x 256 and
 // 256 x 128 take 1.1 us a step, 256 x 256 1.4.  Tiles of 64 x 128, 64 x 256, 32 x 64 and 32 x 128 were within 5 % of the better of the
@@ -650,7 +653,8 @@ struct LogitsForm {
 constexpr double kNever = 1e9;
 constexpr LogitsForm kForms[] = {{64, 64, {3.0, 4.7, 5.0, 5.4}, {0.25, 0.8, 1.0, 1.08}},
                                  {128, 128, {3.0, 6.0, 6.5, 7.0}, {0.66, 1.5, 2.4, 3.0}},
-                                 {128, 192, {4.5, kNever, kNever, kNever}, {0.85, kNever, kNever, kNever}}};
+                                 {128, 192, {4.5, kNever, kNever, kNever}, {0.85, kNever, kNever, kNever}},
+                                 {128, 32, {kNever, 5.0, 5.4, 5.0}, {kNever, 0.95, 1.1, 1.75}}};
 struct LogitsPlan {
   int form = -1;  // -1: product_split
   uint32_t splits = 1, steps_per_split = 0;
@@ -732,6 +736,8 @@ template <class T, class W> int launch_form(int form, const TilesDev &a, hipStre
   if (form == 0) return launch_tiles<T, W, 64, 64, 2, 2, 4>(a, s);
   if constexpr (sizeof(W) == 2) {
     if (form == 2) return launch_tiles<T, W, 128, 192, 2, 2, 3>(a, s);
+  } else {
+    if (form == 3) return launch_tiles<T, W, 128, 32, 4, 1, sizeof(T) == 2 ? 5 : 3>(a, s);
   }
   return launch_tiles<T, W, 128, 128, 2, 4, sizeof(W) == 2 ? 4 : 2>(a, s);
 }

@@ -329,6 +329,9 @@ LOGITS = [
     (2050, 72, 136, F16, F16),
     (4100, 256, 200, BF16, BF16),
     (16400, 300, 200, F16, F16),
+    (5000, 30, 4104, BF16, F32),
+    (5000, 8, 4096, F32, F32),
+    (16384, 30, 1032, F16, F32),
     (3001, 384, 7168, BF16, BF16),
     (8200, 300, 2048, BF16, BF16),
     (1000, 300, 1024, BF16, F32),
