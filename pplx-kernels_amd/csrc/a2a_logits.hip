@@ -637,13 +637,16 @@ template <class K> void allow_lds(K *kernel, uint32_t bytes) {
 // and 128 x 192, for 16-bit operands, beside 128 x 128:
 //   both bf16       16384 x 384 x 7168  91 (1) / 143 (1)     8192 x 384 x 7168  57.6 (2) / 72.2 (1)   4096 x 384 x 7168  36.2 (4) / 42.2 (2)   1024 x 384 x 7168  21.4 (14) / 19.7 (8)
 //                   3001 x 384 x 7168  32.2 (4) / 32.8 (3)
+// and 64 x 128, for 16-bit operands of few steps, beside 64 x 64 and 128 x 128:
+//   both bf16       16384 x 128 x 2048  20.4 / 25.1 / 25.4   8192 x 256 x 2048  17.7 / 21.3 / 23.0   4096 x 300 x 2048  15.1 / 17.9 / 18.9
+//                   16384 x 256 x 2048  35.8 / 41.8 / 28.2   2048 x 128 x 4096  14.0 / 12.0 / 16.4
 // and 128 x 32, where operands are cut into pieces (what a wave cuts of the rows is not cut by a second one), beside 64 x 64:
 //   bf16, fp32      16384 x 8 x 4096  38.4 (4) / 60.4 (1)    4096 x 32 x 2048  12.8 (8) / 13.6 (4)   64 x 8 x 4096  7.9 (32) / 8.7 (16)
 //   both fp32       16384 x 8 x 4096  63.5 (2) / 89.0 (2)    4096 x 32 x 2048  14.4 (8) / 17.8 (4)   both bf16, 16384 x 8 x 4096  30.4 (4) / 29.1 (4)
 // What bounds a tile of 128 x 128 is what a compute unit fetches into its LDS, 31 bytes a cycle: 0.43 us a step with rows in L2, and
 // 0.63 with rows out of HBM, whose latency its four steps do not cover.  Larger tiles fetch less and hold fewer steps: 128 x 256 and
-// 256 x 128 take 1.1 us a step, 256 x 256 1.4.  Tiles of 64 x 128, 64 x 256, 32 x 64 and 32 x 128 were within 5 % of the better of the
-// first two, or slower, in all of twenty products.
+// 256 x 128 take 1.1 us a step, 256 x 256 1.4.  Tiles of 64 x 192, 64 x 256, 32 x 64 and 32 x 128 were within 5 % of the best of
+// these, or slower, in all of thirty products.
 // product_split, which is one launch: 4 x 64 x 2048 4.3 (tiles 5.8), 1 x 256 x 7168 9.5 (6.5), 64 x 256 x 7168 14.2, with fp32
 // weights 20.9: its loads take a cycle for each row of 64 bytes, whatever else is under way.
 struct LogitsForm {
@@ -654,7 +657,8 @@ constexpr double kNever = 1e9;
 constexpr LogitsForm kForms[] = {{64, 64, {3.0, 4.7, 5.0, 5.4}, {0.25, 0.8, 1.0, 1.08}},
                                  {128, 128, {3.0, 6.0, 6.5, 7.0}, {0.66, 1.5, 2.4, 3.0}},
                                  {128, 192, {4.5, kNever, kNever, kNever}, {0.85, kNever, kNever, kNever}},
-                                 {128, 32, {kNever, 5.0, 5.4, 5.0}, {kNever, 0.95, 1.1, 1.75}}};
+                                 {128, 32, {kNever, 5.0, 5.4, 5.0}, {kNever, 0.95, 1.1, 1.75}},
+                                 {64, 128, {3.0, kNever, kNever, kNever}, {0.48, kNever, kNever, kNever}}};
 struct LogitsPlan {
   int form = -1;  // -1: product_split
   uint32_t splits = 1, steps_per_split = 0;
@@ -736,6 +740,7 @@ template <class T, class W> int launch_form(int form, const TilesDev &a, hipStre
   if (form == 0) return launch_tiles<T, W, 64, 64, 2, 2, 4>(a, s);
   if constexpr (sizeof(W) == 2) {
     if (form == 2) return launch_tiles<T, W, 128, 192, 2, 2, 3>(a, s);
+    if (form == 4) return launch_tiles<T, W, 64, 128, 2, 2, 4>(a, s);
   } else {
     if (form == 3) return launch_tiles<T, W, 128, 32, 4, 1, sizeof(T) == 2 ? 5 : 3>(a, s);
   }

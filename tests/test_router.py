@@ -375,6 +375,45 @@ def test_router_logits(device, m, experts, hidden, dtype, weight_dtype):
     assert (room[:, :3] == 7).all() and (room[:, 3 + experts :] == 7).all()
 
 
+EVERY_TILE = {
+    # what a product's sizes choose: each tile, with a multiple of 64 to add up and not, split and not
+    (F32, F32): [
+        (40, 5, 4096), (40, 5, 4104), (257, 5, 4096), (1000, 5, 4104), (1500, 200, 1032), (2050, 384, 72), (2050, 384, 128),
+        (4100, 70, 1024), (4100, 200, 136), (8200, 384, 72), (8200, 384, 128), (12000, 150, 64),
+    ],
+    (BF16, F32): [
+        (40, 5, 4096), (40, 5, 4104), (1000, 5, 4096), (1000, 130, 2048), (2050, 150, 520), (2050, 384, 72), (2050, 384, 128),
+        (3000, 70, 1032), (4100, 200, 136), (8200, 384, 64), (12000, 150, 64), (16400, 100, 72),
+    ],
+    (BF16, BF16): [
+        (40, 5, 4096), (40, 5, 4104), (1030, 384, 72), (1500, 200, 2056), (2050, 300, 64), (3000, 70, 2048), (3000, 70, 2056),
+        (4100, 130, 4096), (4100, 130, 4104), (4100, 200, 64), (8200, 70, 72), (12000, 384, 256), (12000, 384, 264),
+        (16400, 70, 64), (16400, 70, 72),
+    ],
+    (F16, F32): [
+        (40, 5, 4096), (40, 5, 4104), (65, 200, 4104), (520, 5, 4096), (700, 384, 2048), (1000, 384, 1032), (2050, 384, 136),
+        (4100, 200, 136), (8200, 300, 64), (8200, 384, 64), (8200, 384, 72), (16400, 150, 64),
+    ],
+    (F16, F16): [
+        (40, 5, 4096), (40, 5, 4104), (1030, 384, 72), (1500, 200, 2056), (2050, 300, 64), (3000, 70, 2048), (3000, 70, 2056),
+        (4100, 130, 4096), (4100, 130, 4104), (4100, 200, 64), (8200, 70, 72), (12000, 384, 256), (12000, 384, 264),
+        (16400, 70, 64), (16400, 70, 72),
+    ],
+}  # fmt: skip
+
+
+@gpu
+@pytest.mark.parametrize("dtype,weight_dtype,m,experts,hidden", [(*types, *size) for types, sizes in EVERY_TILE.items() for size in sizes])
+def test_router_logits_of_every_tile(device, dtype, weight_dtype, m, experts, hidden):
+    gen = torch.Generator().manual_seed(m + hidden)
+    x, weight = (t.to(device) for t in router(m, experts, hidden, dtype, weight_dtype, gen))
+    want, off = product(x, weight.t(), hidden)
+    room = torch.full((m, experts + 3), 7.0, device=device)
+    router_logits(x, weight, out=room[:, 1 : 1 + experts])
+    assert_within(room[:, 1 : 1 + experts], want.cpu(), off.cpu())
+    assert (room[:, 0] == 7).all() and (room[:, 1 + experts :] == 7).all()
+
+
 @gpu
 @pytest.mark.parametrize("dtype,weight_dtype", [(F32, F32), (BF16, F32), (F16, F32), (F16, F16), (BF16, BF16)])
 def test_router_logits_hold_every_bit(device, dtype, weight_dtype):
