@@ -309,7 +309,7 @@ __device__ __forceinline__ void load_some(const PPLX_GLOBAL T *row, uint32_t bas
 }
 
 // A token's choice in F, with its logits and biases in registers: of experts `base` on in this lane, which are of `group`.  False,
-// with nothing stored, if fp32 doesn't tell.  SCORED: keys or the groups' sums are scores, not logits.
+// with nothing stored, if fp32 doesn't tell.  SCORED: keys (with a bias) or the groups' sums are scores, not logits.
 template <class F, int PER, bool SCORED>
 __device__ __forceinline__ bool choose(const PicksDev &a, uint32_t t, uint32_t lane, uint32_t group, uint32_t base, const float *l,
                                        const float *bias, float most) {
@@ -345,7 +345,8 @@ __device__ __forceinline__ bool choose(const PicksDev &a, uint32_t t, uint32_t l
   // of two groups by four times; the sums with the bias and of two scores round by 2^-24 of what they come to.
   const float off = !kWatched ? 0.f : softmax ? 0x1p-18f / (float)total : 0x1p-21f;
   auto are_near = [](float larger, float smaller, float off) {
-    return larger - smaller <= __builtin_fmaf(0x1p-22f, __builtin_fabsf(larger) + __builtin_fabsf(smaller), off);
+    // (so that what is no number, the difference of sums that fp32 does not hold, is near)
+    return !(larger - smaller > __builtin_fmaf(0x1p-22f, __builtin_fabsf(larger) + __builtin_fabsf(smaller), off));
   };
   bool near = false;
   if (grouped) {
@@ -376,9 +377,10 @@ __device__ __forceinline__ bool choose(const PicksDev &a, uint32_t t, uint32_t l
       const float next = wave_max_of_lanes(taken || group >= a.groups ? kNoLogit : (float)sum);
       near |= next > kNoLogit && are_near(last, next, 2 * off);
     }
-    if (!taken) {
 #pragma unroll
-      for (int j = 0; j < PER; ++j) key[j] = none;
+    for (int j = 0; j < PER; ++j) {
+      if (!a.bias) key[j] = order_of((F)l[j]);  // (equal scores may be of logits that are not)
+      key[j] = taken ? key[j] : none;
     }
   }
   // The largest key of each lane; the largest of all is taken, and its lane looks for its next one.
@@ -418,7 +420,7 @@ __device__ __forceinline__ bool choose(const PicksDev &a, uint32_t t, uint32_t l
     }
   }
   const bool picked = own < a.experts;
-  if constexpr (kWatched) {
+  if (kWatched && a.bias) {
     // Each pick beside the next, the last one beside all that are left.  Equal logits with equal biases are equal in any arithmetic.
     const PPLX_GLOBAL float *biases = as_global(a.bias);
     const float next_key = __shfl(own_key, (int)(lane + 1));
@@ -426,20 +428,20 @@ __device__ __forceinline__ bool choose(const PicksDev &a, uint32_t t, uint32_t l
     if (__ballot(close)) {
       const float next_logit = __shfl(own_logit, (int)(lane + 1));
       const uint32_t next = __shfl(own, (int)(lane + 1));
-      if (close) near |= !(own_logit == next_logit && (!a.bias || biases[own] == biases[next]));
+      if (close) near |= !(own_logit == next_logit && biases[own] == biases[next]);
     }
     const Order order = wave_largest(head);
     const float last_key = of_lane(own_key, (int)a.picks - 1), last_logit = of_lane(own_logit, (int)a.picks - 1);
     const int last = of_lane((int)own, (int)a.picks - 1);
     if (order != none && are_near(last_key, number_of(order), off)) {
-      const float last_bias = a.bias ? biases[last] : 0.f;
+      const float last_bias = biases[last];
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
         near |= key[j] != none && are_near(last_key, number_of(key[j]), off) && !(l[j] == last_logit && bias[j] == last_bias);
       }
     }
-    if (__ballot(near)) return false;
   }
+  if (kWatched && __ballot(near)) return false;
   float w;
   if (sizeof(F) == 4 && picks_are_near(picked, own_logit, most)) {
     w = (float)weight_of_pick<F>(picked, own_logit, softmax, a.renormalize, most, total) * a.weight_scale;

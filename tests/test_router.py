@@ -667,6 +667,31 @@ def test_route_tokens_tells_picks_from_runners_up(device, scores, experts, group
 
 
 @gpu
+@pytest.mark.parametrize("experts,groups", [(64, 8), (128, 4), (250, 5), (1200, 6)])
+def test_route_tokens_without_a_bias_keeps_the_logits_order(device, experts, groups):
+    """Logits whose sigmoid is 1 in 64 bits too: groups are equal then, experts are not."""
+    gen = torch.Generator().manual_seed(experts)
+    logits = 38 + 60 * torch.rand(50, experts, generator=gen)
+    logits[:, ::3] -= 40
+    more = dict(scores="sigmoid", num_groups=groups, top_groups=2)
+    got, weights = route_tokens(logits.to(device), 6, **more)
+    want, want_weights = ref_route(logits, 6, **more)
+    assert torch.equal(got.view(torch.int32).cpu(), want)
+    assert_within(weights, want_weights, rounded(want_weights, F32, want_weights * weight_error(experts)))
+
+
+@gpu
+def test_route_tokens_with_biases_whose_sums_leave_fp32(device):
+    gen = torch.Generator().manual_seed(4)
+    logits, bias = torch.randn(20, 64, generator=gen), torch.full((64,), -3e38)
+    bias[:32] = 2e38 + 1e38 * torch.rand(32, generator=gen)
+    more = dict(scores="sigmoid", num_groups=8, top_groups=2)
+    got, _ = route_tokens(logits.to(device), 5, bias=bias.to(device), **more)
+    want, _ = ref_route(logits, 5, bias, **more)
+    assert torch.equal(got.view(torch.int32).cpu(), want)
+
+
+@gpu
 @pytest.mark.parametrize("bad", [float("inf"), float("nan")])
 @pytest.mark.parametrize("bias", [False, True])
 def test_route_tokens_of_logits_that_are_no_numbers(device, bad, bias):
