@@ -204,11 +204,11 @@ __global__ __launch_bounds__(WM *WN * 64) void logits_tiles(TilesDev a) {
   }
   // Load number i of a step.  Behind k a lane fetches the first chunk of its line; what it brings is taken for zeros.  Loads of
   // steps that do not exist bring nothing, and count.
-  auto fetch = [&](int i, uint32_t step, uint32_t stage) __attribute__((always_inline)) {
+  auto fetch = [&](auto last, int i, uint32_t step, uint32_t stage) __attribute__((always_inline)) {
     const bool of_a = i < kLoadsA;
     const uint32_t bytes = of_a ? LA::kBytes : LB::kBytes, size = of_a ? sizeof(TA) : sizeof(TB);
     const int8_t *base = (of_a ? first_a : first_b) + (uint64_t)step * bytes;
-    const bool behind = TAIL && step * 64 + chunk[i] * (16 / size) >= a.k;
+    const bool behind = decltype(last)::value && step * 64 + chunk[i] * (16 / size) >= a.k;
     const uint32_t place = of_a ? i * kWaves + wave : (i - kLoadsA) * kWaves + wave;
     load_to_lds(base, behind ? offset[i] - chunk[i] * 16 : offset[i], lds0 + stage * kStage + (of_a ? 0 : kPlaceB) + place * 1024,
                 step < end ? ~0u : 0u);
@@ -216,33 +216,34 @@ __global__ __launch_bounds__(WM *WN * 64) void logits_tiles(TilesDev a) {
   typename Eight<TA>::raw ra[2][MF];
   typename Eight<TB>::raw rb[2][NF];
   constexpr int kReads = MF + NF;
-  auto read_line = [&](auto &to, auto lines, const uint8_t *line, int kk, uint32_t step) __attribute__((always_inline)) {
+  auto read_line = [&](auto last, auto &to, auto lines, const uint8_t *line, int kk, uint32_t step) __attribute__((always_inline)) {
     typedef decltype(lines) L;
     u32x4 v[L::kChunks / 8];
 #pragma unroll
     for (uint32_t h = 0; h < L::kChunks / 8; ++h) {
       const uint32_t c = (2 * kk + lane / 32) * (L::kChunks / 8) + h;
       v[h] = *reinterpret_cast<const u32x4 *>(line + (c ^ L::exchange(lane % 32)) * 16);
-      if constexpr (TAIL) v[h] &= step * 64 + kk * 16 + lane / 32 * 8 < a.k ? ~0u : 0u;
+      if constexpr (decltype(last)::value) v[h] &= step * 64 + kk * 16 + lane / 32 * 8 < a.k ? ~0u : 0u;
     }
     __builtin_memcpy(&to, v, sizeof(v));
   };
-  auto read = [&](int i, int to, int kk, uint32_t step, uint32_t stage) __attribute__((always_inline)) {
+  auto read = [&](auto last, int i, int to, int kk, uint32_t step, uint32_t stage) __attribute__((always_inline)) {
     const uint8_t *lines = lds + stage * kStage;
-    if (i < MF) read_line(ra[to][i], LA{}, lines + (wm * kRows + i * 32 + lane % 32) * LA::kBytes, kk, step);
-    else read_line(rb[to][i - MF], LB{}, lines + kPlaceB + (wn * kColumns + (i - MF) * 32 + lane % 32) * LB::kBytes, kk, step);
+    if (i < MF) read_line(last, ra[to][i], LA{}, lines + (wm * kRows + i * 32 + lane % 32) * LA::kBytes, kk, step);
+    else read_line(last, rb[to][i - MF], LB{}, lines + kPlaceB + (wn * kColumns + (i - MF) * 32 + lane % 32) * LB::kBytes, kk, step);
   };
+  typedef std::bool_constant<TAIL> Tail;
   f32x16 acc[NF][MF] = {};
 #pragma unroll
   for (int s = 0; s < STAGES; ++s) {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) fetch(i, begin + s, s);
+    for (int i = 0; i < kLoads; ++i) fetch(Tail{}, i, begin + s, s);
   }
   wait_loads<(STAGES - 1) * kLoads>();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < kReads; ++i) read(i, 0, 0, begin, 0);
+  for (int i = 0; i < kReads; ++i) read(Tail{}, i, 0, 0, begin, 0);
   typedef Operand<TA, TB> OA;
   typedef Operand<TB, TA> OB;
   constexpr int kMost = OA::count + OB::count - 2 < 2 ? OA::count + OB::count - 2 : 2;
@@ -282,19 +283,27 @@ __global__ __launch_bounds__(WM *WN * 64) void logits_tiles(TilesDev a) {
       }
     }
   };
-  uint32_t stage = 0;
-  for (uint32_t step = begin; step < end; ++step) {
+  uint32_t stage = 0, step = begin;
+  auto take = [&](auto last_read, auto last_fetched) __attribute__((always_inline)) {
     const uint32_t next = stage + 1 == STAGES ? 0 : stage + 1;
 #pragma unroll
     for (int kk = 0; kk < 3; ++kk) {
-      multiply(kk % 2, [&](int r) { read(r, (kk + 1) % 2, kk + 1, step, stage); }, [](int) {});
+      multiply(kk % 2, [&](int r) { read(last_read, r, (kk + 1) % 2, kk + 1, step, stage); }, [](int) {});
     }
     // Loads under way are those of steps step + 1 .. step + STAGES - 1; this step's place is free behind the barrier.
     wait_loads<(STAGES - 2) * kLoads, true>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    multiply(1, [&](int r) { read(r, 0, 0, step + 1, next); }, [&](int l) { fetch(l, step + STAGES, stage); });
+    multiply(1, [&](int r) { read(last_read, r, 0, 0, step + 1, next); }, [&](int l) { fetch(last_fetched, l, step + STAGES, stage); });
     stage = next;
+    ++step;
+  };
+  // (what lies behind k is looked for in the last steps only)
+  const uint32_t last = all_steps - 1;
+  while (step < end && (!TAIL || step + STAGES < last)) take(std::false_type{}, std::false_type{});
+  if constexpr (TAIL) {
+    while (step < end && step + 1 < last) take(std::false_type{}, std::true_type{});
+    while (step < end) take(std::true_type{}, std::true_type{});
   }
   wait_loads<0, true>();
   // Lane l holds row l % 32 of each fragment and columns 4 (l / 32) .. + 3 of every eight.
