@@ -605,13 +605,13 @@ __global__ __launch_bounds__(WAVES * 64) void gradient_of_weight(GradientDev a, 
 #pragma unroll
   for (uint32_t i = 0; i < WAVES; ++i) fa[i].load(from, first + i, all);
   uint32_t buffer = 0, at = begin;
-  auto take = [&](auto last) __attribute__((always_inline)) {
-    constexpr bool kLast = decltype(last)::value;
+  auto take = [&](auto last, auto idle) __attribute__((always_inline)) {
+    constexpr bool kLast = decltype(last)::value, kIdle = decltype(idle)::value;
     b.store(lds + buffer * size + wave * B::kBytes, left_at(at + wave * 16 + half), lane);
     __syncthreads();
     if constexpr (!kLast) b.load(a, there ? column : 0, at + step + wave * 16 + half);
 #pragma unroll
-    for (uint32_t u = 0; u < WAVES; ++u) {
+    for (uint32_t u = 0; u < (kIdle ? 0 : WAVES); ++u) {
       const uint32_t now = at / 16 + u;
       if (!kLast || now < all) multiply_turned<B::kPieces, NV>(fa[u], lds + buffer * size + u * B::kBytes, lane, acc);
       if constexpr (!kLast) fa[u].load(from, now + WAVES, all);
@@ -619,8 +619,14 @@ __global__ __launch_bounds__(WAVES * 64) void gradient_of_weight(GradientDev a, 
     buffer ^= 1;
     at += step;
   };
-  while (at + step < end) take(std::false_type{});
-  take(std::true_type{});
+  // (waves without experts turn rows for the others, and leave the matrix cores to them)
+  if (m0 < a.rows) {
+    while (at + step < end) take(std::false_type{}, std::false_type{});
+    take(std::true_type{}, std::false_type{});
+  } else {
+    while (at + step < end) take(std::false_type{}, std::true_type{});
+    take(std::true_type{}, std::true_type{});
+  }
   if (there && m0 < a.rows) store_turned<O, NV>(a, part * a.out_split, m0, column, lane, acc);
 }
 
