@@ -774,6 +774,11 @@ template <class TB, int ORDER> constexpr int kColumnsOfLane = Pieces<TB, ORDER>:
 struct WeightShares {
   uint32_t waves, row_blocks, parts, tokens_per_part;
 };
+// Into how many parts the tokens go, by cost in us: a start, a step of 16 tokens for each wave, and the parts' sums.  Up to 64 experts
+// leave two of four waves without work for the matrix cores, and a second workgroup costs a compute unit half a step.  The products alone:
+// 8192 x 4096 of 8 in 8 parts 19.1 and in 16 (two to a unit) 14.3; of 64 in fp16 32.5 and 24.6; but 8192 x 2048 of 128 in 16 parts 16.1
+// and in 32 23.3, and 3001 x 7168 of 256 in 4 parts 26.2 and in 8 30.8.  Workgroups of two waves, each in its best parts and with the
+// sums: 8192 x 4096 of 8 17.4 and not 16.9, 4452 x 1960 of 47 in fp32 18.2 and not 18.3, 2000 x 2048 of 60 12.7 and not 8.0.
 WeightShares weight_shares(uint64_t m, uint64_t experts, uint64_t hidden, uint32_t columns) {
   WeightShares w{};
   w.waves = experts > 128 ? 8 : 4;
@@ -783,8 +788,9 @@ WeightShares weight_shares(uint64_t m, uint64_t experts, uint64_t hidden, uint32
   for (uint64_t most = steps; most >= 1; most = most > 8 ? most * 7 / 8 : most - 1) {
     const uint64_t parts = ceil_div(steps, most), per = ceil_div(steps, parts);
     if (parts > 32) break;
-    const double rounds = std::ceil((double)(blocks * parts) / kComputeUnits);
-    const double cost = rounds * ((double)per * (w.waves == 8 ? 3.2 : 1.2) + 2.0) + (parts > 1 ? 2.0 + (double)(parts * experts * hidden) * 8 / 6e6 : 0.0);
+    const double at_once = (double)ceil_div(blocks * parts, kComputeUnits), shared = at_once > 1 && experts <= 64 ? at_once - 0.5 : at_once;
+    const double cost = shared * (double)per * (w.waves == 8 ? 3.2 : 1.2) + 2.0 * at_once +
+                        (parts > 1 ? 2.0 + (double)(parts * experts * hidden) * 8 / 6e6 : 0.0);
     if (w.parts == 0 || cost < least) {
       least = cost;
       w.parts = (uint32_t)parts;
