@@ -593,8 +593,14 @@ extern "C" int pplx_a2a_rms_norm_backward(int device, const pplx_a2a_rms_norm_ba
       constexpr bool kAhead = sizeof(T) == 2;  // (32 elements of fp32 in a thread fill its registers once)
       W *out = static_cast<W *>(p.grad_weight);
       if (a.width > kMostInRegisters) {
-        PPLX_LAUNCH(launch_kernel(norm_backward_long<T, W>, dim3(groups), dim3(kLongLanes), 0, s, a));
+        // (the weight's gradient reads grad_y once more: grad_h over it comes last, by a launch of its own)
+        const bool over = out && a.grad_h && a.grad_h == a.grad_y;
+        NormBackwardDev first = a;
+        if (over) first.grad_h = nullptr;
+        PPLX_LAUNCH(launch_kernel(norm_backward_long<T, W>, dim3(groups), dim3(kLongLanes), 0, s, first));
         if (out) PPLX_LAUNCH(launch_kernel(norm_weight_gradient_long<T, W>, dim3(columns), dim3(kSumThreads), 0, s, a, out));
+        a.partial = nullptr;
+        if (over) PPLX_LAUNCH(launch_kernel(norm_backward_long<T, W>, dim3(groups), dim3(kLongLanes), 0, s, a));
         return (int)PPLX_A2A_OK;
       }
       if (a.width <= 512) PPLX_LAUNCH(launch_kernel(norm_backward_rows<T, W, 64, 1, true>, dim3(groups), dim3(256), 0, s, a));

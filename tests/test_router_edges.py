@@ -265,3 +265,17 @@ def test_gradients_with_picks_taken_out(device):
     few = at[:, [0, 1, 3]].contiguous().view(torch.uint32)
     want = route_tokens_backward(grad[:, [0, 1, 3]].contiguous(), logits, few, renormalize=False)
     assert torch.isfinite(got).all() and same(got, want) and (got[5] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("hidden", [256, 2048, 7168, 16384, 20000])
+@pytest.mark.parametrize("over_sum", [False, True])
+def test_the_gradient_of_a_norm_over_its_own_operand(device, hidden, over_sum):
+    """Into grad_y or grad_sum, beside the weight's gradient: the bits that buffers of their own get."""
+    gen = torch.Generator().manual_seed(hidden)
+    h, grad, grad_sum = (torch.randn(37, hidden, generator=gen).to(torch.bfloat16).to(device) for _ in range(3))
+    weight = torch.randn(hidden, generator=gen).to(device)
+    want, want_weight = rms_norm_backward(grad, h, weight, grad_sum=grad_sum)
+    over, of_weight = (grad_sum if over_sum else grad), torch.empty_like(weight)
+    rms_norm_backward(grad, h, weight, grad_sum=grad_sum, out=(over, of_weight))
+    assert torch.equal(over, want) and torch.equal(of_weight, want_weight)
