@@ -7,7 +7,7 @@
 // A wave takes a token, whose logits it reads once.  What bounds it is the instructions of the choice, six dependent steps over the wave for
 // each pick, 0.16 us of a wave: 256 experts in fp32, a pick and eight, us in a graph: 64 tokens 2.4 and 3.5, with scores and biases
 // 3.0 and 4.3, with groups too 3.8 and 5.0; 8192 tokens 3.7 and 6.9 (1.2 TB/s of logits), with scores and biases 5.6 and 11.6, with
-// groups too 7.8 and 14.2, of which some tokens' second choice is 2 to 4.
+// groups too 7.8 and 15.1, of which some tokens' second choice is 2 to 4.
 #include <cfloat>
 #include <climits>
 #include <cmath>
@@ -372,10 +372,15 @@ __device__ __forceinline__ bool choose(const PicksDev &a, uint32_t t, uint32_t l
     }
     const bool taken = before < a.top_groups;
     if (kWatched) {
-      // Of the groups that are taken the last, and the first of the others.
-      const float last = -wave_max_of_lanes(taken ? -(float)sum : kNoLogit);
-      const float next = wave_max_of_lanes(taken || group >= a.groups ? kNoLogit : (float)sum);
-      near |= next > kNoLogit && are_near(last, next, 2 * off);
+      // Of the groups that are taken the least that the last may come to, and the most of the others.  Keys round by their own size, which
+      // the sum of two of different signs does not show.  (A sum that fp32 does not hold is not told; one of a single expert is -inf.)
+      const bool whole = a.group_top == 1 ? first > (F)kNone : second > (F)kNone;
+      const float size = a.group_top == 1 ? __builtin_fabsf((float)first) : __builtin_fabsf((float)first) + __builtin_fabsf((float)second);
+      const float error = __builtin_fmaf(0x1p-22f, size, off);
+      near |= whole && !(size <= FLT_MAX);
+      const float last = -wave_max_of_lanes(!taken ? kNoLogit : whole ? error - (float)sum : HUGE_VALF);
+      const float next = wave_max_of_lanes(taken || !whole ? kNoLogit : (float)sum + error);
+      near |= next > kNoLogit && !(last > next);
     }
 #pragma unroll
     for (int j = 0; j < PER; ++j) {

@@ -279,3 +279,37 @@ def test_the_gradient_of_a_norm_over_its_own_operand(device, hidden, over_sum):
     over, of_weight = (grad_sum if over_sum else grad), torch.empty_like(weight)
     rms_norm_backward(grad, h, weight, grad_sum=grad_sum, out=(over, of_weight))
     assert torch.equal(over, want) and torch.equal(of_weight, want_weight)
+
+
+def groups_by_sums(logits, bias, groups, top, k):
+    """Choices of `k` in 64 bits, by the two best keys of each group."""
+    keys = torch.sigmoid(logits.double()) + bias.double()
+    sums = keys.view(len(keys), groups, -1).topk(2, 2).values.sum(2)
+    inside = torch.zeros(sums.shape, dtype=torch.bool).scatter_(1, sums.sort(dim=1, descending=True, stable=True).indices[:, :top], True)
+    keys = torch.where(inside.repeat_interleave(keys.shape[1] // groups, 1), keys, float("-inf"))
+    return keys.sort(dim=1, descending=True, stable=True).indices[:, :k].to(torch.int32)
+
+
+@gpu
+@pytest.mark.parametrize("experts,groups", [(32, 4), (256, 8), (250, 5), (512, 64)])
+def test_groups_whose_sums_fp32_holds_for_nothing(device, experts, groups):
+    """Two biases around -3e38 leave fp32 at its lower end: the group is there all the same."""
+    gen = torch.Generator().manual_seed(experts)
+    logits = torch.randn(20, experts, generator=gen)
+    bias = -3e38 + 1e38 * torch.rand(experts, generator=gen)
+    got, _ = route_tokens(logits.to(device), 3, bias=bias.to(device), scores="sigmoid", num_groups=groups, top_groups=2)
+    assert torch.equal(got.view(torch.int32).cpu(), groups_by_sums(logits, bias, groups, 2, 3))
+
+
+@gpu
+@pytest.mark.parametrize("experts,groups", [(32, 4), (256, 8), (250, 5), (512, 64)])
+@pytest.mark.parametrize("size", [100.0, 3e4])
+def test_groups_whose_best_two_cancel(device, experts, groups, size):
+    """Keys are rounded by their size, which the sum of two does not show."""
+    gen = torch.Generator().manual_seed(experts)
+    logits = torch.randn(2000, experts, generator=gen)
+    bias = torch.full((groups, experts // groups), -1e6)
+    bias[:, 0], bias[:, 1] = -size, size
+    bias = bias.flatten()
+    got, _ = route_tokens(logits.to(device), 3, bias=bias.to(device), scores="sigmoid", num_groups=groups, top_groups=2)
+    assert torch.equal(got.view(torch.int32).cpu(), groups_by_sums(logits, bias, groups, 2, 3))
