@@ -659,7 +659,8 @@ template <class K> void allow_lds(K *kernel, uint32_t bytes) {
 //   bf16, fp32      16384 x 8 x 4096  38.4 (4) / 60.4 (1)    4096 x 32 x 2048  12.8 (8) / 13.6 (4)   64 x 8 x 4096  7.9 (32) / 8.7 (16)
 //   both fp32       16384 x 8 x 4096  63.5 (2) / 89.0 (2)    4096 x 32 x 2048  14.4 (8) / 17.8 (4)   both bf16, 16384 x 8 x 4096  30.4 (4) / 29.1 (4)
 // What bounds a tile of 128 x 128 is what a compute unit fetches into its LDS, 31 bytes a cycle: 0.43 us a step with rows in L2, and
-// 0.63 with rows out of HBM, whose latency its four steps do not cover.  Larger tiles fetch less and hold fewer steps: 128 x 256 and
+// 0.63 with rows out of HBM.  (Not for their latency: with a wave of its own that reads them into L2 one to eight steps ahead,
+// 16384 x 512 x 7168 takes 147 to 151 and not 145.)  Larger tiles fetch less and hold fewer steps: 128 x 256 and
 // 256 x 128 take 1.1 us a step, 256 x 256 1.4.  Tiles of 64 x 192, 64 x 256, 32 x 64 and 32 x 128 were within 5 % of the best of
 // these, or slower, in all of thirty products.
 // product_split, which is one launch: 4 x 64 x 2048 4.3 (tiles 5.8), 1 x 256 x 7168 9.5 (6.5), 64 x 256 x 7168 14.2, with fp32
