@@ -381,6 +381,13 @@ __device__ __forceinline__ bool choose(const PicksDev &a, uint32_t t, uint32_t l
       const float last = -wave_max_of_lanes(!taken ? kNoLogit : whole ? error - (float)sum : HUGE_VALF);
       const float next = wave_max_of_lanes(taken || !whole ? kNoLogit : (float)sum + error);
       near |= next > kNoLogit && !(last > next);
+    } else if (!SCORED) {
+      // Groups by their largest logit: the order of the scores, but where two of these are one in 64 bits.  They are not for logits 2^-20
+      // apart, of which the less is not beyond 12 (a sigmoid's slope is 2^-18 there) and the larger one's exponential is a normal number.
+      const float last = -wave_max_of_lanes(taken ? -(float)sum : kNoLogit), mine = (float)sum;
+      const float more = mine > last ? mine : last, less = mine > last ? last : mine;
+      const bool apart = more - less > 0x1p-20f && (softmax ? more - most > -700.f : less < 12.f && more > -700.f);
+      near |= group < a.groups && mine != last && less > kNoLogit && !apart;
     }
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
@@ -446,7 +453,7 @@ __device__ __forceinline__ bool choose(const PicksDev &a, uint32_t t, uint32_t l
       }
     }
   }
-  if (kWatched && __ballot(near)) return false;
+  if (sizeof(F) == 4 && __ballot(near)) return false;
   float w;
   if (sizeof(F) == 4 && picks_are_near(picked, own_logit, most)) {
     w = (float)weight_of_pick<F>(picked, own_logit, softmax, a.renormalize, most, total) * a.weight_scale;
@@ -488,7 +495,7 @@ template <class T, int PER, bool SCORED> __global__ __launch_bounds__(64 * kToke
   if (__ballot(bad)) return store_bad(a, t, lane);
   most = wave_max_of_lanes(most);
   if (choose<float, PER, SCORED>(a, t, lane, group, base, l, bias, most)) return;
-  if constexpr (SCORED) choose<double, PER, true>(a, t, lane, group, base, l, bias, most);
+  choose<double, PER, true>(a, t, lane, group, base, l, bias, most);
 }
 
 struct PicksBackwardDev {

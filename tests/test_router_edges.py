@@ -313,3 +313,25 @@ def test_groups_whose_best_two_cancel(device, experts, groups, size):
     bias = bias.flatten()
     got, _ = route_tokens(logits.to(device), 3, bias=bias.to(device), scores="sigmoid", num_groups=groups, top_groups=2)
     assert torch.equal(got.view(torch.int32).cpu(), groups_by_sums(logits, bias, groups, 2, 3))
+
+
+@gpu
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts,groups", [(32, 4), (128, 2), (250, 5), (512, 64), (1200, 6), (1320, 330)])
+def test_groups_by_their_best_expert_where_scores_meet(device, scores, experts, groups):
+    """Scores of different logits that are one in 64 bits: near 1, near 0, of logits near 0, and beside ones that are not."""
+    gen = torch.Generator().manual_seed(experts)
+    size = experts // groups
+    logits = torch.randn(120, experts, generator=gen) - 40
+    best = torch.randn(120, groups, generator=gen)
+    best[:30] = 10 + 40 * torch.rand(30, groups, generator=gen)  # sigmoids that meet, and ones that do not
+    best[30:60] = 1e-30 * best[30:60].round()  # 0.5, or one exponential
+    best[60:90] = best[60:90].round() * (1 + 2.0**-23 * torch.randint(0, 2, (30, groups), generator=gen))  # a last bit apart
+    logits.view(120, groups, size)[:, :, size // 2] = best
+    logits[90:105] = logits[90:105] * 30 - 800  # sigmoids of 0
+    for top in (1, groups // 2):
+        more = dict(scores=scores, num_groups=groups, top_groups=top, group_top=1)
+        got, weights = route_tokens(logits.to(device), 2, **more)
+        want, want_weights = ref_route(logits, 2, **more)
+        assert torch.equal(got.view(torch.int32).cpu(), want)
+        assert torch.isfinite(weights).all()
