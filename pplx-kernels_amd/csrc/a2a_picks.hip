@@ -308,6 +308,7 @@ __device__ __forceinline__ void load_some(const PPLX_GLOBAL T *row, uint32_t bas
   }
 }
 
+constexpr int kMostExperts = 16;  // of a lane
 // A token's choice in F, with its logits and biases in registers: of experts `base` on in this lane, which are of `group`.  False,
 // with nothing stored, if fp32 doesn't tell.  SCORED: keys (with a bias) or the groups' sums are scores, not logits.
 template <class F, int PER, bool SCORED>
@@ -315,7 +316,7 @@ __device__ __forceinline__ bool choose(const PicksDev &a, uint32_t t, uint32_t l
                                        const float *bias, float most) {
   constexpr bool kWatched = SCORED && sizeof(F) == 4;
   typedef decltype(order_of(F())) Order;
-  const bool softmax = a.scores == PPLX_A2A_SOFTMAX, grouped = a.top_groups < a.groups;
+  const bool softmax = a.scores == PPLX_A2A_SOFTMAX, grouped = (SCORED || PER < kMostExperts) && a.top_groups < a.groups;
   const Order none = order_of((F)kNone);
   F score[PER], total = 0;
   if (softmax && (SCORED || !a.renormalize)) {
@@ -495,7 +496,7 @@ template <class T, int PER, bool SCORED> __global__ __launch_bounds__(64 * kToke
   if (__ballot(bad)) return store_bad(a, t, lane);
   most = wave_max_of_lanes(most);
   if (choose<float, PER, SCORED>(a, t, lane, group, base, l, bias, most)) return;
-  choose<double, PER, true>(a, t, lane, group, base, l, bias, most);
+  if constexpr (SCORED || PER < kMostExperts) choose<double, PER, true>(a, t, lane, group, base, l, bias, most);
 }
 
 struct PicksBackwardDev {
@@ -645,7 +646,7 @@ extern "C" int pplx_a2a_route_tokens(int device, const pplx_a2a_route_args_t *ar
   return guarded(device, [&] {
     return with_type(p.dtype, [&](auto tag) {
       typedef typename decltype(tag)::type T;
-      const bool grouped = a.top_groups < a.groups, scored = a.bias || (grouped && a.group_top > 1);
+      const bool grouped = a.top_groups < a.groups;
       // Experts of a lane: as few as hold all of them, where no lane has some of two groups, whose lanes are a power of two.  (More
       // experts in a lane make its choice of the next one longer: 64 tokens of 256 experts 5.0 us, of 512 in 64 groups 8.0.)  What sixteen to
       // a lane do not hold is chosen for in LDS in 64 bits.
@@ -656,10 +657,10 @@ extern "C" int pplx_a2a_route_tokens(int device, const pplx_a2a_route_args_t *ar
         while (lanes * per < size) lanes *= 2;
         return lanes;
       };
-      while (per <= 16 && (grouped ? (uint64_t)a.groups * lanes_of_group() > 64 : a.experts > 64 * per)) per *= 2;
+      while (per <= kMostExperts && (grouped ? (uint64_t)a.groups * lanes_of_group() > 64 : a.experts > 64 * per)) per *= 2;
       a.group_lanes = grouped ? lanes_of_group() : 64;
       a.lanes_shift = (uint32_t)__builtin_ctz(a.group_lanes);
-      if (per > 16) {
+      if (per > kMostExperts) {
         // (5461 experts in as many groups take 85 KiB)
         const uint32_t lds = 8 * (a.experts + (grouped ? a.groups : 0));
         auto kernel = pick_experts_exactly<T>;
@@ -671,6 +672,8 @@ extern "C" int pplx_a2a_route_tokens(int device, const pplx_a2a_route_args_t *ar
         PPLX_LAUNCH(launch_groups(kernel, kernel, a.m, 64, lds, (hipStream_t)stream, a));
         return (int)PPLX_A2A_OK;
       }
+      // (a choice in 64 bits that may follow one of sixteen logits in a lane takes more registers than there are: groups of so many go by scores)
+      const bool scored = a.bias || (grouped && (a.group_top > 1 || per == kMostExperts));
       auto launch = [&](auto count) {
         constexpr int PER = decltype(count)::value;
         auto kernel = scored ? pick_experts<T, PER, true> : pick_experts<T, PER, false>;
@@ -683,7 +686,7 @@ extern "C" int pplx_a2a_route_tokens(int device, const pplx_a2a_route_args_t *ar
         case 2: return launch(std::integral_constant<int, 2>{});
         case 4: return launch(std::integral_constant<int, 4>{});
         case 8: return launch(std::integral_constant<int, 8>{});
-        default: return launch(std::integral_constant<int, 16>{});
+        default: return launch(std::integral_constant<int, kMostExperts>{});
       }
     });
   });

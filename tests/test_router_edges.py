@@ -317,7 +317,7 @@ def test_groups_whose_best_two_cancel(device, experts, groups, size):
 
 @gpu
 @pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
-@pytest.mark.parametrize("experts,groups", [(32, 4), (128, 2), (250, 5), (512, 64), (1200, 6), (1320, 330)])
+@pytest.mark.parametrize("experts,groups", [(32, 4), (128, 2), (250, 5), (512, 64), (1000, 4), (1200, 6), (1320, 330)])
 def test_groups_by_their_best_expert_where_scores_meet(device, scores, experts, groups):
     """Scores of different logits that are one in 64 bits: near 1, near 0, of logits near 0, and beside ones that are not."""
     gen = torch.Generator().manual_seed(experts)
