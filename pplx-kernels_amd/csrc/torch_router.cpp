@@ -402,18 +402,52 @@ Normed normed_rows_meta(const at::Tensor &x, const at::Tensor &, opt_tensor resi
           residual ? fresh_traced(x.sym_sizes(), x, x.scalar_type()) : fresh({0}, x, x.scalar_type())};
 }
 
+// (y, sum, q, scale): rows in int8, or else e4m3; without a residual there is no sum (of the registered op: it is empty)
+using Quantized = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
+Quantized empty_quantized(const at::Tensor &x, bool add, bool int8) {
+  TORCH_CHECK(x.dim() == 2, "Tensor x must be 2 dimensional");
+  const c10::SymInt m = x.sym_size(0), h = x.sym_size(1);
+  return {fresh_traced({m, h}, x, x.scalar_type()), add ? fresh_traced({m, h}, x, x.scalar_type()) : at::Tensor(),
+          fresh_traced({m, h}, x, int8 ? at::kChar : at::kFloat8_e4m3fn),
+          int8 ? fresh_traced({m}, x, at::kFloat) : fresh_traced({m, (h + (kBlock - 1)) / kBlock}, x, at::kFloat)};
+}
+Quantized quantized_rows_op(const at::Tensor &x, const at::Tensor &weight, opt_tensor residual, double eps, bool int8) {
+  TORCH_CHECK(x.is_cuda(), "Tensor x must be on GPU");
+  Quantized made = empty_quantized(x, residual.has_value(), int8);
+  auto &[y, sum, q, scale] = made;
+  rms_norm(&y, defined(sum), &q, &scale, x, weight, opt(residual), eps);
+  if (!residual) sum = fresh({0}, x, x.scalar_type());
+  return made;
+}
+Quantized quantized_rows_meta(const at::Tensor &x, const at::Tensor &, opt_tensor residual, double, bool int8) {
+  Quantized made = empty_quantized(x, residual.has_value(), int8);
+  if (!residual) std::get<1>(made) = fresh({0}, x, x.scalar_type());
+  return made;
+}
+
+// Of both: `format` is pplx_a2a_row_format, and with rows in 8 bits these and their scales, which have no gradient, come behind y and sum.
 struct NormFunction : torch::autograd::Function<NormFunction> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x, const at::Tensor &weight,
-                                                const std::optional<at::Tensor> &residual, double eps) {
+                                                const std::optional<at::Tensor> &residual, double eps, int64_t format) {
     at::AutoDispatchBelowADInplaceOrView below;
-    static auto op = op_handle<Normed(const at::Tensor &, const at::Tensor &, opt_tensor, double)>("pplx_kernels::normed_rows");
-    auto [y, sum] = op.call(x, weight, residual, eps);
-    ctx->save_for_backward({residual ? sum : x, weight});
+    torch::autograd::variable_list made, fixed;
+    if (format == PPLX_A2A_ROWS_PLAIN) {
+      static auto op = op_handle<decltype(normed_rows_op)>("pplx_kernels::normed_rows");
+      auto [y, sum] = op.call(x, weight, residual, eps);
+      made = {y, sum};
+    } else {
+      static auto op = op_handle<decltype(quantized_rows_op)>("pplx_kernels::quantized_rows");
+      auto [y, sum, q, scale] = op.call(x, weight, residual, eps, format == PPLX_A2A_ROWS_INT8);
+      made = {y, sum, q, scale};
+      fixed = {q, scale};
+    }
+    if (!residual) fixed.push_back(made[1]);
+    ctx->save_for_backward({residual ? made[1] : x, weight});
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["add"] = residual.has_value();
-    if (!residual) ctx->mark_non_differentiable({sum});
+    ctx->mark_non_differentiable(fixed);
     ctx->set_materialize_grads(false);
-    return {y, sum};
+    return made;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
@@ -432,14 +466,19 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
     } else if (grads[1].defined()) {
       grad_h = grads[1];  // (of the sum alone)
     }
-    return differentiable_once({for_x ? grad_h : at::Tensor(), grad_weight, for_residual ? grad_h : at::Tensor(), at::Tensor()},
-                               kDifferentiable);
+    return differentiable_once(
+        {for_x ? grad_h : at::Tensor(), grad_weight, for_residual ? grad_h : at::Tensor(), at::Tensor(), at::Tensor()}, kDifferentiable);
   }
 };
 Normed normed_rows_autograd(const at::Tensor &x, const at::Tensor &weight, opt_tensor residual, double eps) {
   check_no_tangent({&x, &weight, opt(residual)}, kDifferentiable);
-  auto made = NormFunction::apply(x, weight, residual, eps);
+  auto made = NormFunction::apply(x, weight, residual, eps, (int64_t)PPLX_A2A_ROWS_PLAIN);
   return {made[0], made[1]};
+}
+Quantized quantized_rows_autograd(const at::Tensor &x, const at::Tensor &weight, opt_tensor residual, double eps, bool int8) {
+  check_no_tangent({&x, &weight, opt(residual)}, kDifferentiable);
+  auto made = NormFunction::apply(x, weight, residual, eps, (int64_t)(int8 ? PPLX_A2A_ROWS_INT8 : PPLX_A2A_ROWS_E4M3));
+  return {made[0], made[1], made[2], made[3]};
 }
 
 at::Tensor new_logits_op(const at::Tensor &x, const at::Tensor &weight) {
@@ -583,6 +622,9 @@ TORCH_LIBRARY_FRAGMENT(pplx_kernels, m) {
          &route_tokens_backward_op);
   define_differentiable(m, "normed_rows", "(Tensor x, Tensor weight, Tensor? residual, float eps) -> (Tensor, Tensor)",
                         &normed_rows_op, &normed_rows_meta, &normed_rows_autograd);
+  define_differentiable(m, "quantized_rows",
+                        "(Tensor x, Tensor weight, Tensor? residual, float eps, bool int8) -> (Tensor, Tensor, Tensor, Tensor)",
+                        &quantized_rows_op, &quantized_rows_meta, &quantized_rows_autograd);
   define_differentiable(m, "new_logits", "(Tensor x, Tensor weight) -> Tensor", &new_logits_op, &new_logits_meta, &new_logits_autograd);
   define_differentiable(m, "routed_tokens",
                         "(Tensor logits, int experts_per_token, Tensor? bias, Tensor? bound_m, int num_groups, int top_groups, "
@@ -671,20 +713,20 @@ PyObject *py_normed_rows(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// quantized_rows(x, weight, residual, eps, int8) -> (y, sum, q, scale): rows in int8, or else e4m3
+// quantized_rows(x, weight, residual, eps, int8, record) -> (y, sum, q, scale): rows in int8, or else e4m3; y and sum are
+// differentiable if `record`
 PyObject *py_quantized_rows(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  arity("quantized_rows", nargs, 5);
+  arity("quantized_rows", nargs, 6);
   const at::Tensor &x = tensor_arg(args[0], "x"), &weight = tensor_arg(args[1], "weight");
   const at::Tensor *residual = optional_tensor_arg(args[2], "residual");
   const double eps = float_arg(args[3], "eps");
-  const bool int8 = bool_arg(args[4]);
-  TORCH_CHECK(x.dim() == 2, "Tensor x must be 2 dimensional");
-  const c10::SymInt m = x.sym_size(0), h = x.sym_size(1);
-  const at::Tensor y = fresh_traced({m, h}, x, x.scalar_type());
-  const at::Tensor sum = residual ? fresh_traced({m, h}, x, x.scalar_type()) : at::Tensor();
-  const at::Tensor q = fresh_traced({m, h}, x, int8 ? at::kChar : at::kFloat8_e4m3fn);
-  const at::Tensor scale = int8 ? fresh_traced({m}, x, at::kFloat) : fresh_traced({m, (h + (kBlock - 1)) / kBlock}, x, at::kFloat);
+  const bool int8 = bool_arg(args[4]), record = bool_arg(args[5]);
+  if (record) {
+    const auto [y, sum, q, scale] = quantized_rows_autograd(x, weight, maybe(residual), eps, int8);
+    return normed(y, residual ? sum : at::Tensor(), q, scale);
+  }
+  const auto [y, sum, q, scale] = empty_quantized(x, residual, int8);
   if (straight({&x, &weight, residual})) {
     rms_norm(&y, defined(sum), &q, &scale, x, weight, residual, eps);
   } else {
@@ -855,7 +897,7 @@ PyObject *py_router_build_id(PyObject *, PyObject *) { return PyUnicode_FromStri
 PyMethodDef kRouterMethods[] = {
     {"rms_norm", PPLX_FASTCALL(py_rms_norm), "rms_norm(y, sum, q, scale, x, weight, residual, eps)"},
     {"normed_rows", PPLX_FASTCALL(py_normed_rows), "normed_rows(x, weight, residual, eps, record) -> (y, sum, None, None)"},
-    {"quantized_rows", PPLX_FASTCALL(py_quantized_rows), "quantized_rows(x, weight, residual, eps, int8) -> (y, sum, q, scale)"},
+    {"quantized_rows", PPLX_FASTCALL(py_quantized_rows), "quantized_rows(x, weight, residual, eps, int8, record) -> (y, sum, q, scale)"},
     {"rms_norm_backward", PPLX_FASTCALL(py_rms_norm_backward),
      "rms_norm_backward(grad_h, grad_weight, grad_y, grad_sum, h, weight, eps, workspace)"},
     {"rms_norm_workspace", PPLX_FASTCALL(py_rms_norm_workspace), "rms_norm_workspace(tokens, width) -> bytes that its gradients take"},

@@ -6,9 +6,10 @@ experts with its weights, with the gradients of all three.
     indices, weights = route_tokens(logits, 8, bias=bias, scores="sigmoid", num_groups=8, top_groups=4, scale=2.5)
     ata.dispatch(..., dp_x=n.q, dp_x_scale=n.scale, indices=indices)        # and weights to combine
 
-A rank that holds its experts itself gives ``indices`` and ``weights`` to ``sort_tokens`` and ``unsort_tokens``; all of it is
-differentiable, so the same calls make a training step.  Calls run on the current stream of the tensors' device and keep nothing
-between calls.  With ``out=``, and ``workspace=`` where there is one, a call allocates nothing and can be captured as it is; without
+A rank that holds its experts itself gives ``indices`` and ``weights`` to ``sort_tokens`` and ``unsort_tokens``, with rows of ``n.y``.
+``n.y``, ``n.sum``, the logits and the weights are differentiable, and so are the sorted rows and their sum, so that the same calls
+make a training step; ``n.q`` and ``n.scale`` have no gradient, and ``dispatch`` and ``combine`` pass none on.  Calls run on the current
+stream of the tensors' device and keep nothing between calls.  With ``out=``, and ``workspace=`` where there is one, a call allocates nothing and can be captured as it is; without
 ``workspace`` it takes that from torch's allocator, which keeps it for a graph that torch captures, not for one that
 ``LoopbackWorld.capture`` does.  Gradients are those of reverse mode; under capture they go through the ``_backward`` functions.
 """
@@ -87,8 +88,8 @@ def rms_norm(
     an infinity or a NaN becomes NaN (``q`` zeros, its scales NaN).
 
     ``x`` is ``[m, H]`` of float32, bfloat16 or float16, its rows 16-byte aligned and ``H`` a multiple of 8 (with ``quantize`` of 16);
-    ``weight`` is ``[H]`` of its type or float32.  Differentiable in ``x``, ``residual`` and ``weight``, through ``y`` and ``sum``, unless
-    ``quantize`` or ``out`` is given.  ``out`` may leave ``y`` out (None) where it has ``q``, and ``y`` and ``sum`` may be ``x`` and
+    ``weight`` is ``[H]`` of its type or float32.  Differentiable in ``x``, ``residual`` and ``weight``, through ``y`` and ``sum`` (``q`` and
+    ``scale`` have no gradient), unless ``out`` is given.  ``out`` may leave ``y`` out (None) where it has ``q``, and ``y`` and ``sum`` may be ``x`` and
     ``residual`` themselves."""
     if out is not None:
         if quantize is not None and (out.q is None or out.q.dtype != quantize):
@@ -98,13 +99,13 @@ def rms_norm(
         return out
     if quantize is not None:
         _check_quantize(quantize)
-        x, weight, residual = (t if t is None or not t.requires_grad else t.detach() for t in (x, weight, residual))
-        if not _is_compiling():
-            return NormedRows._make(_C.quantized_rows(x, weight, residual, eps, quantize == torch.int8))
-        if x.dim() != 2:
-            raise RuntimeError("Tensor x must be 2 dimensional")
-        made = NormedRows.empty(*x.shape, x.dtype, x.device, residual=residual is not None, quantize=quantize)
-        return rms_norm(x, weight, residual, eps=eps, out=made)
+        if _is_compiling():
+            y, total, q, scale = _ops.quantized_rows(x, weight, residual, eps, quantize == torch.int8)
+            return NormedRows(y, None if residual is None else total, q, scale)
+        record = _wants_grad(x, weight, residual)
+        if record:
+            _check_recording(x)
+        return NormedRows._make(_C.quantized_rows(x, weight, residual, eps, quantize == torch.int8, record))
     if _is_compiling():
         y, total = _ops.normed_rows(x, weight, residual, eps)
         return NormedRows(y, None if residual is None else total)

@@ -1,0 +1,143 @@
+"""Gradients of the operators before dispatch that come by less common ways: beside rows in 8 bits."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+from pplx_kernels import rms_norm, route_tokens, router_logits
+from tests.test_experts import BF16, F16, F32
+from tests.test_router import E4M3
+from tests.test_router_path import make_step, same
+
+gpu = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------
+# Rows in 8 bits: y and sum beside them are differentiable
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("quantize", [torch.int8, E4M3])
+@pytest.mark.parametrize("which", ["x", "weight", "residual"])
+def test_quantised_norms_are_recorded(quantize, which):
+    """Without a device: tensors that have none of their data."""
+    made = {name: torch.empty(*shape, device="meta") for name, shape in (("x", (6, 256)), ("weight", (256,)), ("residual", (6, 256)))}
+    made[which].requires_grad_(True)
+    for residual in (made["residual"], None) if which != "residual" else (made["residual"],):
+        n = rms_norm(made["x"], made["weight"], residual, quantize=quantize)
+        assert n.y.requires_grad and not n.q.requires_grad and not n.scale.requires_grad
+        assert n.q.dtype == quantize and n.scale.shape == ((6,) if quantize == torch.int8 else (6, 2))
+        assert n.sum is None if residual is None else n.sum.requires_grad
+        with torch.no_grad(), pytest.raises(RuntimeError, match="must be on GPU"):  # (nothing to record: the call itself)
+            rms_norm(made["x"], made["weight"], residual, quantize=quantize)
+
+
+def check_tangents_of_quantised_norms(device):
+    x, weight = torch.ones(4, 16, device=device), torch.ones(16, device=device)
+    with forward_ad.dual_level():
+        dx, dw = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, weight))
+        for quantize in (torch.int8, E4M3):
+            for args in ((dx, weight), (x, dw), (x, weight, dx)):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    rms_norm(*args, quantize=quantize)
+                with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                    rms_norm(*args, quantize=quantize)
+
+
+def test_tangents_of_quantised_norms_are_refused_before_the_device_is_looked_at():
+    check_tangents_of_quantised_norms("cpu")
+
+
+@gpu
+def test_tangents_of_quantised_norms_are_refused(device):
+    check_tangents_of_quantised_norms(device)
+
+
+@gpu
+@pytest.mark.parametrize("quantize", [torch.int8, E4M3])
+@pytest.mark.parametrize("m,hidden,dtype,weight_dtype", [
+    (1, 16, F32, F32), (33, 528, F16, F16), (70, 2048, BF16, F32), (9, 7168, BF16, BF16), (3, 20000, F16, F32), (0, 64, BF16, BF16),
+])  # fmt: skip
+@pytest.mark.parametrize("add", [False, True])
+def test_gradients_through_quantised_norms(device, m, hidden, dtype, weight_dtype, add, quantize):
+    """The bits that the norm without rows in 8 bits gives, results and gradients."""
+    gen = torch.Generator().manual_seed(hidden)
+    x, residual, weight, *_ = make_step(device, gen, m, hidden, 4, dtype, weight_dtype)
+    grads = [torch.randn(m, hidden, generator=gen).to(dtype).to(device) for _ in range(1 + add)]
+    got = []
+    for more in (dict(), dict(quantize=quantize)):
+        leaves = [t.detach().requires_grad_(True) for t in ((x, weight, residual) if add else (x, weight))]
+        n = rms_norm(*leaves, **more)
+        outs = [n.y, n.sum] if add else [n.y]
+        got.append([t.detach() for t in outs] + list(torch.autograd.grad(outs, leaves, grads, retain_graph=True)))
+        if add:  # of the sum alone
+            got[-1] += torch.autograd.grad(n.sum, leaves[::2], grads[1])
+    assert all(same(a, b) for a, b in zip(*got))
+    assert not n.q.requires_grad and not n.scale.requires_grad
+    with torch.no_grad():  # and the rows themselves are those of a call that records nothing
+        plain = rms_norm(x, weight, residual if add else None, quantize=quantize)
+        assert same(plain.q, n.q) and same(plain.scale, n.scale) and not plain.y.requires_grad
+
+
+@gpu
+def test_quantised_norms_under_autograd(device):
+    """Differentiable once, told of what changed, refused under capture."""
+    gen = torch.Generator().manual_seed(4)
+    x, residual, weight, *_ = make_step(device, gen, 9, 64, 8, F32)
+    leaf = x.clone().requires_grad_(True)
+    (got,) = torch.autograd.grad(rms_norm(leaf, weight, quantize=torch.int8).y.square().sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        got.sum().backward()
+    n = rms_norm(leaf * 1.0, weight, residual, quantize=E4M3)
+    with torch.no_grad():
+        n.sum.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        n.y.sum().backward()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        with pytest.raises(RuntimeError, match="not recorded under stream capture"):
+            rms_norm(leaf, weight, quantize=torch.int8)
+        with torch.no_grad():
+            captured = rms_norm(leaf, weight, quantize=torch.int8)
+    for _ in range(3):
+        captured.y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = rms_norm(x, weight, quantize=torch.int8)
+        assert same(captured.y, eager.y) and same(captured.q, eager.q) and same(captured.scale, eager.scale)
+
+
+@gpu
+@pytest.mark.parametrize("quantize", [torch.int8, E4M3])
+def test_a_step_whose_rows_are_sent_in_8_bits_trains_its_router(device, quantize):
+    """The norm that makes the rows for dispatch makes the router's rows too: gradients reach x, the residual and the norm's weight."""
+    gen = torch.Generator().manual_seed(5)
+    x, residual, norm_weight, gate, bias = make_step(device, gen, 40, 256, 16, BF16, F32)
+    results = []
+    for more in (dict(), dict(quantize=quantize)):
+        leaves = [t.detach().requires_grad_(True) for t in (x, residual, norm_weight, gate)]
+        n = rms_norm(leaves[0], leaves[2], leaves[1], **more)
+        _, weights = route_tokens(router_logits(n.y, leaves[3]), 4, bias=bias, scores="sigmoid")
+        results.append(torch.autograd.grad(weights.square().sum() + n.sum.float().sum(), leaves))
+    assert all(same(a, b) and a.abs().sum() > 0 for a, b in zip(*results))
+
+
+@gpu
+def test_quantised_norms_are_traced_with_their_gradients(device):
+    gen = torch.Generator().manual_seed(6)
+
+    def step(x, weight, residual):
+        n = rms_norm(x * 1.0, weight, residual, quantize=torch.int8)
+        e = rms_norm(n.y, weight, quantize=E4M3)
+        return n.y, n.sum, n.q, n.scale, e.y, e.scale
+
+    compiled = torch.compile(step, backend="aot_eager", fullgraph=True)
+    x, residual, weight, *_ = make_step(device, gen, 30, 256, 8, F32)
+    for record in (True, False):
+        leaves = [t.detach().requires_grad_(record) for t in (x, weight, residual)]
+        want, got = step(*leaves), compiled(*leaves)
+        assert all(same(a, b) and a.requires_grad == b.requires_grad for a, b in zip(got, want))
+        if record:
+            grads = [torch.autograd.grad(out[0].sum() + out[4].square().sum(), leaves) for out in (want, got)]
+            assert all(torch.allclose(a, b, rtol=1e-5, atol=1e-6) for a, b in zip(*grads))
