@@ -613,7 +613,8 @@ typedef struct pplx_a2a_route_args {
 int pplx_a2a_route_tokens(int device, const pplx_a2a_route_args_t *args, void *stream);
 
 /* The gradient of the weights with respect to the logits, for the picks (distinct in each token) that route_tokens made;
- * picks with an index of num_experts or more have none.  Every logit's gradient is written. */
+ * picks with an index of num_experts or more have none.  Every logit's gradient is written: NaN for all of a token's that has picks
+ * and a logit that is NaN or +inf.  (The bias is not read: a token whose weights are NaN by the bias alone has a gradient all the same.) */
 typedef struct pplx_a2a_route_backward_args {
   const float *grad_weights;   /* [m, experts_per_token] contiguous */
   const void *logits;          /* [m, num_experts] of dtype, as above */

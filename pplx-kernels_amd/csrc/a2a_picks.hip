@@ -134,10 +134,10 @@ __device__ __forceinline__ float wave_max_of_lanes(float v) { return number_of(w
 __device__ __forceinline__ double wave_max_of_lanes(double v) { return number_of(wave_largest(order_of(v))); }
 __device__ __forceinline__ double wave_total(double v) { return wave_sum_of(v); }
 
-// exp(x) to two ulps, of x <= 88 (of more, exp(88)): 2^p for the rounded product p = x log2(e), times 1 + what the rounding left, in two
-// steps where the result is subnormal (the instruction has none).
+// exp(x) to two ulps, of x <= 88 (of more, exp(88); of NaN, NaN): 2^p for the rounded product p = x log2(e), times 1 + what the rounding
+// left, in two steps where the result is subnormal (the instruction has none).
 __device__ __forceinline__ float exp_of(float x) {
-  x = x < 88.f ? x : 88.f;
+  x = x > 88.f ? 88.f : x;
   constexpr float kLog2e = 1.44269504088896340736f, kRest = 1.925963033500865e-8f;  // (their sum is log2(e))
   const float p = x * kLog2e;
   const float left = __builtin_fmaf(x, kLog2e, -p) + x * kRest;
@@ -526,8 +526,10 @@ __device__ __forceinline__ F gradient_of_pick(const PicksBackwardDev &a, bool pi
   return picked ? part * (F)a.weight_scale : (F)0;
 }
 
-// A wave to a token, PER consecutive experts in a lane and 64 PER at a time; rows of up to that are read once.  An expert's own part goes
-// through LDS to the lane that writes it.  16384 tokens of 256 experts, softmax without renormalisation: 11.9 us, 2.8 TB/s.
+// A wave to a token, PER consecutive experts in a lane and 64 PER at a time; rows of up to that are read once, whole in every form: a
+// token with a logit that is NaN or +inf has weights of NaN, and so has its gradient.  An expert's own part goes through LDS to the lane
+// that writes it.  16384 tokens of 256 experts, us in a graph: softmax without renormalisation 13.5 (2.5 TB/s), the other forms 10.4 (8.4
+// if they read the picks' logits alone).
 template <class T, int PER> __global__ __launch_bounds__(64 * kTokensAtOnce) void pick_gradient(PicksBackwardDev a) {
   extern __shared__ float of_picks[];  // [waves][experts]: an expert's own part
   const uint32_t lane = lane_id(), wave = wave_id(), E = a.experts;
@@ -542,12 +544,17 @@ template <class T, int PER> __global__ __launch_bounds__(64 * kTokensAtOnce) voi
   const bool dense = a.scores == PPLX_A2A_SOFTMAX && !a.renormalize, once = E <= 64 * PER;
   float l[PER];
   float most = kNoLogit, total = 0.f;
-  if (dense) {
-    for (uint32_t first = 0; first < E; first += 64 * PER) {
-      load_some<T, PER>(logits, first + lane * PER, E, kNoLogit, l);
+  bool bad = false;
+  for (uint32_t first = 0; first < E; first += 64 * PER) {
+    load_some<T, PER>(logits, first + lane * PER, E, kNoLogit, l);
 #pragma unroll
-      for (int j = 0; j < PER; ++j) most = l[j] > most ? l[j] : most;
+    for (int j = 0; j < PER; ++j) {
+      bad |= !(l[j] < HUGE_VALF);
+      most = l[j] > most ? l[j] : most;
     }
+  }
+  bad = __ballot(bad) && __ballot(picked);  // (without picks it has no part in anything)
+  if (dense) {
     most = wave_max_of_lanes(most);
     for (uint32_t first = 0; first < E; first += 64 * PER) {
       if (!once) load_some<T, PER>(logits, first + lane * PER, E, kNoLogit, l);
@@ -578,6 +585,7 @@ template <class T, int PER> __global__ __launch_bounds__(64 * kTokensAtOnce) voi
     for (int j = 0; j < PER; ++j) {
       d[j] = base + j < E ? own_parts[base + j] : 0.f;
       if (dense && inner != 0.f) d[j] -= l[j] == kNoLogit ? 0.f : exp_of(l[j] - most) * share;
+      if (bad) d[j] = __uint_as_float(0x7fc00000u);
     }
     if constexpr (PER > 1) {
       typedef T vec __attribute__((ext_vector_type(PER), aligned(sizeof(T))));

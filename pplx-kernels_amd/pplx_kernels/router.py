@@ -248,7 +248,8 @@ def route_tokens_backward(
     out: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """The gradient of the weights of :func:`route_tokens` with respect to ``logits``, for the picks in ``indices`` that it made (no
-    expert twice in a token).  Every logit's is written, zeros where there is none."""
+    expert twice in a token).  Every logit's is written, zeros where there is none, and NaN for a token that has picks and a NaN or
+    +inf among its logits.  The bias has no part in it: where only the bias made the weights NaN, the gradient is that of the scores."""
     if out is None:
         out = torch.empty_like(logits, memory_format=torch.contiguous_format)
     fn = _ops.route_tokens_backward if _is_compiling() else _C.route_tokens_backward

@@ -1,4 +1,5 @@
-"""Gradients of the operators before dispatch that come by less common ways: beside rows in 8 bits."""
+"""Gradients of the operators before dispatch that come by less common ways: beside rows in 8 bits, of tokens whose logits are
+no numbers."""
 
 from __future__ import annotations
 
@@ -6,7 +7,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
-from pplx_kernels import rms_norm, route_tokens, router_logits
+from pplx_kernels import rms_norm, route_tokens, route_tokens_backward, router_logits
 from tests.test_experts import BF16, F16, F32
 from tests.test_router import E4M3
 from tests.test_router_path import make_step, same
@@ -141,3 +142,50 @@ def test_quantised_norms_are_traced_with_their_gradients(device):
         if record:
             grads = [torch.autograd.grad(out[0].sum() + out[4].square().sum(), leaves) for out in (want, got)]
             assert all(torch.allclose(a, b, rtol=1e-5, atol=1e-6) for a, b in zip(*grads))
+
+
+# ---------------------------------------------------------------------------
+# Tokens whose logits are no numbers
+# ---------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renormalize", [False, True])
+@pytest.mark.parametrize("experts,dtype", [(40, F32), (64, F16), (130, BF16), (256, F32), (500, F16), (700, F32), (1500, BF16)])
+def test_tokens_of_bad_logits_have_gradients_of_nan(device, experts, dtype, scores, renormalize, bad):
+    """Their weights are NaN, and so is what depends on them: at any expert, one of the picks or not.  The other tokens have the bits
+    that they have without them."""
+    gen = torch.Generator().manual_seed(experts)
+    m, k = 13, 3
+    logits = (2 * torch.randn(m, experts, generator=gen)).to(dtype)
+    logits[::2, experts // 3] = float("-inf")
+    grad = torch.randn(m, k, generator=gen).to(device)
+    more = dict(scores=scores, renormalize=renormalize, scale=1.5)
+    spoiled = {1: 0, 4: k - 1, 5: k, 8: experts // 2, 12: experts - 1}
+    mixed = logits.clone()
+    for t, e in spoiled.items():
+        mixed[t, e] = bad
+    leaf, clean = mixed.to(device).requires_grad_(True), logits.to(device).requires_grad_(True)
+    indices, weights = route_tokens(leaf, k, **more)
+    (got,) = torch.autograd.grad(weights, leaf, grad)
+    (want,) = torch.autograd.grad(route_tokens(clean, k, **more)[1], clean, grad)
+    rest = [t for t in range(m) if t not in spoiled]
+    assert torch.isnan(weights[list(spoiled)]).all() and torch.isnan(got[list(spoiled)]).all()
+    assert torch.isfinite(got[rest]).all() and same(got[rest], want[rest])
+    # a token whose picks are all taken out has no part in anything, another one's pick that is taken out leaves it what it is
+    at = indices.view(torch.int32).clone()
+    at[1], at[8, 1], at[2] = experts, experts, experts
+    got = route_tokens_backward(grad, mixed.to(device), at.view(torch.uint32), **more)
+    assert (got[[1, 2]] == 0).all() and torch.isnan(got[[4, 5, 8, 12]]).all()
+
+
+@gpu
+@pytest.mark.parametrize("renormalize", [False, True])
+def test_tokens_behind_the_last_have_no_gradient_whatever_their_logits(device, renormalize):
+    logits = torch.randn(12, 256, generator=torch.Generator().manual_seed(1))
+    logits[8:] = float("nan")
+    leaf = logits.to(device).requires_grad_(True)
+    bound = torch.tensor([8], dtype=torch.int32, device=device).view(torch.uint32)
+    _, weights = route_tokens(leaf, 4, bound_m=bound, renormalize=renormalize)
+    (got,) = torch.autograd.grad(weights.square().sum(), leaf)
+    assert (got[8:] == 0).all() and torch.isfinite(got).all() and got[:8].abs().sum() > 0
