@@ -654,6 +654,10 @@ PyObject *py_int8_matmul(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
 #define PPLX_EXPERTS_SOURCE_ID "unknown"
 #endif
 PyObject *py_experts_build_id(PyObject *, PyObject *) { return PyUnicode_FromString(PPLX_EXPERTS_SOURCE_ID); }
+#ifndef PPLX_EXPERTS_HEADERS_ID
+#define PPLX_EXPERTS_HEADERS_ID "unknown"
+#endif
+PyObject *py_experts_headers_id(PyObject *, PyObject *) { return PyUnicode_FromString(PPLX_EXPERTS_HEADERS_ID); }
 
 #define PPLX_FASTCALL(fn) (PyCFunction)(void (*)(void))fn, METH_FASTCALL
 PyMethodDef kExpertsMethods[] = {
@@ -672,6 +676,7 @@ PyMethodDef kExpertsMethods[] = {
     {"int8_matmul", PPLX_FASTCALL(py_int8_matmul),
      "int8_matmul(out, x, x_scale, weight, weight_scale, num_tokens, offsets)"},
     {"experts_build_id", py_experts_build_id, METH_NOARGS, "hash of the sources that these functions were built from"},
+    {"experts_headers_id", py_experts_headers_id, METH_NOARGS, "hash of the binding's headers that they were built with"},
     {nullptr, nullptr, 0, nullptr},
 };
 

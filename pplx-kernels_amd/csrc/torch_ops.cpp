@@ -934,9 +934,15 @@ PyObject *py_held_tensors(PyObject *, PyObject *arg) {
 #endif
 // build_id() -> hash of the sources this module was built from (a stale build shows up in a test)
 PyObject *py_build_id(PyObject *, PyObject *) { return PyUnicode_FromString(PPLX_BINDING_SOURCE_ID); }
+#ifndef PPLX_BINDING_HEADERS_ID
+#define PPLX_BINDING_HEADERS_ID "unknown"
+#endif
+// headers_id() -> the same of the binding's own headers
+PyObject *py_headers_id(PyObject *, PyObject *) { return PyUnicode_FromString(PPLX_BINDING_HEADERS_ID); }
 
 PyMethodDef kMethods[] = {
     {"build_id", py_build_id, METH_NOARGS, "hash of the sources the module was built from"},
+    {"headers_id", py_headers_id, METH_NOARGS, "hash of the binding's headers the module was built with"},
     {"dispatch", (PyCFunction)(void (*)(void))py_dispatch, METH_FASTCALL,
      "dispatch(fptr, out_expert_num_tokens, out_expert_x, out_expert_x_scale, dp_x, dp_x_scale, indices, "
      "bound_m, do_send, do_recv): all_to_all_*_dispatch without the op dispatcher"},

@@ -2,11 +2,14 @@
 
 from __future__ import annotations
 
+import hashlib
 import os
 import re
 import subprocess
 
 import pytest
+
+from pplx_kernels import ops
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "pplx-kernels_amd", "csrc")
@@ -44,3 +47,16 @@ def test_objects_are_made_again_when_a_header_changes(source):
     stem = os.path.splitext(source)[0]
     target = f"{stem}.o" if f"{stem}.o" in RULES else stem
     assert included(source) - RULES[target] == set()
+
+
+@pytest.mark.parametrize("made,sources", [
+    ("headers_id", ["torch_common.h"]),
+    ("experts_headers_id", ["torch_common.h", "torch_tensors.h"]),
+])  # fmt: skip
+def test_the_layer_is_built_with_the_headers_in_the_tree(made, sources):
+    """Beside the ids of the sources themselves: which headers each object of the binding was compiled with."""
+    h = hashlib.sha256()
+    for name in sources:
+        with open(os.path.join(CSRC, name), "rb") as f:
+            h.update(f.read())
+    assert getattr(ops._C, made)() == h.hexdigest()[:16], "pplx_kernels/_C.so is stale: run `make -C pplx-kernels_amd/csrc`"
