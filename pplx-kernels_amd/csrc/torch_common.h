@@ -78,6 +78,12 @@ inline int64_t int_arg(PyObject *obj, const char *name) {
   return v;
 }
 
+inline bool bool_arg(PyObject *obj) {
+  const int v = PyObject_IsTrue(obj);
+  if (v < 0) throw python_error();  // (what its __bool__ raised)
+  return v;
+}
+
 inline void arity(const char *fn, Py_ssize_t got, Py_ssize_t want) {
   TORCH_CHECK_TYPE(got == want, fn, "() takes ", want, " positional arguments but ", got, " were given");
 }

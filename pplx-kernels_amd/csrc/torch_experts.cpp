@@ -509,7 +509,7 @@ PyObject *py_sort_tokens(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   const at::Tensor &x = tensor_arg(args[0], "x"), &indices = tensor_arg(args[1], "indices");
   const int64_t experts = int_arg(args[2], "num_experts");
   const at::Tensor *bound_m = optional_tensor_arg(args[3], "bound_m");
-  const bool int8 = PyObject_IsTrue(args[4]) == 1;
+  const bool int8 = bool_arg(args[4]);
   Sorted s;
   if (straight({&x, &indices, bound_m})) {
     s = sort_new(x, indices, experts, bound_m, int8);
@@ -620,7 +620,7 @@ PyObject *py_quantize_rows(PyObject *, PyObject *const *args, Py_ssize_t nargs) 
   arity("quantize_rows", nargs, 6);
   const at::Tensor &out = tensor_arg(args[0], "out"), &scale = tensor_arg(args[1], "scale"), &x = tensor_arg(args[2], "x");
   const at::Tensor *num_tokens = optional_tensor_arg(args[3], "num_tokens"), *offsets = optional_tensor_arg(args[4], "offsets");
-  const bool swiglu = PyObject_IsTrue(args[5]) == 1;
+  const bool swiglu = bool_arg(args[5]);
   if (straight({&out, &scale, &x, num_tokens, offsets})) {
     quantize_rows(out, scale, x, num_tokens, offsets, swiglu);
   } else {

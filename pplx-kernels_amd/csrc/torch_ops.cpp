@@ -639,7 +639,7 @@ PyObject *py_dispatch(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
                 tensor_arg(args[2], "out_expert_x"), optional_tensor_arg(args[3], "out_expert_x_scale"),
                 tensor_arg(args[4], "dp_x"), optional_tensor_arg(args[5], "dp_x_scale"),
                 tensor_arg(args[6], "indices"), optional_tensor_arg(args[7], "bound_m"),
-                PyObject_IsTrue(args[8]) == 1, PyObject_IsTrue(args[9]) == 1, args + 1);
+                bool_arg(args[8]), bool_arg(args[9]), args + 1);
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -650,8 +650,8 @@ PyObject *py_combine(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   arity("combine", nargs, 8);
   combine_core(int_arg(args[0], "fptr"), tensor_arg(args[1], "out_tokens"), tensor_arg(args[2], "indices"),
                tensor_arg(args[3], "weights"), tensor_arg(args[4], "expert_y"),
-               optional_tensor_arg(args[5], "bound_m"), PyObject_IsTrue(args[6]) == 1,
-               PyObject_IsTrue(args[7]) == 1, args + 1);
+               optional_tensor_arg(args[5], "bound_m"), bool_arg(args[6]),
+               bool_arg(args[7]), args + 1);
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }

@@ -650,7 +650,6 @@ uint64_t count_arg(PyObject *obj, const char *name) {
   TORCH_CHECK(v >= 0 && v < (1ll << 31), "pplx_kernels: invalid argument: ", name, " out of range");
   return (uint64_t)v;
 }
-bool bool_arg(PyObject *obj) { return PyObject_IsTrue(obj) == 1; }
 
 PyObject *pair(const at::Tensor &a, const at::Tensor &b) {
   PyObject *out = PyTuple_New(2);
@@ -816,10 +815,11 @@ PyObject *py_router_workspace(PyObject *, PyObject *const *args, Py_ssize_t narg
   HANDLE_TH_ERRORS
   arity("router_workspace", nargs, 3);
   const at::Tensor &x = tensor_arg(args[0], "x"), &weight = tensor_arg(args[1], "weight");
+  const bool backward = bool_arg(args[2]);
   check_router(x, weight);
   uint64_t bytes = 0;
   A2A_CHECK(pplx_a2a_router_workspace(tokens_of(x), (uint32_t)weight.sizes()[0], (uint64_t)x.sizes()[1], dtype_code(x.scalar_type()),
-                                      dtype_code(weight.scalar_type()), bool_arg(args[2]), &bytes));
+                                      dtype_code(weight.scalar_type()), backward, &bytes));
   return PyLong_FromUnsignedLongLong(bytes);
   END_HANDLE_TH_ERRORS
 }
