@@ -1,5 +1,5 @@
 """Gradients of the operators before dispatch that come by less common ways: beside rows in 8 bits, of tokens whose logits are
-no numbers."""
+no numbers, of more experts than a workgroup holds at once.  Tolerances count roundings, as in test_router.py."""
 
 from __future__ import annotations
 
@@ -7,9 +7,9 @@ import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
-from pplx_kernels import rms_norm, route_tokens, route_tokens_backward, router_logits
-from tests.test_experts import BF16, F16, F32
-from tests.test_router import E4M3
+from pplx_kernels import rms_norm, route_tokens, route_tokens_backward, router_logits, router_logits_backward
+from tests.test_experts import BF16, F16, F32, assert_within, rounded
+from tests.test_router import E4M3, gradient, router
 from tests.test_router_path import make_step, same
 
 gpu = pytest.mark.gpu
@@ -189,3 +189,35 @@ def test_tokens_behind_the_last_have_no_gradient_whatever_their_logits(device, r
     _, weights = route_tokens(leaf, 4, bound_m=bound, renormalize=renormalize)
     (got,) = torch.autograd.grad(weights.square().sum(), leaf)
     assert (got[8:] == 0).all() and torch.isfinite(got).all() and got[:8].abs().sum() > 0
+
+
+# ---------------------------------------------------------------------------
+# The router's product
+# ---------------------------------------------------------------------------
+MANY_EXPERTS = [
+    # more experts than a workgroup of grad_x holds of the weight at once (256 to 512, by their types), and than one of grad_weight
+    # takes; tokens that leave waves of the last round without rows
+    (300, 257, 264, F16, F32), (37, 300, 136, BF16, F32), (515, 330, 136, F32, F32), (700, 520, 520, BF16, BF16), (290, 384, 72, F16, F16),
+    (1, 513, 2056, BF16, BF16), (530, 1100, 64, BF16, F32), (70, 1333, 328, F32, F32), (20, 5461, 40, F16, F16), (33, 5461, 64, BF16, BF16),
+]  # fmt: skip
+
+
+@gpu
+@pytest.mark.parametrize("m,experts,hidden,dtype,weight_dtype", MANY_EXPERTS)
+def test_gradients_of_router_logits_of_many_experts(device, m, experts, hidden, dtype, weight_dtype):
+    gen = torch.Generator().manual_seed(m + hidden)
+    x, weight = router(m, experts, hidden, dtype, weight_dtype, gen)
+    grad = 1e-2 * torch.randn(m, experts, generator=gen)
+    leaves = [t.to(device).requires_grad_(True) for t in (x, weight)]
+    gx, gw = torch.autograd.grad(router_logits(*leaves), leaves, grad.to(device))
+    want, off = gradient(grad, weight, experts, dtype)
+    want_w, off_w = gradient(grad.t(), x, m, weight_dtype)
+    assert_within(gx, want, rounded(want, dtype, off))
+    assert_within(gw, want_w, rounded(want_w, weight_dtype, off_w))
+    dev = [t.to(device) for t in (grad, x, weight)]
+    room = torch.full((m, hidden + 16), 7.0, dtype=dtype, device=device), torch.full((experts, hidden + 16), 7.0, dtype=weight_dtype, device=device)
+    inner = [t[:, 8 : 8 + hidden] for t in room]
+    router_logits_backward(*dev, out=(inner[0], None))
+    router_logits_backward(*dev, out=(None, inner[1]))
+    assert same(inner[0], gx) and same(inner[1], gw)
+    assert all((t[:, :8] == 7).all() and (t[:, 8 + hidden :] == 7).all() for t in room)
