@@ -559,9 +559,8 @@ int pplx_a2a_router_workspace(uint32_t m, uint32_t num_experts, uint64_t hidden_
                               int32_t backward, uint64_t *bytes);
 int pplx_a2a_router_logits(int device, const pplx_a2a_router_logits_args_t *args, void *stream);
 
-/* Its gradients: grad_x = grad_logits * weight and grad_weight = grad_logits^T * x, added up in fp32 and rounded once.  For results of
- * 16 bits grad_logits, and the other operand where it is not bf16, count to 2^-18 of each value; for fp32 to 24 bits.  Either may
- * be left out (NULL). */
+/* Its gradients: grad_x = grad_logits * weight and grad_weight = grad_logits^T * x, added up in fp32 and rounded once.  For bf16
+ * results grad_logits, and weights of fp32, count to 2^-18 of each value; for fp16 and fp32 to 24 bits.  Either may be left out (NULL). */
 typedef struct pplx_a2a_router_logits_backward_args {
   const float *grad_logits;    /* [m, num_experts], 4-byte aligned */
   int64_t grad_logits_stride_row; /* floats */

@@ -766,9 +766,11 @@ template <class T, class W> int launch_form(int form, const TilesDev &a, hipStre
 // ---------------------------------------------------------------------------
 // The gradients' shares
 // ---------------------------------------------------------------------------
-// Results of 16 bits are sums of operands that count to two pieces, 2^-18 of each value, a hundredth of what the result is rounded by
-// and less: with three, 3001 x 7168 of 256 takes 33 us and not 26.
-template <class O> constexpr int kOrder = sizeof(O) == 4 ? 2 : 1;
+// Results of bf16 are sums of operands that count to two pieces, 2^-18 of each value, beside 2^-9 of the result that they are rounded by;
+// products of two second pieces, 2^-18 too, are left out.  Three pieces cost 33 us and not 26 for grad_x of 3001 x 7168.  fp16 is rounded by
+// 2^-12, so that two pieces would show where products cancel to a fiftieth: it has three, as fp32 has (two and three, with all launches:
+// 3001 x 7168 of 256 grad_x 43 and 58, with weights in fp32 38 and 66, grad_weight 49 and 62; 16384 x 4096 of 64 grad_weight 56 and 69).
+template <class O> constexpr int kOrder = std::is_same_v<O, __bf16> ? 1 : 2;
 // Columns of a lane: four where their pieces fit LDS.
 template <class TB, int ORDER> constexpr int kColumnsOfLane = Pieces<TB, ORDER>::count <= 2 ? 4 : 2;
 

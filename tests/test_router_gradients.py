@@ -1,5 +1,5 @@
 """Gradients of the operators before dispatch that come by less common ways: beside rows in 8 bits, of tokens whose logits are
-no numbers, of more experts than a workgroup holds at once.  Tolerances count roundings, as in test_router.py."""
+no numbers, of more experts than a workgroup holds at once, of sums that cancel.  Tolerances count roundings, as in test_router.py."""
 
 from __future__ import annotations
 
@@ -9,7 +9,7 @@ import torch.autograd.forward_ad as forward_ad
 
 from pplx_kernels import rms_norm, route_tokens, route_tokens_backward, router_logits, router_logits_backward
 from tests.test_experts import BF16, F16, F32, assert_within, rounded
-from tests.test_router import E4M3, gradient, router
+from tests.test_router import E4M3, gradient, product, router
 from tests.test_router_path import make_step, same
 
 gpu = pytest.mark.gpu
@@ -221,3 +221,29 @@ def test_gradients_of_router_logits_of_many_experts(device, m, experts, hidden, 
     router_logits_backward(*dev, out=(None, inner[1]))
     assert same(inner[0], gx) and same(inner[1], gw)
     assert all((t[:, :8] == 7).all() and (t[:, 8 + hidden :] == 7).all() for t in room)
+
+
+@gpu
+@pytest.mark.parametrize("weight_dtype", [F16, F32])
+def test_half_precision_gradients_of_products_that_cancel(device, weight_dtype):
+    """Two products that cancel to a five-hundredth and less: what is left shows the bits of grad_logits far behind those that the
+    result has.  Only fp32's roundings are allowed for."""
+    gen = torch.Generator().manual_seed(12)
+
+    def two(n):  # n pairs of fp32 numbers whose sum is 2^-9 to 2^-8 of them
+        a = 1 + torch.rand(n, 1, generator=gen)
+        return torch.cat([a, -a * (1 + 2.0**-9 * (1 + torch.rand(n, 1, generator=gen)))], 1)
+
+    # of the rows: 64 tokens, two experts with one weight
+    weight = (1 + torch.rand(1, 512, generator=gen)).to(weight_dtype).expand(2, 512).contiguous()
+    x, grad = torch.randn(64, 512, generator=gen).to(F16), two(64)
+    got, _ = router_logits_backward(grad.to(device), x.to(device), weight.to(device))
+    want, off = product(grad, weight, 2)
+    assert_within(got, want, rounded(want, F16, off))
+    # of the weight: 64 experts, two tokens with one row
+    if weight_dtype == F16:
+        x, grad = (1 + torch.rand(1, 512, generator=gen)).to(F16).expand(2, 512).contiguous(), two(64).t().contiguous()
+        weight = torch.randn(64, 512, generator=gen).to(F16)
+        _, got = router_logits_backward(grad.to(device), x.to(device), weight.to(device))
+        want, off = product(grad.t(), x, 2)
+        assert_within(got, want, rounded(want, F16, off))
