@@ -539,7 +539,7 @@ int pplx_a2a_rms_norm_workspace(uint32_t m, uint64_t hidden_dim, uint64_t *bytes
 int pplx_a2a_rms_norm_backward(int device, const pplx_a2a_rms_norm_backward_args_t *args, void *stream);
 
 /* The router's product: logits[t, e] = sum over k of x[t, k] * weight[e, k], added up in fp32.  Products of 16-bit elements are
- * exact; fp32 elements count to 24 bits (an infinity among them, or a value above 3.38e38, makes a NaN). */
+ * exact; fp32 elements count to 24 bits.  (With weights of fp32 an infinity in a row or a weight, or a value above 3.38e38, makes a NaN.) */
 typedef struct pplx_a2a_router_logits_args {
   const void *x;               /* [m, hidden_dim] of dtype; rows 16-byte aligned, strides in bytes, multiples of 16 */
   int64_t x_stride_row;
@@ -559,8 +559,9 @@ int pplx_a2a_router_workspace(uint32_t m, uint32_t num_experts, uint64_t hidden_
                               int32_t backward, uint64_t *bytes);
 int pplx_a2a_router_logits(int device, const pplx_a2a_router_logits_args_t *args, void *stream);
 
-/* Its gradients: grad_x = grad_logits * weight and grad_weight = grad_logits^T * x, added up in fp32 and rounded once.  For bf16
- * results grad_logits, and weights of fp32, count to 2^-18 of each value; for fp16 and fp32 to 24 bits.  Either may be left out (NULL). */
+/* Its gradients: grad_x = grad_logits * weight and grad_weight = grad_logits^T * x, added up in fp32 and rounded once.  Operands count to 24
+ * bits whatever the results' type; an infinity, or a value above 3.38e38, may make a NaN of what it has a part in.  Either may be left out
+ * (NULL). */
 typedef struct pplx_a2a_router_logits_backward_args {
   const float *grad_logits;    /* [m, num_experts], 4-byte aligned */
   int64_t grad_logits_stride_row; /* floats */

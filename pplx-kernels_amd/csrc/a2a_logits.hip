@@ -46,10 +46,9 @@ template <int N> __device__ __forceinline__ void cut(f32x8 v, bf16x8 *p) {
     p[n] = __builtin_bit_cast(bf16x8, w);
   }
 }
-// Pieces that hold a value in full, or the first ORDER + 1 of them.
-template <class T, int ORDER = 2> struct Pieces {
-  static constexpr int kFull = std::is_same_v<T, __bf16> ? 1 : std::is_same_v<T, _Float16> ? 2 : 3;
-  static constexpr int count = kFull < ORDER + 1 ? kFull : ORDER + 1;
+// Pieces that hold a value in full.
+template <class T> struct Pieces {
+  static constexpr int count = std::is_same_v<T, __bf16> ? 1 : std::is_same_v<T, _Float16> ? 2 : 3;
   static __device__ __forceinline__ void of(typename Eight<T>::raw v, bf16x8 *p) {
     if constexpr (std::is_same_v<T, __bf16>) p[0] = v;
     else cut<count>(Eight<T>::wide(v), p);
@@ -384,7 +383,13 @@ template <class O> int launch_sum(const SumDev &a, hipStream_t s) {
 // The matrix cores want eight consecutive k of a column in a lane.  A lane fetches NV consecutive columns of eight rows of b, and the
 // vectors are turned in its registers: fragment f has the columns f, NV + f, 2 NV + f .. of a block of 32 NV, and the sums of a lane,
 // one for each fragment, are consecutive columns again.  Fragments go to LDS, from where all waves of a workgroup take them.
-// The other operand, grad_logits, is cut into pieces once, by split_gradient, and lies in the order in which lanes take them.
+// The other operand, grad_logits, is cut into pieces once, by split_gradient, and lies in the order in which lanes take them.  It has
+// all three pieces whatever the results' type: two leave out up to 2^-17 of a value (and the products of second pieces 2^-16), which shows
+// in a result of 16 bits where products cancel.  What the third one costs, us with all launches, two pieces and three:
+//   both bf16       3001 x 7168 of 256  grad_x 34 / 44, grad_weight 38 / 48     8192 x 7168 of 256  78 / 103, 81 / 107
+//                   8192 x 4096 of 8  17 / 18, 20 / 21
+//   both fp16       3001 x 7168 of 256  45 / 61, 50 / 63     16384 x 4096 of 64  44 / 58, 59 / 75
+//   bf16, fp32      3001 x 7168 of 256  44 / 76 (two pieces of the weight too, without the product of second pieces)
 struct GradientDev {
   const uint8_t *a;  // [blocks of 32 rows][sixteens of k][pieces][64 lanes] of 16 bytes
   const uint8_t *b;
@@ -397,8 +402,8 @@ struct GradientDev {
   uint32_t first_group;
 };
 
-template <class TB, int NV, int ORDER> struct Turned {
-  typedef Pieces<TB, ORDER> Cut;
+template <class TB, int NV> struct Turned {
+  typedef Pieces<TB> Cut;
   static constexpr int kPieces = Cut::count;
   static constexpr int kBytes = kPieces * NV * 1024;  // of sixteen k in LDS
   typedef TB vec __attribute__((ext_vector_type(NV)));
@@ -427,25 +432,26 @@ template <class TB, int NV, int ORDER> struct Turned {
 };
 
 typedef const PPLX_GLOBAL bf16x8 *FragmentPtr;
-template <int ORDER> struct Fragments {  // of 32 rows and sixteen k
-  bf16x8 p[ORDER + 1];
+constexpr int kPiecesOfGradient = 3;
+struct Fragments {  // of 32 rows and sixteen k
+  bf16x8 p[kPiecesOfGradient];
   // Number i of those at `from`, the first where there are not so many.
   __device__ __forceinline__ void load(FragmentPtr from, uint32_t i, uint32_t all) {
-    from += (uint64_t)(i < all ? i : 0) * (64 * (ORDER + 1));
+    from += (uint64_t)(i < all ? i : 0) * (64 * kPiecesOfGradient);
 #pragma unroll
-    for (int n = 0; n <= ORDER; ++n) p[n] = from[n * 64];
+    for (int n = 0; n < kPiecesOfGradient; ++n) p[n] = from[n * 64];
   }
 };
 // Their products with the columns' fragments at `from`.
-template <int PIECES, int NV, int ORDER>
-__device__ __forceinline__ void multiply_turned(const Fragments<ORDER> &fa, const uint8_t *from, uint32_t lane, f32x16 *acc) {
+template <int PIECES, int NV>
+__device__ __forceinline__ void multiply_turned(const Fragments &fa, const uint8_t *from, uint32_t lane, f32x16 *acc) {
 #pragma unroll
   for (int pb = PIECES - 1; pb >= 0; --pb) {
     bf16x8 fb[NV];
 #pragma unroll
     for (int f = 0; f < NV; ++f) fb[f] = *reinterpret_cast<const bf16x8 *>(from + ((pb * NV + f) * 64 + lane) * 16);
 #pragma unroll
-    for (int pa = ORDER - pb; pa >= 0; --pa) {
+    for (int pa = kPiecesOfGradient - 1 - pb; pa >= 0; --pa) {
 #pragma unroll
       for (int f = 0; f < NV; ++f) acc[f] = multiply_32(fa.p[pa], fb[f], acc[f]);
     }
@@ -458,7 +464,6 @@ struct PiecesDev {
   int64_t in_stride;  // elements
   uint32_t rows, columns;
   uint8_t *by_rows, *by_columns;
-  uint32_t pieces_by_rows, pieces_by_columns;
   uint32_t first_group;
 };
 // A workgroup to 32 rows by 32 columns, of which a wave each takes half a block of rows, and of columns.
@@ -478,29 +483,27 @@ __global__ __launch_bounds__(128) void split_gradient(PiecesDev a) {
 #pragma unroll
   for (uint32_t i = 0; i < 8; ++i) tile[i * 4 + y][x] = r0 + i * 4 + y < a.rows && c0 + x < a.columns ? in[i] : 0.f;
   __syncthreads();
-  auto write = [&](uint8_t *to, uint64_t fragment, uint32_t pieces, auto at) {
+  auto write = [&](uint8_t *to, uint64_t fragment, auto at) {
     f32x8 v;
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = at(lane % 32, wave * 16 + lane / 32 * 8 + i);
-    bf16x8 p[3];
-    cut<3>(v, p);
-    PPLX_GLOBAL bf16x8 *out = as_global(reinterpret_cast<bf16x8 *>(to)) + fragment * pieces * 64 + lane;
+    bf16x8 p[kPiecesOfGradient];
+    cut<kPiecesOfGradient>(v, p);
+    PPLX_GLOBAL bf16x8 *out = as_global(reinterpret_cast<bf16x8 *>(to)) + fragment * (64 * kPiecesOfGradient) + lane;
 #pragma unroll
-    for (uint32_t i = 0; i < 3; ++i) {
-      if (i < pieces) out[i * 64] = p[i];
-    }
+    for (int i = 0; i < kPiecesOfGradient; ++i) out[i * 64] = p[i];
   };
   const uint32_t row_sixteens = (a.rows + 15) / 16, column_sixteens = (a.columns + 15) / 16;
   if (a.by_rows && column_block * 2 + wave < column_sixteens) {
-    write(a.by_rows, (uint64_t)block * column_sixteens + column_block * 2 + wave, a.pieces_by_rows,
+    write(a.by_rows, (uint64_t)block * column_sixteens + column_block * 2 + wave,
           [&](uint32_t r, uint32_t k) { return tile[r][k]; });
   }
   if (a.by_columns && block * 2 + wave < row_sixteens) {
-    write(a.by_columns, (uint64_t)column_block * row_sixteens + block * 2 + wave, a.pieces_by_columns,
+    write(a.by_columns, (uint64_t)column_block * row_sixteens + block * 2 + wave,
           [&](uint32_t c, uint32_t k) { return tile[k][c]; });
   }
 }
-uint64_t fragment_bytes(uint64_t rows, uint64_t k, int pieces) { return (rows + 31) / 32 * ((k + 15) / 16) * (1024 * pieces); }
+uint64_t fragment_bytes(uint64_t rows, uint64_t k) { return (rows + 31) / 32 * ((k + 15) / 16) * (1024 * kPiecesOfGradient); }
 int launch_split(const PiecesDev &a, hipStream_t s) {
   return launch_groups(split_gradient, split_gradient, ((uint64_t)a.rows + 31) / 32 * ((a.columns + 31) / 32), 128, 0, s, a);
 }
@@ -521,13 +524,13 @@ __device__ __forceinline__ void store_turned(const GradientDev &a, uint64_t firs
 }
 
 // Of x: a workgroup keeps the fragments of 32 NV columns of the weight in LDS, CHUNK k of them at a time, and its waves take 32 rows
-// of grad_logits each, a round after the other.  3001 x 7168 of 256 in bf16: 28 us, with two pieces of grad_logits 790 TFLOP/s; the products
-// alone take 18, the stores 6 and the loads 2 to 4 (what another order of loads and stores, priorities of waves or fewer rows to a
-// workgroup do not hide).
+// of grad_logits each, a round after the other.  3001 x 7168 of 256 in bf16: 38 us, 860 TFLOP/s with the three pieces of grad_logits.  With
+// two of them 28, of which the products alone took 18, the stores 6 and the loads 2 to 4 (what another order of loads and stores,
+// priorities of waves or fewer rows to a workgroup do not hide).
 constexpr int kGradientWaves = 8;
-template <class TB, class O, int NV, int ORDER>
+template <class TB, class O, int NV>
 __global__ __launch_bounds__(kGradientWaves * 64) void gradient_of_rows(GradientDev a, uint32_t chunk) {
-  typedef Turned<TB, NV, ORDER> B;
+  typedef Turned<TB, NV> B;
   extern __shared__ __align__(16) uint8_t lds[];  // [chunk / 16][pieces][NV][64 lanes]
   const uint32_t lane = lane_id(), wave = wave_id(), half = lane / 32 * 8;
   const uint32_t group = a.first_group + blockIdx.x;
@@ -552,9 +555,9 @@ __global__ __launch_bounds__(kGradientWaves * 64) void gradient_of_rows(Gradient
   const uint32_t all = (a.k + 15) / 16;
   for (uint32_t round = part; round < rounds; round += a.parts) {
     const uint32_t block = round * kGradientWaves + wave, m0 = block * 32;
-    const FragmentPtr from = as_global(reinterpret_cast<const bf16x8 *>(a.a)) + (uint64_t)(m0 < a.rows ? block : 0) * all * (64 * (ORDER + 1)) + lane;
+    const FragmentPtr from = as_global(reinterpret_cast<const bf16x8 *>(a.a)) + (uint64_t)(m0 < a.rows ? block : 0) * all * (64 * kPiecesOfGradient) + lane;
     constexpr int kAhead = 4;  // fragments under way
-    Fragments<ORDER> fa[kAhead];
+    Fragments fa[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) fa[i].load(from, i, all);
     f32x16 acc[NV] = {};
@@ -581,11 +584,11 @@ __global__ __launch_bounds__(kGradientWaves * 64) void gradient_of_rows(Gradient
 
 // Of the weight: waves take 32 experts each, a workgroup all of a block of them, and go through the tokens sixteen for each wave at a
 // time: every wave turns sixteen of x, and all multiply with what the others turned.  Parts of the tokens add up in sum_splits.
-// Memory answers a wave in order: the fragments of a step are all under way before the rows of x that come after it (four of eight:
-// 30.5 us, all: 26.5 for 256 x 7168 of 3001 in bf16, 830 TFLOP/s with two pieces, and 6 for the sum of the parts).
-template <class TB, class O, int NV, int ORDER, int WAVES>
+// 256 x 7168 of 3001 in bf16: 38 us, 860 TFLOP/s with the three pieces, and 6 for the sum of the parts.  Memory answers a wave in order: the
+// fragments of a step are all under way before the rows of x that come after it (with two pieces four of eight 30.5 us, all 26.5).
+template <class TB, class O, int NV, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void gradient_of_weight(GradientDev a, uint32_t tokens_per_part, uint32_t row_blocks) {
-  typedef Turned<TB, NV, ORDER> B;
+  typedef Turned<TB, NV> B;
   extern __shared__ __align__(16) uint8_t lds[];  // [2][waves][pieces][NV][64 lanes]
   const uint32_t lane = lane_id(), wave = wave_id(), half = lane / 32 * 8;
   const uint32_t group = a.first_group + blockIdx.x;
@@ -596,12 +599,12 @@ __global__ __launch_bounds__(WAVES * 64) void gradient_of_weight(GradientDev a, 
   const uint32_t begin = part * tokens_per_part, end = a.k - begin < tokens_per_part ? a.k : begin + tokens_per_part;
   constexpr uint32_t step = 16 * WAVES, size = WAVES * B::kBytes;
   const uint32_t all = (a.k + 15) / 16, first = begin / 16;
-  const FragmentPtr from = as_global(reinterpret_cast<const bf16x8 *>(a.a)) + (uint64_t)(m0 < a.rows ? m0 / 32 : 0) * all * (64 * (ORDER + 1)) + lane;
+  const FragmentPtr from = as_global(reinterpret_cast<const bf16x8 *>(a.a)) + (uint64_t)(m0 < a.rows ? m0 / 32 : 0) * all * (64 * kPiecesOfGradient) + lane;
   auto left_at = [&](uint32_t k) { return k < end ? end - k : 0u; };
   B b;
   f32x16 acc[NV] = {};
   b.load(a, there ? column : 0, begin + wave * 16 + half);
-  Fragments<ORDER> fa[WAVES];
+  Fragments fa[WAVES];
 #pragma unroll
   for (uint32_t i = 0; i < WAVES; ++i) fa[i].load(from, first + i, all);
   uint32_t buffer = 0, at = begin;
@@ -766,22 +769,18 @@ template <class T, class W> int launch_form(int form, const TilesDev &a, hipStre
 // ---------------------------------------------------------------------------
 // The gradients' shares
 // ---------------------------------------------------------------------------
-// Results of bf16 are sums of operands that count to two pieces, 2^-18 of each value, beside 2^-9 of the result that they are rounded by;
-// products of two second pieces, 2^-18 too, are left out.  Three pieces cost 33 us and not 26 for grad_x of 3001 x 7168.  fp16 is rounded by
-// 2^-12, so that two pieces would show where products cancel to a fiftieth: it has three, as fp32 has (two and three, with all launches:
-// 3001 x 7168 of 256 grad_x 43 and 58, with weights in fp32 38 and 66, grad_weight 49 and 62; 16384 x 4096 of 64 grad_weight 56 and 69).
-template <class O> constexpr int kOrder = std::is_same_v<O, __bf16> ? 1 : 2;
 // Columns of a lane: four where their pieces fit LDS.
-template <class TB, int ORDER> constexpr int kColumnsOfLane = Pieces<TB, ORDER>::count <= 2 ? 4 : 2;
+template <class TB> constexpr int kColumnsOfLane = Pieces<TB>::count <= 2 ? 4 : 2;
 
 struct WeightShares {
   uint32_t waves, row_blocks, parts, tokens_per_part;
 };
 // Into how many parts the tokens go, by cost in us: a start, a step of 16 tokens for each wave, and the parts' sums.  Up to 64 experts
-// leave two of four waves without work for the matrix cores, and a second workgroup costs a compute unit half a step.  The products alone:
-// 8192 x 4096 of 8 in 8 parts 19.1 and in 16 (two to a unit) 14.3; of 64 in fp16 32.5 and 24.6; but 8192 x 2048 of 128 in 16 parts 16.1
-// and in 32 23.3, and 3001 x 7168 of 256 in 4 parts 26.2 and in 8 30.8.  Workgroups of two waves, each in its best parts and with the
-// sums: 8192 x 4096 of 8 17.4 and not 16.9, 4452 x 1960 of 47 in fp32 18.2 and not 18.3, 2000 x 2048 of 60 12.7 and not 8.0.
+// leave two of four waves without work for the matrix cores, and a second workgroup costs a compute unit half a step.  With all launches:
+// 8192 x 4096 of 8 in 8 parts 30.4 and in 16 (two to a unit) 22.0; 16384 x 4096 of 64 in fp16 in 8, 16 and 32 parts 83.5, 68.4 and 71.7; but
+// 8192 x 2048 of 128 in 16 parts 28.8 and in 32 34.0, and 3001 x 7168 of 256 in 4 parts 47.1 and in 8 58.8 (the best of all parts in each of
+// eleven such sizes, or within 2 %).  Workgroups of two waves, each in its best parts, with two pieces of grad_logits: 8192 x 4096 of 8 17.4
+// and not 16.9, 4452 x 1960 of 47 in fp32 18.2 and not 18.3, 2000 x 2048 of 60 12.7 and not 8.0.
 WeightShares weight_shares(uint64_t m, uint64_t experts, uint64_t hidden, uint32_t columns) {
   WeightShares w{};
   w.waves = experts > 128 ? 8 : 4;
@@ -807,18 +806,18 @@ struct BackwardSpace {
   WeightShares shares;
   uint64_t by_columns, sums, bytes;  // (fragments of the rows come first)
 };
-template <class T, class W> BackwardSpace backward_space(uint64_t m, uint64_t experts, uint64_t hidden) {
+template <class T> BackwardSpace backward_space(uint64_t m, uint64_t experts, uint64_t hidden) {
   BackwardSpace s{};
-  s.shares = weight_shares(m, experts, hidden, 32 * kColumnsOfLane<T, kOrder<W>>);
-  s.by_columns = fragment_bytes(m, experts, kOrder<T> + 1);
-  s.sums = s.by_columns + fragment_bytes(experts, m, kOrder<W> + 1);
+  s.shares = weight_shares(m, experts, hidden, 32 * kColumnsOfLane<T>);
+  s.by_columns = fragment_bytes(m, experts);
+  s.sums = s.by_columns + fragment_bytes(experts, m);
   s.bytes = s.sums + (s.shares.parts > 1 ? 4 * s.shares.parts * experts * hidden : 0);
   return s;
 }
 
 template <class T, class W> int launch_gradient_of_rows(GradientDev a, hipStream_t s) {
-  constexpr int kOrd = kOrder<T>, kNV = kColumnsOfLane<W, kOrd>;
-  typedef Turned<W, kNV, kOrd> B;
+  constexpr int kNV = kColumnsOfLane<W>;
+  typedef Turned<W, kNV> B;
   constexpr uint32_t kMost = kLdsBytes / B::kBytes / 4 * 64;  // k of a chunk
   const uint32_t whole = (a.k + 15) / 16 * 16, chunk = whole < kMost ? whole : kMost;
   a.column_blocks = (uint32_t)ceil_div(a.columns, 32 * kNV);
@@ -832,28 +831,28 @@ template <class T, class W> int launch_gradient_of_rows(GradientDev a, hipStream
       a.parts = (uint32_t)parts;
     }
   }
-  auto kernel = gradient_of_rows<W, T, kNV, kOrd>;
+  auto kernel = gradient_of_rows<W, T, kNV>;
   const uint32_t lds = chunk / 16 * B::kBytes;
   allow_lds(kernel, lds);
   return launch_groups(kernel, kernel, (uint64_t)a.column_blocks * a.parts, kGradientWaves * 64, lds, s, a, chunk);
 }
 
 template <class T, class W> int launch_gradient_of_weight(GradientDev a, const WeightShares &w, float *sums, hipStream_t s) {
-  constexpr int kOrd = kOrder<W>, kNV = kColumnsOfLane<T, kOrd>;
+  constexpr int kNV = kColumnsOfLane<T>;
   a.column_blocks = (uint32_t)ceil_div(a.columns, 32 * kNV);
   a.parts = w.parts;
   const uint64_t groups = (uint64_t)a.column_blocks * w.row_blocks * w.parts;
-  const uint32_t lds = 2 * w.waves * Turned<T, kNV, kOrd>::kBytes;
+  const uint32_t lds = 2 * w.waves * Turned<T, kNV>::kBytes;
   auto launch = [&](auto kernel) {
     allow_lds(kernel, lds);
     return launch_groups(kernel, kernel, groups, w.waves * 64, lds, s, a, w.tokens_per_part, w.row_blocks);
   };
-  if (w.parts == 1) return w.waves == 8 ? launch(gradient_of_weight<T, W, kNV, kOrd, 8>) : launch(gradient_of_weight<T, W, kNV, kOrd, 4>);
+  if (w.parts == 1) return w.waves == 8 ? launch(gradient_of_weight<T, W, kNV, 8>) : launch(gradient_of_weight<T, W, kNV, 4>);
   const SumDev sum{sums, (uint64_t)a.rows * a.columns, a.out, a.out_stride, a.rows, a.columns, a.columns, w.parts, 0};
   a.out = reinterpret_cast<uint8_t *>(sums);
   a.out_stride = a.columns;
   a.out_split = sum.split;
-  const int err = w.waves == 8 ? launch(gradient_of_weight<T, float, kNV, kOrd, 8>) : launch(gradient_of_weight<T, float, kNV, kOrd, 4>);
+  const int err = w.waves == 8 ? launch(gradient_of_weight<T, float, kNV, 8>) : launch(gradient_of_weight<T, float, kNV, 4>);
   return err ? err : launch_sum<W>(sum, s);
 }
 
@@ -882,8 +881,8 @@ extern "C" int pplx_a2a_router_workspace(uint32_t m, uint32_t num_experts, uint6
     *bytes = plan_logits(m, num_experts, hidden_dim, dtype, weight_dtype, false).bytes;
     return PPLX_A2A_OK;
   }
-  return with_weight_type(dtype, weight_dtype, [&](auto tag, auto weight_tag) {
-    *bytes = backward_space<typename decltype(tag)::type, typename decltype(weight_tag)::type>(m, num_experts, hidden_dim).bytes;
+  return with_type(dtype, [&](auto tag) {
+    *bytes = backward_space<typename decltype(tag)::type>(m, num_experts, hidden_dim).bytes;
     return (int)PPLX_A2A_OK;
   });
 }
@@ -967,7 +966,7 @@ extern "C" int pplx_a2a_router_logits_backward(int device, const pplx_a2a_router
       typedef typename decltype(tag)::type T;
       typedef typename decltype(weight_tag)::type W;
       hipStream_t s = (hipStream_t)stream;
-      const BackwardSpace space = backward_space<T, W>(p.m, p.num_experts, p.hidden_dim);
+      const BackwardSpace space = backward_space<T>(p.m, p.num_experts, p.hidden_dim);
       uint8_t *work = static_cast<uint8_t *>(p.workspace);
       PiecesDev pieces{};
       pieces.in = p.grad_logits;
@@ -976,8 +975,6 @@ extern "C" int pplx_a2a_router_logits_backward(int device, const pplx_a2a_router
       pieces.columns = p.num_experts;
       pieces.by_rows = p.grad_x ? work : nullptr;
       pieces.by_columns = p.grad_weight ? work + space.by_columns : nullptr;
-      pieces.pieces_by_rows = kOrder<T> + 1;
-      pieces.pieces_by_columns = kOrder<W> + 1;
       PPLX_LAUNCH(launch_split(pieces, s));
       if (p.grad_x) {
         GradientDev a{};

@@ -172,8 +172,7 @@ def router_logits_backward(
     workspace: torch.Tensor | None = None,
 ) -> tuple[torch.Tensor | None, torch.Tensor | None]:
     """The gradients of :func:`router_logits`: ``grad_logits @ weight`` and ``grad_logits.T @ x``, added up in float32 and rounded
-    once.  For bfloat16 results ``grad_logits`` (and float32 weights) count to 2**-18 of each value, for float16 and float32 to 24
-    bits.  In ``out`` either may be None, which leaves it out.  ``workspace`` is of :func:`router_workspace`."""
+    once; operands count to 24 bits whatever the results' type.  In ``out`` either may be None, which leaves it out.  ``workspace`` is of :func:`router_workspace`."""
     if out is None:
         out = (
             torch.empty_like(x, memory_format=torch.contiguous_format),

@@ -224,26 +224,25 @@ def test_gradients_of_router_logits_of_many_experts(device, m, experts, hidden, 
 
 
 @gpu
-@pytest.mark.parametrize("weight_dtype", [F16, F32])
-def test_half_precision_gradients_of_products_that_cancel(device, weight_dtype):
-    """Two products that cancel to a five-hundredth and less: what is left shows the bits of grad_logits far behind those that the
-    result has.  Only fp32's roundings are allowed for."""
+@pytest.mark.parametrize("dtype,weight_dtype,bits", [(F16, F16, 9), (F16, F32, 9), (BF16, BF16, 13), (BF16, F32, 13), (F32, F32, 16)])
+def test_gradients_of_products_that_cancel(device, dtype, weight_dtype, bits):
+    """Two products that cancel to 2^-bits of them: what is left shows the bits of grad_logits far behind those that a result of 16 bits
+    has.  Only fp32's roundings are allowed for."""
     gen = torch.Generator().manual_seed(12)
 
-    def two(n):  # n pairs of fp32 numbers whose sum is 2^-9 to 2^-8 of them
+    def two(n):  # n pairs of fp32 numbers whose sum is 2^-bits to twice that of them
         a = 1 + torch.rand(n, 1, generator=gen)
-        return torch.cat([a, -a * (1 + 2.0**-9 * (1 + torch.rand(n, 1, generator=gen)))], 1)
+        return torch.cat([a, -a * (1 + 2.0**-bits * (1 + torch.rand(n, 1, generator=gen)))], 1)
 
     # of the rows: 64 tokens, two experts with one weight
     weight = (1 + torch.rand(1, 512, generator=gen)).to(weight_dtype).expand(2, 512).contiguous()
-    x, grad = torch.randn(64, 512, generator=gen).to(F16), two(64)
+    x, grad = torch.randn(64, 512, generator=gen).to(dtype), two(64)
     got, _ = router_logits_backward(grad.to(device), x.to(device), weight.to(device))
     want, off = product(grad, weight, 2)
-    assert_within(got, want, rounded(want, F16, off))
+    assert_within(got, want, rounded(want, dtype, off))
     # of the weight: 64 experts, two tokens with one row
-    if weight_dtype == F16:
-        x, grad = (1 + torch.rand(1, 512, generator=gen)).to(F16).expand(2, 512).contiguous(), two(64).t().contiguous()
-        weight = torch.randn(64, 512, generator=gen).to(F16)
-        _, got = router_logits_backward(grad.to(device), x.to(device), weight.to(device))
-        want, off = product(grad.t(), x, 2)
-        assert_within(got, want, rounded(want, F16, off))
+    x, grad = (1 + torch.rand(1, 512, generator=gen)).to(dtype).expand(2, 512).contiguous(), two(64).t().contiguous()
+    weight = torch.randn(64, 512, generator=gen).to(weight_dtype)
+    _, got = router_logits_backward(grad.to(device), x.to(device), weight.to(device))
+    want, off = product(grad.t(), x, 2)
+    assert_within(got, want, rounded(want, weight_dtype, off))
