@@ -485,9 +485,10 @@ int pplx_a2a_int8_matmul_plan(const pplx_a2a_rows_t *rows, uint64_t n, uint64_t 
  *   v = h * weight / sqrt(mean(h^2) + eps), in fp32, rounded to dtype      -> y
  *   the quantised v, of which y is not a part                              -> q, scale
  * PPLX_A2A_ROWS_INT8: one scale a row, as pplx_a2a_quantize_rows.  PPLX_A2A_ROWS_E4M3: one scale for each 128 columns, which
- * is how dispatch carries fp8 rows: a = max(max |v|, 2^-100), scale = a / 448, q = v * (448 / a) rounded to e4m3.  A row that
- * holds an infinity or a NaN becomes NaN: y and the scales are NaN, q is zeros.  y and sum may be x or residual themselves (same
- * address and stride). */
+ * is how dispatch carries fp8 rows: a = max(max |v|, 2^-100), scale = a / 448, q = v * (448 / a) rounded to e4m3.  (A v that lies in the
+ * middle between two codes but for the roundings of fp32 has either of them; the same inputs have the same.)  A row that holds an
+ * infinity or a NaN becomes NaN: y and the scales are NaN, q is zeros.  y and sum may be x or residual themselves (same address and
+ * stride). */
 typedef enum pplx_a2a_row_format { PPLX_A2A_ROWS_PLAIN = 0, PPLX_A2A_ROWS_INT8 = 1, PPLX_A2A_ROWS_E4M3 = 2 } pplx_a2a_row_format;
 typedef struct pplx_a2a_rms_norm_args {
   const void *x;               /* [m, hidden_dim] of dtype; all rows 16-byte aligned, strides in bytes, multiples of 16 */
@@ -539,7 +540,7 @@ int pplx_a2a_rms_norm_workspace(uint32_t m, uint64_t hidden_dim, uint64_t *bytes
 int pplx_a2a_rms_norm_backward(int device, const pplx_a2a_rms_norm_backward_args_t *args, void *stream);
 
 /* The router's product: logits[t, e] = sum over k of x[t, k] * weight[e, k], added up in fp32.  Products of 16-bit elements are
- * exact; fp32 elements count to 24 bits.  (With weights of fp32 an infinity in a row or a weight, or a value above 3.38e38, makes a NaN.) */
+ * exact; fp32 elements count to 24 bits.  (With weights of fp32 an infinity in a row or a weight, or a value above 3.38e38, may make a NaN.) */
 typedef struct pplx_a2a_router_logits_args {
   const void *x;               /* [m, hidden_dim] of dtype; rows 16-byte aligned, strides in bytes, multiples of 16 */
   int64_t x_stride_row;

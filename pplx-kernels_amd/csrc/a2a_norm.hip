@@ -460,9 +460,10 @@ template <class T, class W> __global__ __launch_bounds__(kSumThreads) void norm_
 constexpr uint64_t kMostInRegisters = 8 * 4 * 512;
 
 // The gradients' workgroups, each with a share of the weight's gradient to add up: as few as keep memory busy.  One of them has 8192
-// elements of each operand under way, or 4096 of rows of up to that, 2048 of short ones.  With the sum, us:
-//   8192 x 7168  256: 89, 512: 96, 1024: 102       8192 x 4096 with weights in fp32  256: 62, 512: 57     4096 x 2048  256: 18.2, 512: 19.2
-//   16384 x 512  256: 19.7, 512: 18.8, 1024: 21.5   262144 x 128  256: 177, 512: 113, 1024: 83
+// elements of each operand under way, or 4096 of rows of up to that, 2048 of short ones.  Both launches, with grad_sum, in a graph over
+// tensors and results that no cache holds, us (a step's own results may lie in the caches: 8192 x 4096 then takes 43 + 5):
+//   8192 x 7168  256: 89, 512: 97, 1024: 104       8192 x 4096 with weights in fp32  256: 60, 512: 57, 1024: 61     4096 x 2048  256: 17.9, 512: 19.2
+//   16384 x 512  256: 19.1, 512: 17.7, 1024: 20.6   262144 x 128  256: 178, 512: 113, 1024: 84
 uint32_t backward_groups(uint32_t m, uint64_t width) {
   const uint64_t rows = width <= 2048 ? ((uint64_t)m + 3) / 4 : m;
   const uint64_t most = width <= 128 ? 1024 : width <= 512 || (width > 2048 && width <= 4096) ? 512 : 256;

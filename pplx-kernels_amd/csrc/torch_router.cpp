@@ -46,9 +46,9 @@ const at::Tensor *unless_same(const at::Tensor *x, const at::Tensor *out) { retu
 
 float as_float(double v) { return (float)v; }
 
-// Bytes for a call's own use, which go back to torch's allocator with the call: a later one on the same stream may have them,
-// and a captured one has them to itself.
-// `given`, or memory of torch's allocator, which a capture by torch keeps in its graph's pool.
+// Bytes for a call's own use: the caller's, `given`, checked against what else the call reads and writes, or memory of torch's
+// allocator, which goes back to it with the call: a later one on the same stream may have it, and a capture by torch keeps it in its
+// graph's pool.
 at::Tensor space(uint64_t bytes, const at::Tensor &with, const at::Tensor *given, std::initializer_list<const at::Tensor *> others) {
   if (!given) return fresh({(int64_t)bytes}, with, at::kByte);
   check_dense(*given, at::kByte, 1, with, "workspace");

@@ -84,8 +84,9 @@ def rms_norm(
     """``h = x + residual``, rounded to the type of ``x``, and ``v = h * weight / sqrt(mean(h**2) + eps)`` in fp32: ``sum`` is ``h``
     (None without ``residual``) and ``y`` is ``v``, rounded once.  With ``quantize`` also ``v`` in 8 bits: ``torch.int8`` with one scale
     a row, as by :func:`quantize_rows`, or ``torch.float8_e4m3fn`` with one scale for each 128 columns, ``a = max(max |v|, 2**-100)``,
-    ``q = e4m3(v * (448 / a))``, ``scale = a / 448``, which is what ``dispatch`` takes as ``dp_x`` and ``dp_x_scale``.  A row that holds
-    an infinity or a NaN becomes NaN (``q`` zeros, its scales NaN).
+    ``q = e4m3(v * (448 / a))``, ``scale = a / 448``, which is what ``dispatch`` takes as ``dp_x`` and ``dp_x_scale``.  (Where ``v`` lies in
+    the middle between two codes, fp32's roundings decide: another order of its sums may take the other one.)  A row that holds an
+    infinity or a NaN becomes NaN (``q`` zeros, its scales NaN).
 
     ``x`` is ``[m, H]`` of float32, bfloat16 or float16, its rows 16-byte aligned and ``H`` a multiple of 8 (with ``quantize`` of 16);
     ``weight`` is ``[H]`` of its type or float32.  Differentiable in ``x``, ``residual`` and ``weight``, through ``y`` and ``sum`` (``q`` and
